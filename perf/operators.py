@@ -194,10 +194,11 @@ def _rotate(x, pos, state):
 def _write(state, which, rows, phys, slot):
     fmt = state["case"]["fmt"]
     amax = rows.abs().amax(-1).clamp_min(MIN_AMAX)
-    scaled = rows * (Q_MAX[fmt] / amax)[..., None]
+    top = torch.full_like(amax, Q_MAX[fmt])              # (a tensor over a tensor: one rounded division, with no reciprocal between)
+    scaled = rows * (top / amax)[..., None]
     codes = scaled.round().to(torch.int8) if fmt == "i8" else scaled.to(torch.float8_e4m3fn)
     state["codes"][which].view(torch.uint8)[phys, slot] = codes.view(torch.uint8)
-    state["scales"][which][phys, :, slot] = amax / Q_MAX[fmt]
+    state["scales"][which][phys, :, slot] = amax / top
 
 
 def _append(state):
@@ -342,7 +343,7 @@ def exact(case, seed):
             if case["op"] != "read":
                 fresh = turned(state["k"][at:at + n], p) if i == 0 else state["v"][at:at + n].double()
                 amax = fresh.abs().amax(-1, keepdim=True).clamp_min(MIN_AMAX)
-                y = fresh.float() * (top / amax.float())       # the codes are defined by these two fp32 operations
+                y = fresh.float() * (torch.full_like(amax, top).float() / amax.float())       # the codes are defined by these two fp32 operations
                 y = y.round() if fmt == "i8" else y.to(torch.float8_e4m3fn)
                 x[p - lo:] = y.double() * (amax / top)
             kv.append(x)
