@@ -19,7 +19,8 @@ LIB_PATH = os.environ.get("NOVA_B200_LIB") or os.path.join(HERE, "libnova_b200.s
 OK = 0
 ERR_INVALID, ERR_POOL_FULL, ERR_NO_SLICE, ERR_NO_SESSION, ERR_CUDA = -1, -2, -3, -4, -5
 ERR_BAD_TABLE, ERR_TIMEOUT, ERR_UNSUPPORTED, ERR_TOO_LARGE, ERR_BUSY = -6, -7, -8, -9, -10
-KV_F32, KV_F16 = 0, 1
+KV_F32, KV_F16, KV_I8, KV_E4M3 = 0, 1, 2, 3
+IO_F32, IO_F16, IO_BF16 = 0, 1, 2
 
 c_i32p = C.POINTER(C.c_int32)
 c_f32p = C.POINTER(C.c_float)
@@ -47,6 +48,21 @@ class KvShape(C.Structure):
 class KvBlock(C.Structure):
     _fields_ = [("prefix", C.c_uint64), ("suffix", C.c_uint64), ("session", C.c_int32),
                 ("turn", C.c_int32), ("pos0", C.c_int64), ("pos1", C.c_int64)]
+
+
+class Q8Cache(C.Structure):
+    """nova_q8_cache: pages of 8-bit codes with their scales, block tables and rotary tables.  Pointers are addresses."""
+    _fields_ = [("shape", KvShape), ("layer", C.c_int32), ("nb", C.c_int32), ("pool_k", C.c_void_p), ("pool_v", C.c_void_p),
+                ("scale_k", C.c_void_p), ("scale_v", C.c_void_p), ("tables", C.c_void_p), ("table_stride", C.c_int64),
+                ("slice_ids", C.c_void_p), ("rope_cs", C.c_void_p), ("rope_sn", C.c_void_p), ("rope_rows", C.c_int64),
+                ("status", C.c_void_p)]
+
+
+class Q8Rows(C.Structure):
+    """nova_q8_rows: which rows of q / k / v / out belong to which session, and at which positions."""
+    _fields_ = [("n_sessions", C.c_int32), ("n_tokens", C.c_int32), ("max_tokens", C.c_int32), ("io_dtype", C.c_int32),
+                ("n_past", C.c_void_p), ("tok_start", C.c_void_p), ("q_stride", C.c_int64), ("k_stride", C.c_int64),
+                ("v_stride", C.c_int64), ("out_stride", C.c_int64)]
 
 
 vp, i32, i64, u64, sz = C.c_void_p, C.c_int, C.c_int64, C.c_uint64, C.c_size_t
@@ -107,6 +123,11 @@ SIGNATURES = {
     "nova_launch_attn_decode_paged": (i32, [C.POINTER(KvShape), vp, vp, vp, vp, i32, i32, i32, vp, vp, vp]),
     "nova_attn_static_scratch_max_heads": (sz, []),
     "nova_launch_attn_decode_paged_static": (i32, [C.POINTER(KvShape), vp, vp, vp, vp, i32, i32, i32, vp, vp]),
+    "nova_launch_q8_append": (i32, [C.POINTER(Q8Cache), C.POINTER(Q8Rows), vp, vp, vp]),
+    "nova_launch_q8_read": (i32, [C.POINTER(Q8Cache), C.POINTER(Q8Rows), vp, vp, vp]),
+    "nova_q8_workspace_bytes": (sz, [C.POINTER(KvShape), C.POINTER(Q8Rows)]),
+    "nova_launch_q8_attn": (i32, [C.POINTER(Q8Cache), C.POINTER(Q8Rows), vp, vp, i32, vp, sz, vp]),
+    "nova_launch_q8_append_attn": (i32, [C.POINTER(Q8Cache), C.POINTER(Q8Rows), vp, vp, vp, vp, i32, vp, sz, vp]),
     "nova_synth_key": (u64, [u64, u64, u64, u64]), "nova_synth_normal": (i32, [vp, sz, u64, u64, vp]),
     "nova_batch_create": (i32, [vp, c_i32p, i32, C.POINTER(vp)]), "nova_batch_destroy": (None, [vp]),
     "nova_batch_size": (i32, [vp]), "nova_batch_sync_positions": (i32, [vp, vp]),
@@ -281,6 +302,28 @@ class PoolView:
                     tables={s: self.table(s).tolist() for s in live},
                     n_past={s: self.n_past(s) for s in live},
                     need_copy={s: list(self.need_copy(s)) for s in live})
+
+
+# ------------------------------------------------------------------------------ 8-bit paged cache
+# The operators of nova_launch_q8_*: cache and rows are Q8Cache / Q8Rows, everything else device addresses and a stream handle.
+def q8_append(cache: Q8Cache, rows: Q8Rows, k, v, stream=None):
+    return check(lib.nova_launch_q8_append(cache, rows, k, v, stream), "q8_append")
+
+
+def q8_read(cache: Q8Cache, rows: Q8Rows, k_out, v_out, stream=None):
+    return check(lib.nova_launch_q8_read(cache, rows, k_out, v_out, stream), "q8_read")
+
+
+def q8_workspace_bytes(shape: KvShape, rows: Q8Rows) -> int:
+    return int(lib.nova_q8_workspace_bytes(shape, rows))
+
+
+def q8_attn(cache: Q8Cache, rows: Q8Rows, q, out, window, work, work_bytes, stream=None):
+    return check(lib.nova_launch_q8_attn(cache, rows, q, out, window, work, work_bytes, stream), "q8_attn")
+
+
+def q8_append_attn(cache: Q8Cache, rows: Q8Rows, q, k, v, out, window, work, work_bytes, stream=None):
+    return check(lib.nova_launch_q8_append_attn(cache, rows, q, k, v, out, window, work, work_bytes, stream), "q8_append_attn")
 
 
 # ------------------------------------------------------------------------------ device helpers

@@ -1,0 +1,172 @@
+// q8_common.cuh — what the kernels of the 8-bit paged cache share: the launch description, the rows of a session, the
+// element types of activations and codes.
+//
+// The cache: value = code * scale.  Codes [layer][NB][page tokens][NKV][128], one byte each (int8, or e4m3); one fp32
+// scale per (token, kv head) [layer][NB][NKV][page tokens], kv head major within a page so that the scales of one
+// head's tile of keys are one contiguous piece.
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_fp8.h>
+
+#include "common.cuh"
+
+namespace novab {
+
+// A row that is all zeros (or nearly) still gets a positive scale: amax is taken to be at least this.
+constexpr float kQ8MinAmax = 8.6736173798840355e-19f;      // 2^-60
+// ... and attention takes a scale of V to be at least this, so that its logarithm and reciprocal are finite for pages
+// that were never written (zeroed scales).  Codes up to 448 times it are below 1e-18.
+constexpr float kQ8MinScale = 8.4703294725430034e-22f;     // 2^-70
+
+struct Q8Launch {
+    void* pool_k;
+    void* pool_v;
+    float* scale_k;
+    float* scale_v;
+    const int32_t* tables;
+    int64_t table_stride;
+    const int32_t* slice_ids;     // nullptr: session s uses table s
+    const int32_t* n_past;        // [S] position of the first row of each session
+    const int32_t* tok_start;     // [S + 1] rows of session s: [tok_start[s], tok_start[s + 1]); nullptr: uniform_tokens each
+    const void* q;                // [n_tokens][NH][128], io type, rows q_stride elements apart
+    const void* k;                // [n_tokens][NKV][128]
+    const void* v;
+    void* out;                    // [n_tokens][NH][128]
+    void* k_out;                  // read back: [n_tokens][NKV][128]
+    void* v_out;
+    float* q_rot;                 // append only (fp32 activations): rotate q / k in place as well, or nullptr
+    float* k_rot;
+    int64_t q_stride, k_stride, v_stride, out_stride;
+    const float* rope_cs;         // nullptr: q and k are taken as they are
+    const float* rope_sn;
+    int64_t rope_rows;
+    int32_t* status;
+    float* part;                  // workspace of the attention
+    int32_t n_sessions, n_tokens, max_tokens, uniform_tokens;
+    int32_t io, fmt, neox;
+    int32_t layer, nb, n_heads, n_kv_heads, kv_shift;
+    int32_t window;
+    int32_t append;               // attention: write the (single) new token of every session on the way
+};
+
+#ifdef __CUDACC__
+
+// Rows of session s, never outside [0, n_tokens) whatever tok_start holds.
+__device__ __forceinline__ void q8_rows(const Q8Launch& a, int s, int& first, int& count) {
+    if (!a.tok_start) {
+        first = s * a.uniform_tokens;
+        count = a.uniform_tokens;
+        return;
+    }
+    int f = __ldg(a.tok_start + s), e = __ldg(a.tok_start + s + 1);
+    f = f < 0 ? 0 : (f > a.n_tokens ? a.n_tokens : f);
+    e = e < f ? f : (e > a.n_tokens ? a.n_tokens : e);
+    first = f;
+    count = e - f < a.max_tokens ? e - f : a.max_tokens;
+}
+
+// Session and token-within-session of row r: the last session that starts at or before r (-1: the row is nobody's).
+__device__ __forceinline__ int q8_session_of(const Q8Launch& a, int r, int& t) {
+    if (!a.tok_start) {
+        const int s = r / a.uniform_tokens;
+        t = r - s * a.uniform_tokens;
+        return s < a.n_sessions ? s : -1;
+    }
+    int lo = 0, up = a.n_sessions;
+    while (up - lo > 1) {
+        const int mid = (lo + up) >> 1;
+        if (__ldg(a.tok_start + mid) <= r) lo = mid; else up = mid;
+    }
+    int first, count;
+    q8_rows(a, lo, first, count);
+    t = r - first;
+    return t >= 0 && t < count ? lo : -1;
+}
+
+__device__ __forceinline__ const int32_t* q8_table(const Q8Launch& a, int s) {
+    return a.tables + (int64_t)(a.slice_ids ? __ldg(a.slice_ids + s) : s) * a.table_stride;
+}
+
+__device__ __forceinline__ void q8_flag(const Q8Launch& a, int code) {
+    if (a.status) atomicCAS(a.status, 0, code);
+}
+
+// ---- activations: four consecutive values as fp32
+template <typename T> struct Q8Io;
+template <> struct Q8Io<float> {
+    static __device__ __forceinline__ float4 load4(const float* p) { return *reinterpret_cast<const float4*>(p); }
+    static __device__ __forceinline__ void store4(float* p, float4 v) { *reinterpret_cast<float4*>(p) = v; }
+};
+template <> struct Q8Io<__half> {
+    static __device__ __forceinline__ float4 load4(const __half* p) {
+        const uint2 u = *reinterpret_cast<const uint2*>(p);
+        const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&u.x)), b = __half22float2(*reinterpret_cast<const __half2*>(&u.y));
+        return make_float4(a.x, a.y, b.x, b.y);
+    }
+    static __device__ __forceinline__ void store4(__half* p, float4 v) {
+        const __half2 a = __floats2half2_rn(v.x, v.y), b = __floats2half2_rn(v.z, v.w);
+        *reinterpret_cast<uint2*>(p) = make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
+    }
+};
+template <> struct Q8Io<__nv_bfloat16> {
+    static __device__ __forceinline__ float4 load4(const __nv_bfloat16* p) {
+        const uint2 u = *reinterpret_cast<const uint2*>(p);
+        return make_float4(__uint_as_float(u.x << 16), __uint_as_float(u.x & 0xffff0000u), __uint_as_float(u.y << 16),
+                           __uint_as_float(u.y & 0xffff0000u));
+    }
+    static __device__ __forceinline__ void store4(__nv_bfloat16* p, float4 v) {
+        const __nv_bfloat162 a = __floats2bfloat162_rn(v.x, v.y), b = __floats2bfloat162_rn(v.z, v.w);
+        *reinterpret_cast<uint2*>(p) = make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
+    }
+};
+// The same with the type known only at run time (a few loads per row: the branch is uniform).
+__device__ __forceinline__ float4 q8_load4(const void* base, int64_t elem, int io) {
+    if (io == NOVA_IO_F32) return Q8Io<float>::load4(static_cast<const float*>(base) + elem);
+    if (io == NOVA_IO_F16) return Q8Io<__half>::load4(static_cast<const __half*>(base) + elem);
+    return Q8Io<__nv_bfloat16>::load4(static_cast<const __nv_bfloat16*>(base) + elem);
+}
+__device__ __forceinline__ void q8_store4(void* base, int64_t elem, int io, float4 v) {
+    if (io == NOVA_IO_F32) Q8Io<float>::store4(static_cast<float*>(base) + elem, v);
+    else if (io == NOVA_IO_F16) Q8Io<__half>::store4(static_cast<__half*>(base) + elem, v);
+    else Q8Io<__nv_bfloat16>::store4(static_cast<__nv_bfloat16*>(base) + elem, v);
+}
+
+// ---- codes: four of them in a word
+template <int kFmt> __device__ __forceinline__ float4 q8_decode4(uint32_t w) {
+    if constexpr (kFmt == NOVA_KV_I8) {
+        return make_float4((float)(int8_t)(w & 0xff), (float)(int8_t)((w >> 8) & 0xff), (float)(int8_t)((w >> 16) & 0xff), (float)(int8_t)(w >> 24));
+    } else {
+        uint32_t h0, h1;
+        asm("{ .reg .b16 l, h; mov.b32 {l, h}, %2; cvt.rn.f16x2.e4m3x2 %0, l; cvt.rn.f16x2.e4m3x2 %1, h; }" : "=r"(h0), "=r"(h1) : "r"(w));
+        const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&h0)), b = __half22float2(*reinterpret_cast<const __half2*>(&h1));
+        return make_float4(a.x, a.y, b.x, b.y);
+    }
+}
+// Round to nearest, ties to even, in both formats.  |x| <= Q but for the rounding of the product; a NaN becomes code 0
+// (int8) or NaN (e4m3).
+template <int kFmt> __device__ __forceinline__ uint32_t q8_encode4(float4 x) {
+    if constexpr (kFmt == NOVA_KV_I8) {
+        auto code = [](float f) -> uint32_t {
+            int c = __float2int_rn(f);
+            c = c > 127 ? 127 : (c < -127 ? -127 : c);
+            return (uint32_t)c & 0xffu;
+        };
+        return code(x.x) | (code(x.y) << 8) | (code(x.z) << 16) | (code(x.w) << 24);
+    } else {
+        uint32_t w;
+        asm("{ .reg .b16 l, h; cvt.rn.satfinite.e4m3x2.f32 l, %2, %1; cvt.rn.satfinite.e4m3x2.f32 h, %4, %3; mov.b32 %0, {l, h}; }"
+            : "=r"(w) : "f"(x.x), "f"(x.y), "f"(x.z), "f"(x.w));
+        return w;
+    }
+}
+template <int kFmt> __device__ __forceinline__ constexpr float q8_qmax() { return kFmt == NOVA_KV_I8 ? 127.f : 448.f; }
+
+#endif  // __CUDACC__
+
+// q8_cache.cu / q8_attn.cu
+int launch_q8_append(const Q8Launch& a, cudaStream_t s);
+int launch_q8_read(const Q8Launch& a, cudaStream_t s);
+int launch_q8_attn(const Q8Launch& a, size_t work_bytes, cudaStream_t s);
+size_t q8_work_bytes(int n_heads, int n_kv_heads, int n_sessions, int n_tokens, int max_tokens);
+
+}  // namespace novab

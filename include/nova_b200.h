@@ -42,6 +42,15 @@ const char* nova_last_cuda_error(void);
 /* KV element type of the page pools. */
 #define NOVA_KV_F32 0   /* the reference's format (float* pool_k/pool_v, include/nova/model.h:173-174) */
 #define NOVA_KV_F16 1   /* IEEE half, value = round-to-nearest-even of the fp32 value */
+/* 8-bit pages (no counterpart in the reference): value = code * scale, one fp32 scale per (token, kv head).  See the
+ * "8-bit paged cache" section for the layout and the rounding. */
+#define NOVA_KV_I8   2  /* int8 codes, -127..127 */
+#define NOVA_KV_E4M3 3  /* 8-bit floats: 4 exponent bits, 3 mantissa bits, largest value 448 */
+
+/* Element type of activations (8-bit cache operators; everything else takes fp32). */
+#define NOVA_IO_F32  0
+#define NOVA_IO_F16  1
+#define NOVA_IO_BF16 2
 
 /* Opaque CUDA stream (cudaStream_t).  NULL = the legacy default stream. */
 typedef void* nova_stream_t;
@@ -301,6 +310,64 @@ int nova_launch_attn_decode_paged_static(const nova_kv_shape* sh, const float* q
                                          const void* pool_k, const void* pool_v,
                                          const int32_t* table, int layer, int nb, int n_keys,
                                          float* o, nova_stream_t s);
+
+/* ------------------------------------------------------- 8-bit paged cache */
+/* Operators on pages of 8-bit codes, for any number of sessions per launch (no counterpart in the reference).
+ *   codes  pool_k / pool_v   [layers][nb][kv_block][n_kv_heads][128], one byte each (shape.kv_dtype: NOVA_KV_I8 | NOVA_KV_E4M3)
+ *   scales scale_k / scale_v [layers][nb][n_kv_heads][kv_block] fp32
+ * A row (one token of one kv head) is written as  amax = max(max|x|, 2^-60),  scale = amax / Q,  code = rn(x * (Q / amax)),
+ * Q = 127 or 448, in fp32 with one rounding per operation (ties to even).  A NaN becomes code 0 (int8) or NaN (e4m3); a row
+ * with an infinity gets an infinite scale and reads back as NaN.
+ * The block tables are those of the rest of this header: `tables` is an array of tables of table_stride entries, session s
+ * uses table slice_ids[s] (slice_ids NULL: table s).  An entry outside [0, nb) is never followed: its keys are skipped, its
+ * rows are neither written nor read back, and *status (device, may be NULL) becomes NOVA_ERR_BAD_TABLE.
+ * rope_cs / rope_sn [rope_rows][64] (both NULL: no rotation): k is rotated at its position before it is quantised, q when it
+ * is read; neither buffer is changed.  A position beyond the tables is skipped and flagged (NOVA_ERR_INVALID).
+ * All pointers 16-byte aligned (tables, positions and status: 4).  All calls act on the calling thread's current device,
+ * are asynchronous, keep nothing from one call to the next, allocate nothing, and may be captured into a graph. */
+typedef struct {
+    nova_kv_shape  shape;
+    int32_t        layer;          /* which layer of the pools this call works on */
+    int32_t        nb;             /* pages per layer */
+    void          *pool_k, *pool_v;
+    float         *scale_k, *scale_v;
+    const int32_t *tables;
+    int64_t        table_stride;
+    const int32_t *slice_ids;
+    const float   *rope_cs, *rope_sn;
+    int64_t        rope_rows;
+    int32_t       *status;
+} nova_q8_cache;
+
+/* The rows of one call: session s has the rows [tok_start[s], tok_start[s+1]) of q / k / v / out (any number, none included),
+ * at the positions n_past[s], n_past[s] + 1, ...  tok_start NULL: every session has n_tokens / n_sessions rows.  Rows of the
+ * buffers that belong to no session are left as they are. */
+typedef struct {
+    int32_t        n_sessions;
+    int32_t        n_tokens;       /* rows of all sessions together */
+    int32_t        max_tokens;     /* the most rows that one session has (rows beyond it are not worked on) */
+    int32_t        io_dtype;       /* of q, k, v and out: NOVA_IO_F32 | NOVA_IO_F16 | NOVA_IO_BF16 */
+    const int32_t *n_past;         /* device [n_sessions] */
+    const int32_t *tok_start;      /* device [n_sessions + 1], ascending, or NULL */
+    int64_t        q_stride, k_stride, v_stride, out_stride;   /* elements from row to row, multiples of 16 bytes; 0: dense */
+} nova_q8_rows;
+
+/* Write the rows of k and v ([n_tokens][n_kv_heads][128]) into the cache. */
+int nova_launch_q8_append(const nova_q8_cache* c, const nova_q8_rows* r, const void* k, const void* v, nova_stream_t s);
+/* Read the cached rows at those positions back: k_out / v_out [n_tokens][n_kv_heads][128], dense, io_dtype, code * scale
+ * rounded once (keys come back as they are stored: rotated). */
+int nova_launch_q8_read(const nova_q8_cache* c, const nova_q8_rows* r, void* k_out, void* v_out, nova_stream_t s);
+/* Attention of the rows of q ([n_tokens][n_heads][128]) over the cached keys: the query at position p sees the keys [0, p], or
+ * (p - window, p] where window > 0.  The keys of the new rows must be in the cache; a query that sees none gets zeros.
+ * q is taken to fp16 where a session has several rows or a kv head more than 8 query heads, to fp16 hi + lo parts otherwise;
+ * sums and the softmax are fp32.  q and out must not overlap.  work: nova_q8_workspace_bytes() bytes, no state in it
+ * between calls; calls that may overlap on the GPU need a workspace each. */
+size_t nova_q8_workspace_bytes(const nova_kv_shape* sh, const nova_q8_rows* r);
+int nova_launch_q8_attn(const nova_q8_cache* c, const nova_q8_rows* r, const void* q, void* out, int window, void* work,
+                        size_t work_bytes, nova_stream_t s);
+/* nova_launch_q8_append followed by nova_launch_q8_attn: one decode step, or one chunk of a prompt, of a layer. */
+int nova_launch_q8_append_attn(const nova_q8_cache* c, const nova_q8_rows* r, const void* q, const void* k, const void* v, void* out,
+                               int window, void* work, size_t work_bytes, nova_stream_t s);
 
 /* ------------------------------------------- batched decode over sessions */
 /* Engine::decode_batch's hot-path calls (model.cpp:281-289) for any number of

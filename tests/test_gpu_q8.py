@@ -1,0 +1,313 @@
+"""The 8-bit paged cache: writing it (rotation, scales, codes bit for bit), reading it back, decode and chunk attention over it,
+against plain 64-bit forms (q8_plain.py).  Rows that nobody may look at hold NaN scales and, in e4m3, NaN codes; table entries
+behind the last page are -1; output rows behind the last session hold a value that must stay."""
+import math
+
+import pytest
+import torch
+
+from q8_plain import HD, IO, Cache, attention_bound, call
+
+pytestmark = pytest.mark.gpu
+
+
+def same_bits(x, y):
+    x, y = x.cpu().contiguous(), y.contiguous()
+    return x.shape == y.shape and bool((x.view(torch.uint8) == y.view(torch.uint8)).all())
+
+
+def run_and_check(nv, case, what="append_attn", extra_rows=3):
+    d = case.device(nv, extra_rows=extra_rows)
+    case.append()
+    if what == "attn":
+        call(nv, d, "append")
+    call(nv, d, what, case.window)
+    torch.cuda.synchronize()
+    assert int(d["status"]) == 0
+    check_cache(case, d)
+    check_out(case, d)
+    return d
+
+
+def check_cache(case, d):
+    for i in (0, 1):
+        assert same_bits(d["codes"][i], case.codes[i]), "codes"
+        assert same_bits(d["scales"][i], case.scales[i]), "scales"
+
+
+def check_out(case, d):
+    T = sum(case.new)
+    got = d["out"].cpu()
+    assert bool((got[T:] == 7).all()), "rows behind the last session"
+    o, a, spread = case.attend()
+    exact_q = max(case.new) == 1 and case.H // case.N <= 8
+    bound = attention_bound(case, o, a, spread, exact_q)
+    off = (got[:T].double() - o).abs()
+    assert bool(torch.isfinite(got[:T]).all()), "finite"
+    assert bool((off <= bound).all()), f"off by {float((off / bound).max()):.3g} of the bound at {divmod(int((off / bound).argmax()), HD)}"
+
+
+@pytest.mark.parametrize("rope", ["neox", "pairs", "none"])
+@pytest.mark.parametrize("fmt", ["i8", "e4m3"])
+@pytest.mark.parametrize("io,page,packed", [("f32", 16, False), ("f16", 8, True), ("bf16", 64, True), ("bf16", 32, False)])
+def test_append_and_read_back(nv, io, page, packed, fmt, rope):
+    for N, past, new in ((1, [0], [1]), (3, [5, 0, 63, 16], [0, 70, 1, 17]), (8, [130, 7], [33, 64])):
+        case = Cache(past, new, 2 * N, N, page, fmt, io, rope=rope, packed=packed, seed=N)
+        d = case.device(nv, extra_rows=2)
+        case.append()
+        call(nv, d, "append")
+        call(nv, d, "read")
+        torch.cuda.synchronize()
+        assert int(d["status"]) == 0
+        check_cache(case, d)
+        for got, want in zip(d["back"], case.read()):
+            T = sum(new)
+            assert bool((got[T:] == 7).all())
+            assert same_bits(got[:T], want)
+
+
+@pytest.mark.parametrize("fmt", ["i8", "e4m3"])
+def test_append_of_extreme_rows(nv, fmt):
+    """Zero rows, rows of the type's smallest and largest values, one outlier among zeros: the scale stays positive and finite."""
+    case = Cache([3], [8], 2, 2, 16, fmt, "f32", rope="none")
+    case.k.zero_()
+    case.v.zero_()
+    case.k[1] = 1e-45
+    case.k[2] = 3.3e38
+    case.k[3, :, 77] = -5.0
+    case.v[4] = -1e-30
+    case.v[5] = torch.finfo(torch.float32).tiny
+    case.v[6, :, ::2] = 3e38
+    d = case.device(nv)
+    case.append()
+    call(nv, d, "append")
+    call(nv, d, "read")
+    torch.cuda.synchronize()
+    check_cache(case, d)
+    assert bool((d["scales"][0][1].isfinite() | d["scales"][0][1].isnan()).all())
+    for got, want in zip(d["back"], case.read()):
+        assert same_bits(got, want) and bool(want.isfinite().all())
+
+
+@pytest.mark.parametrize("fmt", ["i8", "e4m3"])
+def test_append_of_values_that_are_no_numbers(nv, fmt):
+    """A NaN becomes code 0 (int8) or NaN (e4m3) and leaves the row's other values alone; a row with an infinity reads back as NaN."""
+    case = Cache([0], [2], 1, 1, 16, fmt, "f32", rope="none")
+    case.k[0, 0, 5] = math.nan
+    case.v[1, 0, 9] = math.inf
+    d = case.device(nv)
+    call(nv, d, "append")
+    call(nv, d, "read")
+    torch.cuda.synchronize()
+    k, v = (x.cpu() for x in d["back"])
+    keep = torch.arange(HD) != 5
+    assert bool(k[0, 0, keep].isfinite().all()) and (float(k[0, 0, 5]) == 0 if fmt == "i8" else bool(k[0, 0, 5].isnan()))
+    assert bool(k[1].isfinite().all()) and bool(v[0].isfinite().all())
+    assert bool(v[1, 0].isnan().all())
+
+
+LENGTHS = [0, 1, 2, 7, 8, 9, 15, 16, 17, 31, 32, 33, 63, 64, 65, 127, 128, 129, 255, 600]
+
+
+@pytest.mark.parametrize("fmt", ["i8", "e4m3"])
+@pytest.mark.parametrize("page", [8, 16, 32, 64])
+def test_decode_lengths(nv, page, fmt):
+    run_and_check(nv, Cache(LENGTHS, [1] * len(LENGTHS), 14, 2, page, fmt, "f32", seed=page, uniform=page != 16, packed=page == 32))
+
+
+@pytest.mark.parametrize("heads,kv_heads", [(1, 1), (8, 1), (2, 2), (10, 2), (9, 3), (15, 3), (4, 4), (28, 4), (32, 4), (12, 6), (40, 8), (20, 5), (32, 32), (16, 1), (64, 1), (36, 2)])
+@pytest.mark.parametrize("io", ["f16", "bf16", "f32"])
+def test_decode_heads(nv, heads, kv_heads, io):
+    run_and_check(nv, Cache([200, 0, 33], [1, 1, 1], heads, kv_heads, 16, "i8" if heads % 3 else "e4m3", io, seed=heads, rope=["neox", "pairs", "none"][heads % 3]))
+
+
+@pytest.mark.parametrize("window", [1, 2, 15, 16, 17, 100, 10 ** 9])
+def test_decode_window(nv, window):
+    run_and_check(nv, Cache(LENGTHS, [1] * len(LENGTHS), 14, 2, 16, "e4m3", "f32", window=window, seed=3))
+    run_and_check(nv, Cache([0, 5, 40, 300], [1] * 4, 8, 4, 8, "i8", "bf16", window=window, seed=4))
+
+
+def test_decode_sessions_without_a_token(nv):
+    run_and_check(nv, Cache([40, 0, 17, 99, 5], [1, 0, 1, 0, 1], 8, 4, 16, "i8", "f32"))
+    run_and_check(nv, Cache([40, 9, 17], [0, 1, 0], 7, 1, 8, "e4m3", "f16"))
+
+
+def test_decode_many_sessions(nv):
+    g = torch.Generator().manual_seed(5)
+    past = torch.randint(0, 90, (700,), generator=g).tolist()
+    run_and_check(nv, Cache(past, [1] * 700, 4, 2, 16, "i8", "bf16", layers=1, layer=0))
+    run_and_check(nv, Cache(past[:300], [1] * 300, 8, 8, 8, "e4m3", "f16", layers=1, layer=0))
+
+
+def test_decode_long_context(nv):
+    """One session over many CTAs, the merge of their partial rows included; the same position far behind the first pages."""
+    run_and_check(nv, Cache([20011], [1], 14, 2, 16, "i8", "f32", layers=1, layer=0, poison=False))
+    run_and_check(nv, Cache([9000, 3, 5000], [1] * 3, 4, 4, 64, "e4m3", "f32", layers=1, layer=0, poison=False, window=4321))
+
+
+def test_decode_scales_far_apart(nv):
+    """Scales of neighbouring keys that differ by many orders of magnitude, and sharp score distributions."""
+    run_and_check(nv, Cache([500, 100], [1, 1], 8, 2, 16, "i8", "f32", scale_spread=4.0, seed=1))
+    run_and_check(nv, Cache([500, 100], [1, 1], 8, 2, 16, "e4m3", "f16", scale_spread=1.0, q_gain=8.0, seed=2))
+
+
+CHUNKS = [([0], [1]), ([0, 0, 7], [2, 17, 40]), ([70, 5, 0, 200], [0, 3, 1, 65]), ([300], [129]), ([15, 16, 17, 31], [1, 16, 15, 2])]
+
+
+@pytest.mark.parametrize("fmt", ["i8", "e4m3"])
+@pytest.mark.parametrize("page", [8, 16, 32, 64])
+@pytest.mark.parametrize("io", ["f16", "bf16", "f32"])
+def test_chunk(nv, io, page, fmt):
+    for i, (past, new) in enumerate(CHUNKS):
+        run_and_check(nv, Cache(past, new, 14, 2, page, fmt, io, seed=i, packed=i % 2 == 1, rope=["neox", "pairs", "none"][i % 3]))
+
+
+@pytest.mark.parametrize("heads,kv_heads", [(1, 1), (8, 8), (3, 1), (9, 3), (28, 4), (40, 8), (16, 1), (100, 1), (128, 1), (256, 2)])
+def test_chunk_heads(nv, heads, kv_heads):
+    run_and_check(nv, Cache([100, 0, 31], [9, 40, 2], heads, kv_heads, 16, "i8", "bf16", seed=heads))
+
+
+@pytest.mark.parametrize("window", [1, 2, 16, 63, 64, 65, 200])
+def test_chunk_window(nv, window):
+    run_and_check(nv, Cache([0, 90, 300], [70, 33, 5], 6, 2, 16, "i8", "f16", window=window))
+    run_and_check(nv, Cache([0, 90, 300], [70, 33, 5], 6, 2, 64, "e4m3", "bf16", window=window))
+
+
+def test_chunk_long(nv):
+    run_and_check(nv, Cache([1500, 40], [300, 700], 7, 1, 16, "i8", "bf16", layers=1, layer=0, poison=False))
+    run_and_check(nv, Cache([6000, 2500, 900], [5, 1, 8], 14, 2, 32, "e4m3", "f16", layers=1, layer=0, poison=False))
+    run_and_check(nv, Cache([300, 20], [12, 9], 8, 2, 16, "i8", "f16", scale_spread=3.0))
+
+
+def test_attention_of_written_keys(nv):
+    """The attention alone, on keys that an earlier call has written."""
+    run_and_check(nv, Cache([70, 5], [1, 1], 14, 2, 16, "i8", "f32"), what="attn")
+    run_and_check(nv, Cache([70, 5], [6, 21], 14, 2, 8, "e4m3", "bf16"), what="attn")
+
+
+def test_a_conversation(nv):
+    """The operators as they are used together: a prompt in two chunks, then single tokens, then drafted tokens, then everything
+    read back; every step against the plain form."""
+    pieces = [[30, 11], [19, 40], [1, 1], [1, 1], [4, 0], [1, 1]]
+    total = [sum(p[s] for p in pieces) for s in (0, 1)]
+    last = None
+    for io in ("bf16",):
+        past = [0, 0]
+        for i, new in enumerate(pieces):
+            case = Cache(past, new, 14, 2, 16, "i8", io, seed=10 + i, poison=last is None)
+            case.nb = sum((t + 15) // 16 for t in total) + 2
+            case.tables = torch.full((2, 9), -1, dtype=torch.int32)
+            case.slices = torch.tensor([1, 0], dtype=torch.int32)
+            case.tables[1, :7] = torch.arange(0, 7, dtype=torch.int32)
+            case.tables[0, :7] = torch.arange(7, 14, dtype=torch.int32)
+            case.nb = 14
+            case.codes = [torch.full((2, 14, 16, 2, HD), 0x7f, dtype=torch.uint8) for _ in range(2)] if last is None else last.codes
+            case.scales = [torch.full((2, 14, 2, 16), math.nan) for _ in range(2)] if last is None else last.scales
+            run_and_check(nv, case)
+            last, past = case, [p + n for p, n in zip(past, new)]
+        end = Cache([0, 0], total, 14, 2, 16, "i8", io)
+        for name in ("nb", "tables", "slices", "codes", "scales"):
+            setattr(end, name, getattr(last, name))
+        d = end.device(nv)
+        call(nv, d, "read")
+        torch.cuda.synchronize()
+        for got, want in zip(d["back"], end.read()):
+            assert same_bits(got, want)
+
+
+def test_bad_table_entries_are_skipped_and_flagged(nv):
+    """A table entry outside the pool: nothing is written or read there, the status says so, other sessions are not touched."""
+    for entry in (-1, 10 ** 6):
+        for new in ([1, 1], [5, 9]):
+            case = Cache([40, 60], new, 4, 2, 16, "i8", "f32" if new[0] == 1 else "bf16", poison=False)
+            good = Cache([40, 60], new, 4, 2, 16, "i8", case.io, poison=False)
+            good.append()
+            o, a, spread = good.attend()
+            case.tables[int(case.slices[0]), 1] = entry
+            d = case.device(nv)
+            call(nv, d, "append_attn")
+            torch.cuda.synchronize()
+            assert int(d["status"]) == nv.ERR_BAD_TABLE
+            rows = slice(new[0], sum(new))
+            bound = attention_bound(case, o, a, spread, new[0] == 1)
+            assert bool(((d["out"].cpu().double() - o).abs() <= bound)[rows].all())
+            # the entry that takes the new row
+            case.tables = good.tables.clone()
+            case.tables[int(case.slices[0]), 40 // 16] = entry
+            d = case.device(nv)
+            call(nv, d, "append")
+            call(nv, d, "read")
+            torch.cuda.synchronize()
+            assert int(d["status"]) == nv.ERR_BAD_TABLE
+            assert bool((d["back"][0][0] == 7).all()) and bool((d["back"][1][0] == 7).all())
+
+
+def test_positions_beyond_the_rotary_tables(nv):
+    case = Cache([40, 60], [1, 1], 4, 2, 16, "i8", "f32", poison=False)
+    d = case.device(nv)
+    d["cache"].rope_rows = 50
+    call(nv, d, "append_attn")
+    torch.cuda.synchronize()
+    assert int(d["status"]) == nv.ERR_INVALID
+
+
+def test_row_starts_that_are_out_of_range(nv):
+    """tok_start is device data: whatever it holds, no row outside the buffers is touched."""
+    for new in ([1, 1, 1], [4, 5, 6]):
+        case = Cache([20, 30, 40], new, 4, 2, 16, "i8", "bf16", poison=False)
+        d = case.device(nv, extra_rows=1)
+        d["start"].copy_(torch.tensor([0, -50, 10 ** 9, 10 ** 9], dtype=torch.int32))
+        call(nv, d, "append_attn")
+        call(nv, d, "read")
+        d["start"].copy_(torch.tensor([7, 3, 2, 1], dtype=torch.int32))
+        call(nv, d, "append_attn")
+        torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("new", [[1, 1, 1], [3, 0, 20]])
+def test_graph_replay_and_streams(nv, new):
+    """Captured once, replayed on other inputs and positions, two graphs with a workspace each running at once."""
+    cases, ds, graphs = [], [], []
+    for i in range(2):
+        case = Cache([50, 10, 90], new, 14, 2, 16, "i8", "bf16", seed=i, poison=False)
+        d = case.device(nv)
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            call(nv, d, "append_attn")                      # first use outside of the capture
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=side):
+            call(nv, d, "append_attn")
+        cases.append(case)
+        ds.append(d)
+        graphs.append((g, side))
+    other = Cache([50, 10, 90], new, 14, 2, 16, "i8", "bf16", seed=7, poison=False)
+    for case, d in zip(cases, ds):
+        d["qkv"].zero_()
+        for x in "qkv":
+            d[x].copy_(getattr(other, x))
+            getattr(case, x).copy_(getattr(other, x))
+        d["out"].fill_(7)
+    torch.cuda.synchronize()
+    for _ in range(3):
+        for g, side in graphs:
+            with torch.cuda.stream(side):
+                g.replay()
+    torch.cuda.synchronize()
+    for case, d in zip(cases, ds):
+        case.append()
+        check_cache(case, d)
+        check_out(case, d)
+
+
+def test_same_call_twice_gives_the_same_bits(nv):
+    for new in ([1] * 5, [7, 1, 33, 0, 4]):
+        case = Cache([5000, 12, 999, 64, 1], new, 14, 2, 16, "e4m3", "f16", layers=1, layer=0, poison=False)
+        d = case.device(nv)
+        call(nv, d, "append_attn")
+        first = d["out"].clone()
+        d["work"].fill_(0xff)
+        call(nv, d, "append_attn")
+        torch.cuda.synchronize()
+        assert same_bits(d["out"], first.cpu())
