@@ -678,7 +678,7 @@ bool attn_mma_built() { return true; }
 int attn_default_ctas_mma() { return sm_count(); }
 size_t attn_tmap_bytes() { return sizeof(CUtensorMap); }
 
-// Tensor map over one fp16 pool [rows = L*NB*page tokens][NKV][128]: dim0 = 128 dims, dim1 = slot rows
+// Tensor map over one pool (fp16; fp32 and 8-bit codes: the same with 4 or 1 bytes an element) [rows = L*NB*page tokens][NKV][128]: dim0 = 128 dims, dim1 = slot rows
 // (stride NKV*256 B), dim2 = kv head (stride 256 B); box = [64][box_rows = 16 or 8][kv_group], 128-byte swizzle.
 int attn_make_tmap(void* out_map, void* pool, int64_t slot_rows, int n_kv_heads, int kv_group, int box_rows, int elem_bytes) {
     static EncodeTiledFn encode = nullptr;
@@ -693,12 +693,12 @@ int attn_make_tmap(void* out_map, void* pool, int64_t slot_rows, int n_kv_heads,
         encode = (EncodeTiledFn)fn;
     }
     if (slot_rows <= 0 || slot_rows > 0x7fffffffLL) return NOVA_ERR_TOO_LARGE;
-    if ((box_rows != 8 && box_rows != 16) || (elem_bytes != 2 && elem_bytes != 4)) return NOVA_ERR_INVALID;
+    if ((box_rows != 8 && box_rows != 16) || (elem_bytes != 1 && elem_bytes != 2 && elem_bytes != 4)) return NOVA_ERR_INVALID;
     const cuuint64_t dims[3] = {(cuuint64_t)kHeadDim, (cuuint64_t)slot_rows, (cuuint64_t)n_kv_heads};
     const cuuint64_t strides[2] = {(cuuint64_t)n_kv_heads * kHeadDim * (cuuint64_t)elem_bytes, (cuuint64_t)kHeadDim * (cuuint64_t)elem_bytes};
     const cuuint32_t box[3] = {(cuuint32_t)(128 / elem_bytes), (cuuint32_t)box_rows, (cuuint32_t)kv_group};      // 128-byte lines
     const cuuint32_t estr[3] = {1, 1, 1};
-    const CUresult r = encode(static_cast<CUtensorMap*>(out_map), elem_bytes == 2 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32,
+    const CUresult r = encode(static_cast<CUtensorMap*>(out_map), elem_bytes == 1 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : elem_bytes == 2 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32,
                               3, pool, dims, strides,
                               box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
                               CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);

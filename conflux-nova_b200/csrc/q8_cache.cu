@@ -11,31 +11,6 @@
 namespace novab {
 namespace {
 
-__device__ __forceinline__ float warp_amax(float4 x) {
-    float m = fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w)));
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-    return m;
-}
-
-// Rotates the row whose values 4i .. 4i + 3 lane i holds.  All 32 lanes.
-__device__ __forceinline__ float4 q8_rotate(float4 x, int64_t pos, int lane, const Q8Launch& a) {
-    if (a.neox) {               // pairs (d, d + 64): the partner sits 16 lanes away
-        const float4 y = make_float4(__shfl_xor_sync(0xffffffffu, x.x, 16), __shfl_xor_sync(0xffffffffu, x.y, 16),
-                                     __shfl_xor_sync(0xffffffffu, x.z, 16), __shfl_xor_sync(0xffffffffu, x.w, 16));
-        const int i = 4 * (lane & 15);
-        const float4 c = *reinterpret_cast<const float4*>(a.rope_cs + pos * 64 + i), s = *reinterpret_cast<const float4*>(a.rope_sn + pos * 64 + i);
-        if (lane < 16)
-            return make_float4(__fmaf_rn(x.x, c.x, -__fmul_rn(y.x, s.x)), __fmaf_rn(x.y, c.y, -__fmul_rn(y.y, s.y)),
-                               __fmaf_rn(x.z, c.z, -__fmul_rn(y.z, s.z)), __fmaf_rn(x.w, c.w, -__fmul_rn(y.w, s.w)));
-        return make_float4(__fmaf_rn(y.x, s.x, __fmul_rn(x.x, c.x)), __fmaf_rn(y.y, s.y, __fmul_rn(x.y, c.y)),
-                           __fmaf_rn(y.z, s.z, __fmul_rn(x.z, c.z)), __fmaf_rn(y.w, s.w, __fmul_rn(x.w, c.w)));
-    }
-    const float2 c = *reinterpret_cast<const float2*>(a.rope_cs + pos * 64 + 2 * lane), s = *reinterpret_cast<const float2*>(a.rope_sn + pos * 64 + 2 * lane);
-    return make_float4(__fmaf_rn(x.x, c.x, -__fmul_rn(x.y, s.x)), __fmaf_rn(x.x, s.x, __fmul_rn(x.y, c.x)),
-                       __fmaf_rn(x.z, c.y, -__fmul_rn(x.w, s.y)), __fmaf_rn(x.z, s.y, __fmul_rn(x.w, c.y)));
-}
-
 // One warp per (row, head): heads [0, NKV) are K, [NKV, 2 NKV) V, and, when q is rotated in place too, the rest q.
 template <int kFmt>
 __global__ void __launch_bounds__(256) q8_append_kernel(Q8Launch a) {
@@ -72,7 +47,7 @@ __global__ void __launch_bounds__(256) q8_append_kernel(Q8Launch a) {
         if (lane == 0) q8_flag(a, NOVA_ERR_BAD_TABLE);
         return;
     }
-    const float amax = fmaxf(warp_amax(x), kQ8MinAmax);
+    const float amax = fmaxf(q8_amax(x), kQ8MinAmax);
     const float inv = __fdiv_rn(q8_qmax<kFmt>(), amax);
     const uint32_t w = q8_encode4<kFmt>(make_float4(__fmul_rn(x.x, inv), __fmul_rn(x.y, inv), __fmul_rn(x.z, inv), __fmul_rn(x.w, inv)));
     const int64_t page = (int64_t)a.layer * a.nb + phys;
@@ -215,8 +190,7 @@ static int q8_attn(const nova_q8_cache* c, const nova_q8_rows* r, const void* q,
     if (append) {
         if (!k || !v || misaligned(k) || misaligned(v)) return NOVA_ERR_INVALID;
         a.k = k; a.v = v;
-        rc = launch_q8_append(a, (cudaStream_t)s);
-        if (rc != NOVA_OK) return rc;
+        a.append = 1;
     }
     return launch_q8_attn(a, work_bytes, (cudaStream_t)s);
 }

@@ -161,6 +161,32 @@ template <int kFmt> __device__ __forceinline__ uint32_t q8_encode4(float4 x) {
 }
 template <int kFmt> __device__ __forceinline__ constexpr float q8_qmax() { return kFmt == NOVA_KV_I8 ? 127.f : 448.f; }
 
+// ---- one row over a warp: lane i holds the values 4i .. 4i + 3
+__device__ __forceinline__ float q8_amax(float4 x) {
+    float m = fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w)));
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    return m;
+}
+
+// Rotates it for position pos, in the fused form of the append kernel (rope_append.cu).  All 32 lanes.
+__device__ __forceinline__ float4 q8_rotate(float4 x, int64_t pos, int lane, const Q8Launch& a) {
+    if (a.neox) {               // pairs (d, d + 64): the partner sits 16 lanes away
+        const float4 y = make_float4(__shfl_xor_sync(0xffffffffu, x.x, 16), __shfl_xor_sync(0xffffffffu, x.y, 16),
+                                     __shfl_xor_sync(0xffffffffu, x.z, 16), __shfl_xor_sync(0xffffffffu, x.w, 16));
+        const int i = 4 * (lane & 15);
+        const float4 c = *reinterpret_cast<const float4*>(a.rope_cs + pos * 64 + i), s = *reinterpret_cast<const float4*>(a.rope_sn + pos * 64 + i);
+        if (lane < 16)
+            return make_float4(__fmaf_rn(x.x, c.x, -__fmul_rn(y.x, s.x)), __fmaf_rn(x.y, c.y, -__fmul_rn(y.y, s.y)),
+                               __fmaf_rn(x.z, c.z, -__fmul_rn(y.z, s.z)), __fmaf_rn(x.w, c.w, -__fmul_rn(y.w, s.w)));
+        return make_float4(__fmaf_rn(y.x, s.x, __fmul_rn(x.x, c.x)), __fmaf_rn(y.y, s.y, __fmul_rn(x.y, c.y)),
+                           __fmaf_rn(y.z, s.z, __fmul_rn(x.z, c.z)), __fmaf_rn(y.w, s.w, __fmul_rn(x.w, c.w)));
+    }
+    const float2 c = *reinterpret_cast<const float2*>(a.rope_cs + pos * 64 + 2 * lane), s = *reinterpret_cast<const float2*>(a.rope_sn + pos * 64 + 2 * lane);
+    return make_float4(__fmaf_rn(x.x, c.x, -__fmul_rn(x.y, s.x)), __fmaf_rn(x.x, s.x, __fmul_rn(x.y, c.x)),
+                       __fmaf_rn(x.z, c.y, -__fmul_rn(x.w, s.y)), __fmaf_rn(x.z, s.y, __fmul_rn(x.w, c.y)));
+}
+
 #endif  // __CUDACC__
 
 // q8_cache.cu / q8_attn.cu
