@@ -6,17 +6,22 @@
 //
 //   * One persistent CTA per SM; the 16-key tiles of all (session, kv group) rows form one line that is dealt out evenly
 //     (attn_plan.cuh); rows that several CTAs worked on are merged by the kernel behind it.
-//   * A producer warp brings the tiles in with TMA: boxes [128 B][16 slots][kv group] of codes, 128-byte swizzle (a row of codes
-//     is one swizzle line), and the tile's scales with plain bulk copies.
-//   * Eight consumer warps: 8 / KVG of them per kv head, each with its own running maximum, sums and accumulators over every
-//     (8 / KVG)-th tile; merged once per row.  Codes become fp16 in registers (exactly: both formats fit fp16's mantissa)
-//     and go to mma.sync m16n8k16.  A lane reads 32 consecutive codes of a key: the contraction index of S = Q.K^T may be permuted
-//     freely as long as q's fragments follow, so no transposition is needed; for P.V the columns are permuted the same
-//     way (column n of product j is dim 16 n + j) and pairs of keys are interleaved with byte permutes.
-//   * The at most 8 query heads of a kv head fill half of the 16 rows.  The other half holds the low parts: q = hi + lo and
-//     p = hi + lo in fp16, both halves in one instruction, so scores and outputs keep fp32-level accuracy at no cost.
-//   * The scale of K multiplies the finished score.  The scale of V goes into the exponent: w_j = 2^(x_j + log2 sv_j - m), so
-//     the weights that multiply the codes never leave fp16's range whatever the scales are; the softmax sum adds w_j / sv_j.
+//   * Four producer warps.  Two bring in the codes of K and V with TMA: boxes [128 B][16 slots][kv group], 128-byte swizzle (a row
+//     of codes is one swizzle line).  Two load the scales, four keys of a head per lane, and leave what the consumers need
+//     of them in shared memory.
+//   * Twelve consumer warps: 12 / KVG of them per kv head, each with its own reference maxima, sums and accumulators over
+//     every (12 / KVG)-th tile; merged once per row.  Codes become fp16 in registers, exactly, and go to mma.sync m16n8k16 as the
+//     16-row operand: S^T = K.Q^T (16 keys x 8 query heads) and O^T += V^T.P^T (16 dims x 8 heads), so that none of the
+//     instruction's rows is padding but for the heads beyond G.  A lane reads 32 consecutive codes of a key: the
+//     contraction index may be permuted freely as long as q's fragments follow.  V needs pairs of keys side by side: bytes are
+//     interleaved with permutes, and the rows of product j are the dims 16 g + 2 j (+ 1).  P goes from the accumulator layout to
+//     the operand layout with movmatrix.
+//   * int8 K: the byte code + 128 is taken as an fp16 subnormal, (code + 128) 2^-24, which costs no arithmetic; the accumulators start
+//     at -128 2^-24 sum(q).  (Not for V: there the offset would be a sum of weights, hundreds of times the result.)
+//   * fp32 activations: q and p as fp16 hi + lo, two instructions each, so scores and outputs keep fp32-level accuracy.  16-bit
+//     activations: q (rotated) and p rounded to fp16.
+//   * The scale of K multiplies the finished score.  The scale of V goes into the exponent: w_j = 2^(x_j + log2 sv_j - ref), so
+//     the weights that multiply the codes stay inside fp16's range whatever the scales are; the softmax sum adds w_j / sv_j.
 #include "attn_plan.cuh"
 #include "mma_common.cuh"
 #include "q8_common.cuh"
@@ -35,7 +40,7 @@ __device__ __forceinline__ float rcp(float x) {
     return y;
 }
 
-// Two codes (the low 16 bits of lo16: first code in the low byte) ... four codes of a word -> two pairs of fp16, exactly.
+// Four codes of a word -> two pairs of fp16, exactly.
 template <int kFmt> __device__ __forceinline__ void q8_to_h2(uint32_t w, uint32_t& h0, uint32_t& h1) {
     if constexpr (kFmt == NOVA_KV_I8) {
         // 0x6400 | (code + 128) is the fp16 number 1024 + 128 + code
@@ -50,33 +55,57 @@ template <int kFmt> __device__ __forceinline__ void q8_to_h2(uint32_t w, uint32_
     }
 }
 
+// The same for K: int8 codes as (code + 128) 2^-24, an fp16 subnormal whose bits are the byte.
+template <int kFmt> __device__ __forceinline__ void q8_k_to_h2(uint32_t w, uint32_t& h0, uint32_t& h1) {
+    if constexpr (kFmt == NOVA_KV_I8) {
+        const uint32_t u = w ^ 0x80808080u;
+        h0 = __byte_perm(u, 0u, 0x4140);
+        h1 = __byte_perm(u, 0u, 0x4342);
+    } else {
+        q8_to_h2<kFmt>(w, h0, h1);
+    }
+}
+
 __device__ __forceinline__ uint4 lds128(uint32_t addr) {
     uint4 v;
     asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr));
     return v;
 }
-__device__ __forceinline__ float2 lds_f2(uint32_t addr) {
-    float2 v;
-    asm volatile("ld.shared.v2.f32 {%0,%1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(addr));
+__device__ __forceinline__ float lds_f1(uint32_t addr) {
+    float v;
+    asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(addr));
     return v;
 }
-__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
-    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
+__device__ __forceinline__ void sts_f1(uint32_t addr, float v) { asm volatile("st.shared.f32 [%0], %1;" ::"r"(addr), "f"(v) : "memory"); }
+__device__ __forceinline__ void sts128(uint32_t addr, float4 v) {
+    asm volatile("st.shared.v4.f32 [%0], {%1,%2,%3,%4};" ::"r"(addr), "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w) : "memory");
 }
-
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+// Transpose of an 8 x 8 matrix of 16-bit values over the warp (lane 4 r + c holds row r, columns 2c and 2c + 1).
+__device__ __forceinline__ uint32_t movmatrix(uint32_t x) {
+    uint32_t y;
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
+}
 constexpr int kSetupTiles = 2;       // work-split weight of starting a row inside a CTA, in tiles
 constexpr int kMinTiles = 4;         // a CTA gets at least that many tiles (fewer partial rows to merge for short contexts)
 
 template <int KVG>
 struct DecCfg {
-    static constexpr int kSub = 8 / KVG;                    // consumer warps per kv head
-    static constexpr int kStages = 32 / KVG;                // 128 KiB of tiles in flight
+    static constexpr int kCons = 12;                        // consumer warps; with four producers 16, which leave 128 registers a thread
+    static constexpr int kSub = kCons / KVG;                // ... per kv head
+    static constexpr int kStages = 36 / KVG;                // 144 KiB of tiles in flight; a stage always goes to the same warps
     static constexpr int kHalf = KVG * 2048;                // K (or V) codes of a tile
     static constexpr int kTile = 2 * kHalf;
-    static constexpr int kScales = KVG * 128;               // K scales | V scales
-    static constexpr int kMergeFloats = KVG * (kSub - 1) * 34 * 32;
-    static constexpr int kSmem = kStages * (kTile + kScales) + kMergeFloats * 4 + 1024;
-    static constexpr int kThreads = 288;
+    static constexpr int kScales = KVG * 192;               // K scales | logarithms of V's | reciprocals of V's
+    static constexpr int kMergeFloats = KVG * (kSub - 1) * 36 * 32;
+    static constexpr int kRawSteps = 8;                     // rings of raw scales (K, V), steps of 512 bytes
+    static constexpr int kSmem = kStages * (kTile + kScales) + 2 * kRawSteps * 512 + kMergeFloats * 4 + 1024;
+    static constexpr int kThreads = 32 * (kCons + 4);
+    static constexpr int kBatch = 8 / KVG;                  // tiles that a producer of codes issues at a time
+    static_assert(kStages % kSub == 0, "stages and consumer warps");
 };
 
 // Keys, first tile and tile count of every (session, group) row; a row without a new token has no tiles.
@@ -142,7 +171,8 @@ __device__ __forceinline__ PlanView dec_view(const Q8Launch& a, const DecPlan& p
     return pv;
 }
 
-template <int KVG, int kFmt>
+// kLo: q and p in two fp16 parts (fp32 activations)
+template <int KVG, int kFmt, bool kLo>
 __global__ void __launch_bounds__(DecCfg<KVG>::kThreads, 1)
 q8_decode_kernel(Q8Launch a, const __grid_constant__ CUtensorMap tmk, const __grid_constant__ CUtensorMap tmv) {
     using Cfg = DecCfg<KVG>;
@@ -160,15 +190,16 @@ q8_decode_kernel(Q8Launch a, const __grid_constant__ CUtensorMap tmk, const __gr
     const int heads_per_row = KVG * G;
     const uint32_t tile0 = (smem_u32(smem_raw) + 1023u) & ~1023u;
     const uint32_t scale0 = tile0 + kStages * Cfg::kTile;
-    float* const merge = reinterpret_cast<float*>(smem_raw + (scale0 - smem_u32(smem_raw)) + kStages * Cfg::kScales);
+    float* const merge = reinterpret_cast<float*>(smem_raw + (scale0 - smem_u32(smem_raw)) + kStages * Cfg::kScales + 2 * Cfg::kRawSteps * 512);
+    // the operands are q / 8 (rotated fp16 values stay inside fp16) and codes, those of int8 K times 2^-24
+    constexpr float kToLog2 = kAttnScale * kLog2e * 8.f * (kFmt == NOVA_KV_I8 ? 16777216.f : 1.f);
     // a page of 8 tokens is half a tile: two boxes of 8 slots, [half][kv head][8]; otherwise [kv head][16]
     const bool p8 = a.kv_shift == 3;
     const uint32_t head_step = p8 ? 1024u : 2048u, half_step = p8 ? KVG * 1024u : 1024u;
-    const uint32_t sc_head = p8 ? 32u : 64u, sc_half = p8 ? KVG * 32u : 32u;
 
-    if (threadIdx.x == 256) {
+    if (threadIdx.x == 32 * Cfg::kCons) {
         for (int i = 0; i < kStages; ++i) {
-            mbar_init(smem_u32(&s_full[i]), 1);
+            mbar_init(smem_u32(&s_full[i]), 4);        // codes and scales of K and V
             mbar_init(smem_u32(&s_empty[i]), KVG);
         }
         s_abort = 0;
@@ -185,97 +216,176 @@ q8_decode_kernel(Q8Launch a, const __grid_constant__ CUtensorMap tmk, const __gr
     if (pv.pages_total == 0 || (int)blockIdx.x >= pv.n_ctas) return;
     const int64_t lo = plan_cta_begin(pv, (int)blockIdx.x), hi = plan_cta_begin(pv, (int)blockIdx.x + 1);
 
-    // ------------------------------------------------------------------------------------------------ producer
-    if (warp == 8) {
+    // ------------------------------------------------------------------------------------------------ producers
+    // Each of the four goes through ALL tiles in order: a stage's fill waits for the release of the fill before, which the same
+    // warp has taken part in, so a parity is never taken for the one two fills ago.
+    const int tpp = a.kv_shift > 4 ? a.kv_shift - 4 : 0;               // log2(tiles per page)
+    // entries of the block table behind tile i of a segment (the second: 8-token pages); -1: a bad one, -2: nothing to bring
+    auto fetch = [&](const int32_t* table, int keys, int t, bool real, int& e0, int& e1) {
+        auto entry = [&](int64_t page, int first_key) -> int {
+            if (first_key >= keys) return -2;
+            if (page >= a.table_stride) return -1;
+            const int e = __ldg(table + page);
+            return e >= 0 && e < a.nb ? e : -1;
+        };
+        e0 = e1 = -2;
+        if (!real) return;
+        if (p8) {
+            e0 = entry(2 * (int64_t)t, 16 * t);
+            e1 = entry(2 * (int64_t)t + 1, 16 * t + 8);
+        } else {
+            e0 = entry(t >> tpp, 16 * t);
+        }
+    };
+    if (warp < Cfg::kCons + 2 && warp >= Cfg::kCons) {
+        // Codes of K and of V, a batch of tiles at a time, one lane per tile: what a copy costs its thread (wait, byte count,
+        // issue: several hundred cycles) is then paid once per batch.  A batch waits for all its stages, so it is a small part of the
+        // ring: the rest stays in flight meanwhile.
+        const bool is_v = warp == Cfg::kCons + 1;
         const unsigned long long policy = l2_policy_evict_first();
-        // what this lane copies of every tile: K or V codes (one box, or one per page of 8), K or V scales (one run of the kv
-        // group per page of 8 or 16, one run per head in longer pages)
-        const int n_box = p8 ? 2 : 1, n_sc = p8 ? 2 : (a.kv_shift == 4 ? 1 : KVG), jobs = 2 * (n_box + n_sc);
-        const bool is_box = lane < 2 * n_box;
-        const int j = is_box ? lane : lane - 2 * n_box;
-        const bool is_v = j >= (is_box ? n_box : n_sc);
-        const int part = is_v ? j - (is_box ? n_box : n_sc) : j;           // page of the tile, or head
-        const uint32_t sc_bytes = (uint32_t)(p8 ? KVG * 32 : (a.kv_shift == 4 ? KVG * 64 : 64));
-        const uint32_t my_off = is_box ? (uint32_t)(is_v ? Cfg::kHalf : 0) + (p8 ? part * half_step : 0u)
-                                       : (uint32_t)(is_v ? KVG * 64 : 0) + part * sc_bytes;
-        const float* const my_scale = is_v ? a.scale_v : a.scale_k;
-        const int tpp = a.kv_shift > 4 ? a.kv_shift - 4 : 0;               // log2(tiles per page)
-        uint32_t it = 0;
+        const CUtensorMap* const tm = is_v ? &tmv : &tmk;
+        const int row0 = (a.layer * a.nb) << a.kv_shift;
+        uint32_t it0 = 0;                                                   // tiles before this segment
         for (int64_t pos = lo; pos < hi;) {
             const Segment sg = plan_segment(pv, pos, hi, kSetupTiles);
             pos += sg.span;
             const int keys = s_plan.keys[sg.session];
             const int t0 = dec_first_tile(a, keys) + sg.page_first, low = a.window > 0 && keys > a.window ? keys - a.window : 0;
             const int32_t* table = a.tables + (int64_t)s_plan.slice[sg.session] * a.table_stride;
-            auto entry = [&](int64_t page, int first_key) -> int {        // block-table entry of a page that starts at first_key
-                if (first_key >= keys) return -2;                           // behind the last key: nothing to bring
-                if (page >= a.table_stride) return -1;
-                const int e = __ldg(table + page);
-                return e >= 0 && e < a.nb ? e : -1;
-            };
-            auto fetch = [&](int t, int& e0, int& e1) {
-                e0 = e1 = -2;
-                if (t < t0 + sg.page_count) {
-                    if (p8) {
-                        e0 = entry(2 * (int64_t)t, 16 * t);
-                        e1 = entry(2 * (int64_t)t + 1, 16 * t + 8);
-                    } else {
-                        e0 = entry(t >> tpp, 16 * t);
-                    }
+            int n0, n1, c0 = 0, c1 = 0;
+            fetch(table, keys, t0 + lane, lane < sg.page_count, n0, n1);
+            uint32_t stage = (it0 + (uint32_t)lane) % kStages, round = (it0 + (uint32_t)lane) / kStages;
+#pragma unroll 1
+            for (int b = 0; b < sg.page_count; b += Cfg::kBatch) {
+                if ((b & 31) == 0) {                                        // 32 entries at a time, the next 32 on their way
+                    c0 = n0;
+                    c1 = n1;
+                    const int nx = b + 32 + lane;
+                    fetch(table, keys, t0 + nx, nx < sg.page_count, n0, n1);
                 }
-            };
-            int n0, n1;
-            fetch(t0 + lane, n0, n1);
-            for (int b = 0; b < sg.page_count; b += 32) {
-                const int c0 = n0, c1 = n1;
-                fetch(t0 + b + 32 + lane, n0, n1);
-                const int n = sg.page_count - b < 32 ? sg.page_count - b : 32;
-                for (int i = 0; i < n; ++i, ++it) {
-                    const int e0 = __shfl_sync(0xffffffffu, c0, i), e1 = __shfl_sync(0xffffffffu, c1, i);
-                    const int t = t0 + b + i, stage = (int)(it % kStages);
-                    const uint32_t round = it / kStages;
-                    if (round > 0 && !__all_sync(0xffffffffu, mbar_wait(smem_u32(&s_empty[stage]), (round - 1) & 1, &s_abort))) {
-                        if (lane == 0) q8_flag(a, NOVA_ERR_TIMEOUT);
-                        return;
-                    }
+                const int i = b + lane, t = t0 + i;
+                const int e0 = __shfl_sync(0xffffffffu, c0, i & 31);
+                int e1 = -2;
+                if (p8) e1 = __shfl_sync(0xffffffffu, c1, i & 31);
+                const bool mine = lane < Cfg::kBatch && i < sg.page_count;
+                const bool free = !mine || round == 0 || mbar_wait(smem_u32(&s_empty[stage]), (round - 1) & 1, &s_abort);
+                if (!__all_sync(0xffffffffu, free)) {
+                    if (lane == 0) q8_flag(a, NOVA_ERR_TIMEOUT);
+                    return;
+                }
+                if (mine) {
                     const uint32_t bar = smem_u32(&s_full[stage]);
-                    if (lane == 0) {
+                    const uint32_t dst = tile0 + stage * Cfg::kTile + (is_v ? (uint32_t)Cfg::kHalf : 0u);
+                    const int slot = p8 ? 0 : (t << 4) & ((1 << a.kv_shift) - 1);
+                    const uint32_t halves = (uint32_t)(p8 ? (e0 >= 0) + (e1 >= 0) : 2 * (e0 >= 0));
+                    if (!is_v) {
                         if (e0 == -1 || e1 == -1) q8_flag(a, NOVA_ERR_BAD_TABLE);
                         uint32_t mask = p8 ? (e0 >= 0 ? 0xffu : 0u) | (e1 >= 0 ? 0xff00u : 0u) : (e0 >= 0 ? 0xffffu : 0u);
                         if (keys - 16 * t < 16) mask &= (1u << (keys - 16 * t)) - 1u;
                         if (low > 16 * t) mask &= ~((1u << (low - 16 * t < 16 ? low - 16 * t : 16)) - 1u);
                         s_mask[stage] = mask;
                         s_phys[stage] = p8 && e1 >= 0 ? e1 : e0;
-                        const uint32_t bytes = (uint32_t)(p8 ? ((e0 >= 0) + (e1 >= 0)) * (Cfg::kTile + Cfg::kScales) / 2 : (e0 >= 0 ? Cfg::kTile + Cfg::kScales : 0));
-                        if (bytes) mbar_expect_tx(bar, bytes);
-                        else mbar_arrive(bar);
                     }
-                    __syncwarp();
-                    if (lane < jobs) {
-                        const int e = p8 && part == 1 ? e1 : e0;
-                        if (e >= 0) {
-                            const int64_t page = (int64_t)a.layer * a.nb + e;
-                            const int slot = p8 ? 0 : (t << 4) & ((1 << a.kv_shift) - 1);
-                            if (is_box) {
-                                tma_load_3d_hint(tile0 + (uint32_t)stage * Cfg::kTile + my_off, is_v ? &tmv : &tmk, 0, (int)((page << a.kv_shift) + slot),
-                                                 sg.group * KVG, bar, policy);
-                            } else {
-                                const int h = sg.group * KVG + (a.kv_shift > 4 ? part : 0);
-                                bulk_load(scale0 + (uint32_t)stage * Cfg::kScales + my_off, my_scale + ((page * a.n_kv_heads + h) << a.kv_shift) + slot, sc_bytes, bar);
-                            }
-                        }
-                    }
+                    if (halves) mbar_expect_tx(bar, halves * (uint32_t)(Cfg::kHalf / 2));
+                    else mbar_arrive(bar);
+                    if (e0 >= 0) tma_load_3d_hint(dst, tm, 0, row0 + (e0 << a.kv_shift) + slot, sg.group * KVG, bar, policy);
+                    if (p8 && e1 >= 0) tma_load_3d_hint(dst + half_step, tm, 0, row0 + (e1 << a.kv_shift), sg.group * KVG, bar, policy);
+                }
+                __syncwarp();
+                stage += Cfg::kBatch;
+                if (stage >= kStages) {
+                    stage -= kStages;
+                    ++round;
                 }
             }
+            it0 += (uint32_t)sg.page_count;
         }
+        return;
+    }
+    if (warp >= Cfg::kCons + 2) {
+        // Scales of K and of V: a lane takes four keys of one head of a tile, 8 / KVG tiles at a time, and leaves what the consumers
+        // multiply with: K's scale times 1/sqrt(128) log2 e (and what the operands were scaled by), V's logarithm and reciprocal.
+        // The raw scales arrive (cp.async) in a ring of the warp's own, far enough ahead of their use: they are short runs all over
+        // the pools, about 2 us away when HBM is busy.
+        constexpr int kPer = 8 / KVG, kDepth = Cfg::kRawSteps - 1;           // tiles of a step (512 bytes of scales); steps ahead
+        const bool is_v = warp == Cfg::kCons + 3;
+        const int sub_tile = lane / (4 * KVG), quad = lane & 3, h = (lane >> 2) % KVG;
+        const uint32_t raw0 = scale0 + kStages * Cfg::kScales + (uint32_t)(is_v ? Cfg::kRawSteps * 512 : 0) + (uint32_t)lane * 16u;
+        const uint32_t dst0 = scale0 + (uint32_t)((is_v ? KVG * 64 : 0) + h * 64 + quad * 16);
+        const int slot_mask = p8 ? 0 : (1 << a.kv_shift) - 1, slot_add = p8 ? 4 * (quad & 1) : 4 * quad;
+        uint32_t it0 = 0;
+        for (int64_t pos = lo; pos < hi;) {
+            const Segment sg = plan_segment(pv, pos, hi, kSetupTiles);
+            pos += sg.span;
+            const int keys = s_plan.keys[sg.session], t0 = dec_first_tile(a, keys) + sg.page_first;
+            const int32_t* table = a.tables + (int64_t)s_plan.slice[sg.session] * a.table_stride;
+            const float* const mine0 = (is_v ? a.scale_v : a.scale_k) + ((((int64_t)a.layer * a.nb) * a.n_kv_heads + sg.group * KVG + h) << a.kv_shift);
+            const int steps = (sg.page_count + kPer - 1) / kPer;
+            int n0, n1, c0 = 0, c1 = 0;
+            fetch(table, keys, t0 + lane, lane < sg.page_count, n0, n1);
+            uint32_t stage = (it0 + (uint32_t)sub_tile) % kStages, round = (it0 + (uint32_t)sub_tile) / kStages;
+            int i = sub_tile - kDepth * kPer;                               // the tile that this step converts
+#pragma unroll 1
+            for (int step = 0; step < steps + kDepth; ++step, i += kPer) {
+                if (step < steps) {
+                    const int f = step * kPer;
+                    if ((f & 31) == 0) {                                    // 32 entries at a time, the next 32 on their way
+                        c0 = n0;
+                        c1 = n1;
+                        const int nx = f + 32 + lane;
+                        fetch(table, keys, t0 + nx, nx < sg.page_count, n0, n1);
+                    }
+                    int e = __shfl_sync(0xffffffffu, c0, (f + sub_tile) & 31);       // (below 0 behind the segment's last tile too)
+                    if (p8) {
+                        const int f1 = __shfl_sync(0xffffffffu, c1, (f + sub_tile) & 31);
+                        if (quad >= 2) e = f1;
+                    }
+                    const int slot = (((t0 + f + sub_tile) << 4) & slot_mask) + slot_add;
+                    const uint32_t raw = raw0 + (uint32_t)(step & (Cfg::kRawSteps - 1)) * 512u;
+                    if (e >= 0) cp_async16(raw, mine0 + (((int64_t)e * a.n_kv_heads) << a.kv_shift) + slot);
+                    else sts128(raw, make_float4(0.f, 0.f, 0.f, 0.f));
+                }
+                asm volatile("cp.async.commit_group;" ::: "memory");
+                if (step < kDepth) continue;
+                asm volatile("cp.async.wait_group %0;" ::"n"(kDepth) : "memory");
+                const bool mine = i < sg.page_count;                        // a lane converts what it has brought itself
+                const uint4 u = lds128(raw0 + (uint32_t)((step - kDepth) & (Cfg::kRawSteps - 1)) * 512u);
+                const float4 v = make_float4(__uint_as_float(u.x), __uint_as_float(u.y), __uint_as_float(u.z), __uint_as_float(u.w));
+                const bool free = !mine || round == 0 || mbar_wait(smem_u32(&s_empty[stage]), (round - 1) & 1, &s_abort);
+                if (!__all_sync(0xffffffffu, free)) {
+                    if (lane == 0) q8_flag(a, NOVA_ERR_TIMEOUT);
+                    break;
+                }
+                const uint32_t dst = dst0 + stage * Cfg::kScales;
+                if (mine) {
+                    if (!is_v) {
+                        sts128(dst, make_float4(v.x * kToLog2, v.y * kToLog2, v.z * kToLog2, v.w * kToLog2));
+                    } else {
+                        const float4 m = make_float4(fmaxf(v.x, kQ8MinScale), fmaxf(v.y, kQ8MinScale), fmaxf(v.z, kQ8MinScale), fmaxf(v.w, kQ8MinScale));
+                        sts128(dst, make_float4(lg2(m.x), lg2(m.y), lg2(m.z), lg2(m.w)));
+                        sts128(dst + KVG * 64, make_float4(rcp(m.x), rcp(m.y), rcp(m.z), rcp(m.w)));
+                    }
+                }
+                __syncwarp();
+                if (mine && lane % (4 * KVG) == 0) mbar_arrive(smem_u32(&s_full[stage]));
+                stage += kPer;
+                if (stage >= kStages) {
+                    stage -= kStages;
+                    ++round;
+                }
+            }
+            it0 += (uint32_t)sg.page_count;
+        }
+        asm volatile("cp.async.wait_all;" ::: "memory");
         return;
     }
 
     // ------------------------------------------------------------------------------------------------ consumers
     const int w = warp % KVG, sub = warp / KVG;       // kv head of the group, which of its warps
     const int g = lane >> 2, t = lane & 3;
-    constexpr float kToLog2 = kAttnScale * kLog2e * 8.f;      // q goes in divided by 8: rotated fp16 values stay inside fp16
-    uint32_t it = 0;
+    uint32_t it = 0;                                  // tiles of the segments before
+    int stage = sub;                                  // of this warp's next tile, and the parity of its fill
+    uint32_t parity = 0;
     for (int64_t pos = lo; pos < hi;) {
         const Segment sg = plan_segment(pv, pos, hi, kSetupTiles);
         pos += sg.span;
@@ -283,9 +393,11 @@ q8_decode_kernel(Q8Launch a, const __grid_constant__ CUtensorMap tmk, const __gr
         const int keys = s_plan.keys[s], row = s_plan.row[s], t0 = dec_first_tile(a, keys) + sg.page_first;
         const int head = kvh * G + (g < G ? g : 0);
 
-        // q fragments of head g: this lane's dims are 32 t .. 32 t + 31 (four per contraction step), rows 8-15 hold the low parts
-        uint32_t qh[8][2], ql[8][2];
+        // q fragments of head g: this lane's dims are 32 t .. 32 t + 31, four per contraction step
+        uint32_t qh[8][2], ql[kLo ? 8 : 1][2];
+        float off0 = 0.f, off1 = 0.f;             // what the accumulators of heads 2 t and 2 t + 1 start at
         {
+            float qsum = 0.f;
             const int64_t qe = (int64_t)row * a.q_stride + (int64_t)head * kHeadDim;
 #pragma unroll
             for (int ks = 0; ks < 8; ++ks) {
@@ -313,25 +425,33 @@ q8_decode_kernel(Q8Launch a, const __grid_constant__ CUtensorMap tmk, const __gr
                     const __half2 h = __floats2half2_rn(f[2 * e], f[2 * e + 1]);
                     const float2 b = __half22float2(h);
                     qh[ks][e] = g < G ? *reinterpret_cast<const uint32_t*>(&h) : 0u;
-                    ql[ks][e] = g < G ? pack_h2(f[2 * e] - b.x, f[2 * e + 1] - b.y) : 0u;
+                    qsum += kLo ? f[2 * e] + f[2 * e + 1] : b.x + b.y;
+                    if constexpr (kLo) ql[ks][e] = g < G ? pack_h2(f[2 * e] - b.x, f[2 * e + 1] - b.y) : 0u;
                 }
             }
+            if constexpr (kFmt == NOVA_KV_I8) {
+                qsum += __shfl_xor_sync(0xffffffffu, qsum, 1);
+                qsum += __shfl_xor_sync(0xffffffffu, qsum, 2);
+                if (g >= G) qsum = 0.f;
+                off0 = -7.62939453125e-06f * __shfl_sync(0xffffffffu, qsum, 8 * t);             // 128 * 2^-24
+                off1 = -7.62939453125e-06f * __shfl_sync(0xffffffffu, qsum, 8 * t + 4);
+            }
         }
-        float m = -INFINITY, l = 0.f;
-        float o[16][4];
+        // heads 2 t and 2 t + 1: reference maximum (log2 units), this lane's share of the sum, dims 16 g .. 16 g + 15
+        float ref0 = -INFINITY, ref1 = -INFINITY, l0 = 0.f, l1 = 0.f;
+        float o[8][4];
 #pragma unroll
-        for (int j = 0; j < 16; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
+        for (int j = 0; j < 8; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
 
         const uint32_t it_end = it + (uint32_t)sg.page_count;
         for (uint32_t i = it + (((uint32_t)sub + kSub - it % kSub) % kSub); i < it_end; i += kSub) {
-            const int stage = (int)(i % kStages);
-            if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(&s_full[stage]), (i / kStages) & 1, &s_abort))) {
+            if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(&s_full[stage]), parity, &s_abort))) {
                 if (lane == 0) q8_flag(a, NOVA_ERR_TIMEOUT);      // the result is void; the warp still meets its siblings below
                 break;
             }
             const uint32_t mask = s_mask[stage];
             const uint32_t sk = tile0 + (uint32_t)stage * Cfg::kTile + w * head_step, sv = sk + Cfg::kHalf;
-            const uint32_t ck = scale0 + (uint32_t)stage * Cfg::kScales + w * sc_head, cv = ck + KVG * 64;
+            const uint32_t ck = scale0 + (uint32_t)stage * Cfg::kScales + w * 64u;
             const int tile = t0 + (int)(i - it);
             bool patched = false;
             if (a.append && tile == (keys - 1) >> 4 && (mask >> ((keys - 1) & 15) & 1)) {
@@ -356,84 +476,92 @@ q8_decode_kernel(Q8Launch a, const __grid_constant__ CUtensorMap tmk, const __gr
                     asm volatile("st.shared.u32 [%0], %1;" ::"r"(dst), "r"(code) : "memory");
                     if (lane == 0) {
                         (i2 ? a.scale_v : a.scale_k)[((page * a.n_kv_heads + kvh) << a.kv_shift) + pslot] = scale;
-                        asm volatile("st.shared.f32 [%0], %1;" ::"r"((i2 ? cv : ck) + (slot >> 3) * sc_half + (slot & 7) * 4u), "f"(scale) : "memory");
+                        sts_f1(ck + (i2 ? KVG * 64u : 0u) + slot * 4u, i2 ? lg2(scale) : scale * kToLog2);
+                        if (i2) sts_f1(ck + KVG * 128u + slot * 4u, rcp(scale));
                     }
                 }
                 __syncwarp();
             }
             if (mask) {
-                // S = Q.K^T: lane (g, t) holds codes 32 t .. of keys g and g + 8 (two swizzled 16-byte pieces each)
-                float c[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+                // Everything of the tile into registers, so that the stage can be filled again while the rest is computed: codes 32 t ..
+                // of keys g and g + 8 (two swizzled 16-byte pieces each), codes 16 g .. of keys 2t, 2t + 1, 2t + 8, 2t + 9, scales.
+                uint4 kw[2][2], vw[4];
 #pragma unroll
                 for (int half = 0; half < 2; ++half) {
-                    uint4 kw[2];
-#pragma unroll
-                    for (int nt = 0; nt < 2; ++nt) kw[nt] = lds128(sk + nt * half_step + g * 128u + (((2 * t + half) ^ g) << 4));
-#pragma unroll
-                    for (int k4 = 0; k4 < 4; ++k4) {
-                        const int ks = 4 * half + k4;
-#pragma unroll
-                        for (int nt = 0; nt < 2; ++nt) {
-                            uint32_t b0, b1;
-                            q8_to_h2<kFmt>(k4 == 0 ? kw[nt].x : k4 == 1 ? kw[nt].y : k4 == 2 ? kw[nt].z : kw[nt].w, b0, b1);
-                            mma_full(c[nt], qh[ks][0], ql[ks][0], qh[ks][1], ql[ks][1], b0, b1);
-                        }
-                    }
+                    kw[half][0] = lds128(sk + g * 128u + (((2 * t + half) ^ g) << 4));
+                    kw[half][1] = lds128(sk + half_step + g * 128u + (((2 * t + half) ^ g) << 4));
                 }
-                uint4 vw[4];       // codes 16 g .. 16 g + 15 of keys 2t, 2t + 1, 2t + 8, 2t + 9
 #pragma unroll
                 for (int e = 0; e < 4; ++e) vw[e] = lds128(sv + (e >> 1) * half_step + (2 * t + (e & 1)) * 128u + ((g ^ (2 * t + (e & 1))) << 4));
-                float x[4], r[4];
-                {
-                    const float2 k0 = lds_f2(ck + 8 * t), k1 = lds_f2(ck + sc_half + 8 * t), v0 = lds_f2(cv + 8 * t), v1 = lds_f2(cv + sc_half + 8 * t);
-                    const float fk[4] = {k0.x, k0.y, k1.x, k1.y}, fv[4] = {v0.x, v0.y, v1.x, v1.y};
+                const float ka = lds_f1(ck + 4 * g), kb = lds_f1(ck + 4 * g + 32), la = lds_f1(ck + KVG * 64 + 4 * g), lb = lds_f1(ck + KVG * 64 + 4 * g + 32);
+                float ra = lds_f1(ck + KVG * 128 + 4 * g), rb = lds_f1(ck + KVG * 128 + 4 * g + 32);
+                if (patched) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) mbar_arrive(smem_u32(&s_empty[stage]));
+                // S^T = K.Q^T
+                float c[4] = {off0, off1, off0, off1};
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const float sv_e = fmaxf(fv[e], kQ8MinScale);
-                        r[e] = rcp(sv_e);
-                        x[e] = fmaf(c[e >> 1][e & 1] + c[e >> 1][2 + (e & 1)], fk[e] * kToLog2, lg2(sv_e));
-                    }
+                for (int ks = 0; ks < 8; ++ks) {
+                    const uint4 wa = kw[ks >> 2][0], wb = kw[ks >> 2][1];
+                    const int k4 = ks & 3;
+                    uint32_t a0, a1, a2, a3;
+                    q8_k_to_h2<kFmt>(k4 == 0 ? wa.x : k4 == 1 ? wa.y : k4 == 2 ? wa.z : wa.w, a0, a2);
+                    q8_k_to_h2<kFmt>(k4 == 0 ? wb.x : k4 == 1 ? wb.y : k4 == 2 ? wb.z : wb.w, a1, a3);
+                    mma_full(c, a0, a1, a2, a3, qh[ks][0], qh[ks][1]);
+                    if constexpr (kLo) mma_full(c, a0, a1, a2, a3, ql[ks][0], ql[ks][1]);
                 }
-                if (mask != 0xffffu) {
+                // x[e]: keys g (e = 0, 1) and g + 8 (e = 2, 3), heads 2 t and 2 t + 1
+                float x[4] = {fmaf(c[0], ka, la), fmaf(c[1], ka, la), fmaf(c[2], kb, lb), fmaf(c[3], kb, lb)};
+                if (mask != 0xffffu) {             // what is masked may hold anything
+                    if (!((mask >> g) & 1)) {
+                        x[0] = x[1] = -INFINITY;
+                        ra = 0.f;
+                    }
+                    if (!((mask >> (g + 8)) & 1)) {
+                        x[2] = x[3] = -INFINITY;
+                        rb = 0.f;
+                    }
 #pragma unroll
                     for (int e = 0; e < 4; ++e)
-                        if (!((mask >> (2 * t + (e & 1) + 8 * (e >> 1))) & 1)) {      // what is masked may hold anything
-                            x[e] = -INFINITY;
-                            r[e] = 0.f;
-                            vw[e] = make_uint4(0u, 0u, 0u, 0u);
-                        }
+                        if (!((mask >> (2 * t + (e & 1) + 8 * (e >> 1))) & 1)) vw[e] = make_uint4(0u, 0u, 0u, 0u);
                 }
-                float mx = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
-                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-                const float mn = fmaxf(m, mx);
-                if (__any_sync(0xffffffffu, mn != m)) {
-                    const float corr = ex2(m - mn);
-                    l *= corr;
+                // The reference moves only when a score outgrows it by more than 2^8; the largest weight is then 2^7 .. 2^15, and a
+                // weight keeps fp16's 11 bits down to 2^-21 of the reference (2^7 cancels between the outputs and l).
+                float m0 = fmaxf(x[0], x[2]), m1 = fmaxf(x[1], x[3]);
+                if (__any_sync(0xffffffffu, m0 > ref0 + 8.f || m1 > ref1 + 8.f)) {
 #pragma unroll
-                    for (int j = 0; j < 16; ++j) {
-                        o[j][0] *= corr;
-                        o[j][1] *= corr;
-                        o[j][2] *= corr;
-                        o[j][3] *= corr;
+                    for (int sh = 4; sh < 32; sh <<= 1) {
+                        m0 = fmaxf(m0, __shfl_xor_sync(0xffffffffu, m0, sh));
+                        m1 = fmaxf(m1, __shfl_xor_sync(0xffffffffu, m1, sh));
                     }
-                    m = mn;
-                }
-                // The largest weight is 2^14, not 1: a weight of fp16 then keeps its 11 bits down to 2^-28 of the largest (2^14
-                // cancels between the outputs and l).
-                const float ref = m - 14.f;
-                uint32_t ph[2], pl[2];
+                    m0 = fmaxf(m0, ref0);
+                    m1 = fmaxf(m1, ref1);
+                    const float c0 = ex2(ref0 - m0), c1 = ex2(ref1 - m1);
+                    ref0 = m0;
+                    ref1 = m1;
+                    l0 *= c0;
+                    l1 *= c1;
 #pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    const float p0 = ex2(x[2 * e] - ref), p1 = ex2(x[2 * e + 1] - ref);
-                    l = fmaf(p0, r[2 * e], l);
-                    l = fmaf(p1, r[2 * e + 1], l);
-                    const __half2 h = __floats2half2_rn(p0, p1);
-                    const float2 b = __half22float2(h);
-                    ph[e] = *reinterpret_cast<const uint32_t*>(&h);
-                    pl[e] = pack_h2(p0 - b.x, p1 - b.y);
+                    for (int j = 0; j < 8; ++j) {
+                        o[j][0] *= c0;
+                        o[j][1] *= c1;
+                        o[j][2] *= c0;
+                        o[j][3] *= c1;
+                    }
                 }
-                // O += P.V: product j has the dims 16 n + j, n = 0..7, as its columns
+                const float s0 = ref0 - 7.f, s1 = ref1 - 7.f;
+                const float p0 = ex2(x[0] - s0), p1 = ex2(x[1] - s1), p2 = ex2(x[2] - s0), p3 = ex2(x[3] - s1);
+                l0 = fmaf(p2, rb, fmaf(p0, ra, l0));
+                l1 = fmaf(p3, rb, fmaf(p1, ra, l1));
+                const uint32_t ha = pack_h2(p0, p1), hb = pack_h2(p2, p3);
+                const uint32_t ph0 = movmatrix(ha), ph1 = movmatrix(hb);
+                uint32_t pl0 = 0u, pl1 = 0u;
+                if constexpr (kLo) {
+                    const float2 fa = __half22float2(*reinterpret_cast<const __half2*>(&ha)), fb = __half22float2(*reinterpret_cast<const __half2*>(&hb));
+                    pl0 = movmatrix(pack_h2(p0 - fa.x, p1 - fa.y));
+                    pl1 = movmatrix(pack_h2(p2 - fb.x, p3 - fb.y));
+                }
+                // O^T += V^T.P^T: product j has the dims 16 g + 2 j and 16 g + 2 j + 1 as its rows g and g + 8
 #pragma unroll
                 for (int k4 = 0; k4 < 4; ++k4) {
                     uint32_t wd[4];
@@ -446,61 +574,78 @@ q8_decode_kernel(Q8Launch a, const __grid_constant__ CUtensorMap tmk, const __gr
                         q8_to_h2<kFmt>(__byte_perm(wd[2 * e], wd[2 * e + 1], 0x7362), b[e][2], b[e][3]);
                     }
 #pragma unroll
-                    for (int d = 0; d < 4; ++d) mma_full(o[4 * k4 + d], ph[0], pl[0], ph[1], pl[1], b[0][d], b[1][d]);
+                    for (int d = 0; d < 2; ++d) {
+                        mma_full(o[2 * k4 + d], b[0][2 * d], b[0][2 * d + 1], b[1][2 * d], b[1][2 * d + 1], ph0, ph1);
+                        if constexpr (kLo) mma_full(o[2 * k4 + d], b[0][2 * d], b[0][2 * d + 1], b[1][2 * d], b[1][2 * d + 1], pl0, pl1);
+                    }
                 }
             }
-            if (patched) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            __syncwarp();
-            if (lane == 0) mbar_arrive(smem_u32(&s_empty[stage]));
+            else if (lane == 0) {
+                mbar_arrive(smem_u32(&s_empty[stage]));
+            }
+            stage += kSub;
+            if (stage >= kStages) {
+                stage -= kStages;
+                parity ^= 1;
+            }
         }
         it = it_end;
 
-        // ---- the row's segment is done: high and low parts together, then the head's warps, then memory
-        l += __shfl_xor_sync(0xffffffffu, l, 1);
-        l += __shfl_xor_sync(0xffffffffu, l, 2);
-        float acc[32];             // dims 32 t + i of head g
+        // ---- the row's segment is done: the sums of the key lanes together, then the head's warps, then memory
 #pragma unroll
-        for (int j = 0; j < 16; ++j) {
-            acc[j] = o[j][0] + o[j][2];
-            acc[16 + j] = o[j][1] + o[j][3];
+        for (int sh = 4; sh < 32; sh <<= 1) {
+            l0 += __shfl_xor_sync(0xffffffffu, l0, sh);
+            l1 += __shfl_xor_sync(0xffffffffu, l1, sh);
         }
         if constexpr (kSub > 1) {
-            float* mine = merge + (size_t)(w * (kSub - 1)) * 34 * 32 + lane;
+            float* mine = merge + (size_t)(w * (kSub - 1)) * 36 * 32 + lane;
             if (sub > 0) {
-                float* p = mine + (size_t)(sub - 1) * 34 * 32;
+                float* p = mine + (size_t)(sub - 1) * 36 * 32;
 #pragma unroll
-                for (int j = 0; j < 32; ++j) p[32 * j] = acc[j];
-                p[32 * 32] = m;
-                p[33 * 32] = l;
+                for (int j = 0; j < 32; ++j) p[32 * j] = o[j >> 2][j & 3];
+                p[32 * 32] = ref0;
+                p[33 * 32] = ref1;
+                p[34 * 32] = l0;
+                p[35 * 32] = l1;
             }
             asm volatile("bar.sync %0, %1;" ::"r"(1 + w), "r"(32 * kSub) : "memory");
             if (sub == 0) {
 #pragma unroll 1
                 for (int u = 0; u < kSub - 1; ++u) {
-                    const float* p = mine + (size_t)u * 34 * 32;
-                    const float mu = p[32 * 32], lu = p[33 * 32];
-                    const float mn = fmaxf(m, mu);
-                    const float c0 = m == -INFINITY ? 0.f : ex2(m - mn), c1 = mu == -INFINITY ? 0.f : ex2(mu - mn);
-                    l = l * c0 + lu * c1;
+                    const float* p = mine + (size_t)u * 36 * 32;
+                    const float u0 = p[32 * 32], u1 = p[33 * 32];
+                    const float n0 = fmaxf(ref0, u0), n1 = fmaxf(ref1, u1);
+                    const float a0 = ref0 == -INFINITY ? 0.f : ex2(ref0 - n0), b0 = u0 == -INFINITY ? 0.f : ex2(u0 - n0);
+                    const float a1 = ref1 == -INFINITY ? 0.f : ex2(ref1 - n1), b1 = u1 == -INFINITY ? 0.f : ex2(u1 - n1);
+                    l0 = l0 * a0 + p[34 * 32] * b0;
+                    l1 = l1 * a1 + p[35 * 32] * b1;
 #pragma unroll
-                    for (int j = 0; j < 32; ++j) acc[j] = acc[j] * c0 + p[32 * j] * c1;
-                    m = mn;
+                    for (int j = 0; j < 32; ++j) o[j >> 2][j & 3] = o[j >> 2][j & 3] * (j & 1 ? a1 : a0) + p[32 * j] * (j & 1 ? b1 : b0);
+                    ref0 = n0;
+                    ref1 = n1;
                 }
             }
             asm volatile("bar.sync %0, %1;" ::"r"(1 + w), "r"(32 * kSub) : "memory");
             if (sub > 0) continue;
         }
-        if (g >= G) continue;
-        if (sg.c_last == sg.c_first) {
-            const float inv = l > 0.f ? 1.f / l : 0.f;
-            const int64_t oe = (int64_t)row * a.out_stride + (int64_t)head * kHeadDim + 32 * t;
 #pragma unroll
-            for (int j = 0; j < 32; j += 4) q8_store4(a.out, oe + j, a.io, make_float4(acc[j] * inv, acc[j + 1] * inv, acc[j + 2] * inv, acc[j + 3] * inv));
-        } else {
-            float* p = a.part + ((size_t)((int64_t)blockIdx.x + sg.row_id) * heads_per_row + (size_t)(w * G + g)) * kSlotW;
-            if (t == 0) *reinterpret_cast<float2*>(p) = make_float2(m, l);
+        for (int e = 0; e < 2; ++e) {                       // heads 2 t + e: o[j][e], o[j][2 + e] are the dims 16 g + 2 j, 16 g + 2 j + 1
+            const int hd = 2 * t + e;
+            if (hd >= G) continue;
+            const float l = e ? l1 : l0;
+            if (sg.c_last == sg.c_first) {
+                const float inv = l > 0.f ? 1.f / l : 0.f;
+                const int64_t oe = (int64_t)row * a.out_stride + (int64_t)(kvh * G + hd) * kHeadDim + 16 * g;
 #pragma unroll
-            for (int j = 0; j < 32; j += 4) *reinterpret_cast<float4*>(p + 4 + 32 * t + j) = make_float4(acc[j], acc[j + 1], acc[j + 2], acc[j + 3]);
+                for (int j = 0; j < 8; j += 2)
+                    q8_store4(a.out, oe + 2 * j, a.io, make_float4(o[j][e] * inv, o[j][2 + e] * inv, o[j + 1][e] * inv, o[j + 1][2 + e] * inv));
+            } else {
+                float* p = a.part + ((size_t)((int64_t)blockIdx.x + sg.row_id) * heads_per_row + (size_t)(w * G + hd)) * kSlotW;
+                if (g == 0) *reinterpret_cast<float2*>(p) = make_float2(e ? ref1 : ref0, l);
+#pragma unroll
+                for (int j = 0; j < 8; j += 2)
+                    *reinterpret_cast<float4*>(p + 4 + 16 * g + 2 * j) = make_float4(o[j][e], o[j][2 + e], o[j + 1][e], o[j + 1][2 + e]);
+            }
         }
     }
 }
@@ -630,17 +775,22 @@ __global__ void __launch_bounds__(128) q8_attn_kernel(Q8Launch a) {
 int dec_group(int n_kv_heads) { return n_kv_heads % 4 == 0 ? 4 : (n_kv_heads % 2 == 0 ? 2 : 1); }
 bool is_decode(int n_heads, int n_kv_heads, int max_tokens) { return max_tokens <= 1 && n_heads / n_kv_heads <= 8; }
 
-template <int KVG, int kFmt>
-int launch_decode(const Q8Launch& a, const CUtensorMap& tmk, const CUtensorMap& tmv, int ctas, cudaStream_t s) {
+template <int KVG, int kFmt, bool kLo>
+int launch_decode_as(const Q8Launch& a, const CUtensorMap& tmk, const CUtensorMap& tmv, int ctas, cudaStream_t s) {
     using Cfg = DecCfg<KVG>;
-    NOVA_CUDA_TRY((cudaFuncSetAttribute(q8_decode_kernel<KVG, kFmt>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::kSmem)));
-    const cudaError_t e = launch_kernel_pdl(q8_decode_kernel<KVG, kFmt>, dim3((unsigned)ctas), dim3(Cfg::kThreads), (size_t)Cfg::kSmem, s, true, a, tmk, tmv);
+    NOVA_CUDA_TRY((cudaFuncSetAttribute(q8_decode_kernel<KVG, kFmt, kLo>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::kSmem)));
+    const cudaError_t e = launch_kernel_pdl(q8_decode_kernel<KVG, kFmt, kLo>, dim3((unsigned)ctas), dim3(Cfg::kThreads), (size_t)Cfg::kSmem, s, true, a, tmk, tmv);
     if (e != cudaSuccess) {
         set_cuda_error(e, "8-bit decode attention launch");
         return NOVA_ERR_CUDA;
     }
     NOVA_LAUNCH_CHECK();
     return NOVA_OK;
+}
+
+template <int KVG, int kFmt>
+int launch_decode(const Q8Launch& a, const CUtensorMap& tmk, const CUtensorMap& tmv, int ctas, cudaStream_t s) {
+    return a.io == NOVA_IO_F32 ? launch_decode_as<KVG, kFmt, true>(a, tmk, tmv, ctas, s) : launch_decode_as<KVG, kFmt, false>(a, tmk, tmv, ctas, s);
 }
 
 }  // namespace

@@ -359,8 +359,9 @@ int nova_launch_q8_append(const nova_q8_cache* c, const nova_q8_rows* r, const v
 int nova_launch_q8_read(const nova_q8_cache* c, const nova_q8_rows* r, void* k_out, void* v_out, nova_stream_t s);
 /* Attention of the rows of q ([n_tokens][n_heads][128]) over the cached keys: the query at position p sees the keys [0, p], or
  * (p - window, p] where window > 0.  The keys of the new rows must be in the cache; a query that sees none gets zeros.
- * q is taken to fp16 where a session has several rows or a kv head more than 8 query heads, to fp16 hi + lo parts otherwise;
- * sums and the softmax are fp32.  q and out must not overlap.  work: nova_q8_workspace_bytes() bytes, no state in it
+ * Codes are exact; q (rotated) and the softmax weights are rounded to fp16 on their way into the tensor cores, or, for fp32
+ * activations of one row per session and at most 8 query heads per kv head, taken as two fp16 parts (2^-21); sums and the
+ * softmax are fp32.  q and out must not overlap.  work: nova_q8_workspace_bytes() bytes, no state in it
  * between calls; calls that may overlap on the GPU need a workspace each. */
 size_t nova_q8_workspace_bytes(const nova_kv_shape* sh, const nova_q8_rows* r);
 int nova_launch_q8_attn(const nova_q8_cache* c, const nova_q8_rows* r, const void* q, void* out, int window, void* work,
