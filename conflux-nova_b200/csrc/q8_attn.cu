@@ -23,72 +23,11 @@
 //   * The scale of K multiplies the finished score.  The scale of V goes into the exponent: w_j = 2^(x_j + log2 sv_j - ref), so
 //     the weights that multiply the codes stay inside fp16's range whatever the scales are; the softmax sum adds w_j / sv_j.
 #include "attn_plan.cuh"
-#include "mma_common.cuh"
 #include "q8_common.cuh"
 
 namespace novab {
 namespace {
 
-__device__ __forceinline__ float lg2(float x) {
-    float y;
-    asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-__device__ __forceinline__ float rcp(float x) {
-    float y;
-    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-
-// Four codes of a word -> two pairs of fp16, exactly.
-template <int kFmt> __device__ __forceinline__ void q8_to_h2(uint32_t w, uint32_t& h0, uint32_t& h1) {
-    if constexpr (kFmt == NOVA_KV_I8) {
-        // 0x6400 | (code + 128) is the fp16 number 1024 + 128 + code
-        const uint32_t u = w ^ 0x80808080u;
-        const uint32_t a = __byte_perm(u, 0x64646464u, 0x4140), b = __byte_perm(u, 0x64646464u, 0x4342);
-        const __half2 k = __halves2half2(__ushort_as_half(0x6480), __ushort_as_half(0x6480));      // 1152
-        const __half2 x = __hsub2(*reinterpret_cast<const __half2*>(&a), k), y = __hsub2(*reinterpret_cast<const __half2*>(&b), k);
-        h0 = *reinterpret_cast<const uint32_t*>(&x);
-        h1 = *reinterpret_cast<const uint32_t*>(&y);
-    } else {
-        asm("{ .reg .b16 l, h; mov.b32 {l, h}, %2; cvt.rn.f16x2.e4m3x2 %0, l; cvt.rn.f16x2.e4m3x2 %1, h; }" : "=r"(h0), "=r"(h1) : "r"(w));
-    }
-}
-
-// The same for K: int8 codes as (code + 128) 2^-24, an fp16 subnormal whose bits are the byte.
-template <int kFmt> __device__ __forceinline__ void q8_k_to_h2(uint32_t w, uint32_t& h0, uint32_t& h1) {
-    if constexpr (kFmt == NOVA_KV_I8) {
-        const uint32_t u = w ^ 0x80808080u;
-        h0 = __byte_perm(u, 0u, 0x4140);
-        h1 = __byte_perm(u, 0u, 0x4342);
-    } else {
-        q8_to_h2<kFmt>(w, h0, h1);
-    }
-}
-
-__device__ __forceinline__ uint4 lds128(uint32_t addr) {
-    uint4 v;
-    asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr));
-    return v;
-}
-__device__ __forceinline__ float lds_f1(uint32_t addr) {
-    float v;
-    asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(addr));
-    return v;
-}
-__device__ __forceinline__ void sts_f1(uint32_t addr, float v) { asm volatile("st.shared.f32 [%0], %1;" ::"r"(addr), "f"(v) : "memory"); }
-__device__ __forceinline__ void sts128(uint32_t addr, float4 v) {
-    asm volatile("st.shared.v4.f32 [%0], {%1,%2,%3,%4};" ::"r"(addr), "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w) : "memory");
-}
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
-}
-// Transpose of an 8 x 8 matrix of 16-bit values over the warp (lane 4 r + c holds row r, columns 2c and 2c + 1).
-__device__ __forceinline__ uint32_t movmatrix(uint32_t x) {
-    uint32_t y;
-    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
-    return y;
-}
 constexpr int kSetupTiles = 2;       // work-split weight of starting a row inside a CTA, in tiles
 constexpr int kMinTiles = 4;         // a CTA gets at least that many tiles (fewer partial rows to merge for short contexts)
 
@@ -525,10 +464,9 @@ q8_decode_kernel(Q8Launch a, const __grid_constant__ CUtensorMap tmk, const __gr
                     for (int e = 0; e < 4; ++e)
                         if (!((mask >> (2 * t + (e & 1) + 8 * (e >> 1))) & 1)) vw[e] = make_uint4(0u, 0u, 0u, 0u);
                 }
-                // The reference moves only when a score outgrows it by more than 2^8; the largest weight is then 2^7 .. 2^15, and a
-                // weight keeps fp16's 11 bits down to 2^-21 of the reference (2^7 cancels between the outputs and l).
+                // (2^kQ8Top cancels between the outputs and l)
                 float m0 = fmaxf(x[0], x[2]), m1 = fmaxf(x[1], x[3]);
-                if (__any_sync(0xffffffffu, m0 > ref0 + 8.f || m1 > ref1 + 8.f)) {
+                if (__any_sync(0xffffffffu, m0 > ref0 + kQ8Step || m1 > ref1 + kQ8Step)) {
 #pragma unroll
                     for (int sh = 4; sh < 32; sh <<= 1) {
                         m0 = fmaxf(m0, __shfl_xor_sync(0xffffffffu, m0, sh));
@@ -549,7 +487,7 @@ q8_decode_kernel(Q8Launch a, const __grid_constant__ CUtensorMap tmk, const __gr
                         o[j][3] *= c1;
                     }
                 }
-                const float s0 = ref0 - 7.f, s1 = ref1 - 7.f;
+                const float s0 = ref0 - kQ8Top, s1 = ref1 - kQ8Top;
                 const float p0 = ex2(x[0] - s0), p1 = ex2(x[1] - s1), p2 = ex2(x[2] - s0), p3 = ex2(x[3] - s1);
                 l0 = fmaf(p2, rb, fmaf(p0, ra, l0));
                 l1 = fmaf(p3, rb, fmaf(p1, ra, l1));
@@ -716,62 +654,6 @@ __global__ void __launch_bounds__(128) q8_decode_merge_kernel(Q8Launch a, int kv
     }
 }
 
-__device__ __forceinline__ float warp_total(float v) {
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-    return v;
-}
-
-// Several new tokens per session, or more than 8 query heads per kv head: one warp per (token, query head), a lane owns four
-// dims; online softmax in fp32.
-template <int kFmt>
-__global__ void __launch_bounds__(128) q8_attn_kernel(Q8Launch a) {
-    const int lane = (int)threadIdx.x & 31;
-    const int64_t job = (int64_t)blockIdx.x * 4 + ((int)threadIdx.x >> 5);
-    if (job >= (int64_t)a.n_tokens * a.n_heads) return;
-    const int r = (int)(job / a.n_heads), head = (int)(job - (int64_t)r * a.n_heads);
-    int t;
-    const int s = q8_session_of(a, r, t);
-    if (s < 0) return;
-    const int64_t pos = (int64_t)__ldg(a.n_past + s) + t;
-    if (pos < 0 || (a.rope_cs && pos >= a.rope_rows)) {
-        if (lane == 0) q8_flag(a, NOVA_ERR_INVALID);
-        return;
-    }
-    const int h = head / (a.n_heads / a.n_kv_heads);
-    float4 q = q8_load4(a.q, (int64_t)r * a.q_stride + head * kHeadDim + 4 * lane, a.io);
-    if (a.rope_cs) q = q8_rotate(q, pos, lane, a);
-    const int64_t first = a.window > 0 && pos - a.window + 1 > 0 ? pos - a.window + 1 : 0;
-    const int32_t* table = q8_table(a, s);
-    float m = -INFINITY, l = 0.f;
-    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int64_t j = first; j <= pos; ++j) {
-        const int64_t lb = j >> a.kv_shift;
-        const int phys = lb < a.table_stride ? __ldg(table + lb) : -1;
-        if (phys < 0 || phys >= a.nb) {
-            if (lane == 0) q8_flag(a, NOVA_ERR_BAD_TABLE);
-            continue;
-        }
-        const int64_t page = (int64_t)a.layer * a.nb + phys;
-        const int slot = (int)(j & ((1 << a.kv_shift) - 1));
-        const int64_t row = (((page << a.kv_shift) + slot) * a.n_kv_heads + h) * kHeadDim + 4 * lane;
-        const int64_t sc = ((page * a.n_kv_heads + h) << a.kv_shift) + slot;
-        const float4 k = q8_decode4<kFmt>(*reinterpret_cast<const uint32_t*>(static_cast<const unsigned char*>(a.pool_k) + row));
-        const float4 v = q8_decode4<kFmt>(*reinterpret_cast<const uint32_t*>(static_cast<const unsigned char*>(a.pool_v) + row));
-        const float x = warp_total(q.x * k.x + q.y * k.y + q.z * k.z + q.w * k.w) * (a.scale_k[sc] * kAttnScale);
-        const float mn = fmaxf(m, x);
-        const float corr = expf(m - mn), p = expf(x - mn), pv = p * a.scale_v[sc];
-        m = mn;
-        l = fmaf(l, corr, p);
-        acc.x = fmaf(acc.x, corr, pv * v.x);
-        acc.y = fmaf(acc.y, corr, pv * v.y);
-        acc.z = fmaf(acc.z, corr, pv * v.z);
-        acc.w = fmaf(acc.w, corr, pv * v.w);
-    }
-    const float inv = l > 0.f ? 1.f / l : 0.f;
-    q8_store4(a.out, (int64_t)r * a.out_stride + head * kHeadDim + 4 * lane, a.io, make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv));
-}
-
 int dec_group(int n_kv_heads) { return n_kv_heads % 4 == 0 ? 4 : (n_kv_heads % 2 == 0 ? 2 : 1); }
 bool is_decode(int n_heads, int n_kv_heads, int max_tokens) { return max_tokens <= 1 && n_heads / n_kv_heads <= 8; }
 
@@ -796,7 +678,7 @@ int launch_decode(const Q8Launch& a, const CUtensorMap& tmk, const CUtensorMap& 
 }  // namespace
 
 size_t q8_work_bytes(int n_heads, int n_kv_heads, int n_sessions, int, int max_tokens) {
-    if (!is_decode(n_heads, n_kv_heads, max_tokens)) return 0;
+    if (!is_decode(n_heads, n_kv_heads, max_tokens)) return q8_chunk_work_bytes(n_heads, n_kv_heads, max_tokens);
     const int kvg = dec_group(n_kv_heads), groups = n_kv_heads / kvg;
     const int64_t rows = (int64_t)n_sessions * groups;
     return (size_t)((rows < kMaxRowsSmem ? rows : kMaxRowsSmem) + kMaxSms) * (size_t)(kvg * (n_heads / n_kv_heads)) * kSlotW * sizeof(float);
@@ -857,16 +739,11 @@ int launch_q8_attn(const Q8Launch& a_in, size_t, cudaStream_t s) {
         }
         return NOVA_OK;
     }
-    const int64_t blocks = ((int64_t)a.n_tokens * a.n_heads + 3) / 4;
-    if (blocks > 0x7fffffffLL) return NOVA_ERR_TOO_LARGE;
     if (a.append) {
         const int rc = launch_q8_append(a, s);
         if (rc != NOVA_OK) return rc;
     }
-    if (a.fmt == NOVA_KV_I8) q8_attn_kernel<NOVA_KV_I8><<<(unsigned)blocks, 128, 0, s>>>(a);
-    else q8_attn_kernel<NOVA_KV_E4M3><<<(unsigned)blocks, 128, 0, s>>>(a);
-    NOVA_LAUNCH_CHECK();
-    return NOVA_OK;
+    return launch_q8_chunk(a, s);
 }
 
 }  // namespace novab

@@ -1,0 +1,790 @@
+// q8_chunk.cu — attention of chunks of new tokens over the 8-bit paged cache: a ragged number of tokens per session (drafted
+// tokens, prompt chunks), causal or in a sliding window; also single tokens with more than 8 query heads per kv head.
+//
+// What bounds it: few rows over long contexts, HBM (264 bytes per key and kv head); many rows, the tensor cores and the
+// exponentials (4 * 128 flops and one exponential per (query head, key)).
+//
+//   * tcgen05 with accumulators in tensor memory.  The (token, head) pairs that share a kv head are the rows of a tile: one
+//     half of 128 rows, or two that share every K/V tile.  A unit of work is (session, kv head, tile of tokens); the 64-key tiles
+//     of all units form one line that is dealt out evenly over one CTA per SM, so neither short sessions, nor long ones, nor
+//     the causal triangle leave SMs idle.  Units that several CTAs worked on are merged by the kernel behind it.
+//   * Sixteen warps: 8 softmax (thread = row), 2 issuing MMAs (one per half), 1 copying codes (TMA boxes of 16 slots x 128 B), 1
+//     preparing scales, 4 converting.  The pipe runs on from one unit to the next.
+//   * The tensor cores want fp16 operands, so the codes of a tile are converted in shared memory: exact integers or e4m3 values,
+//     128-byte-swizzle layout, which is the K-major form for S = Q.K^T and the MN-major form for O += P.V.  A lane's rows
+//     are chosen so that neither the reads (rows r and r ^ 5 side by side) nor the writes meet in a bank.
+//   * Scales: x = s * (sk log2 e / sqrt(128)) + log2 sv, packed fp32 pairs, weights w = 2^(x - ref), sum += w / sv (see q8_attn.cu:
+//     weights stay inside fp16 whatever the scales are).  Keys that do not exist get sk = 0, log2 sv = -inf, 1 / sv = 0.
+//   * q is rotated on the way in and rounded to fp16, P is rounded to fp16; everything else is fp32.
+//   * Every wait is bounded; tensor memory is released on every path.
+#include "attn_plan.cuh"
+#include "q8_common.cuh"
+#include "tc5_common.cuh"
+
+namespace novab {
+namespace {
+
+constexpr int kThreads = 512;
+constexpr int kKeys = 64;                             // keys of a tile
+constexpr int kHalfRows = 128;                        // rows of a half = M of the MMAs
+constexpr int kSlab = kKeys * 128;                    // 64 rows x 128 B
+constexpr int kQSlab = kHalfRows * 128;
+constexpr int kRaw = 5;                               // tiles of codes in flight (16 KiB each)
+constexpr int kSc = 4;                                // tiles of prepared scales
+constexpr int kScSteps = 8;                           // ring of raw scales
+constexpr int kMaxSessions = 512;                     // sessions of one launch
+constexpr int kOffK = 4 * kQSlab;                     // two fp16 K tiles (dims 0-63 | 64-127), two V tiles
+constexpr int kOffV = kOffK + 2 * 2 * kSlab;
+constexpr int kOffRaw = kOffV + 2 * 2 * kSlab;        // codes: K 8 KiB | V 8 KiB
+constexpr int kOffSc = kOffRaw + kRaw * 2 * kSlab;    // per tile 64 x (K scale | log of V's | reciprocal of V's)
+constexpr int kOffRawSc = kOffSc + kSc * 768;
+constexpr int kOffPlan = kOffRawSc + kScSteps * 512;
+struct ChunkPlan {
+    long long line[kMaxSessions + 1];                 // where each session's tiles start on the line
+    int first[kMaxSessions], count[kMaxSessions], past[kMaxSessions];
+};
+constexpr int kOffBar = kOffPlan + (int)((sizeof(ChunkPlan) + 15) / 16 * 16);
+constexpr int kSmem = kOffBar + 512;
+static_assert(kSmem <= 232448, "shared memory of one CTA");
+constexpr int kTmemCols = 512;                        // S of half h, buffer b: columns 128 h + 64 b (P over its first 32); O: 256 + 128 h
+constexpr uint32_t kColO = 256;
+constexpr int kSetup = 2;                             // what starting a unit costs, in tiles
+constexpr int kMinTiles = 4;                          // a CTA gets at least that many
+constexpr uint32_t kIdescS = (1u << 4) | ((uint32_t)(kKeys >> 3) << 17) | ((uint32_t)(kHalfRows >> 4) << 24);
+constexpr uint32_t kIdescPV = (1u << 4) | (1u << 16) | ((uint32_t)(kHeadDim >> 3) << 17) | ((uint32_t)(kHalfRows >> 4) << 24);
+
+struct ChunkShape {
+    int tq;              // tokens of a tile
+    int halves;          // 1 or 2
+    int rows_cap;        // rows of a partial slot
+};
+
+// Tiles of a unit: keys [first16 * 16, keys_end) in steps of 64.
+__device__ __forceinline__ int unit_first16(const Q8Launch& a, int past, int t0) {
+    const int first = a.window > 0 && past + t0 - a.window + 1 > 0 ? past + t0 - a.window + 1 : 0;
+    return first >> 4;
+}
+__device__ __forceinline__ int unit_tiles(const Q8Launch& a, int tq, int past, int count, int qt) {
+    const int t1 = (qt + 1) * tq < count ? (qt + 1) * tq : count;
+    return (((past + t1 + 15) >> 4) - unit_first16(a, past, qt * tq) + 3) >> 2;
+}
+
+// All threads of the CTA; ends with __syncthreads().
+__device__ inline void build_plan(const Q8Launch& a, const ChunkShape& sh, ChunkPlan& p, bool flag) {
+    for (int s = (int)threadIdx.x; s < a.n_sessions; s += (int)blockDim.x) {
+        int first, count;
+        q8_rows(a, s, first, count);
+        const int past = __ldg(a.n_past + s);
+        if (count > 0 && (past < 0 || past > 0x7ff00000 - count)) {
+            if (flag) q8_flag(a, NOVA_ERR_INVALID);
+            count = 0;
+        }
+        long long len = 0;
+        for (int qt = 0; qt * sh.tq < count; ++qt) len += unit_tiles(a, sh.tq, past, count, qt) + kSetup;
+        p.line[s + 1] = len * a.n_kv_heads;
+        p.first[s] = first;
+        p.count[s] = count;
+        p.past[s] = past;
+    }
+    __syncthreads();
+    if (threadIdx.x < 32) {
+        const int lane = (int)threadIdx.x;
+        long long carry = 0;
+        if (lane == 0) p.line[0] = 0;
+        for (int base = 0; base < a.n_sessions; base += 32) {
+            long long v = base + lane < a.n_sessions ? p.line[base + lane + 1] : 0;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const long long t = __shfl_up_sync(0xffffffffu, v, o);
+                if (lane >= o) v += t;
+            }
+            if (base + lane < a.n_sessions) p.line[base + lane + 1] = carry + v;
+            carry += __shfl_sync(0xffffffffu, v, 31);
+        }
+    }
+    __syncthreads();
+}
+__device__ __forceinline__ int plan_ctas(long long total, int grid) {
+    const long long most = (total + kMinTiles - 1) / kMinTiles;
+    return most < grid ? (int)most : grid;
+}
+
+struct Unit {
+    int s, kvh, t0, t_cnt, past;     // session, kv head, first token of the tile, its tokens
+    int first16, keys_end, tiles;
+    long long begin, end;            // on the line, set-up weight included
+};
+// The unit at place pos of the line.  All lanes of a warp, same arguments.
+__device__ inline Unit find_unit(const Q8Launch& a, const ChunkShape& sh, const ChunkPlan& p, long long pos) {
+    const int lane = (int)threadIdx.x & 31;
+    int lo = 0, up = a.n_sessions;
+    while (up - lo > 1) {
+        const int mid = (lo + up) >> 1;
+        if (p.line[mid] <= pos) lo = mid; else up = mid;
+    }
+    while (lo + 1 < a.n_sessions && p.line[lo + 1] <= pos) ++lo;      // sessions without tiles
+    Unit u;
+    u.s = lo;
+    u.past = p.past[lo];
+    const int count = p.count[lo], nqt = (count + sh.tq - 1) / sh.tq;
+    const long long off = pos - p.line[lo], per_head = (p.line[lo + 1] - p.line[lo]) / a.n_kv_heads;
+    u.kvh = (int)(off / per_head);
+    long long rem = off - u.kvh * per_head, base = 0;
+    int qt = 0, len = 0;
+    long long before = 0;
+    for (int q0 = 0; q0 < nqt; q0 += 32) {
+        const int v = q0 + lane < nqt ? unit_tiles(a, sh.tq, u.past, count, q0 + lane) + kSetup : 0;
+        long long incl = v;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const long long t = __shfl_up_sync(0xffffffffu, incl, o);
+            if (lane >= o) incl += t;
+        }
+        const unsigned hit = __ballot_sync(0xffffffffu, rem < base + incl);
+        if (hit) {
+            const int l = __ffs(hit) - 1;
+            qt = q0 + l;
+            len = __shfl_sync(0xffffffffu, v, l);
+            before = base + __shfl_sync(0xffffffffu, incl, l) - len;
+            break;
+        }
+        base += __shfl_sync(0xffffffffu, incl, 31);
+    }
+    u.t0 = qt * sh.tq;
+    u.t_cnt = count - u.t0 < sh.tq ? count - u.t0 : sh.tq;
+    u.first16 = unit_first16(a, u.past, u.t0);
+    u.keys_end = u.past + u.t0 + u.t_cnt;
+    u.tiles = len - kSetup;
+    u.begin = pos - rem + before;
+    u.end = u.begin + len;
+    return u;
+}
+// The part [lo, hi) of the line that a CTA takes of a unit, as tiles of the unit.
+__device__ __forceinline__ void unit_part(const Unit& u, long long lo, long long hi, int& tile, int& count) {
+    const long long b = (lo > u.begin ? lo : u.begin) - u.begin - kSetup, e = (hi < u.end ? hi : u.end) - u.begin - kSetup;
+    tile = (int)(b > 0 ? b : 0);
+    count = (int)(e > 0 ? e : 0) - tile;
+    if (count < 0) count = 0;
+}
+
+__device__ __forceinline__ unsigned long long pack_f2(float x, float y) {
+    unsigned long long v;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(x), "f"(y));
+    return v;
+}
+__device__ __forceinline__ void unpack_f2(unsigned long long v, float& x, float& y) { asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(v)); }
+__device__ __forceinline__ unsigned long long fma_f2(unsigned long long x, unsigned long long y, unsigned long long z) {
+    unsigned long long v;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(v) : "l"(x), "l"(y), "l"(z));
+    return v;
+}
+__device__ __forceinline__ unsigned long long add_f2(unsigned long long x, unsigned long long y) {
+    unsigned long long v;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(v) : "l"(x), "l"(y));
+    return v;
+}
+__device__ __forceinline__ void lds_2x64(uint32_t addr, unsigned long long& x, unsigned long long& y) {
+    asm volatile("ld.shared.v2.b64 {%0, %1}, [%2];" : "=l"(x), "=l"(y) : "r"(addr));
+}
+template <int kRegs> __device__ __forceinline__ void regs_up() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegs)); }
+template <int kRegs> __device__ __forceinline__ void regs_down() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegs)); }
+
+template <int kFmt>
+__global__ void __launch_bounds__(kThreads, 1)
+q8_chunk_kernel(Q8Launch a, const __grid_constant__ CUtensorMap tmk, const __grid_constant__ CUtensorMap tmv, ChunkShape sh) {
+    // No static shared memory: the dynamic region then starts at the front of the CTA's window, which is 1024-byte aligned as the
+    // swizzled tiles need (checked).
+    extern __shared__ unsigned char smem_raw[];
+    ChunkPlan& plan = *reinterpret_cast<ChunkPlan*>(smem_raw + kOffPlan);
+    uint32_t& s_tmem = *reinterpret_cast<uint32_t*>(smem_raw + kOffBar + 400);
+    volatile int& s_abort = *reinterpret_cast<volatile int*>(smem_raw + kOffBar + 404);
+    unsigned long long* const s_rmask = reinterpret_cast<unsigned long long*>(smem_raw + kOffBar + 408);      // [kRaw] which keys of the raw tile exist
+    const int lane = (int)threadIdx.x & 31;
+    const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0);
+    const int G = a.n_heads / a.n_kv_heads;
+    const uint32_t base = smem_u32(smem_raw);
+    const uint32_t bar = base + kOffBar;
+    const uint32_t bar_rawfull = bar, bar_rawfree = bar + 40, bar_kfull = bar + 80, bar_kfree = bar + 96, bar_vfull = bar + 112, bar_vfree = bar + 128,
+                   bar_sready = bar + 144 /* [half][buffer] */, bar_pready = bar + 176, bar_pvdone = bar + 208, bar_scfull = bar + 240, bar_scfree = bar + 272,
+                   bar_qready = bar + 304 /* [half] */;
+    // Every waiter waits for a phase whose successor on the same barrier needs that waiter's own next action (or one that follows it),
+    // so a parity is never taken for a later one.
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < kRaw; ++i) {
+            mbar_init(bar_rawfull + 8u * i, 1);
+            mbar_init(bar_rawfree + 8u * i, 4);
+        }
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(bar_kfull + 8u * i, 4);
+            mbar_init(bar_kfree + 8u * i, sh.halves);
+            mbar_init(bar_vfull + 8u * i, 4);
+            mbar_init(bar_vfree + 8u * i, sh.halves);
+            mbar_init(bar_qready + 8u * i, kHalfRows);
+        }
+        for (int i = 0; i < 4; ++i) {
+            mbar_init(bar_sready + 8u * i, 1);
+            mbar_init(bar_pready + 8u * i, kHalfRows);
+            mbar_init(bar_pvdone + 8u * i, 1);
+        }
+        for (int i = 0; i < kSc; ++i) {
+            mbar_init(bar_scfull + 8u * i, 1);
+            mbar_init(bar_scfree + 8u * i, 4 * sh.halves);
+        }
+        s_abort = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&tmk) : "memory");
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&tmv) : "memory");
+    }
+    // Nothing of the caller's is read before the kernels before this one are done; the merge kernel, which reads positions and
+    // row starts before its own wait, is let go only then.
+    pdl_wait();
+    pdl_launch_dependents();
+    build_plan(a, sh, plan, blockIdx.x == 0);
+    const long long total = plan.line[a.n_sessions];
+    const int n_ctas = plan_ctas(total, (int)gridDim.x);
+    if ((int)blockIdx.x >= n_ctas || (base & 1023u) != 0) {            // uniform over the CTA; nothing has been allocated yet
+        if ((base & 1023u) != 0 && threadIdx.x == 0) q8_flag(a, NOVA_ERR_UNSUPPORTED);
+        return;
+    }
+    const long long lo = (long long)blockIdx.x * total / n_ctas, hi = ((long long)blockIdx.x + 1) * total / n_ctas;
+    if (warp == 0) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&s_tmem)), "r"((uint32_t)kTmemCols) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = __shfl_sync(0xffffffffu, s_tmem, 0);
+    bool failed = false;
+    int n = 0;                       // tiles of the units before: every ring runs on over the units
+
+    if (warp < 8) {
+        // ---------------------------------------------------------------------------------------- softmax: thread = one row
+        regs_up<168>();
+        const int half = warp >> 2, hrow = (int)threadIdx.x & (kHalfRows - 1);
+        const uint32_t t_lane = tmem + ((uint32_t)(32 * (warp & 3)) << 16);
+        const uint32_t col_s = 128u * (uint32_t)half, col_o = kColO + 128u * (uint32_t)half;
+        const uint32_t my_sready = bar_sready + 16u * (uint32_t)half, my_pready = bar_pready + 16u * (uint32_t)half, my_pvdone = bar_pvdone + 16u * (uint32_t)half;
+        const int row = half * kHalfRows + hrow, tk = row / G, g = row - tk * G;
+        for (long long pos = lo; pos < hi && !failed && half < sh.halves;) {
+            const Unit u = find_unit(a, sh, plan, pos);
+            int tile0, tiles;
+            unit_part(u, lo, hi, tile0, tiles);
+            pos = u.end;
+            if (tiles == 0) continue;
+            // ---- q: rotated, divided by 8 (so that a rotated fp16 value stays inside fp16), fp16, K-major 128-byte swizzle.  The scores of
+            // the unit before are all computed (this thread has waited for the last of them), so the operand can be overwritten.
+            const int row_pos = u.past + u.t0 + tk;
+            const bool in_tile = tk < u.t_cnt, beyond = in_tile && a.rope_cs && row_pos >= a.rope_rows;
+            const bool row_ok = in_tile && !beyond;
+            if (beyond && g == 0) q8_flag(a, NOVA_ERR_INVALID);
+            const int64_t q_row = (int64_t)plan.first[u.s] + u.t0 + tk;
+            {
+                const int64_t qe = q_row * a.q_stride + (int64_t)(u.kvh * G + g) * kHeadDim;
+                const bool rot = row_ok && a.rope_cs;
+#pragma unroll 2
+                for (int c = 0; c < 8; ++c) {                  // dims 8c .. 8c+7 and 64 + 8c ..
+                    float x[16];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const float4 v = row_ok ? q8_load4(a.q, qe + (e >> 1) * 64 + 8 * c + 4 * (e & 1), a.io) : make_float4(0.f, 0.f, 0.f, 0.f);
+                        x[4 * e] = v.x;
+                        x[4 * e + 1] = v.y;
+                        x[4 * e + 2] = v.z;
+                        x[4 * e + 3] = v.w;
+                    }
+                    if (rot && a.neox) {
+                        const float* cr = a.rope_cs + (int64_t)row_pos * 64 + 8 * c;
+                        const float* sr = a.rope_sn + (int64_t)row_pos * 64 + 8 * c;
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) {
+                            const float cc = __ldg(cr + e), sn = __ldg(sr + e), x0 = x[e], x1 = x[8 + e];
+                            x[e] = __fmaf_rn(x0, cc, -__fmul_rn(x1, sn));
+                            x[8 + e] = __fmaf_rn(x0, sn, __fmul_rn(x1, cc));
+                        }
+                    } else if (rot) {
+#pragma unroll
+                        for (int hf = 0; hf < 2; ++hf)
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) {
+                                const int64_t i = (int64_t)row_pos * 64 + 32 * hf + 4 * c + e;
+                                const float cc = __ldg(a.rope_cs + i), sn = __ldg(a.rope_sn + i), x0 = x[8 * hf + 2 * e], x1 = x[8 * hf + 2 * e + 1];
+                                x[8 * hf + 2 * e] = __fmaf_rn(x0, cc, -__fmul_rn(x1, sn));
+                                x[8 * hf + 2 * e + 1] = __fmaf_rn(x0, sn, __fmul_rn(x1, cc));
+                            }
+                    }
+#pragma unroll
+                    for (int hf = 0; hf < 2; ++hf) {
+                        const uint32_t dst = base + (uint32_t)((2 * half + hf) * kQSlab + hrow * 128 + ((c ^ (hrow & 7)) << 4));
+                        const float* y = x + 8 * hf;
+                        asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(dst), "r"(pack_h2(y[0] * 0.125f, y[1] * 0.125f)),
+                                     "r"(pack_h2(y[2] * 0.125f, y[3] * 0.125f)), "r"(pack_h2(y[4] * 0.125f, y[5] * 0.125f)), "r"(pack_h2(y[6] * 0.125f, y[7] * 0.125f))
+                                     : "memory");
+                    }
+                }
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            mbar_arrive(bar_qready + 8u * (uint32_t)half);
+            // rows that are nobody's see everything: they never slow a warp down, and nothing of them is written
+            const int row_lim = row_ok ? row_pos : 0x7fffffff;
+            const int row_lo = row_ok && a.window > 0 ? row_pos - a.window + 1 : 0;
+            float m_ref = -INFINITY, l = 0.f;
+#pragma unroll 1
+            for (int i = 0; i < tiles; ++i) {
+                const int t = n + i;
+                const uint32_t sc = base + kOffSc + (uint32_t)(t & (kSc - 1)) * 768u;
+                bool ok = t5_wait(bar_scfull + 8u * (uint32_t)(t & (kSc - 1)), (uint32_t)(t / kSc) & 1u, &s_abort);
+                ok = ok && t5_wait(my_sready + 8u * (uint32_t)(t & 1), (uint32_t)(t >> 1) & 1u, &s_abort);
+                if (!__all_sync(0xffffffffu, ok)) { failed = true; break; }
+                tc_fence_after();
+                uint32_t sv[2][32];
+                tmem_ld32(t_lane + col_s + 64u * (uint32_t)(t & 1), sv[0]);
+                tmem_ld32(t_lane + col_s + 64u * (uint32_t)(t & 1) + 32, sv[1]);
+                tmem_wait_ld();
+#pragma unroll
+                for (int c = 0; c < 64; c += 4) {               // scores in log2 units, with the logarithm of V's scale
+                    unsigned long long k0, k1, v0, v1;
+                    lds_2x64(sc + 4 * c, k0, k1);
+                    lds_2x64(sc + 256 + 4 * c, v0, v1);
+                    float y[4];
+                    unpack_f2(fma_f2(pack_f2(__uint_as_float(sv[c >> 5][c & 31]), __uint_as_float(sv[c >> 5][(c + 1) & 31])), k0, v0), y[0], y[1]);
+                    unpack_f2(fma_f2(pack_f2(__uint_as_float(sv[c >> 5][(c + 2) & 31]), __uint_as_float(sv[c >> 5][(c + 3) & 31])), k1, v1), y[2], y[3]);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) sv[c >> 5][(c + e) & 31] = __float_as_uint(y[e]);
+                }
+                const int key0 = (u.first16 << 4) + (tile0 + i) * kKeys;
+                const int hi_k = row_lim - key0, lo_k = row_lo - key0;       // first and last visible column
+                float mx = -INFINITY;
+                if (__all_sync(0xffffffffu, hi_k >= kKeys - 1 && lo_k <= 0)) {
+#pragma unroll
+                    for (int c = 0; c < 64; ++c) mx = fmaxf(mx, __uint_as_float(sv[c >> 5][c & 31]));
+                } else {
+#pragma unroll
+                    for (int c = 0; c < 64; ++c) {
+                        float v = __uint_as_float(sv[c >> 5][c & 31]);
+                        v = (c <= hi_k && c >= lo_k) ? v : -INFINITY;
+                        sv[c >> 5][c & 31] = __float_as_uint(v);
+                        mx = fmaxf(mx, v);
+                    }
+                }
+                float scale = 1.f;
+                if (mx > m_ref + kQ8Step || (m_ref == -INFINITY && mx > -INFINITY)) {
+                    scale = m_ref == -INFINITY ? 0.f : ex2(m_ref - mx);
+                    m_ref = mx;
+                }
+                const float ms = m_ref == -INFINITY ? 0.f : kQ8Top - m_ref;         // nothing visible yet: keep exp arguments finite
+                const unsigned long long ms2 = pack_f2(ms, ms);
+                uint32_t pk[32];
+                unsigned long long sum2 = 0ull;
+#pragma unroll
+                for (int c = 0; c < 64; c += 4) {
+                    unsigned long long r0, r1;
+                    lds_2x64(sc + 512 + 4 * c, r0, r1);
+                    float y[4];
+                    unpack_f2(add_f2(pack_f2(__uint_as_float(sv[c >> 5][c & 31]), __uint_as_float(sv[c >> 5][(c + 1) & 31])), ms2), y[0], y[1]);
+                    unpack_f2(add_f2(pack_f2(__uint_as_float(sv[c >> 5][(c + 2) & 31]), __uint_as_float(sv[c >> 5][(c + 3) & 31])), ms2), y[2], y[3]);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) y[e] = ex2(y[e]);
+                    sum2 = fma_f2(pack_f2(y[0], y[1]), r0, sum2);
+                    sum2 = fma_f2(pack_f2(y[2], y[3]), r1, sum2);
+                    pk[c >> 1] = pack_h2(y[0], y[1]);
+                    pk[(c >> 1) + 1] = pack_h2(y[2], y[3]);
+                }
+                __syncwarp();
+                if (lane == 0) mbar_arrive(bar_scfree + 8u * (uint32_t)(t & (kSc - 1)));
+                float s0, s1;
+                unpack_f2(sum2, s0, s1);
+                l = fmaf(l, scale, s0 + s1);
+                if (i > 0 && __any_sync(0xffffffffu, scale != 1.f)) {
+                    // O is rescaled between two P.V products: the previous one must be done
+                    if (!__all_sync(0xffffffffu, t5_wait(my_pvdone + 8u * (uint32_t)((t - 1) & 1), (uint32_t)((t - 1) >> 1) & 1u, &s_abort))) { failed = true; break; }
+                    tc_fence_after();
+#pragma unroll 1
+                    for (int cc = 0; cc < 4; ++cc) {
+                        uint32_t ov[32];
+                        tmem_ld32(t_lane + col_o + 32u * (uint32_t)cc, ov);
+                        tmem_wait_ld();
+#pragma unroll
+                        for (int c = 0; c < 32; ++c) ov[c] = __float_as_uint(__uint_as_float(ov[c]) * scale);
+                        tmem_st32(t_lane + col_o + 32u * (uint32_t)cc, ov);
+                    }
+                    tmem_wait_st();
+                }
+                tmem_st32(t_lane + col_s + 64u * (uint32_t)(t & 1), pk);
+                tmem_wait_st();
+                tc_fence_before();
+                mbar_arrive(my_pready + 8u * (uint32_t)(t & 1));
+            }
+            n += tiles;
+            if (failed) break;
+            // ---- the unit's part is done: outputs, or a partial slot for the merge
+            if (!__all_sync(0xffffffffu, t5_wait(my_pvdone + 8u * (uint32_t)((n - 1) & 1), (uint32_t)((n - 1) >> 1) & 1u, &s_abort))) { failed = true; break; }
+            tc_fence_after();
+            const bool whole = tiles == u.tiles;
+            const float inv = whole ? (l > 0.f ? 1.f / l : 0.f) : 1.f;
+            const int64_t oe = q_row * a.out_stride + (int64_t)(u.kvh * G + g) * kHeadDim;
+            // slot: (m, l) of every row, then the accumulators, four dims of every row side by side
+            float* const slot = a.part + (size_t)(2 * blockIdx.x + (u.begin > lo ? 1 : 0)) * ((size_t)sh.rows_cap * kSlotW);
+            if (!whole && row_ok) *reinterpret_cast<float2*>(slot + 2 * row) = make_float2(m_ref, l);
+#pragma unroll 1
+            for (int cc = 0; cc < 4; ++cc) {
+                uint32_t ov[32];
+                tmem_ld32(t_lane + col_o + 32u * (uint32_t)cc, ov);
+                tmem_wait_ld();
+                if (row_ok) {
+#pragma unroll
+                    for (int c = 0; c < 32; c += 4) {
+                        const float4 v = make_float4(__uint_as_float(ov[c]) * inv, __uint_as_float(ov[c + 1]) * inv, __uint_as_float(ov[c + 2]) * inv,
+                                                     __uint_as_float(ov[c + 3]) * inv);
+                        if (whole) q8_store4(a.out, oe + 32 * cc + c, a.io, v);
+                        else *reinterpret_cast<float4*>(slot + 4 * (size_t)sh.rows_cap + ((size_t)(8 * cc + (c >> 2)) * sh.rows_cap + row) * 4) = v;
+                    }
+                }
+            }
+            tc_fence_before();
+        }
+    } else if (warp < 12) {
+        regs_down<80>();
+        if (warp < 10) {
+            // ------------------------------------------------------------------------------------ MMA issue: one warp per half
+            const int h = warp - 8;
+            const uint32_t q_lo0 = umma_desc_lo(base + (uint32_t)(2 * h) * kQSlab, 16u), k_lo0 = umma_desc_lo(base + kOffK, 16u),
+                           v_lo0 = umma_desc_lo(base + kOffV, (uint32_t)kSlab);
+            const uint32_t col_s = tmem + 128u * (uint32_t)h, col_o = tmem + kColO + 128u * (uint32_t)h;
+            auto issue_s = [&](int t) -> bool {
+                const uint32_t k_lo = k_lo0 + (uint32_t)(t & 1) * ((2 * kSlab) >> 4), d_s = col_s + 64u * (uint32_t)(t & 1);
+                if (!__all_sync(0xffffffffu, t5_wait(bar_kfull + 8u * (uint32_t)(t & 1), (uint32_t)(t >> 1) & 1u, &s_abort))) return false;
+                tc_fence_after();
+                if (elect_one()) {
+#pragma unroll
+                    for (int j = 0; j < 8; ++j)
+                        umma_f16(d_s, umma_desc_of(q_lo0 + (uint32_t)((j >> 2) * (kQSlab >> 4) + (j & 3) * 2)),
+                                 umma_desc_of(k_lo + (uint32_t)((j >> 2) * (kSlab >> 4) + (j & 3) * 2)), kIdescS, j > 0 ? 1u : 0u);
+                    umma_commit(bar_sready + 8u * (uint32_t)(2 * h + (t & 1)));
+                    umma_commit(bar_kfree + 8u * (uint32_t)(t & 1));
+                }
+                __syncwarp();
+                return true;
+            };
+            uint32_t seg = 0;
+            for (long long pos = lo; pos < hi && !failed && h < sh.halves;) {
+                const Unit u = find_unit(a, sh, plan, pos);
+                int tile0, tiles;
+                unit_part(u, lo, hi, tile0, tiles);
+                pos = u.end;
+                if (tiles == 0) continue;
+                if (!__all_sync(0xffffffffu, t5_wait(bar_qready + 8u * (uint32_t)h, seg & 1u, &s_abort))) { failed = true; break; }
+                ++seg;
+                if (!issue_s(n)) { failed = true; break; }
+                for (int i = 0; i < tiles; ++i) {
+                    const int t = n + i;
+                    const uint32_t v_lo = v_lo0 + (uint32_t)(t & 1) * ((2 * kSlab) >> 4), p_col = col_s + 64u * (uint32_t)(t & 1);
+                    // the scores of the next 64 keys first: they are computed while the softmax warps work on this tile
+                    if (i + 1 < tiles && !issue_s(t + 1)) { failed = true; break; }
+                    if (!__all_sync(0xffffffffu, t5_wait(bar_vfull + 8u * (uint32_t)(t & 1), (uint32_t)(t >> 1) & 1u, &s_abort))) { failed = true; break; }
+                    if (!__all_sync(0xffffffffu, t5_wait(bar_pready + 8u * (uint32_t)(2 * h + (t & 1)), (uint32_t)(t >> 1) & 1u, &s_abort))) { failed = true; break; }
+                    tc_fence_after();
+                    if (elect_one()) {
+#pragma unroll
+                        for (int j = 0; j < 4; ++j)
+                            umma_f16_ts(col_o, p_col + (uint32_t)(8 * j), umma_desc_of(v_lo + (uint32_t)(j * (2048 >> 4))), kIdescPV, (j > 0 || i > 0) ? 1u : 0u);
+                        umma_commit(bar_pvdone + 8u * (uint32_t)(2 * h + (t & 1)));
+                        umma_commit(bar_vfree + 8u * (uint32_t)(t & 1));
+                    }
+                    __syncwarp();
+                }
+                n += tiles;
+            }
+        } else {
+            // ------------------------------------------------------------------------------------ copies
+            const bool p8 = a.kv_shift == 3;
+            const int slot_mask = (1 << a.kv_shift) - 1;
+            // block-table entry of the page that holds a key; -1: a bad one, -2: there is no such key
+            auto entry = [&](const int32_t* table, int key, int keys_end) -> int {
+                if (key >= keys_end) return -2;
+                const int64_t page = key >> a.kv_shift;
+                if (page >= a.table_stride) return -1;
+                const int e = __ldg(table + page);
+                return e >= 0 && e < a.nb ? e : -1;
+            };
+            if (warp == 10) {
+                // codes: lane = (K or V, box of 16 slots, or of 8 in pages of 8), one box per tile
+                const int boxes = p8 ? 8 : 4, box_keys = p8 ? 8 : 16;
+                const int j = lane & 7, is_v = lane >> 3 & 1;
+                const bool mine = lane < 16 && j < boxes;
+                const CUtensorMap* const tm = is_v ? &tmv : &tmk;
+                const int row0 = (a.layer * a.nb) << a.kv_shift;
+                uint32_t stage = 0, round = 0;
+                for (long long pos = lo; pos < hi && !failed;) {
+                    const Unit u = find_unit(a, sh, plan, pos);
+                    int tile0, tiles;
+                    unit_part(u, lo, hi, tile0, tiles);
+                    pos = u.end;
+                    if (tiles == 0) continue;
+                    const int32_t* table = q8_table(a, u.s);
+                    const int key_a = (u.first16 << 4) + tile0 * kKeys + j * box_keys;       // this lane's first key of tile 0
+                    auto get = [&](int i) -> int { return mine && i < tiles ? entry(table, key_a + i * kKeys, u.keys_end) : -2; };
+                    int e0 = get(0), e1 = get(1), e2 = get(2);
+#pragma unroll 1
+                    for (int i = 0; i < tiles; ++i) {
+                        const int e = e0;
+                        e0 = e1;
+                        e1 = e2;
+                        e2 = get(i + 3);
+                        if (round > 0 && !__all_sync(0xffffffffu, t5_wait(bar_rawfree + 8u * stage, (round - 1) & 1u, &s_abort))) { failed = true; break; }
+                        const unsigned have = __ballot_sync(0xffffffffu, e >= 0) & 0xffu, bad = __ballot_sync(0xffffffffu, e == -1);
+                        if (lane == 0) {
+                            if (bad) q8_flag(a, NOVA_ERR_BAD_TABLE);
+                            unsigned long long mask = 0ull;
+                            for (int b = 0; b < boxes; ++b)
+                                if (have >> b & 1) mask |= (p8 ? 0xffull : 0xffffull) << (b * box_keys);
+                            const int left = u.keys_end - ((u.first16 << 4) + (tile0 + i) * kKeys);
+                            if (left < kKeys) mask &= (1ull << left) - 1ull;
+                            s_rmask[stage] = mask;
+                            const uint32_t bytes = 2u * (uint32_t)__popc(have) * (uint32_t)(box_keys * 128);
+                            if (bytes) mbar_expect_tx(bar_rawfull + 8u * stage, bytes);
+                            else mbar_arrive(bar_rawfull + 8u * stage);
+                        }
+                        __syncwarp();
+                        if (e >= 0)
+                            tma_load_3d(base + kOffRaw + stage * (2 * kSlab) + (uint32_t)(is_v * kSlab + j * box_keys * 128), tm, 0,
+                                        row0 + (e << a.kv_shift) + ((key_a + i * kKeys) & slot_mask), u.kvh, bar_rawfull + 8u * stage);
+                        if (++stage == kRaw) {
+                            stage = 0;
+                            ++round;
+                        }
+                    }
+                }
+            } else {
+                // scales: lane = (K or V, four keys); they arrive a few tiles ahead in a ring of the warp's own
+                constexpr int kDepth = kScSteps - 1;
+                const int quad = lane & 15;
+                const bool is_v = lane >= 16;
+                const uint32_t raw0 = base + kOffRawSc + (uint32_t)lane * 16u;
+                for (long long pos = lo; pos < hi && !failed;) {
+                    const Unit u = find_unit(a, sh, plan, pos);
+                    int tile0, tiles;
+                    unit_part(u, lo, hi, tile0, tiles);
+                    pos = u.end;
+                    if (tiles == 0) continue;
+                    const int32_t* table = q8_table(a, u.s);
+                    const float* const mine0 = (is_v ? a.scale_v : a.scale_k) + ((((int64_t)a.layer * a.nb) * a.n_kv_heads + u.kvh) << a.kv_shift);
+                    const int key_a = (u.first16 << 4) + tile0 * kKeys + 4 * quad;
+                    auto get = [&](int i) -> int { return i < tiles ? entry(table, key_a + i * kKeys, u.keys_end) : -2; };
+                    int e0 = get(0), e1 = get(1), e2 = get(2);
+                    unsigned have = 0u;                          // bit i: the quad of step i exists (a ring of kScSteps bits would do)
+#pragma unroll 1
+                    for (int step = 0; step < tiles + kDepth; ++step) {
+                        if (step < tiles) {
+                            const int e = e0;
+                            e0 = e1;
+                            e1 = e2;
+                            e2 = get(step + 3);
+                            const uint32_t raw = raw0 + (uint32_t)(step & (kScSteps - 1)) * 512u;
+                            if (e >= 0) cp_async16(raw, mine0 + (((int64_t)e * a.n_kv_heads) << a.kv_shift) + ((key_a + step * kKeys) & slot_mask));
+                            have = (have << 1) | (e >= 0 ? 1u : 0u);
+                        } else {
+                            have <<= 1;
+                        }
+                        asm volatile("cp.async.commit_group;" ::: "memory");
+                        if (step < kDepth) continue;
+                        asm volatile("cp.async.wait_group %0;" ::"n"(kDepth) : "memory");
+                        const int i = step - kDepth, t = n + i, stage = t & (kSc - 1);
+                        if (t >= kSc && !__all_sync(0xffffffffu, t5_wait(bar_scfree + 8u * (uint32_t)stage, (uint32_t)(t / kSc - 1) & 1u, &s_abort))) { failed = true; break; }
+                        const bool there = have >> kDepth & 1u;
+                        const uint4 w = lds128(raw0 + (uint32_t)(i & (kScSteps - 1)) * 512u);
+                        float v[4] = {__uint_as_float(w.x), __uint_as_float(w.y), __uint_as_float(w.z), __uint_as_float(w.w)}, r[4];
+                        const int left = u.keys_end - (key_a + i * kKeys);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const bool real = there && e < left;
+                            const float f = fmaxf(v[e], kQ8MinScale);
+                            r[e] = real ? rcp(f) : 0.f;
+                            v[e] = is_v ? (real ? lg2(f) : -INFINITY) : (real ? v[e] * (kAttnScale * kLog2e * 8.f) : 0.f);
+                        }
+                        const uint32_t dst = base + kOffSc + (uint32_t)stage * 768u + (uint32_t)(quad * 16) + (is_v ? 256u : 0u);
+                        sts128(dst, make_float4(v[0], v[1], v[2], v[3]));
+                        if (is_v) sts128(dst + 256u, make_float4(r[0], r[1], r[2], r[3]));
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(bar_scfull + 8u * (uint32_t)stage);
+                    }
+                    n += tiles;
+                }
+                asm volatile("cp.async.wait_all;" ::: "memory");
+            }
+        }
+    } else {
+        // ---------------------------------------------------------------------------------------- codes -> fp16 operands
+        regs_down<96>();
+        const int w = warp - 12;
+        // eight lanes share two rows that differ in bits 0 and 2: four 16-byte pieces of each, apart both where they are read
+        // (piece c of row r sits at c ^ (r & 7)) and where they are written (pieces 2c and 2c + 1 of the fp16 row, likewise)
+        const int r8 = (lane >> 3) ^ (5 * (lane >> 2 & 1)), c4 = lane & 3;
+        uint32_t stage = 0, round = 0;
+        for (long long pos = lo; pos < hi && !failed;) {
+            const Unit u = find_unit(a, sh, plan, pos);
+            int tile0, tiles;
+            unit_part(u, lo, hi, tile0, tiles);
+            pos = u.end;
+#pragma unroll 1
+            for (int i = 0; i < tiles; ++i) {
+                const int t = n + i;
+                bool ok = t5_wait(bar_rawfull + 8u * stage, round & 1u, &s_abort);
+                ok = ok && (t < 2 || t5_wait(bar_kfree + 8u * (uint32_t)(t & 1), (uint32_t)(t / 2 - 1) & 1u, &s_abort));
+                if (!__all_sync(0xffffffffu, ok)) { failed = true; break; }
+                const unsigned long long mask = s_rmask[stage];
+                const uint32_t raw = base + kOffRaw + stage * (2 * kSlab);
+#pragma unroll
+                for (int which = 0; which < 2; ++which) {
+                    if (which && t >= 2 && !__all_sync(0xffffffffu, t5_wait(bar_vfree + 8u * (uint32_t)(t & 1), (uint32_t)(t / 2 - 1) & 1u, &s_abort))) { failed = true; break; }
+                    const uint32_t src = raw + (uint32_t)(which * kSlab), dst = base + (which ? kOffV : kOffK) + (uint32_t)(t & 1) * (2 * kSlab);
+                    uint4 code[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {                      // rows 16 w + 8 (e >> 1) + r8, dims of slab e & 1
+                        const uint32_t r = (uint32_t)(16 * w + 8 * (e >> 1) + r8), c = (uint32_t)(4 * (e & 1) + c4);
+                        code[e] = lds128(src + r * 128u + ((c ^ (r & 7u)) << 4));
+                        // e4m3: what is not there may read as NaN, which no weight of 0 would hide
+                        if (kFmt == NOVA_KV_E4M3 && !(mask >> r & 1ull)) code[e] = make_uint4(0u, 0u, 0u, 0u);
+                    }
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const uint32_t r = (uint32_t)(16 * w + 8 * (e >> 1) + r8), d = dst + (uint32_t)((e & 1) * kSlab) + r * 128u;
+                        uint32_t h[8];
+                        q8_to_h2<kFmt>(code[e].x, h[0], h[1]);
+                        q8_to_h2<kFmt>(code[e].y, h[2], h[3]);
+                        q8_to_h2<kFmt>(code[e].z, h[4], h[5]);
+                        q8_to_h2<kFmt>(code[e].w, h[6], h[7]);
+                        asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(d + (((uint32_t)(2 * c4) ^ (r & 7u)) << 4)), "r"(h[0]), "r"(h[1]), "r"(h[2]), "r"(h[3]) : "memory");
+                        asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(d + (((uint32_t)(2 * c4 + 1) ^ (r & 7u)) << 4)), "r"(h[4]), "r"(h[5]), "r"(h[6]), "r"(h[7]) : "memory");
+                    }
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive((which ? bar_vfull : bar_kfull) + 8u * (uint32_t)(t & 1));
+                }
+                if (failed) break;
+                if (lane == 0) mbar_arrive(bar_rawfree + 8u * stage);
+                if (++stage == kRaw) {
+                    stage = 0;
+                    ++round;
+                }
+            }
+            n += tiles;
+        }
+    }
+    if (failed && lane == 0) q8_flag(a, NOVA_ERR_TIMEOUT);
+    // ---- release the tensor memory (every path of every thread ends here)
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 0) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"((uint32_t)kTmemCols) : "memory");
+}
+
+// Merge of the units that several CTAs worked on: the unit that the place where CTA blockIdx.x + 1 begins falls into, unless an
+// earlier such place falls into it too.  blockIdx.y takes a share of the (32-row, 4-dim) pieces; thread = row.
+__global__ void __launch_bounds__(128) q8_chunk_merge_kernel(Q8Launch a, ChunkShape sh, int grid_split) {
+    __shared__ ChunkPlan plan;
+    const int lane = (int)threadIdx.x & 31, warp = (int)threadIdx.x >> 5;
+    const int G = a.n_heads / a.n_kv_heads;
+    pdl_launch_dependents();
+    build_plan(a, sh, plan, false);       // (positions and row starts: written before the attention kernel, which waited)
+    const long long total = plan.line[a.n_sessions];
+    const int n_ctas = plan_ctas(total, grid_split), c1 = (int)blockIdx.x + 1;
+    auto begin = [&](int c) -> long long { return (long long)c * total / n_ctas; };
+    Unit u = {};
+    int tile, count, c_end = 0;
+    bool todo = c1 < n_ctas;
+    if (todo) {
+        u = find_unit(a, sh, plan, begin(c1));
+        todo = begin(c1) != u.begin && begin(c1 - 1) <= u.begin;        // a seam of this unit, and its first
+        for (c_end = c1; c_end < n_ctas && begin(c_end) < u.end; ++c_end) {}      // contributors c1 - 1 .. c_end - 1
+        // (one of two contributors may have got nothing but the set-up weight)
+        unit_part(u, begin(c1 - 1), begin(c1), tile, count);
+        if (count == u.tiles) todo = false;
+        unit_part(u, begin(c1), begin(c1 + 1), tile, count);
+        if (c_end == c1 + 1 && count == u.tiles) todo = false;
+    }
+    pdl_wait();                            // by every CTA: this grid must not be done before the one that it follows
+    if (!todo) return;
+    const size_t slot_floats = (size_t)sh.rows_cap * kSlotW;
+    const int rows = u.t_cnt * G, blocks = (rows + 31) / 32;
+    for (int piece = (int)blockIdx.y * 4 + warp; piece < blocks * 32; piece += (int)gridDim.y * 4) {
+        const int row = (piece >> 5) * 32 + lane, d4 = piece & 31;
+        if (row >= rows) continue;
+        float M = -INFINITY, L = 0.f;
+        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int c = c1 - 1; c < c_end; ++c) {
+            unit_part(u, begin(c), begin(c + 1), tile, count);
+            if (count == 0) continue;
+            const float* slot = a.part + (size_t)(2 * c + (u.begin > begin(c) ? 1 : 0)) * slot_floats;
+            const float2 ml = __ldcg(reinterpret_cast<const float2*>(slot + 2 * row));
+            const float4 x = __ldcg(reinterpret_cast<const float4*>(slot + 4 * (size_t)sh.rows_cap + ((size_t)d4 * sh.rows_cap + row) * 4));
+            if (!(ml.y > 0.f)) continue;
+            const float mn = fmaxf(M, ml.x), cm = M == -INFINITY ? 0.f : ex2(M - mn), cx = ex2(ml.x - mn);
+            M = mn;
+            L = L * cm + ml.y * cx;
+            acc = make_float4(acc.x * cm + x.x * cx, acc.y * cm + x.y * cx, acc.z * cm + x.z * cx, acc.w * cm + x.w * cx);
+        }
+        const int tk = row / G, g = row - tk * G;
+        if (a.rope_cs && u.past + u.t0 + tk >= a.rope_rows) continue;
+        const float inv = L > 0.f ? 1.f / L : 0.f;
+        q8_store4(a.out, ((int64_t)plan.first[u.s] + u.t0 + tk) * a.out_stride + (int64_t)(u.kvh * G + g) * kHeadDim + 4 * d4, a.io,
+                  make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv));
+    }
+}
+
+ChunkShape chunk_shape(int n_heads, int n_kv_heads, int max_tokens) {
+    ChunkShape sh;
+    const int G = n_heads / n_kv_heads;
+    const int64_t most = (int64_t)max_tokens * G;                       // rows of the longest chunk
+    sh.halves = most <= kHalfRows ? 1 : 2;
+    sh.tq = kHalfRows * sh.halves / G;
+    sh.rows_cap = most < kHalfRows * sh.halves ? (int)((most + 31) / 32 * 32) : kHalfRows * sh.halves;
+    return sh;
+}
+
+}  // namespace
+
+size_t q8_chunk_work_bytes(int n_heads, int n_kv_heads, int max_tokens) {
+    return (size_t)2 * kMaxSms * chunk_shape(n_heads, n_kv_heads, max_tokens).rows_cap * kSlotW * sizeof(float);
+}
+
+int launch_q8_chunk(const Q8Launch& a, cudaStream_t s) {
+    alignas(64) CUtensorMap tmk, tmv;
+    const int64_t slot_rows = ((int64_t)(a.layer + 1) * a.nb) << a.kv_shift;
+    const int box = a.kv_shift == 3 ? 8 : 16;
+    int rc = attn_make_tmap(&tmk, a.pool_k, slot_rows, a.n_kv_heads, 1, box, 1);
+    if (rc == NOVA_OK) rc = attn_make_tmap(&tmv, a.pool_v, slot_rows, a.n_kv_heads, 1, box, 1);
+    if (rc != NOVA_OK) return rc;
+    const ChunkShape sh = chunk_shape(a.n_heads, a.n_kv_heads, a.max_tokens);
+    int ctas = sm_count();
+    if (ctas > kMaxSms) ctas = kMaxSms;
+    const size_t io_bytes = a.io == NOVA_IO_F32 ? 4 : 2;
+    for (int s0 = 0; s0 < a.n_sessions; s0 += kMaxSessions) {           // (the plan's size)
+        Q8Launch b = a;
+        b.n_sessions = a.n_sessions - s0 < kMaxSessions ? a.n_sessions - s0 : kMaxSessions;
+        b.n_past = a.n_past + s0;
+        if (a.slice_ids) b.slice_ids = a.slice_ids + s0;
+        else b.tables = a.tables + (int64_t)s0 * a.table_stride;
+        if (a.tok_start) {
+            b.tok_start = a.tok_start + s0;
+        } else {
+            const int64_t rows = (int64_t)s0 * a.uniform_tokens;
+            b.q = static_cast<const unsigned char*>(a.q) + rows * a.q_stride * (int64_t)io_bytes;
+            b.out = static_cast<unsigned char*>(a.out) + rows * a.out_stride * (int64_t)io_bytes;
+        }
+        auto* kernel = a.fmt == NOVA_KV_I8 ? q8_chunk_kernel<NOVA_KV_I8> : q8_chunk_kernel<NOVA_KV_E4M3>;
+        NOVA_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem));
+        cudaError_t e = launch_kernel_pdl(kernel, dim3((unsigned)ctas), dim3(kThreads), (size_t)kSmem, s, true, b, tmk, tmv, sh);
+        if (e == cudaSuccess) {
+            count_launch();
+            e = launch_kernel_pdl(q8_chunk_merge_kernel, dim3((unsigned)ctas - 1, 4u), dim3(128), 0, s, true, b, sh, ctas);
+        }
+        if (e != cudaSuccess) {
+            set_cuda_error(e, "8-bit chunk attention launch");
+            return NOVA_ERR_CUDA;
+        }
+        NOVA_LAUNCH_CHECK();
+    }
+    return NOVA_OK;
+}
+
+}  // namespace novab

@@ -8,7 +8,7 @@
 #include <cuda_bf16.h>
 #include <cuda_fp8.h>
 
-#include "common.cuh"
+#include "mma_common.cuh"
 
 namespace novab {
 
@@ -17,6 +17,11 @@ constexpr float kQ8MinAmax = 8.6736173798840355e-19f;      // 2^-60
 // ... and attention takes a scale of V to be at least this, so that its logarithm and reciprocal are finite for pages
 // that were never written (zeroed scales).  Codes up to 448 times it are below 1e-18.
 constexpr float kQ8MinScale = 8.4703294725430034e-22f;     // 2^-70
+
+// The softmax reference of a row moves only when a score outgrows it by more than kQ8Step (log2 units), so accumulators are
+// rescaled rarely; weights are 2^kQ8Top times 2^(x - ref).  The largest is then 2^11 .. 2^15, inside fp16, and a weight
+// keeps fp16's 11 bits down to 2^-25 of the reference (below: steps of 2^-35 of it).
+constexpr float kQ8Step = 4.f, kQ8Top = 11.f;
 
 struct Q8Launch {
     void* pool_k;
@@ -187,12 +192,76 @@ __device__ __forceinline__ float4 q8_rotate(float4 x, int64_t pos, int lane, con
                        __fmaf_rn(x.z, c.y, -__fmul_rn(x.w, s.y)), __fmaf_rn(x.z, s.y, __fmul_rn(x.w, c.y)));
 }
 
+// ---- arithmetic and shared-memory access of the attention kernels
+__device__ __forceinline__ float lg2(float x) {
+    float y;
+    asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ float rcp(float x) {
+    float y;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// Four codes of a word -> two pairs of fp16, exactly.
+template <int kFmt> __device__ __forceinline__ void q8_to_h2(uint32_t w, uint32_t& h0, uint32_t& h1) {
+    if constexpr (kFmt == NOVA_KV_I8) {
+        // 0x6400 | (code + 128) is the fp16 number 1024 + 128 + code
+        const uint32_t u = w ^ 0x80808080u;
+        const uint32_t a = __byte_perm(u, 0x64646464u, 0x4140), b = __byte_perm(u, 0x64646464u, 0x4342);
+        const __half2 k = __halves2half2(__ushort_as_half(0x6480), __ushort_as_half(0x6480));      // 1152
+        const __half2 x = __hsub2(*reinterpret_cast<const __half2*>(&a), k), y = __hsub2(*reinterpret_cast<const __half2*>(&b), k);
+        h0 = *reinterpret_cast<const uint32_t*>(&x);
+        h1 = *reinterpret_cast<const uint32_t*>(&y);
+    } else {
+        asm("{ .reg .b16 l, h; mov.b32 {l, h}, %2; cvt.rn.f16x2.e4m3x2 %0, l; cvt.rn.f16x2.e4m3x2 %1, h; }" : "=r"(h0), "=r"(h1) : "r"(w));
+    }
+}
+
+// The same for K: int8 codes as (code + 128) 2^-24, an fp16 subnormal whose bits are the byte.
+template <int kFmt> __device__ __forceinline__ void q8_k_to_h2(uint32_t w, uint32_t& h0, uint32_t& h1) {
+    if constexpr (kFmt == NOVA_KV_I8) {
+        const uint32_t u = w ^ 0x80808080u;
+        h0 = __byte_perm(u, 0u, 0x4140);
+        h1 = __byte_perm(u, 0u, 0x4342);
+    } else {
+        q8_to_h2<kFmt>(w, h0, h1);
+    }
+}
+
+__device__ __forceinline__ uint4 lds128(uint32_t addr) {
+    uint4 v;
+    asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr));
+    return v;
+}
+__device__ __forceinline__ float lds_f1(uint32_t addr) {
+    float v;
+    asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(addr));
+    return v;
+}
+__device__ __forceinline__ void sts_f1(uint32_t addr, float v) { asm volatile("st.shared.f32 [%0], %1;" ::"r"(addr), "f"(v) : "memory"); }
+__device__ __forceinline__ void sts128(uint32_t addr, float4 v) {
+    asm volatile("st.shared.v4.f32 [%0], {%1,%2,%3,%4};" ::"r"(addr), "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w) : "memory");
+}
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+// Transpose of an 8 x 8 matrix of 16-bit values over the warp (lane 4 r + c holds row r, columns 2c and 2c + 1).
+__device__ __forceinline__ uint32_t movmatrix(uint32_t x) {
+    uint32_t y;
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
+}
+
 #endif  // __CUDACC__
 
-// q8_cache.cu / q8_attn.cu
+// q8_cache.cu, q8_attn.cu (single tokens), q8_chunk.cu (everything else)
 int launch_q8_append(const Q8Launch& a, cudaStream_t s);
 int launch_q8_read(const Q8Launch& a, cudaStream_t s);
 int launch_q8_attn(const Q8Launch& a, size_t work_bytes, cudaStream_t s);
+int launch_q8_chunk(const Q8Launch& a, cudaStream_t s);
+size_t q8_chunk_work_bytes(int n_heads, int n_kv_heads, int max_tokens);
 size_t q8_work_bytes(int n_heads, int n_kv_heads, int n_sessions, int n_tokens, int max_tokens);
 
 }  // namespace novab

@@ -124,9 +124,10 @@ class Cache:
         return [torch.cat(x).to(IO[self.io]) for x in parts]
 
     def attend(self):
-        """(o, a, spread): the outputs in 64 bits, the sum of weights times |v|, and per row the largest sum of |q k| / sqrt(128)."""
+        """(o, a, spread, floor): the outputs in 64 bits, the sum of weights times |v|, per row the largest sum of |q k| / sqrt(128), and
+        the sum of |codes of v| times the row's largest weight (p times v's scale)."""
         o = torch.zeros(sum(self.new), self.H, HD, dtype=torch.float64)
-        a, spread = o.clone(), torch.zeros(sum(self.new), self.H, dtype=torch.float64)
+        a, spread, floor = o.clone(), torch.zeros(sum(self.new), self.H, dtype=torch.float64), o.clone()
         pos = self.positions()
         q = rotate(self.q, pos, self.cs, self.sn, self.rope).double()
         G, at = self.H // self.N, 0
@@ -144,9 +145,13 @@ class Cache:
                 w = torch.softmax(score.masked_fill(~seen, -math.inf), -1)
                 o[at:at + n, h] = w @ vh
                 a[at:at + n, h] = w @ vh.abs()
+                j = torch.arange(p + n)
+                ph, slot = self.tables[int(self.slices[s])].long()[j // self.page], j % self.page
+                sv = self.scales[1][self.layer][ph, h // G, slot].double()
+                floor[at:at + n, h] = (w * sv).amax(-1, keepdim=True) * (seen.double() @ (vh / sv[:, None]).abs())
                 spread[at:at + n, h] = ((qh.abs() @ kh.abs().T) * HD ** -0.5).masked_fill(~seen, 0).amax(-1)
             at += n
-        return o, a, spread
+        return o, a, spread, floor
 
     # ---- the framework's side
     def device(self, nv, dev="cuda", extra_rows=0, status=True):
@@ -196,17 +201,19 @@ def call(nv, d, what, window=0, stream=None):
                           d["work"].numel(), stream)
 
 
-def attention_bound(case, o, a, spread, exact_q):
+def attention_bound(case, o, a, spread, floor, exact_q):
     """How far an output may be off.
     One step of the sum: weights p = exp(s), so a score off by e takes p off by e (1 + e) and the quotient off by 2 e at most,
     relative to a = sum p |v|.  Scores: q goes to fp16 (2^-11 relative, exact_q: fp16 hi + lo, 2^-21), which moves a score by at most
     that times spread = sum |q k| / sqrt(128); the fp32 accumulation of 128 products by 2^-19 times spread (17 additions rounded or
     truncated to 24 bits), the exponential's argument by 2^-23 of a magnitude below 2 spread.  Weights go to fp16 (2^-11; hi + lo: 2^-21),
-    their sums are rounded once per 16 keys (2^-23 each).  Last the rounding of the output itself, half a step."""
+    their sums are rounded once per 16 keys (2^-23 each).  A weight below fp16's normal range is off by 2^-25 whatever it is, and
+    the largest weight of a row (p times v's scale) goes in as 2^11 or more: floor 2^-36 in all.  Last the rounding of the output
+    itself, half a step."""
     keys = max([p + n for p, n in zip(case.past, case.new)] + [1])
     q_err, p_err = (2.0 ** -21, 2.0 ** -21) if exact_q else (2.0 ** -11, 2.0 ** -11)
     e = spread * (q_err + 2.0 ** -19 + 2.0 ** -22)
     rel = 2 * (e * (1 + e) + p_err) + (keys / 16 + 64) * 2.0 ** -23
     half = {"f32": 2.0 ** -24, "f16": 2.0 ** -11, "bf16": 2.0 ** -8}[case.io]
     tiny = {"f32": 1e-37, "f16": 2.0 ** -25, "bf16": 1e-37}[case.io]
-    return a * rel[..., None] + o.abs() * half + tiny
+    return a * rel[..., None] + floor * 2.0 ** -36 + o.abs() * half + tiny

@@ -39,9 +39,9 @@ def check_out(case, d):
     T = sum(case.new)
     got = d["out"].cpu()
     assert bool((got[T:] == 7).all()), "rows behind the last session"
-    o, a, spread = case.attend()
+    o, a, spread, floor = case.attend()
     exact_q = case.io == "f32" and max(case.new) == 1 and case.H // case.N <= 8        # fp16 hi + lo, by the header's word
-    bound = attention_bound(case, o, a, spread, exact_q)
+    bound = attention_bound(case, o, a, spread, floor, exact_q)
     off = (got[:T].double() - o).abs()
     assert bool(torch.isfinite(got[:T]).all()), "finite"
     assert bool((off <= bound).all()), f"off by {float((off / bound).max()):.3g} of the bound at {divmod(int((off / bound).argmax()), HD)}"
@@ -229,14 +229,14 @@ def test_bad_table_entries_are_skipped_and_flagged(nv):
             case = Cache([40, 60], new, 4, 2, 16, "i8", "f32" if new[0] == 1 else "bf16", poison=False)
             good = Cache([40, 60], new, 4, 2, 16, "i8", case.io, poison=False)
             good.append()
-            o, a, spread = good.attend()
+            o, a, spread, floor = good.attend()
             case.tables[int(case.slices[0]), 1] = entry
             d = case.device(nv)
             call(nv, d, "append_attn")
             torch.cuda.synchronize()
             assert int(d["status"]) == nv.ERR_BAD_TABLE
             rows = slice(new[0], sum(new))
-            bound = attention_bound(case, o, a, spread, new[0] == 1)
+            bound = attention_bound(case, o, a, spread, floor, new[0] == 1)
             assert bool(((d["out"].cpu().double() - o).abs() <= bound)[rows].all())
             # the entry that takes the new row
             case.tables = good.tables.clone()
