@@ -9,13 +9,14 @@
 //     of all units form one line that is dealt out evenly over one CTA per SM, so neither short sessions, nor long ones, nor
 //     the causal triangle leave SMs idle.  Units that several CTAs worked on are merged by the kernel behind it.
 //   * Sixteen warps: 8 softmax (thread = row), 2 issuing MMAs (one per half), 1 copying codes (TMA boxes of 16 slots x 128 B), 1
-//     preparing scales, 4 converting.  The pipe runs on from one unit to the next.
-//   * The tensor cores want fp16 operands, so the codes of a tile are converted in shared memory: exact integers or e4m3 values,
-//     128-byte-swizzle layout, which is the K-major form for S = Q.K^T and the MN-major form for O += P.V.  A lane's rows
-//     are chosen so that neither the reads (rows r and r ^ 5 side by side) nor the writes meet in a bank.
-//   * Scales: x = s * (sk log2 e / sqrt(128)) + log2 sv, packed fp32 pairs, weights w = 2^(x - ref), sum += w / sv (see q8_attn.cu:
-//     weights stay inside fp16 whatever the scales are).  Keys that do not exist get sk = 0, log2 sv = -inf, 1 / sv = 0.
-//   * q is rotated on the way in and rounded to fp16, P is rounded to fp16; everything else is fp32.
+//     copying scales, 4 converting.  The pipe runs on from one unit to the next.
+//   * The tensor cores want fp16 operands, so a tile's codes become fp16 VALUES in shared memory, code times scale, in the
+//     128-byte-swizzle layout that is the K-major form for S = Q.K^T and the MN-major form for O += P.V.  A scale (K's over 16;
+//     q is multiplied by 16 / sqrt(128) log2 e) goes in as two fp16 parts and the product is rounded once (2^-11).
+//     With exact codes as operands and the scales in the softmax instead, every thread had to read three floats per key
+//     from shared memory, which took 1500 cycles of a 64-key tile.  So |K| saturates at 2^20 and |V| at 65504 here.
+//     A lane's rows are chosen so that neither the reads (rows r and r ^ 5 side by side) nor the writes meet in a bank.
+//   * q (rotated) and P are rounded to fp16; everything else is fp32.
 //   * Every wait is bounded; tensor memory is released on every path.
 #include "attn_plan.cuh"
 #include "q8_common.cuh"
@@ -30,15 +31,13 @@ constexpr int kHalfRows = 128;                        // rows of a half = M of t
 constexpr int kSlab = kKeys * 128;                    // 64 rows x 128 B
 constexpr int kQSlab = kHalfRows * 128;
 constexpr int kRaw = 5;                               // tiles of codes in flight (16 KiB each)
-constexpr int kSc = 4;                                // tiles of prepared scales
-constexpr int kScSteps = 8;                           // ring of raw scales
+constexpr int kMasks = 8;                             // ring of "which keys exist", for the softmax
 constexpr int kMaxSessions = 512;                     // sessions of one launch
 constexpr int kOffK = 4 * kQSlab;                     // two fp16 K tiles (dims 0-63 | 64-127), two V tiles
 constexpr int kOffV = kOffK + 2 * 2 * kSlab;
 constexpr int kOffRaw = kOffV + 2 * 2 * kSlab;        // codes: K 8 KiB | V 8 KiB
-constexpr int kOffSc = kOffRaw + kRaw * 2 * kSlab;    // per tile 64 x (K scale | log of V's | reciprocal of V's)
-constexpr int kOffRawSc = kOffSc + kSc * 768;
-constexpr int kOffPlan = kOffRawSc + kScSteps * 512;
+constexpr int kOffSc = kOffRaw + kRaw * 2 * kSlab;    // per tile 64 scales of K, 64 of V
+constexpr int kOffPlan = kOffSc + kRaw * 512;
 struct ChunkPlan {
     long long line[kMaxSessions + 1];                 // where each session's tiles start on the line
     int first[kMaxSessions], count[kMaxSessions], past[kMaxSessions];
@@ -48,6 +47,7 @@ constexpr int kSmem = kOffBar + 512;
 static_assert(kSmem <= 232448, "shared memory of one CTA");
 constexpr int kTmemCols = 512;                        // S of half h, buffer b: columns 128 h + 64 b (P over its first 32); O: 256 + 128 h
 constexpr uint32_t kColO = 256;
+constexpr float kKDiv = 16.f;                         // K goes in divided by this: magnitudes up to 2^20
 constexpr int kSetup = 2;                             // what starting a unit costs, in tiles
 constexpr int kMinTiles = 4;                          // a CTA gets at least that many
 constexpr uint32_t kIdescS = (1u << 4) | ((uint32_t)(kKeys >> 3) << 17) | ((uint32_t)(kHalfRows >> 4) << 24);
@@ -173,18 +173,16 @@ __device__ __forceinline__ unsigned long long pack_f2(float x, float y) {
     return v;
 }
 __device__ __forceinline__ void unpack_f2(unsigned long long v, float& x, float& y) { asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(v)); }
-__device__ __forceinline__ unsigned long long fma_f2(unsigned long long x, unsigned long long y, unsigned long long z) {
-    unsigned long long v;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(v) : "l"(x), "l"(y), "l"(z));
-    return v;
-}
 __device__ __forceinline__ unsigned long long add_f2(unsigned long long x, unsigned long long y) {
     unsigned long long v;
     asm("add.rn.f32x2 %0, %1, %2;" : "=l"(v) : "l"(x), "l"(y));
     return v;
 }
-__device__ __forceinline__ void lds_2x64(uint32_t addr, unsigned long long& x, unsigned long long& y) {
-    asm volatile("ld.shared.v2.b64 {%0, %1}, [%2];" : "=l"(x), "=l"(y) : "r"(addr));
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr), "r"(r[0]), "r"(r[1]),
+                 "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]),
+                 "r"(r[14]), "r"(r[15])
+                 : "memory");
 }
 template <int kRegs> __device__ __forceinline__ void regs_up() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegs)); }
 template <int kRegs> __device__ __forceinline__ void regs_down() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegs)); }
@@ -198,20 +196,20 @@ q8_chunk_kernel(Q8Launch a, const __grid_constant__ CUtensorMap tmk, const __gri
     ChunkPlan& plan = *reinterpret_cast<ChunkPlan*>(smem_raw + kOffPlan);
     uint32_t& s_tmem = *reinterpret_cast<uint32_t*>(smem_raw + kOffBar + 400);
     volatile int& s_abort = *reinterpret_cast<volatile int*>(smem_raw + kOffBar + 404);
-    unsigned long long* const s_rmask = reinterpret_cast<unsigned long long*>(smem_raw + kOffBar + 408);      // [kRaw] which keys of the raw tile exist
+    unsigned long long* const s_rmask = reinterpret_cast<unsigned long long*>(smem_raw + kOffBar + 320);      // [kRaw] which keys of the raw tile exist
+    unsigned long long* const s_mask = reinterpret_cast<unsigned long long*>(smem_raw + kOffBar + 408);       // [kMasks] the same by tile
     const int lane = (int)threadIdx.x & 31;
     const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0);
     const int G = a.n_heads / a.n_kv_heads;
     const uint32_t base = smem_u32(smem_raw);
     const uint32_t bar = base + kOffBar;
     const uint32_t bar_rawfull = bar, bar_rawfree = bar + 40, bar_kfull = bar + 80, bar_kfree = bar + 96, bar_vfull = bar + 112, bar_vfree = bar + 128,
-                   bar_sready = bar + 144 /* [half][buffer] */, bar_pready = bar + 176, bar_pvdone = bar + 208, bar_scfull = bar + 240, bar_scfree = bar + 272,
-                   bar_qready = bar + 304 /* [half] */;
+                   bar_sready = bar + 144 /* [half][buffer] */, bar_pready = bar + 176, bar_pvdone = bar + 208, bar_qready = bar + 240 /* [half] */;
     // Every waiter waits for a phase whose successor on the same barrier needs that waiter's own next action (or one that follows it),
     // so a parity is never taken for a later one.
     if (threadIdx.x == 0) {
         for (int i = 0; i < kRaw; ++i) {
-            mbar_init(bar_rawfull + 8u * i, 1);
+            mbar_init(bar_rawfull + 8u * i, 33);        // codes, and each lane of the scales' warp
             mbar_init(bar_rawfree + 8u * i, 4);
         }
         for (int i = 0; i < 2; ++i) {
@@ -225,10 +223,6 @@ q8_chunk_kernel(Q8Launch a, const __grid_constant__ CUtensorMap tmk, const __gri
             mbar_init(bar_sready + 8u * i, 1);
             mbar_init(bar_pready + 8u * i, kHalfRows);
             mbar_init(bar_pvdone + 8u * i, 1);
-        }
-        for (int i = 0; i < kSc; ++i) {
-            mbar_init(bar_scfull + 8u * i, 1);
-            mbar_init(bar_scfree + 8u * i, 4 * sh.halves);
         }
         s_abort = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -272,7 +266,7 @@ q8_chunk_kernel(Q8Launch a, const __grid_constant__ CUtensorMap tmk, const __gri
             unit_part(u, lo, hi, tile0, tiles);
             pos = u.end;
             if (tiles == 0) continue;
-            // ---- q: rotated, divided by 8 (so that a rotated fp16 value stays inside fp16), fp16, K-major 128-byte swizzle.  The scores of
+            // ---- q: rotated, scaled, fp16, K-major 128-byte swizzle.  The scores of
             // the unit before are all computed (this thread has waited for the last of them), so the operand can be overwritten.
             const int row_pos = u.past + u.t0 + tk;
             const bool in_tile = tk < u.t_cnt, beyond = in_tile && a.rope_cs && row_pos >= a.rope_rows;
@@ -282,6 +276,7 @@ q8_chunk_kernel(Q8Launch a, const __grid_constant__ CUtensorMap tmk, const __gri
             {
                 const int64_t qe = q_row * a.q_stride + (int64_t)(u.kvh * G + g) * kHeadDim;
                 const bool rot = row_ok && a.rope_cs;
+                constexpr float kQ = kAttnScale * kLog2e * kKDiv;
 #pragma unroll 2
                 for (int c = 0; c < 8; ++c) {                  // dims 8c .. 8c+7 and 64 + 8c ..
                     float x[16];
@@ -317,8 +312,8 @@ q8_chunk_kernel(Q8Launch a, const __grid_constant__ CUtensorMap tmk, const __gri
                     for (int hf = 0; hf < 2; ++hf) {
                         const uint32_t dst = base + (uint32_t)((2 * half + hf) * kQSlab + hrow * 128 + ((c ^ (hrow & 7)) << 4));
                         const float* y = x + 8 * hf;
-                        asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(dst), "r"(pack_h2(y[0] * 0.125f, y[1] * 0.125f)),
-                                     "r"(pack_h2(y[2] * 0.125f, y[3] * 0.125f)), "r"(pack_h2(y[4] * 0.125f, y[5] * 0.125f)), "r"(pack_h2(y[6] * 0.125f, y[7] * 0.125f))
+                        asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(dst), "r"(pack_h2(y[0] * kQ, y[1] * kQ)), "r"(pack_h2(y[2] * kQ, y[3] * kQ)),
+                                     "r"(pack_h2(y[4] * kQ, y[5] * kQ)), "r"(pack_h2(y[6] * kQ, y[7] * kQ))
                                      : "memory");
                     }
                 }
@@ -332,40 +327,36 @@ q8_chunk_kernel(Q8Launch a, const __grid_constant__ CUtensorMap tmk, const __gri
 #pragma unroll 1
             for (int i = 0; i < tiles; ++i) {
                 const int t = n + i;
-                const uint32_t sc = base + kOffSc + (uint32_t)(t & (kSc - 1)) * 768u;
-                bool ok = t5_wait(bar_scfull + 8u * (uint32_t)(t & (kSc - 1)), (uint32_t)(t / kSc) & 1u, &s_abort);
-                ok = ok && t5_wait(my_sready + 8u * (uint32_t)(t & 1), (uint32_t)(t >> 1) & 1u, &s_abort);
-                if (!__all_sync(0xffffffffu, ok)) { failed = true; break; }
+                if (!__all_sync(0xffffffffu, t5_wait(my_sready + 8u * (uint32_t)(t & 1), (uint32_t)(t >> 1) & 1u, &s_abort))) { failed = true; break; }
                 tc_fence_after();
-                uint32_t sv[2][32];
-                tmem_ld32(t_lane + col_s + 64u * (uint32_t)(t & 1), sv[0]);
-                tmem_ld32(t_lane + col_s + 64u * (uint32_t)(t & 1) + 32, sv[1]);
-                tmem_wait_ld();
-#pragma unroll
-                for (int c = 0; c < 64; c += 4) {               // scores in log2 units, with the logarithm of V's scale
-                    unsigned long long k0, k1, v0, v1;
-                    lds_2x64(sc + 4 * c, k0, k1);
-                    lds_2x64(sc + 256 + 4 * c, v0, v1);
-                    float y[4];
-                    unpack_f2(fma_f2(pack_f2(__uint_as_float(sv[c >> 5][c & 31]), __uint_as_float(sv[c >> 5][(c + 1) & 31])), k0, v0), y[0], y[1]);
-                    unpack_f2(fma_f2(pack_f2(__uint_as_float(sv[c >> 5][(c + 2) & 31]), __uint_as_float(sv[c >> 5][(c + 3) & 31])), k1, v1), y[2], y[3]);
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) sv[c >> 5][(c + e) & 31] = __float_as_uint(y[e]);
-                }
+                const uint32_t s_col = t_lane + col_s + 64u * (uint32_t)(t & 1);
                 const int key0 = (u.first16 << 4) + (tile0 + i) * kKeys;
                 const int hi_k = row_lim - key0, lo_k = row_lo - key0;       // first and last visible column
+                const unsigned long long there = s_mask[t & (kMasks - 1)];    // (a page missing, or the last key passed)
+                const bool all_seen = __all_sync(0xffffffffu, hi_k >= kKeys - 1 && lo_k <= 0) && there == ~0ull;
+                // Two passes over the scores, 32 columns at a time, both read from tensor memory: half the code and half the registers
+                // of one pass over 64 (with that, instruction fetches were the largest stall: sixteen warps run five loops here).
                 float mx = -INFINITY;
-                if (__all_sync(0xffffffffu, hi_k >= kKeys - 1 && lo_k <= 0)) {
+#pragma unroll 1
+                for (int hf = 0; hf < 2; ++hf) {
+                    uint32_t sv[32];
+                    tmem_ld32(s_col + 32u * (uint32_t)hf, sv);
+                    tmem_wait_ld();
+                    if (!all_seen) {
+                        const int hk = hi_k - 32 * hf, lk = lo_k - 32 * hf;
+                        uint32_t vis = (uint32_t)(there >> (32 * hf));
+                        if (hk < 31) vis &= hk < 0 ? 0u : (2u << hk) - 1u;
+                        if (lk > 0) vis &= lk > 31 ? 0u : ~((1u << lk) - 1u);
 #pragma unroll
-                    for (int c = 0; c < 64; ++c) mx = fmaxf(mx, __uint_as_float(sv[c >> 5][c & 31]));
-                } else {
-#pragma unroll
-                    for (int c = 0; c < 64; ++c) {
-                        float v = __uint_as_float(sv[c >> 5][c & 31]);
-                        v = (c <= hi_k && c >= lo_k) ? v : -INFINITY;
-                        sv[c >> 5][c & 31] = __float_as_uint(v);
-                        mx = fmaxf(mx, v);
+                        for (int c = 0; c < 32; ++c)
+                            if (!(vis >> c & 1u)) sv[c] = 0xff800000u;          // -inf
+                        tmem_st32(s_col + 32u * (uint32_t)hf, sv);
+                        tmem_wait_st();
                     }
+                    float m4[4] = {mx, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                    for (int c = 0; c < 32; ++c) m4[c & 3] = fmaxf(m4[c & 3], __uint_as_float(sv[c]));
+                    mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
                 }
                 float scale = 1.f;
                 if (mx > m_ref + kQ8Step || (m_ref == -INFINITY && mx > -INFINITY)) {
@@ -374,26 +365,25 @@ q8_chunk_kernel(Q8Launch a, const __grid_constant__ CUtensorMap tmk, const __gri
                 }
                 const float ms = m_ref == -INFINITY ? 0.f : kQ8Top - m_ref;         // nothing visible yet: keep exp arguments finite
                 const unsigned long long ms2 = pack_f2(ms, ms);
-                uint32_t pk[32];
-                unsigned long long sum2 = 0ull;
+                unsigned long long sum2[2] = {0ull, 0ull};
+#pragma unroll 1
+                for (int hf = 0; hf < 2; ++hf) {
+                    uint32_t sv[32], pk[16];
+                    tmem_ld32(s_col + 32u * (uint32_t)hf, sv);
+                    tmem_wait_ld();
 #pragma unroll
-                for (int c = 0; c < 64; c += 4) {
-                    unsigned long long r0, r1;
-                    lds_2x64(sc + 512 + 4 * c, r0, r1);
-                    float y[4];
-                    unpack_f2(add_f2(pack_f2(__uint_as_float(sv[c >> 5][c & 31]), __uint_as_float(sv[c >> 5][(c + 1) & 31])), ms2), y[0], y[1]);
-                    unpack_f2(add_f2(pack_f2(__uint_as_float(sv[c >> 5][(c + 2) & 31]), __uint_as_float(sv[c >> 5][(c + 3) & 31])), ms2), y[2], y[3]);
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) y[e] = ex2(y[e]);
-                    sum2 = fma_f2(pack_f2(y[0], y[1]), r0, sum2);
-                    sum2 = fma_f2(pack_f2(y[2], y[3]), r1, sum2);
-                    pk[c >> 1] = pack_h2(y[0], y[1]);
-                    pk[(c >> 1) + 1] = pack_h2(y[2], y[3]);
+                    for (int c = 0; c < 32; c += 2) {
+                        float y0, y1;
+                        unpack_f2(add_f2(pack_f2(__uint_as_float(sv[c]), __uint_as_float(sv[c + 1])), ms2), y0, y1);
+                        y0 = ex2(y0);
+                        y1 = ex2(y1);
+                        sum2[(c >> 1) & 1] = add_f2(pack_f2(y0, y1), sum2[(c >> 1) & 1]);
+                        pk[c >> 1] = pack_h2(y0, y1);
+                    }
+                    tmem_st16(s_col + 16u * (uint32_t)hf, pk);      // P over scores that have been read
                 }
-                __syncwarp();
-                if (lane == 0) mbar_arrive(bar_scfree + 8u * (uint32_t)(t & (kSc - 1)));
                 float s0, s1;
-                unpack_f2(sum2, s0, s1);
+                unpack_f2(add_f2(sum2[0], sum2[1]), s0, s1);
                 l = fmaf(l, scale, s0 + s1);
                 if (i > 0 && __any_sync(0xffffffffu, scale != 1.f)) {
                     // O is rescaled between two P.V products: the previous one must be done
@@ -410,7 +400,6 @@ q8_chunk_kernel(Q8Launch a, const __grid_constant__ CUtensorMap tmk, const __gri
                     }
                     tmem_wait_st();
                 }
-                tmem_st32(t_lane + col_s + 64u * (uint32_t)(t & 1), pk);
                 tmem_wait_st();
                 tc_fence_before();
                 mbar_arrive(my_pready + 8u * (uint32_t)(t & 1));
@@ -556,11 +545,11 @@ q8_chunk_kernel(Q8Launch a, const __grid_constant__ CUtensorMap tmk, const __gri
                     }
                 }
             } else {
-                // scales: lane = (K or V, four keys); they arrive a few tiles ahead in a ring of the warp's own
-                constexpr int kDepth = kScSteps - 1;
+                // scales: lane = (K or V, four keys), one 16-byte copy per tile; the copies arrive on the tile's barrier by themselves
                 const int quad = lane & 15;
-                const bool is_v = lane >= 16;
-                const uint32_t raw0 = base + kOffRawSc + (uint32_t)lane * 16u;
+                const float* const scales = lane >= 16 ? a.scale_v : a.scale_k;
+                const uint32_t dst0 = base + kOffSc + (uint32_t)lane * 16u;
+                uint32_t stage = 0, round = 0;
                 for (long long pos = lo; pos < hi && !failed;) {
                     const Unit u = find_unit(a, sh, plan, pos);
                     int tile0, tiles;
@@ -568,47 +557,24 @@ q8_chunk_kernel(Q8Launch a, const __grid_constant__ CUtensorMap tmk, const __gri
                     pos = u.end;
                     if (tiles == 0) continue;
                     const int32_t* table = q8_table(a, u.s);
-                    const float* const mine0 = (is_v ? a.scale_v : a.scale_k) + ((((int64_t)a.layer * a.nb) * a.n_kv_heads + u.kvh) << a.kv_shift);
+                    const float* const mine0 = scales + ((((int64_t)a.layer * a.nb) * a.n_kv_heads + u.kvh) << a.kv_shift);
                     const int key_a = (u.first16 << 4) + tile0 * kKeys + 4 * quad;
                     auto get = [&](int i) -> int { return i < tiles ? entry(table, key_a + i * kKeys, u.keys_end) : -2; };
                     int e0 = get(0), e1 = get(1), e2 = get(2);
-                    unsigned have = 0u;                          // bit i: the quad of step i exists (a ring of kScSteps bits would do)
 #pragma unroll 1
-                    for (int step = 0; step < tiles + kDepth; ++step) {
-                        if (step < tiles) {
-                            const int e = e0;
-                            e0 = e1;
-                            e1 = e2;
-                            e2 = get(step + 3);
-                            const uint32_t raw = raw0 + (uint32_t)(step & (kScSteps - 1)) * 512u;
-                            if (e >= 0) cp_async16(raw, mine0 + (((int64_t)e * a.n_kv_heads) << a.kv_shift) + ((key_a + step * kKeys) & slot_mask));
-                            have = (have << 1) | (e >= 0 ? 1u : 0u);
-                        } else {
-                            have <<= 1;
+                    for (int i = 0; i < tiles; ++i) {
+                        const int e = e0;
+                        e0 = e1;
+                        e1 = e2;
+                        e2 = get(i + 3);
+                        if (round > 0 && !__all_sync(0xffffffffu, t5_wait(bar_rawfree + 8u * stage, (round - 1) & 1u, &s_abort))) { failed = true; break; }
+                        if (e >= 0) cp_async16(dst0 + stage * 512u, mine0 + (((int64_t)e * a.n_kv_heads) << a.kv_shift) + ((key_a + i * kKeys) & slot_mask));
+                        asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar_rawfull + 8u * stage) : "memory");
+                        if (++stage == kRaw) {
+                            stage = 0;
+                            ++round;
                         }
-                        asm volatile("cp.async.commit_group;" ::: "memory");
-                        if (step < kDepth) continue;
-                        asm volatile("cp.async.wait_group %0;" ::"n"(kDepth) : "memory");
-                        const int i = step - kDepth, t = n + i, stage = t & (kSc - 1);
-                        if (t >= kSc && !__all_sync(0xffffffffu, t5_wait(bar_scfree + 8u * (uint32_t)stage, (uint32_t)(t / kSc - 1) & 1u, &s_abort))) { failed = true; break; }
-                        const bool there = have >> kDepth & 1u;
-                        const uint4 w = lds128(raw0 + (uint32_t)(i & (kScSteps - 1)) * 512u);
-                        float v[4] = {__uint_as_float(w.x), __uint_as_float(w.y), __uint_as_float(w.z), __uint_as_float(w.w)}, r[4];
-                        const int left = u.keys_end - (key_a + i * kKeys);
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const bool real = there && e < left;
-                            const float f = fmaxf(v[e], kQ8MinScale);
-                            r[e] = real ? rcp(f) : 0.f;
-                            v[e] = is_v ? (real ? lg2(f) : -INFINITY) : (real ? v[e] * (kAttnScale * kLog2e * 8.f) : 0.f);
-                        }
-                        const uint32_t dst = base + kOffSc + (uint32_t)stage * 768u + (uint32_t)(quad * 16) + (is_v ? 256u : 0u);
-                        sts128(dst, make_float4(v[0], v[1], v[2], v[3]));
-                        if (is_v) sts128(dst + 256u, make_float4(r[0], r[1], r[2], r[3]));
-                        __syncwarp();
-                        if (lane == 0) mbar_arrive(bar_scfull + 8u * (uint32_t)stage);
                     }
-                    n += tiles;
                 }
                 asm volatile("cp.async.wait_all;" ::: "memory");
             }
@@ -633,29 +599,50 @@ q8_chunk_kernel(Q8Launch a, const __grid_constant__ CUtensorMap tmk, const __gri
                 ok = ok && (t < 2 || t5_wait(bar_kfree + 8u * (uint32_t)(t & 1), (uint32_t)(t / 2 - 1) & 1u, &s_abort));
                 if (!__all_sync(0xffffffffu, ok)) { failed = true; break; }
                 const unsigned long long mask = s_rmask[stage];
-                const uint32_t raw = base + kOffRaw + stage * (2 * kSlab);
-#pragma unroll
+                if (w == 0 && lane == 0) s_mask[t & (kMasks - 1)] = mask;
+                const uint32_t raw = base + kOffRaw + stage * (2 * kSlab), sc = base + kOffSc + stage * 512u;
+#pragma unroll 1
                 for (int which = 0; which < 2; ++which) {
                     if (which && t >= 2 && !__all_sync(0xffffffffu, t5_wait(bar_vfree + 8u * (uint32_t)(t & 1), (uint32_t)(t / 2 - 1) & 1u, &s_abort))) { failed = true; break; }
                     const uint32_t src = raw + (uint32_t)(which * kSlab), dst = base + (which ? kOffV : kOffK) + (uint32_t)(t & 1) * (2 * kSlab);
                     uint4 code[4];
+                    float scale[2];
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {                      // rows 16 w + 8 (e >> 1) + r8, dims of slab e & 1
                         const uint32_t r = (uint32_t)(16 * w + 8 * (e >> 1) + r8), c = (uint32_t)(4 * (e & 1) + c4);
                         code[e] = lds128(src + r * 128u + ((c ^ (r & 7u)) << 4));
-                        // e4m3: what is not there may read as NaN, which no weight of 0 would hide
-                        if (kFmt == NOVA_KV_E4M3 && !(mask >> r & 1ull)) code[e] = make_uint4(0u, 0u, 0u, 0u);
+                        if ((e & 1) == 0) scale[e >> 1] = lds_f1(sc + (uint32_t)(which * 256) + r * 4u);
+                    }
+                    if (mask != ~0ull) {                               // what does not exist may hold anything: zeros instead
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            if (!(mask >> (16 * w + 8 * (e >> 1) + r8) & 1ull)) {
+                                code[e] = make_uint4(0u, 0u, 0u, 0u);
+                                scale[e >> 1] = 0.f;
+                            }
                     }
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const uint32_t r = (uint32_t)(16 * w + 8 * (e >> 1) + r8), d = dst + (uint32_t)((e & 1) * kSlab) + r * 128u;
-                        uint32_t h[8];
-                        q8_to_h2<kFmt>(code[e].x, h[0], h[1]);
-                        q8_to_h2<kFmt>(code[e].y, h[2], h[3]);
-                        q8_to_h2<kFmt>(code[e].z, h[4], h[5]);
-                        q8_to_h2<kFmt>(code[e].w, h[6], h[7]);
-                        asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(d + (((uint32_t)(2 * c4) ^ (r & 7u)) << 4)), "r"(h[0]), "r"(h[1]), "r"(h[2]), "r"(h[3]) : "memory");
-                        asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(d + (((uint32_t)(2 * c4 + 1) ^ (r & 7u)) << 4)), "r"(h[4]), "r"(h[5]), "r"(h[6]), "r"(h[7]) : "memory");
+                    for (int e2 = 0; e2 < 2; ++e2) {
+                        const float f = fminf(which ? scale[e2] : scale[e2] * (1.f / kKDiv), 65504.f / q8_qmax<kFmt>());
+                        const __half hi1 = __float2half_rn(f);
+                        const __half2 hi2 = __half2half2(hi1), lo2 = __half2half2(__float2half_rn(f - __half2float(hi1)));
+#pragma unroll
+                        for (int e = 2 * e2; e < 2 * e2 + 2; ++e) {
+                            const uint32_t r = (uint32_t)(16 * w + 8 * e2 + r8), d = dst + (uint32_t)((e & 1) * kSlab) + r * 128u;
+                            uint32_t h[8];
+                            q8_to_h2<kFmt>(code[e].x, h[0], h[1]);
+                            q8_to_h2<kFmt>(code[e].y, h[2], h[3]);
+                            q8_to_h2<kFmt>(code[e].z, h[4], h[5]);
+                            q8_to_h2<kFmt>(code[e].w, h[6], h[7]);
+#pragma unroll
+                            for (int b = 0; b < 8; ++b) {
+                                const __half2 x = *reinterpret_cast<const __half2*>(&h[b]);
+                                const __half2 y = __hfma2(x, hi2, __hmul2(x, lo2));
+                                h[b] = *reinterpret_cast<const uint32_t*>(&y);
+                            }
+                            asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(d + (((uint32_t)(2 * c4) ^ (r & 7u)) << 4)), "r"(h[0]), "r"(h[1]), "r"(h[2]), "r"(h[3]) : "memory");
+                            asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(d + (((uint32_t)(2 * c4 + 1) ^ (r & 7u)) << 4)), "r"(h[4]), "r"(h[5]), "r"(h[6]), "r"(h[7]) : "memory");
+                        }
                     }
                     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                     __syncwarp();

@@ -204,16 +204,20 @@ def call(nv, d, what, window=0, stream=None):
 def attention_bound(case, o, a, spread, floor, exact_q):
     """How far an output may be off.
     One step of the sum: weights p = exp(s), so a score off by e takes p off by e (1 + e) and the quotient off by 2 e at most,
-    relative to a = sum p |v|.  Scores: q goes to fp16 (2^-11 relative, exact_q: fp16 hi + lo, 2^-21), which moves a score by at most
-    that times spread = sum |q k| / sqrt(128); the fp32 accumulation of 128 products by 2^-19 times spread (17 additions rounded or
+    relative to a = sum p |v|.  Scores: q goes to fp16 (2^-11 relative, exact_q: fp16 hi + lo, 2^-21), in chunks K too (2^-11 for the
+    product, 2^-14 for a scale whose second part is subnormal), which moves a score by at most that times spread = sum |q k| / sqrt(128); the fp32 accumulation of 128 products by 2^-19 times spread (17 additions rounded or
     truncated to 24 bits), the exponential's argument by 2^-23 of a magnitude below 2 spread.  Weights go to fp16 (2^-11; hi + lo: 2^-21),
+    in chunks V too (2^-11 for its scale, 2^-11 for the product; below fp16's normal range 2^-25),
     their sums are rounded once per 16 keys (2^-23 each).  A weight below fp16's normal range is off by 2^-25 whatever it is, and
     the largest weight of a row (p times v's scale) goes in as 2^11 or more: floor 2^-36 in all.  Last the rounding of the output
     itself, half a step."""
     keys = max([p + n for p, n in zip(case.past, case.new)] + [1])
+    chunk = max(case.new) > 1 or case.H // case.N > 8
     q_err, p_err = (2.0 ** -21, 2.0 ** -21) if exact_q else (2.0 ** -11, 2.0 ** -11)
+    if chunk:
+        q_err, p_err = q_err + 2.0 ** -11 + 2.0 ** -14, p_err + 2 * 2.0 ** -11
     e = spread * (q_err + 2.0 ** -19 + 2.0 ** -22)
     rel = 2 * (e * (1 + e) + p_err) + (keys / 16 + 64) * 2.0 ** -23
     half = {"f32": 2.0 ** -24, "f16": 2.0 ** -11, "bf16": 2.0 ** -8}[case.io]
     tiny = {"f32": 1e-37, "f16": 2.0 ** -25, "bf16": 1e-37}[case.io]
-    return a * rel[..., None] + floor * 2.0 ** -36 + o.abs() * half + tiny
+    return a * rel[..., None] + floor * 2.0 ** -36 + o.abs() * half + tiny + (2.0 ** -25 if chunk else 0.0)
