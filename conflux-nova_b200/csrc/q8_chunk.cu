@@ -5,11 +5,11 @@
 // exponentials (4 * 128 flops and one exponential per (query head, key)).
 //
 //   * tcgen05 with accumulators in tensor memory.  The (token, head) pairs that share a kv head are the rows of a tile: one
-//     half of 128 rows, or two that share every K/V tile.  A unit of work is (session, kv head, tile of tokens); the 64-key tiles
+//     half of 128 rows (held twice, for alternate tiles), or two halves that share every K/V tile.  A unit of work is (session, kv head, tile of tokens); the 64-key tiles
 //     of all units form one line that is dealt out evenly over one CTA per SM, so neither short sessions, nor long ones, nor
 //     the causal triangle leave SMs idle.  Units that several CTAs worked on are merged by the kernel behind it.
-//   * Sixteen warps: 8 softmax (thread = row), 2 issuing MMAs (one per half), 1 copying codes (TMA boxes of 16 slots x 128 B), 1
-//     copying scales, 4 converting.  The pipe runs on from one unit to the next.
+//   * Twenty warps: 8 softmax (thread = row), 2 issuing MMAs (one per half), 1 copying codes (TMA boxes of 16 slots x 128 B), 1
+//     copying scales, 8 converting.  The pipe runs on from one unit to the next.
 //   * The tensor cores want fp16 operands, so a tile's codes become fp16 VALUES in shared memory, code times scale, in the
 //     128-byte-swizzle layout that is the K-major form for S = Q.K^T and the MN-major form for O += P.V.  A scale (K's over 16;
 //     q is multiplied by 16 / sqrt(128) log2 e) goes in as two fp16 parts and the product is rounded once (2^-11).
@@ -25,7 +25,8 @@
 namespace novab {
 namespace {
 
-constexpr int kThreads = 512;
+constexpr int kThreads = 640;
+constexpr int kConv = 8;                              // converting warps
 constexpr int kKeys = 64;                             // keys of a tile
 constexpr int kHalfRows = 128;                        // rows of a half = M of the MMAs
 constexpr int kSlab = kKeys * 128;                    // 64 rows x 128 B
@@ -37,7 +38,8 @@ constexpr int kOffK = 4 * kQSlab;                     // two fp16 K tiles (dims 
 constexpr int kOffV = kOffK + 2 * 2 * kSlab;
 constexpr int kOffRaw = kOffV + 2 * 2 * kSlab;        // codes: K 8 KiB | V 8 KiB
 constexpr int kOffSc = kOffRaw + kRaw * 2 * kSlab;    // per tile 64 scales of K, 64 of V
-constexpr int kOffPlan = kOffSc + kRaw * 512;
+constexpr int kOffX = kOffSc + kRaw * 512;            // (m, l) of the second half's rows on their way to the first
+constexpr int kOffPlan = kOffX + kHalfRows * 8;
 struct ChunkPlan {
     long long line[kMaxSessions + 1];                 // where each session's tiles start on the line
     int first[kMaxSessions], count[kMaxSessions], past[kMaxSessions];
@@ -55,7 +57,8 @@ constexpr uint32_t kIdescPV = (1u << 4) | (1u << 16) | ((uint32_t)(kHeadDim >> 3
 
 struct ChunkShape {
     int tq;              // tokens of a tile
-    int halves;          // 1 or 2
+    int dual;            // 0: the tile's rows are two halves that share every K/V tile; 1: at most 128 rows, both halves hold them
+                         // and take every other K/V tile (few rows leave one half's softmax as the slowest step otherwise)
     int rows_cap;        // rows of a partial slot
 };
 
@@ -204,19 +207,20 @@ q8_chunk_kernel(Q8Launch a, const __grid_constant__ CUtensorMap tmk, const __gri
     const uint32_t base = smem_u32(smem_raw);
     const uint32_t bar = base + kOffBar;
     const uint32_t bar_rawfull = bar, bar_rawfree = bar + 40, bar_kfull = bar + 80, bar_kfree = bar + 96, bar_vfull = bar + 112, bar_vfree = bar + 128,
-                   bar_sready = bar + 144 /* [half][buffer] */, bar_pready = bar + 176, bar_pvdone = bar + 208, bar_qready = bar + 240 /* [half] */;
+                   bar_sready = bar + 144 /* [half][buffer] */, bar_pready = bar + 176, bar_pvdone = bar + 208, bar_qready = bar + 240 /* [half] */,
+                   bar_xfull = bar + 256, bar_xfree = bar + 264;
     // Every waiter waits for a phase whose successor on the same barrier needs that waiter's own next action (or one that follows it),
     // so a parity is never taken for a later one.
     if (threadIdx.x == 0) {
         for (int i = 0; i < kRaw; ++i) {
             mbar_init(bar_rawfull + 8u * i, 33);        // codes, and each lane of the scales' warp
-            mbar_init(bar_rawfree + 8u * i, 4);
+            mbar_init(bar_rawfree + 8u * i, kConv);
         }
         for (int i = 0; i < 2; ++i) {
-            mbar_init(bar_kfull + 8u * i, 4);
-            mbar_init(bar_kfree + 8u * i, sh.halves);
-            mbar_init(bar_vfull + 8u * i, 4);
-            mbar_init(bar_vfree + 8u * i, sh.halves);
+            mbar_init(bar_kfull + 8u * i, kConv);
+            mbar_init(bar_kfree + 8u * i, sh.dual ? 1 : 2);
+            mbar_init(bar_vfull + 8u * i, kConv);
+            mbar_init(bar_vfree + 8u * i, sh.dual ? 1 : 2);
             mbar_init(bar_qready + 8u * i, kHalfRows);
         }
         for (int i = 0; i < 4; ++i) {
@@ -224,6 +228,8 @@ q8_chunk_kernel(Q8Launch a, const __grid_constant__ CUtensorMap tmk, const __gri
             mbar_init(bar_pready + 8u * i, kHalfRows);
             mbar_init(bar_pvdone + 8u * i, 1);
         }
+        mbar_init(bar_xfull, kHalfRows);
+        mbar_init(bar_xfree, kHalfRows);
         s_abort = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("prefetch.tensormap [%0];" ::"l"(&tmk) : "memory");
@@ -254,82 +260,95 @@ q8_chunk_kernel(Q8Launch a, const __grid_constant__ CUtensorMap tmk, const __gri
 
     if (warp < 8) {
         // ---------------------------------------------------------------------------------------- softmax: thread = one row
-        regs_up<168>();
+        regs_up<120>();
         const int half = warp >> 2, hrow = (int)threadIdx.x & (kHalfRows - 1);
         const uint32_t t_lane = tmem + ((uint32_t)(32 * (warp & 3)) << 16);
         const uint32_t col_s = 128u * (uint32_t)half, col_o = kColO + 128u * (uint32_t)half;
         const uint32_t my_sready = bar_sready + 16u * (uint32_t)half, my_pready = bar_pready + 16u * (uint32_t)half, my_pvdone = bar_pvdone + 16u * (uint32_t)half;
-        const int row = half * kHalfRows + hrow, tk = row / G, g = row - tk * G;
-        for (long long pos = lo; pos < hi && !failed && half < sh.halves;) {
+        const int row0 = sh.dual ? 0 : half * kHalfRows, row = row0 + hrow, tk = row / G, g = row - tk * G;
+        uint32_t xround = 0;
+        for (long long pos = lo; pos < hi && !failed;) {
             const Unit u = find_unit(a, sh, plan, pos);
             int tile0, tiles;
             unit_part(u, lo, hi, tile0, tiles);
             pos = u.end;
-            if (tiles == 0) continue;
-            // ---- q: rotated, scaled, fp16, K-major 128-byte swizzle.  The scores of
-            // the unit before are all computed (this thread has waited for the last of them), so the operand can be overwritten.
-            const int row_pos = u.past + u.t0 + tk;
-            const bool in_tile = tk < u.t_cnt, beyond = in_tile && a.rope_cs && row_pos >= a.rope_rows;
-            const bool row_ok = in_tile && !beyond;
-            if (beyond && g == 0) q8_flag(a, NOVA_ERR_INVALID);
-            const int64_t q_row = (int64_t)plan.first[u.s] + u.t0 + tk;
+            // this half's tiles of the unit: every tile, or those whose place on the CTA's line is even (odd)
+            const int mine0 = sh.dual ? (half + n) & 1 : 0, step = sh.dual ? 2 : 1;
+            if (mine0 >= tiles) {
+                n += tiles;
+                continue;
+            }
+            const int64_t tok0 = (int64_t)plan.first[u.s] + u.t0;
             {
-                const int64_t qe = q_row * a.q_stride + (int64_t)(u.kvh * G + g) * kHeadDim;
-                const bool rot = row_ok && a.rope_cs;
+                // ---- q: rotated, scaled, fp16, K-major 128-byte swizzle; eight lanes a row, dims 8c .. and 64 + 8c .. each.  The scores
+                // of the unit before are all computed (this thread has waited for the last of them), so the operand can be overwritten.
                 constexpr float kQ = kAttnScale * kLog2e * kKDiv;
+                const int c = lane & 7;
 #pragma unroll 2
-                for (int c = 0; c < 8; ++c) {                  // dims 8c .. 8c+7 and 64 + 8c ..
+                for (int e8 = 0; e8 < 8; ++e8) {
+                    const int r = 32 * (warp & 3) + 4 * e8 + (lane >> 3), rt = (row0 + r) / G, rg = row0 + r - rt * G;
+                    const int rpos = u.past + u.t0 + rt;
                     float x[16];
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const float4 v = row_ok ? q8_load4(a.q, qe + (e >> 1) * 64 + 8 * c + 4 * (e & 1), a.io) : make_float4(0.f, 0.f, 0.f, 0.f);
-                        x[4 * e] = v.x;
-                        x[4 * e + 1] = v.y;
-                        x[4 * e + 2] = v.z;
-                        x[4 * e + 3] = v.w;
-                    }
-                    if (rot && a.neox) {
-                        const float* cr = a.rope_cs + (int64_t)row_pos * 64 + 8 * c;
-                        const float* sr = a.rope_sn + (int64_t)row_pos * 64 + 8 * c;
+                    for (int e = 0; e < 16; ++e) x[e] = 0.f;
+                    if (rt < u.t_cnt && !(a.rope_cs && rpos >= a.rope_rows)) {
+                        const int64_t qe = (tok0 + rt) * a.q_stride + (int64_t)(u.kvh * G + rg) * kHeadDim + 8 * c;
 #pragma unroll
-                        for (int e = 0; e < 8; ++e) {
-                            const float cc = __ldg(cr + e), sn = __ldg(sr + e), x0 = x[e], x1 = x[8 + e];
-                            x[e] = __fmaf_rn(x0, cc, -__fmul_rn(x1, sn));
-                            x[8 + e] = __fmaf_rn(x0, sn, __fmul_rn(x1, cc));
+                        for (int e = 0; e < 4; ++e) {
+                            const float4 v = q8_load4(a.q, qe + (e >> 1) * 64 + 4 * (e & 1), a.io);
+                            x[4 * e] = v.x;
+                            x[4 * e + 1] = v.y;
+                            x[4 * e + 2] = v.z;
+                            x[4 * e + 3] = v.w;
                         }
-                    } else if (rot) {
+                        if (a.rope_cs) {
+                            const float* cr = a.rope_cs + (int64_t)rpos * 64 + (a.neox ? 8 : 4) * c;
+                            const float* sr = a.rope_sn + (int64_t)rpos * 64 + (a.neox ? 8 : 4) * c;
+                            const int second = a.neox ? 4 : 32;        // neox: the pairs (d, d + 64); else neighbours, in both halves of the dims
+                            const float4 c0 = *reinterpret_cast<const float4*>(cr), c1 = *reinterpret_cast<const float4*>(cr + second);
+                            const float4 s0 = *reinterpret_cast<const float4*>(sr), s1 = *reinterpret_cast<const float4*>(sr + second);
+                            const float cc[8] = {c0.x, c0.y, c0.z, c0.w, c1.x, c1.y, c1.z, c1.w}, ss[8] = {s0.x, s0.y, s0.z, s0.w, s1.x, s1.y, s1.z, s1.w};
 #pragma unroll
-                        for (int hf = 0; hf < 2; ++hf)
-#pragma unroll
-                            for (int e = 0; e < 4; ++e) {
-                                const int64_t i = (int64_t)row_pos * 64 + 32 * hf + 4 * c + e;
-                                const float cc = __ldg(a.rope_cs + i), sn = __ldg(a.rope_sn + i), x0 = x[8 * hf + 2 * e], x1 = x[8 * hf + 2 * e + 1];
-                                x[8 * hf + 2 * e] = __fmaf_rn(x0, cc, -__fmul_rn(x1, sn));
-                                x[8 * hf + 2 * e + 1] = __fmaf_rn(x0, sn, __fmul_rn(x1, cc));
+                            for (int e = 0; e < 8; ++e) {
+                                const float x0 = a.neox ? x[e] : x[2 * e], x1 = a.neox ? x[e + 8] : x[2 * e + 1];
+                                const float y0 = __fmaf_rn(x0, cc[e], -__fmul_rn(x1, ss[e])), y1 = __fmaf_rn(x0, ss[e], __fmul_rn(x1, cc[e]));
+                                if (a.neox) {
+                                    x[e] = y0;
+                                    x[e + 8] = y1;
+                                } else {
+                                    x[2 * e] = y0;
+                                    x[2 * e + 1] = y1;
+                                }
                             }
+                        }
                     }
 #pragma unroll
                     for (int hf = 0; hf < 2; ++hf) {
-                        const uint32_t dst = base + (uint32_t)((2 * half + hf) * kQSlab + hrow * 128 + ((c ^ (hrow & 7)) << 4));
+                        const uint32_t dst = base + (uint32_t)((2 * half + hf) * kQSlab + r * 128 + ((c ^ (r & 7)) << 4));
                         const float* y = x + 8 * hf;
                         asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(dst), "r"(pack_h2(y[0] * kQ, y[1] * kQ)), "r"(pack_h2(y[2] * kQ, y[3] * kQ)),
                                      "r"(pack_h2(y[4] * kQ, y[5] * kQ)), "r"(pack_h2(y[6] * kQ, y[7] * kQ))
                                      : "memory");
                     }
                 }
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                mbar_arrive(bar_qready + 8u * (uint32_t)half);
             }
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            mbar_arrive(bar_qready + 8u * (uint32_t)half);
+            const int row_pos = u.past + u.t0 + tk;
+            const bool in_tile = tk < u.t_cnt, beyond = in_tile && a.rope_cs && row_pos >= a.rope_rows;
+            const bool row_ok = in_tile && !beyond;
+            if (beyond && g == 0) q8_flag(a, NOVA_ERR_INVALID);
             // rows that are nobody's see everything: they never slow a warp down, and nothing of them is written
             const int row_lim = row_ok ? row_pos : 0x7fffffff;
             const int row_lo = row_ok && a.window > 0 ? row_pos - a.window + 1 : 0;
             float m_ref = -INFINITY, l = 0.f;
+            int m = sh.dual ? (n + mine0) >> 1 : n;            // tiles of this half so far: which score buffer, which parity
 #pragma unroll 1
-            for (int i = 0; i < tiles; ++i) {
+            for (int i = mine0; i < tiles; i += step, ++m) {
                 const int t = n + i;
-                if (!__all_sync(0xffffffffu, t5_wait(my_sready + 8u * (uint32_t)(t & 1), (uint32_t)(t >> 1) & 1u, &s_abort))) { failed = true; break; }
+                if (!__all_sync(0xffffffffu, t5_wait(my_sready + 8u * (uint32_t)(m & 1), (uint32_t)(m >> 1) & 1u, &s_abort))) { failed = true; break; }
                 tc_fence_after();
-                const uint32_t s_col = t_lane + col_s + 64u * (uint32_t)(t & 1);
+                const uint32_t s_col = t_lane + col_s + 64u * (uint32_t)(m & 1);
                 const int key0 = (u.first16 << 4) + (tile0 + i) * kKeys;
                 const int hi_k = row_lim - key0, lo_k = row_lo - key0;       // first and last visible column
                 const unsigned long long there = s_mask[t & (kMasks - 1)];    // (a page missing, or the last key passed)
@@ -385,9 +404,9 @@ q8_chunk_kernel(Q8Launch a, const __grid_constant__ CUtensorMap tmk, const __gri
                 float s0, s1;
                 unpack_f2(add_f2(sum2[0], sum2[1]), s0, s1);
                 l = fmaf(l, scale, s0 + s1);
-                if (i > 0 && __any_sync(0xffffffffu, scale != 1.f)) {
+                if (i > mine0 && __any_sync(0xffffffffu, scale != 1.f)) {
                     // O is rescaled between two P.V products: the previous one must be done
-                    if (!__all_sync(0xffffffffu, t5_wait(my_pvdone + 8u * (uint32_t)((t - 1) & 1), (uint32_t)((t - 1) >> 1) & 1u, &s_abort))) { failed = true; break; }
+                    if (!__all_sync(0xffffffffu, t5_wait(my_pvdone + 8u * (uint32_t)((m - 1) & 1), (uint32_t)((m - 1) >> 1) & 1u, &s_abort))) { failed = true; break; }
                     tc_fence_after();
 #pragma unroll 1
                     for (int cc = 0; cc < 4; ++cc) {
@@ -402,46 +421,95 @@ q8_chunk_kernel(Q8Launch a, const __grid_constant__ CUtensorMap tmk, const __gri
                 }
                 tmem_wait_st();
                 tc_fence_before();
-                mbar_arrive(my_pready + 8u * (uint32_t)(t & 1));
+                mbar_arrive(my_pready + 8u * (uint32_t)(m & 1));
             }
             n += tiles;
             if (failed) break;
             // ---- the unit's part is done: outputs, or a partial slot for the merge
-            if (!__all_sync(0xffffffffu, t5_wait(my_pvdone + 8u * (uint32_t)((n - 1) & 1), (uint32_t)((n - 1) >> 1) & 1u, &s_abort))) { failed = true; break; }
+            if (!__all_sync(0xffffffffu, t5_wait(my_pvdone + 8u * (uint32_t)((m - 1) & 1), (uint32_t)((m - 1) >> 1) & 1u, &s_abort))) { failed = true; break; }
             tc_fence_after();
-            const bool whole = tiles == u.tiles;
-            const float inv = whole ? (l > 0.f ? 1.f / l : 0.f) : 1.f;
-            const int64_t oe = q_row * a.out_stride + (int64_t)(u.kvh * G + g) * kHeadDim;
+            const bool whole = tiles == u.tiles, fold = sh.dual && tiles > 1;
+            const uint32_t xbase = base + 2u * kQSlab, xml = base + kOffX;      // (the second half's q is no longer needed)
+            if (fold && half == 1) {
+                // both halves have a share of the rows: the second hands its own over, 64 dims at a time
+                sts_f1(xml + 8u * (uint32_t)hrow, m_ref);
+                sts_f1(xml + 8u * (uint32_t)hrow + 4u, l);
+                for (int part = 0; part < 2 && !failed; ++part) {
+#pragma unroll 1
+                    for (int cc = 0; cc < 2; ++cc) {
+                        uint32_t ov[32];
+                        tmem_ld32(t_lane + col_o + 64u * (uint32_t)part + 32u * (uint32_t)cc, ov);
+                        tmem_wait_ld();
+#pragma unroll
+                        for (int c = 0; c < 32; c += 4)
+                            sts128(xbase + (uint32_t)((8 * cc + (c >> 2)) * kHalfRows + hrow) * 16u,
+                                   make_float4(__uint_as_float(ov[c]), __uint_as_float(ov[c + 1]), __uint_as_float(ov[c + 2]), __uint_as_float(ov[c + 3])));
+                    }
+                    mbar_arrive(bar_xfull);
+                    if (!__all_sync(0xffffffffu, t5_wait(bar_xfree, xround & 1u, &s_abort))) failed = true;
+                    ++xround;
+                }
+                tc_fence_before();
+                continue;
+            }
+            const int64_t oe = (tok0 + tk) * a.out_stride + (int64_t)(u.kvh * G + g) * kHeadDim;
             // slot: (m, l) of every row, then the accumulators, four dims of every row side by side
             float* const slot = a.part + (size_t)(2 * blockIdx.x + (u.begin > lo ? 1 : 0)) * ((size_t)sh.rows_cap * kSlotW);
-            if (!whole && row_ok) *reinterpret_cast<float2*>(slot + 2 * row) = make_float2(m_ref, l);
+            float w0 = 1.f, w1 = 0.f;                 // what this half's and the other half's accumulators are multiplied by
 #pragma unroll 1
             for (int cc = 0; cc < 4; ++cc) {
+                if (fold && (cc & 1) == 0) {
+                    if (!__all_sync(0xffffffffu, t5_wait(bar_xfull, xround & 1u, &s_abort))) { failed = true; break; }
+                    ++xround;
+                }
+                if (cc == 0) {
+                    if (fold) {
+                        const float m1 = lds_f1(xml + 8u * (uint32_t)hrow), l1 = lds_f1(xml + 8u * (uint32_t)hrow + 4u);
+                        const float mm = fmaxf(m_ref, m1);
+                        w0 = m_ref == -INFINITY ? 0.f : ex2(m_ref - mm);
+                        w1 = m1 == -INFINITY ? 0.f : ex2(m1 - mm);
+                        l = l * w0 + l1 * w1;
+                        m_ref = mm;
+                    }
+                    if (whole) {
+                        const float inv = l > 0.f ? 1.f / l : 0.f;
+                        w0 *= inv;
+                        w1 *= inv;
+                    } else if (row_ok) {
+                        *reinterpret_cast<float2*>(slot + 2 * row) = make_float2(m_ref, l);
+                    }
+                }
                 uint32_t ov[32];
                 tmem_ld32(t_lane + col_o + 32u * (uint32_t)cc, ov);
                 tmem_wait_ld();
                 if (row_ok) {
 #pragma unroll
                     for (int c = 0; c < 32; c += 4) {
-                        const float4 v = make_float4(__uint_as_float(ov[c]) * inv, __uint_as_float(ov[c + 1]) * inv, __uint_as_float(ov[c + 2]) * inv,
-                                                     __uint_as_float(ov[c + 3]) * inv);
+                        float4 v = make_float4(__uint_as_float(ov[c]) * w0, __uint_as_float(ov[c + 1]) * w0, __uint_as_float(ov[c + 2]) * w0, __uint_as_float(ov[c + 3]) * w0);
+                        if (fold) {
+                            const uint4 y = lds128(xbase + (uint32_t)((8 * (cc & 1) + (c >> 2)) * kHalfRows + hrow) * 16u);
+                            v = make_float4(fmaf(__uint_as_float(y.x), w1, v.x), fmaf(__uint_as_float(y.y), w1, v.y), fmaf(__uint_as_float(y.z), w1, v.z),
+                                            fmaf(__uint_as_float(y.w), w1, v.w));
+                        }
                         if (whole) q8_store4(a.out, oe + 32 * cc + c, a.io, v);
                         else *reinterpret_cast<float4*>(slot + 4 * (size_t)sh.rows_cap + ((size_t)(8 * cc + (c >> 2)) * sh.rows_cap + row) * 4) = v;
                     }
                 }
+                if (fold && (cc & 1) == 1) mbar_arrive(bar_xfree);
             }
             tc_fence_before();
         }
     } else if (warp < 12) {
-        regs_down<80>();
+        regs_down<64>();
         if (warp < 10) {
             // ------------------------------------------------------------------------------------ MMA issue: one warp per half
             const int h = warp - 8;
             const uint32_t q_lo0 = umma_desc_lo(base + (uint32_t)(2 * h) * kQSlab, 16u), k_lo0 = umma_desc_lo(base + kOffK, 16u),
                            v_lo0 = umma_desc_lo(base + kOffV, (uint32_t)kSlab);
             const uint32_t col_s = tmem + 128u * (uint32_t)h, col_o = tmem + kColO + 128u * (uint32_t)h;
-            auto issue_s = [&](int t) -> bool {
-                const uint32_t k_lo = k_lo0 + (uint32_t)(t & 1) * ((2 * kSlab) >> 4), d_s = col_s + 64u * (uint32_t)(t & 1);
+            // scores of tile t into this half's buffer m & 1
+            auto issue_s = [&](int t, int m) -> bool {
+                const uint32_t k_lo = k_lo0 + (uint32_t)(t & 1) * ((2 * kSlab) >> 4), d_s = col_s + 64u * (uint32_t)(m & 1);
                 if (!__all_sync(0xffffffffu, t5_wait(bar_kfull + 8u * (uint32_t)(t & 1), (uint32_t)(t >> 1) & 1u, &s_abort))) return false;
                 tc_fence_after();
                 if (elect_one()) {
@@ -449,35 +517,40 @@ q8_chunk_kernel(Q8Launch a, const __grid_constant__ CUtensorMap tmk, const __gri
                     for (int j = 0; j < 8; ++j)
                         umma_f16(d_s, umma_desc_of(q_lo0 + (uint32_t)((j >> 2) * (kQSlab >> 4) + (j & 3) * 2)),
                                  umma_desc_of(k_lo + (uint32_t)((j >> 2) * (kSlab >> 4) + (j & 3) * 2)), kIdescS, j > 0 ? 1u : 0u);
-                    umma_commit(bar_sready + 8u * (uint32_t)(2 * h + (t & 1)));
+                    umma_commit(bar_sready + 8u * (uint32_t)(2 * h + (m & 1)));
                     umma_commit(bar_kfree + 8u * (uint32_t)(t & 1));
                 }
                 __syncwarp();
                 return true;
             };
             uint32_t seg = 0;
-            for (long long pos = lo; pos < hi && !failed && h < sh.halves;) {
+            for (long long pos = lo; pos < hi && !failed;) {
                 const Unit u = find_unit(a, sh, plan, pos);
                 int tile0, tiles;
                 unit_part(u, lo, hi, tile0, tiles);
                 pos = u.end;
-                if (tiles == 0) continue;
+                const int mine0 = sh.dual ? (h + n) & 1 : 0, step = sh.dual ? 2 : 1;
+                if (mine0 >= tiles) {
+                    n += tiles;
+                    continue;
+                }
+                int m = sh.dual ? (n + mine0) >> 1 : n;
                 if (!__all_sync(0xffffffffu, t5_wait(bar_qready + 8u * (uint32_t)h, seg & 1u, &s_abort))) { failed = true; break; }
                 ++seg;
-                if (!issue_s(n)) { failed = true; break; }
-                for (int i = 0; i < tiles; ++i) {
+                if (!issue_s(n + mine0, m)) { failed = true; break; }
+                for (int i = mine0; i < tiles; i += step, ++m) {
                     const int t = n + i;
-                    const uint32_t v_lo = v_lo0 + (uint32_t)(t & 1) * ((2 * kSlab) >> 4), p_col = col_s + 64u * (uint32_t)(t & 1);
-                    // the scores of the next 64 keys first: they are computed while the softmax warps work on this tile
-                    if (i + 1 < tiles && !issue_s(t + 1)) { failed = true; break; }
+                    const uint32_t v_lo = v_lo0 + (uint32_t)(t & 1) * ((2 * kSlab) >> 4), p_col = col_s + 64u * (uint32_t)(m & 1);
+                    // the scores of this half's next 64 keys first: they are computed while the softmax warps work on this tile
+                    if (i + step < tiles && !issue_s(t + step, m + 1)) { failed = true; break; }
                     if (!__all_sync(0xffffffffu, t5_wait(bar_vfull + 8u * (uint32_t)(t & 1), (uint32_t)(t >> 1) & 1u, &s_abort))) { failed = true; break; }
-                    if (!__all_sync(0xffffffffu, t5_wait(bar_pready + 8u * (uint32_t)(2 * h + (t & 1)), (uint32_t)(t >> 1) & 1u, &s_abort))) { failed = true; break; }
+                    if (!__all_sync(0xffffffffu, t5_wait(bar_pready + 8u * (uint32_t)(2 * h + (m & 1)), (uint32_t)(m >> 1) & 1u, &s_abort))) { failed = true; break; }
                     tc_fence_after();
                     if (elect_one()) {
 #pragma unroll
                         for (int j = 0; j < 4; ++j)
-                            umma_f16_ts(col_o, p_col + (uint32_t)(8 * j), umma_desc_of(v_lo + (uint32_t)(j * (2048 >> 4))), kIdescPV, (j > 0 || i > 0) ? 1u : 0u);
-                        umma_commit(bar_pvdone + 8u * (uint32_t)(2 * h + (t & 1)));
+                            umma_f16_ts(col_o, p_col + (uint32_t)(8 * j), umma_desc_of(v_lo + (uint32_t)(j * (2048 >> 4))), kIdescPV, (j > 0 || i > mine0) ? 1u : 0u);
+                        umma_commit(bar_pvdone + 8u * (uint32_t)(2 * h + (m & 1)));
                         umma_commit(bar_vfree + 8u * (uint32_t)(t & 1));
                     }
                     __syncwarp();
@@ -581,8 +654,8 @@ q8_chunk_kernel(Q8Launch a, const __grid_constant__ CUtensorMap tmk, const __gri
         }
     } else {
         // ---------------------------------------------------------------------------------------- codes -> fp16 operands
-        regs_down<96>();
-        const int w = warp - 12;
+        regs_down<88>();
+        const int w = warp - 12;              // its rows: 8 w .. 8 w + 7 of the tile
         // eight lanes share two rows that differ in bits 0 and 2: four 16-byte pieces of each, apart both where they are read
         // (piece c of row r sits at c ^ (r & 7)) and where they are written (pieces 2c and 2c + 1 of the fp16 row, likewise)
         const int r8 = (lane >> 3) ^ (5 * (lane >> 2 & 1)), c4 = lane & 3;
@@ -605,44 +678,34 @@ q8_chunk_kernel(Q8Launch a, const __grid_constant__ CUtensorMap tmk, const __gri
                 for (int which = 0; which < 2; ++which) {
                     if (which && t >= 2 && !__all_sync(0xffffffffu, t5_wait(bar_vfree + 8u * (uint32_t)(t & 1), (uint32_t)(t / 2 - 1) & 1u, &s_abort))) { failed = true; break; }
                     const uint32_t src = raw + (uint32_t)(which * kSlab), dst = base + (which ? kOffV : kOffK) + (uint32_t)(t & 1) * (2 * kSlab);
-                    uint4 code[4];
-                    float scale[2];
+                    const uint32_t r = (uint32_t)(8 * w + r8), d = dst + r * 128u;
+                    uint4 code[2];                                      // dims of slab 0 and 1
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {                      // rows 16 w + 8 (e >> 1) + r8, dims of slab e & 1
-                        const uint32_t r = (uint32_t)(16 * w + 8 * (e >> 1) + r8), c = (uint32_t)(4 * (e & 1) + c4);
-                        code[e] = lds128(src + r * 128u + ((c ^ (r & 7u)) << 4));
-                        if ((e & 1) == 0) scale[e >> 1] = lds_f1(sc + (uint32_t)(which * 256) + r * 4u);
+                    for (int e = 0; e < 2; ++e) code[e] = lds128(src + r * 128u + (((uint32_t)(4 * e + c4) ^ (r & 7u)) << 4));
+                    float f = lds_f1(sc + (uint32_t)(which * 256) + r * 4u);
+                    if (!(mask >> r & 1ull)) {                          // what does not exist may hold anything: zeros instead
+                        code[0] = code[1] = make_uint4(0u, 0u, 0u, 0u);
+                        f = 0.f;
                     }
-                    if (mask != ~0ull) {                               // what does not exist may hold anything: zeros instead
+                    f = fminf(which ? f : f * (1.f / kKDiv), 65504.f / q8_qmax<kFmt>());
+                    const __half hi1 = __float2half_rn(f);
+                    const __half2 hi2 = __half2half2(hi1), lo2 = __half2half2(__float2half_rn(f - __half2float(hi1)));
 #pragma unroll
-                        for (int e = 0; e < 4; ++e)
-                            if (!(mask >> (16 * w + 8 * (e >> 1) + r8) & 1ull)) {
-                                code[e] = make_uint4(0u, 0u, 0u, 0u);
-                                scale[e >> 1] = 0.f;
-                            }
-                    }
+                    for (int e = 0; e < 2; ++e) {
+                        uint32_t h[8];
+                        q8_to_h2<kFmt>(code[e].x, h[0], h[1]);
+                        q8_to_h2<kFmt>(code[e].y, h[2], h[3]);
+                        q8_to_h2<kFmt>(code[e].z, h[4], h[5]);
+                        q8_to_h2<kFmt>(code[e].w, h[6], h[7]);
 #pragma unroll
-                    for (int e2 = 0; e2 < 2; ++e2) {
-                        const float f = fminf(which ? scale[e2] : scale[e2] * (1.f / kKDiv), 65504.f / q8_qmax<kFmt>());
-                        const __half hi1 = __float2half_rn(f);
-                        const __half2 hi2 = __half2half2(hi1), lo2 = __half2half2(__float2half_rn(f - __half2float(hi1)));
-#pragma unroll
-                        for (int e = 2 * e2; e < 2 * e2 + 2; ++e) {
-                            const uint32_t r = (uint32_t)(16 * w + 8 * e2 + r8), d = dst + (uint32_t)((e & 1) * kSlab) + r * 128u;
-                            uint32_t h[8];
-                            q8_to_h2<kFmt>(code[e].x, h[0], h[1]);
-                            q8_to_h2<kFmt>(code[e].y, h[2], h[3]);
-                            q8_to_h2<kFmt>(code[e].z, h[4], h[5]);
-                            q8_to_h2<kFmt>(code[e].w, h[6], h[7]);
-#pragma unroll
-                            for (int b = 0; b < 8; ++b) {
-                                const __half2 x = *reinterpret_cast<const __half2*>(&h[b]);
-                                const __half2 y = __hfma2(x, hi2, __hmul2(x, lo2));
-                                h[b] = *reinterpret_cast<const uint32_t*>(&y);
-                            }
-                            asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(d + (((uint32_t)(2 * c4) ^ (r & 7u)) << 4)), "r"(h[0]), "r"(h[1]), "r"(h[2]), "r"(h[3]) : "memory");
-                            asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(d + (((uint32_t)(2 * c4 + 1) ^ (r & 7u)) << 4)), "r"(h[4]), "r"(h[5]), "r"(h[6]), "r"(h[7]) : "memory");
+                        for (int b = 0; b < 8; ++b) {
+                            const __half2 x = *reinterpret_cast<const __half2*>(&h[b]);
+                            const __half2 y = __hfma2(x, hi2, __hmul2(x, lo2));
+                            h[b] = *reinterpret_cast<const uint32_t*>(&y);
                         }
+                        const uint32_t de = d + (uint32_t)(e * kSlab);
+                        asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(de + (((uint32_t)(2 * c4) ^ (r & 7u)) << 4)), "r"(h[0]), "r"(h[1]), "r"(h[2]), "r"(h[3]) : "memory");
+                        asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(de + (((uint32_t)(2 * c4 + 1) ^ (r & 7u)) << 4)), "r"(h[4]), "r"(h[5]), "r"(h[6]), "r"(h[7]) : "memory");
                     }
                     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                     __syncwarp();
@@ -722,9 +785,10 @@ ChunkShape chunk_shape(int n_heads, int n_kv_heads, int max_tokens) {
     ChunkShape sh;
     const int G = n_heads / n_kv_heads;
     const int64_t most = (int64_t)max_tokens * G;                       // rows of the longest chunk
-    sh.halves = most <= kHalfRows ? 1 : 2;
-    sh.tq = kHalfRows * sh.halves / G;
-    sh.rows_cap = most < kHalfRows * sh.halves ? (int)((most + 31) / 32 * 32) : kHalfRows * sh.halves;
+    sh.dual = most <= kHalfRows;
+    const int rows = sh.dual ? kHalfRows : 2 * kHalfRows;
+    sh.tq = rows / G;
+    sh.rows_cap = most < rows ? (int)((most + 31) / 32 * 32) : rows;
     return sh;
 }
 
