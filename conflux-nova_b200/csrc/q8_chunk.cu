@@ -8,8 +8,8 @@
 //     half of 128 rows (held twice, for alternate tiles), or two halves that share every K/V tile.  A unit of work is (session, kv head, tile of tokens); the 64-key tiles
 //     of all units form one line that is dealt out evenly over one CTA per SM, so neither short sessions, nor long ones, nor
 //     the causal triangle leave SMs idle.  Units that several CTAs worked on are merged by the kernel behind it.
-//   * Twenty warps: 8 softmax (thread = row), 2 issuing MMAs (one per half), 1 copying codes (TMA boxes of 16 slots x 128 B), 1
-//     copying scales, 8 converting.  The pipe runs on from one unit to the next.
+//   * Twenty warps: 8 softmax (thread = row), 2 issuing MMAs (one per half), 8 converting, each of which brings in its own 16 keys'
+//     codes and scales.  The pipe runs on from one unit to the next.
 //   * The tensor cores want fp16 operands, so a tile's codes become fp16 VALUES in shared memory, code times scale, in the
 //     128-byte-swizzle layout that is the K-major form for S = Q.K^T and the MN-major form for O += P.V.  A scale (K's over 16;
 //     q is multiplied by 16 / sqrt(128) log2 e) goes in as two fp16 parts and the product is rounded once (2^-11).
@@ -44,8 +44,9 @@ struct ChunkPlan {
     long long line[kMaxSessions + 1];                 // where each session's tiles start on the line
     int first[kMaxSessions], count[kMaxSessions], past[kMaxSessions];
 };
-constexpr int kOffBar = kOffPlan + (int)((sizeof(ChunkPlan) + 15) / 16 * 16);
-constexpr int kSmem = kOffBar + 512;
+constexpr int kOffParts = kOffPlan + (int)((sizeof(ChunkPlan) + 15) / 16 * 16);
+constexpr int kOffBar = kOffParts + 4 * 48;
+constexpr int kSmem = kOffBar + 768;
 static_assert(kSmem <= 232448, "shared memory of one CTA");
 constexpr int kTmemCols = 512;                        // S of half h, buffer b: columns 128 h + 64 b (P over its first 32); O: 256 + 128 h
 constexpr uint32_t kColO = 256;
@@ -162,6 +163,15 @@ __device__ inline Unit find_unit(const Q8Launch& a, const ChunkShape& sh, const 
     u.end = u.begin + len;
     return u;
 }
+// What the warps need to know of the part of a unit that their CTA works on.  One warp walks the line and leaves these in a ring; with
+// the walk in every role the kernel was four times this code, and instruction fetches were its largest stall.
+struct __align__(16) Part {
+    int s, kvh, t0, t_cnt;
+    int past, first16, keys_end, tile0;
+    int tiles, whole, slot, pad;     // tiles 0: that was the last one; slot: which of the CTA's two partial slots
+};
+constexpr int kParts = 4;
+static_assert(sizeof(Part) == 48 && kOffBar - kOffParts == kParts * (int)sizeof(Part), "ring of parts");
 // The part [lo, hi) of the line that a CTA takes of a unit, as tiles of the unit.
 __device__ __forceinline__ void unit_part(const Unit& u, long long lo, long long hi, int& tile, int& count) {
     const long long b = (lo > u.begin ? lo : u.begin) - u.begin - kSetup, e = (hi < u.end ? hi : u.end) - u.begin - kSetup;
@@ -192,34 +202,30 @@ template <int kRegs> __device__ __forceinline__ void regs_down() { asm volatile(
 
 template <int kFmt>
 __global__ void __launch_bounds__(kThreads, 1)
-q8_chunk_kernel(Q8Launch a, const __grid_constant__ CUtensorMap tmk, const __grid_constant__ CUtensorMap tmv, ChunkShape sh) {
+q8_chunk_kernel(Q8Launch a, ChunkShape sh) {
     // No static shared memory: the dynamic region then starts at the front of the CTA's window, which is 1024-byte aligned as the
     // swizzled tiles need (checked).
     extern __shared__ unsigned char smem_raw[];
     ChunkPlan& plan = *reinterpret_cast<ChunkPlan*>(smem_raw + kOffPlan);
-    uint32_t& s_tmem = *reinterpret_cast<uint32_t*>(smem_raw + kOffBar + 400);
-    volatile int& s_abort = *reinterpret_cast<volatile int*>(smem_raw + kOffBar + 404);
-    unsigned long long* const s_rmask = reinterpret_cast<unsigned long long*>(smem_raw + kOffBar + 320);      // [kRaw] which keys of the raw tile exist
-    unsigned long long* const s_mask = reinterpret_cast<unsigned long long*>(smem_raw + kOffBar + 408);       // [kMasks] the same by tile
+    uint32_t& s_tmem = *reinterpret_cast<uint32_t*>(smem_raw + kOffBar + 512);
+    volatile int& s_abort = *reinterpret_cast<volatile int*>(smem_raw + kOffBar + 516);
+    uint16_t* const s_mask = reinterpret_cast<uint16_t*>(smem_raw + kOffBar + 520);       // [kMasks][4] which keys of a tile exist, 16 to a word
+    uint16_t* const s_rmask = reinterpret_cast<uint16_t*>(smem_raw + kOffBar + 584);      // [kConv][kRaw] the same of a converter's 16 keys
     const int lane = (int)threadIdx.x & 31;
     const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0);
     const int G = a.n_heads / a.n_kv_heads;
     const uint32_t base = smem_u32(smem_raw);
     const uint32_t bar = base + kOffBar;
-    const uint32_t bar_rawfull = bar, bar_rawfree = bar + 40, bar_kfull = bar + 80, bar_kfree = bar + 96, bar_vfull = bar + 112, bar_vfree = bar + 128,
-                   bar_sready = bar + 144 /* [half][buffer] */, bar_pready = bar + 176, bar_pvdone = bar + 208, bar_qready = bar + 240 /* [half] */,
-                   bar_xfull = bar + 256, bar_xfree = bar + 264;
+    const uint32_t bar_partfull = bar, bar_partfree = bar + 32, bar_kfull = bar + 320, bar_kfree = bar + 336, bar_vfull = bar + 352, bar_vfree = bar + 368,
+                   bar_sready = bar + 384 /* [half][buffer] */, bar_pready = bar + 416, bar_pvdone = bar + 448, bar_qready = bar + 480 /* [half] */,
+                   bar_xfull = bar + 496, bar_xfree = bar + 504;
     // Every waiter waits for a phase whose successor on the same barrier needs that waiter's own next action (or one that follows it),
     // so a parity is never taken for a later one.
     if (threadIdx.x == 0) {
-        for (int i = 0; i < kRaw; ++i) {
-            mbar_init(bar_rawfull + 8u * i, 33);        // codes, and each lane of the scales' warp
-            mbar_init(bar_rawfree + 8u * i, kConv);
-        }
         for (int i = 0; i < 2; ++i) {
-            mbar_init(bar_kfull + 8u * i, kConv);
+            mbar_init(bar_kfull + 8u * i, kConv / 2);
             mbar_init(bar_kfree + 8u * i, sh.dual ? 1 : 2);
-            mbar_init(bar_vfull + 8u * i, kConv);
+            mbar_init(bar_vfull + 8u * i, kConv / 2);
             mbar_init(bar_vfree + 8u * i, sh.dual ? 1 : 2);
             mbar_init(bar_qready + 8u * i, kHalfRows);
         }
@@ -228,12 +234,14 @@ q8_chunk_kernel(Q8Launch a, const __grid_constant__ CUtensorMap tmk, const __gri
             mbar_init(bar_pready + 8u * i, kHalfRows);
             mbar_init(bar_pvdone + 8u * i, 1);
         }
+        for (int i = 0; i < kParts; ++i) {
+            mbar_init(bar_partfull + 8u * i, 1);
+            mbar_init(bar_partfree + 8u * i, 18);      // every warp but the one that walks and the one that idles
+        }
         mbar_init(bar_xfull, kHalfRows);
         mbar_init(bar_xfree, kHalfRows);
         s_abort = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-        asm volatile("prefetch.tensormap [%0];" ::"l"(&tmk) : "memory");
-        asm volatile("prefetch.tensormap [%0];" ::"l"(&tmv) : "memory");
     }
     // Nothing of the caller's is read before the kernels before this one are done; the merge kernel, which reads positions and
     // row starts before its own wait, is let go only then.
@@ -256,7 +264,27 @@ q8_chunk_kernel(Q8Launch a, const __grid_constant__ CUtensorMap tmk, const __gri
     tc_fence_after();
     const uint32_t tmem = __shfl_sync(0xffffffffu, s_tmem, 0);
     bool failed = false;
-    int n = 0;                       // tiles of the units before: every ring runs on over the units
+    int n = 0;                       // tiles of the parts before: every ring runs on over the parts
+    Part* const ring = reinterpret_cast<Part*>(smem_raw + kOffParts);
+    int k_part = 0;
+    Part u;
+    // The next part into u; false after the last one (or when a wait ran out).  All lanes of a warp.
+    auto next_part = [&]() -> bool {
+        const int slot = k_part & (kParts - 1);
+        if (!__all_sync(0xffffffffu, t5_wait(bar_partfull + 8u * (uint32_t)slot, (uint32_t)(k_part / kParts) & 1u, &s_abort))) {
+            failed = true;
+            return false;
+        }
+        const int4* const src = reinterpret_cast<const int4*>(ring + slot);
+        const int4 x = src[0], y = src[1], z = src[2];
+        u.s = x.x; u.kvh = x.y; u.t0 = x.z; u.t_cnt = x.w;
+        u.past = y.x; u.first16 = y.y; u.keys_end = y.z; u.tile0 = y.w;
+        u.tiles = z.x; u.whole = z.y; u.slot = z.z;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar_partfree + 8u * (uint32_t)slot);
+        ++k_part;
+        return u.tiles > 0;
+    };
 
     if (warp < 8) {
         // ---------------------------------------------------------------------------------------- softmax: thread = one row
@@ -267,11 +295,8 @@ q8_chunk_kernel(Q8Launch a, const __grid_constant__ CUtensorMap tmk, const __gri
         const uint32_t my_sready = bar_sready + 16u * (uint32_t)half, my_pready = bar_pready + 16u * (uint32_t)half, my_pvdone = bar_pvdone + 16u * (uint32_t)half;
         const int row0 = sh.dual ? 0 : half * kHalfRows, row = row0 + hrow, tk = row / G, g = row - tk * G;
         uint32_t xround = 0;
-        for (long long pos = lo; pos < hi && !failed;) {
-            const Unit u = find_unit(a, sh, plan, pos);
-            int tile0, tiles;
-            unit_part(u, lo, hi, tile0, tiles);
-            pos = u.end;
+        while (!failed && next_part()) {
+            const int tiles = u.tiles;
             // this half's tiles of the unit: every tile, or those whose place on the CTA's line is even (odd)
             const int mine0 = sh.dual ? (half + n) & 1 : 0, step = sh.dual ? 2 : 1;
             if (mine0 >= tiles) {
@@ -349,9 +374,9 @@ q8_chunk_kernel(Q8Launch a, const __grid_constant__ CUtensorMap tmk, const __gri
                 if (!__all_sync(0xffffffffu, t5_wait(my_sready + 8u * (uint32_t)(m & 1), (uint32_t)(m >> 1) & 1u, &s_abort))) { failed = true; break; }
                 tc_fence_after();
                 const uint32_t s_col = t_lane + col_s + 64u * (uint32_t)(m & 1);
-                const int key0 = (u.first16 << 4) + (tile0 + i) * kKeys;
+                const int key0 = (u.first16 << 4) + (u.tile0 + i) * kKeys;
                 const int hi_k = row_lim - key0, lo_k = row_lo - key0;       // first and last visible column
-                const unsigned long long there = s_mask[t & (kMasks - 1)];    // (a page missing, or the last key passed)
+                const unsigned long long there = *reinterpret_cast<const unsigned long long*>(s_mask + 4 * (t & (kMasks - 1)));    // (a page missing, or the last key passed)
                 const bool all_seen = __all_sync(0xffffffffu, hi_k >= kKeys - 1 && lo_k <= 0) && there == ~0ull;
                 // Two passes over the scores, 32 columns at a time, both read from tensor memory: half the code and half the registers
                 // of one pass over 64 (with that, instruction fetches were the largest stall: sixteen warps run five loops here).
@@ -428,7 +453,7 @@ q8_chunk_kernel(Q8Launch a, const __grid_constant__ CUtensorMap tmk, const __gri
             // ---- the unit's part is done: outputs, or a partial slot for the merge
             if (!__all_sync(0xffffffffu, t5_wait(my_pvdone + 8u * (uint32_t)((m - 1) & 1), (uint32_t)((m - 1) >> 1) & 1u, &s_abort))) { failed = true; break; }
             tc_fence_after();
-            const bool whole = tiles == u.tiles, fold = sh.dual && tiles > 1;
+            const bool whole = u.whole, fold = sh.dual && tiles > 1;
             const uint32_t xbase = base + 2u * kQSlab, xml = base + kOffX;      // (the second half's q is no longer needed)
             if (fold && half == 1) {
                 // both halves have a share of the rows: the second hands its own over, 64 dims at a time
@@ -454,7 +479,7 @@ q8_chunk_kernel(Q8Launch a, const __grid_constant__ CUtensorMap tmk, const __gri
             }
             const int64_t oe = (tok0 + tk) * a.out_stride + (int64_t)(u.kvh * G + g) * kHeadDim;
             // slot: (m, l) of every row, then the accumulators, four dims of every row side by side
-            float* const slot = a.part + (size_t)(2 * blockIdx.x + (u.begin > lo ? 1 : 0)) * ((size_t)sh.rows_cap * kSlotW);
+            float* const slot = a.part + (size_t)(2 * blockIdx.x + u.slot) * ((size_t)sh.rows_cap * kSlotW);
             float w0 = 1.f, w1 = 0.f;                 // what this half's and the other half's accumulators are multiplied by
 #pragma unroll 1
             for (int cc = 0; cc < 4; ++cc) {
@@ -524,11 +549,8 @@ q8_chunk_kernel(Q8Launch a, const __grid_constant__ CUtensorMap tmk, const __gri
                 return true;
             };
             uint32_t seg = 0;
-            for (long long pos = lo; pos < hi && !failed;) {
-                const Unit u = find_unit(a, sh, plan, pos);
-                int tile0, tiles;
-                unit_part(u, lo, hi, tile0, tiles);
-                pos = u.end;
+            while (!failed && next_part()) {
+                const int tiles = u.tiles;
                 const int mine0 = sh.dual ? (h + n) & 1 : 0, step = sh.dual ? 2 : 1;
                 if (mine0 >= tiles) {
                     n += tiles;
@@ -557,169 +579,177 @@ q8_chunk_kernel(Q8Launch a, const __grid_constant__ CUtensorMap tmk, const __gri
                 }
                 n += tiles;
             }
-        } else {
-            // ------------------------------------------------------------------------------------ copies
-            const bool p8 = a.kv_shift == 3;
-            const int slot_mask = (1 << a.kv_shift) - 1;
-            // block-table entry of the page that holds a key; -1: a bad one, -2: there is no such key
-            auto entry = [&](const int32_t* table, int key, int keys_end) -> int {
-                if (key >= keys_end) return -2;
-                const int64_t page = key >> a.kv_shift;
-                if (page >= a.table_stride) return -1;
-                const int e = __ldg(table + page);
-                return e >= 0 && e < a.nb ? e : -1;
-            };
-            if (warp == 10) {
-                // codes: lane = (K or V, box of 16 slots, or of 8 in pages of 8), one box per tile
-                const int boxes = p8 ? 8 : 4, box_keys = p8 ? 8 : 16;
-                const int j = lane & 7, is_v = lane >> 3 & 1;
-                const bool mine = lane < 16 && j < boxes;
-                const CUtensorMap* const tm = is_v ? &tmv : &tmk;
-                const int row0 = (a.layer * a.nb) << a.kv_shift;
-                uint32_t stage = 0, round = 0;
-                for (long long pos = lo; pos < hi && !failed;) {
-                    const Unit u = find_unit(a, sh, plan, pos);
-                    int tile0, tiles;
-                    unit_part(u, lo, hi, tile0, tiles);
-                    pos = u.end;
-                    if (tiles == 0) continue;
-                    const int32_t* table = q8_table(a, u.s);
-                    const int key_a = (u.first16 << 4) + tile0 * kKeys + j * box_keys;       // this lane's first key of tile 0
-                    auto get = [&](int i) -> int { return mine && i < tiles ? entry(table, key_a + i * kKeys, u.keys_end) : -2; };
-                    int e0 = get(0), e1 = get(1), e2 = get(2);
-#pragma unroll 1
-                    for (int i = 0; i < tiles; ++i) {
-                        const int e = e0;
-                        e0 = e1;
-                        e1 = e2;
-                        e2 = get(i + 3);
-                        if (round > 0 && !__all_sync(0xffffffffu, t5_wait(bar_rawfree + 8u * stage, (round - 1) & 1u, &s_abort))) { failed = true; break; }
-                        const unsigned have = __ballot_sync(0xffffffffu, e >= 0) & 0xffu, bad = __ballot_sync(0xffffffffu, e == -1);
-                        if (lane == 0) {
-                            if (bad) q8_flag(a, NOVA_ERR_BAD_TABLE);
-                            unsigned long long mask = 0ull;
-                            for (int b = 0; b < boxes; ++b)
-                                if (have >> b & 1) mask |= (p8 ? 0xffull : 0xffffull) << (b * box_keys);
-                            const int left = u.keys_end - ((u.first16 << 4) + (tile0 + i) * kKeys);
-                            if (left < kKeys) mask &= (1ull << left) - 1ull;
-                            s_rmask[stage] = mask;
-                            const uint32_t bytes = 2u * (uint32_t)__popc(have) * (uint32_t)(box_keys * 128);
-                            if (bytes) mbar_expect_tx(bar_rawfull + 8u * stage, bytes);
-                            else mbar_arrive(bar_rawfull + 8u * stage);
-                        }
-                        __syncwarp();
-                        if (e >= 0)
-                            tma_load_3d(base + kOffRaw + stage * (2 * kSlab) + (uint32_t)(is_v * kSlab + j * box_keys * 128), tm, 0,
-                                        row0 + (e << a.kv_shift) + ((key_a + i * kKeys) & slot_mask), u.kvh, bar_rawfull + 8u * stage);
-                        if (++stage == kRaw) {
-                            stage = 0;
-                            ++round;
-                        }
-                    }
+        } else if (warp == 10) {
+            // ------------------------------------------------------------------------------------ the walk along the line
+            int k = 0;
+            for (long long pos = lo;;) {
+                Part q;
+                q.tiles = 0;
+                while (pos < hi && q.tiles == 0) {
+                    const Unit v = find_unit(a, sh, plan, pos);
+                    unit_part(v, lo, hi, q.tile0, q.tiles);
+                    pos = v.end;
+                    q.s = v.s; q.kvh = v.kvh; q.t0 = v.t0; q.t_cnt = v.t_cnt; q.past = v.past; q.first16 = v.first16; q.keys_end = v.keys_end;
+                    q.whole = q.tiles == v.tiles;
+                    q.slot = v.begin > lo;
                 }
-            } else {
-                // scales: lane = (K or V, four keys), one 16-byte copy per tile; the copies arrive on the tile's barrier by themselves
-                const int quad = lane & 15;
-                const float* const scales = lane >= 16 ? a.scale_v : a.scale_k;
-                const uint32_t dst0 = base + kOffSc + (uint32_t)lane * 16u;
-                uint32_t stage = 0, round = 0;
-                for (long long pos = lo; pos < hi && !failed;) {
-                    const Unit u = find_unit(a, sh, plan, pos);
-                    int tile0, tiles;
-                    unit_part(u, lo, hi, tile0, tiles);
-                    pos = u.end;
-                    if (tiles == 0) continue;
-                    const int32_t* table = q8_table(a, u.s);
-                    const float* const mine0 = scales + ((((int64_t)a.layer * a.nb) * a.n_kv_heads + u.kvh) << a.kv_shift);
-                    const int key_a = (u.first16 << 4) + tile0 * kKeys + 4 * quad;
-                    auto get = [&](int i) -> int { return i < tiles ? entry(table, key_a + i * kKeys, u.keys_end) : -2; };
-                    int e0 = get(0), e1 = get(1), e2 = get(2);
-#pragma unroll 1
-                    for (int i = 0; i < tiles; ++i) {
-                        const int e = e0;
-                        e0 = e1;
-                        e1 = e2;
-                        e2 = get(i + 3);
-                        if (round > 0 && !__all_sync(0xffffffffu, t5_wait(bar_rawfree + 8u * stage, (round - 1) & 1u, &s_abort))) { failed = true; break; }
-                        if (e >= 0) cp_async16(dst0 + stage * 512u, mine0 + (((int64_t)e * a.n_kv_heads) << a.kv_shift) + ((key_a + i * kKeys) & slot_mask));
-                        asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar_rawfull + 8u * stage) : "memory");
-                        if (++stage == kRaw) {
-                            stage = 0;
-                            ++round;
-                        }
-                    }
+                const int slot = k & (kParts - 1);
+                if (k >= kParts && !__all_sync(0xffffffffu, t5_wait(bar_partfree + 8u * (uint32_t)slot, (uint32_t)(k / kParts - 1) & 1u, &s_abort))) { failed = true; break; }
+                if (lane == 0) {
+                    ring[slot] = q;
+                    mbar_arrive(bar_partfull + 8u * (uint32_t)slot);
                 }
-                asm volatile("cp.async.wait_all;" ::: "memory");
+                __syncwarp();
+                ++k;
+                if (q.tiles == 0) break;
             }
         }
     } else {
         // ---------------------------------------------------------------------------------------- codes -> fp16 operands
+        // Four warps for K, four for V: V's buffer comes free only after the softmax of its tile, and the next K must not wait for that.
+        // A warp owns 16 keys of the tile and brings their codes and scales in itself, kRaw tiles ahead, with 16-byte asynchronous copies
+        // into a ring of its own, which needs no barrier.  (As TMA boxes the rows of one head are 2 KiB a copy, too little: one
+        // warp issuing all of a tile's copies took 1900 cycles, eight warps with a box and a run of scales each 900.)
         regs_down<88>();
-        const int w = warp - 12;              // its rows: 8 w .. 8 w + 7 of the tile
-        // eight lanes share two rows that differ in bits 0 and 2: four 16-byte pieces of each, apart both where they are read
-        // (piece c of row r sits at c ^ (r & 7)) and where they are written (pieces 2c and 2c + 1 of the fp16 row, likewise)
-        const int r8 = (lane >> 3) ^ (5 * (lane >> 2 & 1)), c4 = lane & 3;
-        uint32_t stage = 0, round = 0;
-        for (long long pos = lo; pos < hi && !failed;) {
-            const Unit u = find_unit(a, sh, plan, pos);
-            int tile0, tiles;
-            unit_part(u, lo, hi, tile0, tiles);
-            pos = u.end;
-#pragma unroll 1
-            for (int i = 0; i < tiles; ++i) {
-                const int t = n + i;
-                bool ok = t5_wait(bar_rawfull + 8u * stage, round & 1u, &s_abort);
-                ok = ok && (t < 2 || t5_wait(bar_kfree + 8u * (uint32_t)(t & 1), (uint32_t)(t / 2 - 1) & 1u, &s_abort));
-                if (!__all_sync(0xffffffffu, ok)) { failed = true; break; }
-                const unsigned long long mask = s_rmask[stage];
-                if (w == 0 && lane == 0) s_mask[t & (kMasks - 1)] = mask;
-                const uint32_t raw = base + kOffRaw + stage * (2 * kSlab), sc = base + kOffSc + stage * 512u;
-#pragma unroll 1
-                for (int which = 0; which < 2; ++which) {
-                    if (which && t >= 2 && !__all_sync(0xffffffffu, t5_wait(bar_vfree + 8u * (uint32_t)(t & 1), (uint32_t)(t / 2 - 1) & 1u, &s_abort))) { failed = true; break; }
-                    const uint32_t src = raw + (uint32_t)(which * kSlab), dst = base + (which ? kOffV : kOffK) + (uint32_t)(t & 1) * (2 * kSlab);
-                    const uint32_t r = (uint32_t)(8 * w + r8), d = dst + r * 128u;
-                    uint4 code[2];                                      // dims of slab 0 and 1
-#pragma unroll
-                    for (int e = 0; e < 2; ++e) code[e] = lds128(src + r * 128u + (((uint32_t)(4 * e + c4) ^ (r & 7u)) << 4));
-                    float f = lds_f1(sc + (uint32_t)(which * 256) + r * 4u);
-                    if (!(mask >> r & 1ull)) {                          // what does not exist may hold anything: zeros instead
-                        code[0] = code[1] = make_uint4(0u, 0u, 0u, 0u);
-                        f = 0.f;
-                    }
-                    f = fminf(which ? f : f * (1.f / kKDiv), 65504.f / q8_qmax<kFmt>());
-                    const __half hi1 = __float2half_rn(f);
-                    const __half2 hi2 = __half2half2(hi1), lo2 = __half2half2(__float2half_rn(f - __half2float(hi1)));
-#pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        uint32_t h[8];
-                        q8_to_h2<kFmt>(code[e].x, h[0], h[1]);
-                        q8_to_h2<kFmt>(code[e].y, h[2], h[3]);
-                        q8_to_h2<kFmt>(code[e].z, h[4], h[5]);
-                        q8_to_h2<kFmt>(code[e].w, h[6], h[7]);
-#pragma unroll
-                        for (int b = 0; b < 8; ++b) {
-                            const __half2 x = *reinterpret_cast<const __half2*>(&h[b]);
-                            const __half2 y = __hfma2(x, hi2, __hmul2(x, lo2));
-                            h[b] = *reinterpret_cast<const uint32_t*>(&y);
-                        }
-                        const uint32_t de = d + (uint32_t)(e * kSlab);
-                        asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(de + (((uint32_t)(2 * c4) ^ (r & 7u)) << 4)), "r"(h[0]), "r"(h[1]), "r"(h[2]), "r"(h[3]) : "memory");
-                        asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(de + (((uint32_t)(2 * c4 + 1) ^ (r & 7u)) << 4)), "r"(h[4]), "r"(h[5]), "r"(h[6]), "r"(h[7]) : "memory");
-                    }
-                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive((which ? bar_vfull : bar_kfull) + 8u * (uint32_t)(t & 1));
+        const int which = warp >= 16, w = warp & 3, me = warp - 12;
+        const bool p8 = a.kv_shift == 3;
+        const unsigned char* const pool = static_cast<const unsigned char*>(which ? a.pool_v : a.pool_k);
+        const float* const scales = which ? a.scale_v : a.scale_k;
+        const int lrow = lane >> 3, lch = lane & 7;        // this lane's rows (and + 4) and 16-byte piece of every copy
+        const int slot_mask = (1 << a.kv_shift) - 1;
+        // ---- what is copied next
+        u.tiles = 0;
+        const int32_t* table = nullptr;
+        const unsigned char* pool_u = nullptr;             // rows of the part's kv head, this lane's row and piece
+        const float* scale_u = nullptr;
+        const uint32_t row_bytes = (uint32_t)a.n_kv_heads * kHeadDim, page_bytes = row_bytes << a.kv_shift, page_scales = (uint32_t)a.n_kv_heads << a.kv_shift;
+        bool more = true;
+        int c_i = 0, c_key = 0, b0 = 0, b1 = 0, n0 = 0, n1 = 0, issued = 0;
+        uint32_t c_stage = 0;
+        // block-table entry of the page that holds a key; -1: a bad one, -2: there is no such key
+        auto entry = [&](int key) -> int {
+            if (key >= u.keys_end) return -2;
+            const int64_t page = key >> a.kv_shift;
+            if (page >= a.table_stride) return -1;
+            const int e = __ldg(table + page);
+            return e >= 0 && e < a.nb ? e : -1;
+        };
+        auto fetch = [&](int i) {                          // lane's tile of the next 32
+            n0 = n1 = -2;
+            if (i < u.tiles) {
+                n0 = entry(c_key + i * kKeys);
+                if (p8) n1 = entry(c_key + i * kKeys + 8);
+            }
+        };
+        auto issue_next = [&]() {
+            if (!more) return;
+            if (c_i == u.tiles) {
+                if (!next_part()) {
+                    more = false;
+                    return;
                 }
-                if (failed) break;
-                if (lane == 0) mbar_arrive(bar_rawfree + 8u * stage);
-                if (++stage == kRaw) {
-                    stage = 0;
-                    ++round;
+                c_i = 0;
+                table = q8_table(a, u.s);
+                c_key = (u.first16 << 4) + u.tile0 * kKeys + 16 * w;
+                const int64_t page0 = (int64_t)a.layer * a.nb;
+                pool_u = pool + page0 * page_bytes + (uint32_t)(u.kvh * kHeadDim) + (uint32_t)lrow * row_bytes + 16u * (uint32_t)lch;
+                scale_u = scales + page0 * page_scales + ((uint32_t)u.kvh << a.kv_shift) + 4 * (lane & 1);
+                fetch(lane);
+            }
+            if ((c_i & 31) == 0) {
+                b0 = n0;
+                b1 = n1;
+                fetch(c_i + 32 + lane);
+            }
+            const int e0 = __shfl_sync(0xffffffffu, b0, c_i & 31);
+            int e1 = -2;
+            if (p8) e1 = __shfl_sync(0xffffffffu, b1, c_i & 31);
+            const int key = c_key + c_i * kKeys, left = u.keys_end - key, slot = key & slot_mask;
+            if (lane == 0) {
+                uint32_t mask = p8 ? (e0 >= 0 ? 0xffu : 0u) | (e1 >= 0 ? 0xff00u : 0u) : (e0 >= 0 ? 0xffffu : 0u);
+                if (left < 16) mask &= left > 0 ? (1u << left) - 1u : 0u;
+                s_rmask[me * kRaw + c_stage] = (uint16_t)mask;
+                if (!which && (e0 == -1 || e1 == -1)) q8_flag(a, NOVA_ERR_BAD_TABLE);
+            }
+            const uint32_t dst = base + kOffRaw + c_stage * (2 * kSlab) + (uint32_t)(which * kSlab + w * 2048);
+#pragma unroll
+            for (int hf = 0; hf < 2; ++hf) {               // eight rows each: one page of 8, or half of the 16 slots
+                const int e = p8 && hf ? e1 : e0, s0 = p8 ? 0 : slot + 8 * hf;
+                if (e < 0) continue;
+                const unsigned char* src = pool_u + (uint64_t)(uint32_t)e * page_bytes + (uint32_t)s0 * row_bytes;
+                cp_async16(dst + (uint32_t)((8 * hf + lrow) * 128 + ((lch ^ lrow) << 4)), src);
+                cp_async16(dst + (uint32_t)((8 * hf + lrow + 4) * 128 + ((lch ^ (lrow + 4)) << 4)), src + 4 * row_bytes);
+                if ((lane >> 1) == hf)                      // scales: four keys a lane
+                    cp_async16(base + kOffSc + c_stage * 512u + (uint32_t)(which * 256 + w * 64 + 16 * lane), scale_u + (uint64_t)(uint32_t)e * page_scales + s0);
+            }
+            ++c_i;
+            ++issued;
+            if (++c_stage == kRaw) c_stage = 0;
+        };
+        // ---- what is converted now.  Eight lanes share two rows that differ in bits 0 and 2: four 16-byte pieces of each, apart both
+        // where they are read (piece c of row r sits at c ^ (r & 7)) and where they are written (pieces 2c and 2c + 1, likewise).
+        const int r8 = (lane >> 3) ^ (5 * (lane >> 2 & 1)), c4 = lane & 3;
+        const uint32_t bar_full = which ? bar_vfull : bar_kfull, bar_free = which ? bar_vfree : bar_kfree;
+        const uint32_t dst0 = base + (which ? kOffV : kOffK) + (uint32_t)(16 * w + r8) * 128u, src0 = base + kOffRaw + (uint32_t)(which * kSlab) + (uint32_t)(16 * w + r8) * 128u;
+        const uint32_t sc0 = base + kOffSc + (uint32_t)(which * 256 + (16 * w + r8) * 4);
+        const float div = which ? 1.f : 1.f / kKDiv;
+        for (int k = 0; k < kRaw; ++k) {
+            issue_next();
+            asm volatile("cp.async.commit_group;" ::: "memory");
+        }
+        uint32_t stage = 0;
+#pragma unroll 1
+        for (int t = 0; t < issued; ++t) {
+            asm volatile("cp.async.wait_group %0;" ::"n"(kRaw - 1) : "memory");      // (a group per tile, empty ones at the end)
+            __syncwarp();
+            const bool ok = t < 2 || t5_wait(bar_free + 8u * (uint32_t)(t & 1), (uint32_t)(t / 2 - 1) & 1u, &s_abort);
+            if (!__all_sync(0xffffffffu, ok)) { failed = true; break; }
+            const uint32_t mask = s_rmask[me * kRaw + stage];
+            if (!which && lane == 0) s_mask[4 * (t & (kMasks - 1)) + w] = (uint16_t)mask;
+            const uint32_t src = src0 + stage * (2 * kSlab), dst = dst0 + (uint32_t)(t & 1) * (2 * kSlab);
+            uint4 code[4];                                          // rows r8 and r8 + 8, dims of slab 0 and 1
+            float f[2];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) code[e] = lds128(src + (uint32_t)(e >> 1) * 1024u + (((uint32_t)(4 * (e & 1) + c4) ^ (uint32_t)r8) << 4));
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                f[e] = lds_f1(sc0 + stage * 512u + (uint32_t)e * 32u);
+                if (!(mask >> (8 * e + r8) & 1u)) {                   // what does not exist may hold anything: zeros instead
+                    code[2 * e] = code[2 * e + 1] = make_uint4(0u, 0u, 0u, 0u);
+                    f[e] = 0.f;
                 }
             }
-            n += tiles;
+#pragma unroll
+            for (int e2 = 0; e2 < 2; ++e2) {
+                const float fs = fminf(f[e2] * div, 65504.f / q8_qmax<kFmt>());
+                const __half hi1 = __float2half_rn(fs);
+                const __half2 hi2 = __half2half2(hi1), lo2 = __half2half2(__float2half_rn(fs - __half2float(hi1)));
+#pragma unroll
+                for (int e = 2 * e2; e < 2 * e2 + 2; ++e) {
+                    uint32_t h[8];
+                    q8_to_h2<kFmt>(code[e].x, h[0], h[1]);
+                    q8_to_h2<kFmt>(code[e].y, h[2], h[3]);
+                    q8_to_h2<kFmt>(code[e].z, h[4], h[5]);
+                    q8_to_h2<kFmt>(code[e].w, h[6], h[7]);
+#pragma unroll
+                    for (int b = 0; b < 8; ++b) {
+                        const __half2 x = *reinterpret_cast<const __half2*>(&h[b]);
+                        const __half2 y = __hfma2(x, hi2, __hmul2(x, lo2));
+                        h[b] = *reinterpret_cast<const uint32_t*>(&y);
+                    }
+                    const uint32_t de = dst + (uint32_t)(e2 * 1024 + (e & 1) * kSlab);
+                    asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(de + (((uint32_t)(2 * c4) ^ (uint32_t)r8) << 4)), "r"(h[0]), "r"(h[1]), "r"(h[2]), "r"(h[3]) : "memory");
+                    asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(de + (((uint32_t)(2 * c4 + 1) ^ (uint32_t)r8) << 4)), "r"(h[4]), "r"(h[5]), "r"(h[6]), "r"(h[7]) : "memory");
+                }
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar_full + 8u * (uint32_t)(t & 1));
+            issue_next();                                           // into the stage that has just been read
+            asm volatile("cp.async.commit_group;" ::: "memory");
+            if (++stage == kRaw) stage = 0;
         }
+        asm volatile("cp.async.wait_all;" ::: "memory");           // (nothing may land after the CTA is gone)
     }
     if (failed && lane == 0) q8_flag(a, NOVA_ERR_TIMEOUT);
     // ---- release the tensor memory (every path of every thread ends here)
@@ -799,12 +829,6 @@ size_t q8_chunk_work_bytes(int n_heads, int n_kv_heads, int max_tokens) {
 }
 
 int launch_q8_chunk(const Q8Launch& a, cudaStream_t s) {
-    alignas(64) CUtensorMap tmk, tmv;
-    const int64_t slot_rows = ((int64_t)(a.layer + 1) * a.nb) << a.kv_shift;
-    const int box = a.kv_shift == 3 ? 8 : 16;
-    int rc = attn_make_tmap(&tmk, a.pool_k, slot_rows, a.n_kv_heads, 1, box, 1);
-    if (rc == NOVA_OK) rc = attn_make_tmap(&tmv, a.pool_v, slot_rows, a.n_kv_heads, 1, box, 1);
-    if (rc != NOVA_OK) return rc;
     const ChunkShape sh = chunk_shape(a.n_heads, a.n_kv_heads, a.max_tokens);
     int ctas = sm_count();
     if (ctas > kMaxSms) ctas = kMaxSms;
@@ -824,7 +848,7 @@ int launch_q8_chunk(const Q8Launch& a, cudaStream_t s) {
         }
         auto* kernel = a.fmt == NOVA_KV_I8 ? q8_chunk_kernel<NOVA_KV_I8> : q8_chunk_kernel<NOVA_KV_E4M3>;
         NOVA_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem));
-        cudaError_t e = launch_kernel_pdl(kernel, dim3((unsigned)ctas), dim3(kThreads), (size_t)kSmem, s, true, b, tmk, tmv, sh);
+        cudaError_t e = launch_kernel_pdl(kernel, dim3((unsigned)ctas), dim3(kThreads), (size_t)kSmem, s, true, b, sh);
         if (e == cudaSuccess) {
             count_launch();
             e = launch_kernel_pdl(q8_chunk_merge_kernel, dim3((unsigned)ctas - 1, 4u), dim3(128), 0, s, true, b, sh, ctas);

@@ -247,6 +247,9 @@ __device__ __forceinline__ void sts128(uint32_t addr, float4 v) {
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
+}
 // Transpose of an 8 x 8 matrix of 16-bit values over the warp (lane 4 r + c holds row r, columns 2c and 2c + 1).
 __device__ __forceinline__ uint32_t movmatrix(uint32_t x) {
     uint32_t y;
