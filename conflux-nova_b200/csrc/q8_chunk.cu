@@ -8,7 +8,7 @@
 //     half of 128 rows (held twice, for alternate tiles), or two halves that share every K/V tile.  A unit of work is (session, kv head, tile of tokens); the 64-key tiles
 //     of all units form one line that is dealt out evenly over one CTA per SM, so neither short sessions, nor long ones, nor
 //     the causal triangle leave SMs idle.  Units that several CTAs worked on are merged by the kernel behind it.
-//   * Twenty warps: 8 softmax (thread = row), 2 issuing MMAs (one per half), 8 converting, each of which brings in its own 16 keys'
+//   * Twenty warps: 8 softmax (thread = row), 2 issuing MMAs (one per half), 8 converting, each of which brings in its own keys'
 //     codes and scales.  The pipe runs on from one unit to the next.
 //   * The tensor cores want fp16 operands, so a tile's codes become fp16 VALUES in shared memory, code times scale, in the
 //     128-byte-swizzle layout that is the K-major form for S = Q.K^T and the MN-major form for O += P.V.  A scale (K's over 16;
@@ -31,14 +31,14 @@ constexpr int kKeys = 64;                             // keys of a tile
 constexpr int kHalfRows = 128;                        // rows of a half = M of the MMAs
 constexpr int kSlab = kKeys * 128;                    // 64 rows x 128 B
 constexpr int kQSlab = kHalfRows * 128;
-constexpr int kRaw = 5;                               // tiles of codes in flight (16 KiB each)
+constexpr int kRaw = 2;                               // tiles of its own (every other) that a converting warp has in flight
 constexpr int kMasks = 8;                             // ring of "which keys exist", for the softmax
 constexpr int kMaxSessions = 512;                     // sessions of one launch
 constexpr int kOffK = 4 * kQSlab;                     // two fp16 K tiles (dims 0-63 | 64-127), two V tiles
 constexpr int kOffV = kOffK + 2 * 2 * kSlab;
-constexpr int kOffRaw = kOffV + 2 * 2 * kSlab;        // codes: K 8 KiB | V 8 KiB
-constexpr int kOffSc = kOffRaw + kRaw * 2 * kSlab;    // per tile 64 scales of K, 64 of V
-constexpr int kOffX = kOffSc + kRaw * 512;            // (m, l) of the second half's rows on their way to the first
+constexpr int kOffRaw = kOffV + 2 * 2 * kSlab;        // [converter][kRaw] 32 rows of codes
+constexpr int kOffSc = kOffRaw + kConv * kRaw * 4096;    // [converter][kRaw] their scales
+constexpr int kOffX = kOffSc + kConv * kRaw * 128;            // (m, l) of the second half's rows on their way to the first
 constexpr int kOffPlan = kOffX + kHalfRows * 8;
 struct ChunkPlan {
     long long line[kMaxSessions + 1];                 // where each session's tiles start on the line
@@ -112,6 +112,21 @@ __device__ __forceinline__ int plan_ctas(long long total, int grid) {
     const long long most = (total + kMinTiles - 1) / kMinTiles;
     return most < grid ? (int)most : grid;
 }
+// (a 64-bit division is a hundred instructions and more, and these are on the way to a CTA's first load)
+__device__ __forceinline__ long long div_ll(long long x, long long y) {
+    return ((unsigned long long)x | (unsigned long long)y) >> 32 ? x / y : (long long)((unsigned)x / (unsigned)y);
+}
+// Where CTA c begins: shares that differ by one at most.
+struct Shares {
+    long long each, more;      // the first `more` CTAs get one more than `each`
+};
+__device__ __forceinline__ Shares plan_shares(long long total, int n_ctas) {
+    Shares s;
+    s.each = div_ll(total, n_ctas);
+    s.more = total - s.each * n_ctas;
+    return s;
+}
+__device__ __forceinline__ long long cta_begin(const Shares& s, int c) { return c * s.each + (c < s.more ? c : s.more); }
 
 struct Unit {
     int s, kvh, t0, t_cnt, past;     // session, kv head, first token of the tile, its tokens
@@ -131,8 +146,8 @@ __device__ inline Unit find_unit(const Q8Launch& a, const ChunkShape& sh, const 
     u.s = lo;
     u.past = p.past[lo];
     const int count = p.count[lo], nqt = (count + sh.tq - 1) / sh.tq;
-    const long long off = pos - p.line[lo], per_head = (p.line[lo + 1] - p.line[lo]) / a.n_kv_heads;
-    u.kvh = (int)(off / per_head);
+    const long long off = pos - p.line[lo], per_head = div_ll(p.line[lo + 1] - p.line[lo], a.n_kv_heads);
+    u.kvh = (int)div_ll(off, per_head);
     long long rem = off - u.kvh * per_head, base = 0;
     int qt = 0, len = 0;
     long long before = 0;
@@ -209,8 +224,8 @@ q8_chunk_kernel(Q8Launch a, ChunkShape sh) {
     ChunkPlan& plan = *reinterpret_cast<ChunkPlan*>(smem_raw + kOffPlan);
     uint32_t& s_tmem = *reinterpret_cast<uint32_t*>(smem_raw + kOffBar + 512);
     volatile int& s_abort = *reinterpret_cast<volatile int*>(smem_raw + kOffBar + 516);
-    uint16_t* const s_mask = reinterpret_cast<uint16_t*>(smem_raw + kOffBar + 520);       // [kMasks][4] which keys of a tile exist, 16 to a word
-    uint16_t* const s_rmask = reinterpret_cast<uint16_t*>(smem_raw + kOffBar + 584);      // [kConv][kRaw] the same of a converter's 16 keys
+    uint32_t* const s_mask = reinterpret_cast<uint32_t*>(smem_raw + kOffBar + 520);       // [kMasks][2] which keys of a tile exist
+    uint32_t* const s_rmask = reinterpret_cast<uint32_t*>(smem_raw + kOffBar + 584);      // [kConv][kRaw] the same of a converter's 32 keys
     const int lane = (int)threadIdx.x & 31;
     const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0);
     const int G = a.n_heads / a.n_kv_heads;
@@ -223,9 +238,9 @@ q8_chunk_kernel(Q8Launch a, ChunkShape sh) {
     // so a parity is never taken for a later one.
     if (threadIdx.x == 0) {
         for (int i = 0; i < 2; ++i) {
-            mbar_init(bar_kfull + 8u * i, kConv / 2);
+            mbar_init(bar_kfull + 8u * i, kConv / 4);
             mbar_init(bar_kfree + 8u * i, sh.dual ? 1 : 2);
-            mbar_init(bar_vfull + 8u * i, kConv / 2);
+            mbar_init(bar_vfull + 8u * i, kConv / 4);
             mbar_init(bar_vfree + 8u * i, sh.dual ? 1 : 2);
             mbar_init(bar_qready + 8u * i, kHalfRows);
         }
@@ -254,7 +269,8 @@ q8_chunk_kernel(Q8Launch a, ChunkShape sh) {
         if ((base & 1023u) != 0 && threadIdx.x == 0) q8_flag(a, NOVA_ERR_UNSUPPORTED);
         return;
     }
-    const long long lo = (long long)blockIdx.x * total / n_ctas, hi = ((long long)blockIdx.x + 1) * total / n_ctas;
+    const Shares shares = plan_shares(total, n_ctas);
+    const long long lo = cta_begin(shares, (int)blockIdx.x), hi = cta_begin(shares, (int)blockIdx.x + 1);
     if (warp == 0) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&s_tmem)), "r"((uint32_t)kTmemCols) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
@@ -309,7 +325,7 @@ q8_chunk_kernel(Q8Launch a, ChunkShape sh) {
                 // of the unit before are all computed (this thread has waited for the last of them), so the operand can be overwritten.
                 constexpr float kQ = kAttnScale * kLog2e * kKDiv;
                 const int c = lane & 7;
-#pragma unroll 2
+#pragma unroll 4
                 for (int e8 = 0; e8 < 8; ++e8) {
                     const int r = 32 * (warp & 3) + 4 * e8 + (lane >> 3), rt = (row0 + r) / G, rg = row0 + r - rt * G;
                     const int rpos = u.past + u.t0 + rt;
@@ -366,17 +382,22 @@ q8_chunk_kernel(Q8Launch a, ChunkShape sh) {
             // rows that are nobody's see everything: they never slow a warp down, and nothing of them is written
             const int row_lim = row_ok ? row_pos : 0x7fffffff;
             const int row_lo = row_ok && a.window > 0 ? row_pos - a.window + 1 : 0;
+            const bool idle = __all_sync(0xffffffffu, !row_ok);
             float m_ref = -INFINITY, l = 0.f;
             int m = sh.dual ? (n + mine0) >> 1 : n;            // tiles of this half so far: which score buffer, which parity
 #pragma unroll 1
             for (int i = mine0; i < tiles; i += step, ++m) {
                 const int t = n + i;
                 if (!__all_sync(0xffffffffu, t5_wait(my_sready + 8u * (uint32_t)(m & 1), (uint32_t)(m >> 1) & 1u, &s_abort))) { failed = true; break; }
+                if (idle) {                                     // what P and O hold in these rows is nobody's
+                    mbar_arrive(my_pready + 8u * (uint32_t)(m & 1));
+                    continue;
+                }
                 tc_fence_after();
                 const uint32_t s_col = t_lane + col_s + 64u * (uint32_t)(m & 1);
                 const int key0 = (u.first16 << 4) + (u.tile0 + i) * kKeys;
                 const int hi_k = row_lim - key0, lo_k = row_lo - key0;       // first and last visible column
-                const unsigned long long there = *reinterpret_cast<const unsigned long long*>(s_mask + 4 * (t & (kMasks - 1)));    // (a page missing, or the last key passed)
+                const unsigned long long there = *reinterpret_cast<const unsigned long long*>(s_mask + 2 * (t & (kMasks - 1)));    // (a page missing, or the last key passed)
                 const bool all_seen = __all_sync(0xffffffffu, hi_k >= kKeys - 1 && lo_k <= 0) && there == ~0ull;
                 // Two passes over the scores, 32 columns at a time, both read from tensor memory: half the code and half the registers
                 // of one pass over 64 (with that, instruction fetches were the largest stall: sixteen warps run five loops here).
@@ -461,7 +482,7 @@ q8_chunk_kernel(Q8Launch a, ChunkShape sh) {
                 sts_f1(xml + 8u * (uint32_t)hrow + 4u, l);
                 for (int part = 0; part < 2 && !failed; ++part) {
 #pragma unroll 1
-                    for (int cc = 0; cc < 2; ++cc) {
+                    for (int cc = 0; cc < 2 && !idle; ++cc) {
                         uint32_t ov[32];
                         tmem_ld32(t_lane + col_o + 64u * (uint32_t)part + 32u * (uint32_t)cc, ov);
                         tmem_wait_ld();
@@ -505,8 +526,10 @@ q8_chunk_kernel(Q8Launch a, ChunkShape sh) {
                     }
                 }
                 uint32_t ov[32];
-                tmem_ld32(t_lane + col_o + 32u * (uint32_t)cc, ov);
-                tmem_wait_ld();
+                if (!idle) {
+                    tmem_ld32(t_lane + col_o + 32u * (uint32_t)cc, ov);
+                    tmem_wait_ld();
+                }
                 if (row_ok) {
 #pragma unroll
                     for (int c = 0; c < 32; c += 4) {
@@ -606,12 +629,13 @@ q8_chunk_kernel(Q8Launch a, ChunkShape sh) {
         }
     } else {
         // ---------------------------------------------------------------------------------------- codes -> fp16 operands
-        // Four warps for K, four for V: V's buffer comes free only after the softmax of its tile, and the next K must not wait for that.
-        // A warp owns 16 keys of the tile and brings their codes and scales in itself, kRaw tiles ahead, with 16-byte asynchronous copies
-        // into a ring of its own, which needs no barrier.  (As TMA boxes the rows of one head are 2 KiB a copy, too little: one
-        // warp issuing all of a tile's copies took 1900 cycles, eight warps with a box and a run of scales each 900.)
+        // Four warps for K, four for V (V's buffer comes free only after the softmax of its tile, and the next K must not wait for
+        // that); of the four, two take the even tiles and two the odd ones, 32 keys each.  A warp brings its codes and scales in itself,
+        // kRaw tiles ahead, with 16-byte asynchronous copies into a ring of its own, which needs no barrier.  (As TMA boxes the rows of one
+        // head are 2 KiB a copy, too little: one warp issuing all of a tile's copies took 1900 cycles a tile, eight warps with a box
+        // and a run of scales each 900.  16 keys of every tile a warp: 1500 cycles a tile, most of it latency.)
         regs_down<88>();
-        const int which = warp >= 16, w = warp & 3, me = warp - 12;
+        const int me = warp - 12, which = me >> 2, par = me >> 1 & 1, hw = me & 1;
         const bool p8 = a.kv_shift == 3;
         const unsigned char* const pool = static_cast<const unsigned char*>(which ? a.pool_v : a.pool_k);
         const float* const scales = which ? a.scale_v : a.scale_k;
@@ -624,8 +648,7 @@ q8_chunk_kernel(Q8Launch a, ChunkShape sh) {
         const float* scale_u = nullptr;
         const uint32_t row_bytes = (uint32_t)a.n_kv_heads * kHeadDim, page_bytes = row_bytes << a.kv_shift, page_scales = (uint32_t)a.n_kv_heads << a.kv_shift;
         bool more = true;
-        int c_i = 0, c_key = 0, b0 = 0, b1 = 0, n0 = 0, n1 = 0, issued = 0;
-        uint32_t c_stage = 0;
+        int c_i = 0, c_key = 0, c_own = 0, b0 = 0, b1 = 0, n0 = 0, n1 = 0, issued = 0;      // c_i, c_own: own tiles of the part, done and in all
         // block-table entry of the page that holds a key; -1: a bad one, -2: there is no such key
         auto entry = [&](int key) -> int {
             if (key >= u.keys_end) return -2;
@@ -634,120 +657,128 @@ q8_chunk_kernel(Q8Launch a, ChunkShape sh) {
             const int e = __ldg(table + page);
             return e >= 0 && e < a.nb ? e : -1;
         };
-        auto fetch = [&](int i) {                          // lane's tile of the next 32
+        auto fetch = [&](int i) {                          // of own tiles i .. i + 15: lane = (tile, which 16 of its keys)
             n0 = n1 = -2;
-            if (i < u.tiles) {
-                n0 = entry(c_key + i * kKeys);
-                if (p8) n1 = entry(c_key + i * kKeys + 8);
+            if (i + (lane >> 1) < c_own) {
+                const int key = c_key + (i + (lane >> 1)) * 2 * kKeys + 16 * (lane & 1);
+                n0 = entry(key);
+                if (p8) n1 = entry(key + 8);
             }
         };
+        const uint32_t raw0 = base + kOffRaw + (uint32_t)(me * kRaw * 4096), rsc0 = base + kOffSc + (uint32_t)(me * kRaw * 128);
         auto issue_next = [&]() {
             if (!more) return;
-            if (c_i == u.tiles) {
+            while (c_i == c_own) {
+                n += u.tiles;
                 if (!next_part()) {
                     more = false;
                     return;
                 }
+                const int i0 = (par + n) & 1;
                 c_i = 0;
+                c_own = (u.tiles - i0 + 1) >> 1;
                 table = q8_table(a, u.s);
-                c_key = (u.first16 << 4) + u.tile0 * kKeys + 16 * w;
+                c_key = (u.first16 << 4) + (u.tile0 + i0) * kKeys + 32 * hw;
                 const int64_t page0 = (int64_t)a.layer * a.nb;
                 pool_u = pool + page0 * page_bytes + (uint32_t)(u.kvh * kHeadDim) + (uint32_t)lrow * row_bytes + 16u * (uint32_t)lch;
                 scale_u = scales + page0 * page_scales + ((uint32_t)u.kvh << a.kv_shift) + 4 * (lane & 1);
-                fetch(lane);
+                fetch(0);
             }
-            if ((c_i & 31) == 0) {
+            if ((c_i & 15) == 0) {
                 b0 = n0;
                 b1 = n1;
-                fetch(c_i + 32 + lane);
+                fetch(c_i + 16);
             }
-            const int e0 = __shfl_sync(0xffffffffu, b0, c_i & 31);
-            int e1 = -2;
-            if (p8) e1 = __shfl_sync(0xffffffffu, b1, c_i & 31);
-            const int key = c_key + c_i * kKeys, left = u.keys_end - key, slot = key & slot_mask;
-            if (lane == 0) {
-                uint32_t mask = p8 ? (e0 >= 0 ? 0xffu : 0u) | (e1 >= 0 ? 0xff00u : 0u) : (e0 >= 0 ? 0xffffu : 0u);
-                if (left < 16) mask &= left > 0 ? (1u << left) - 1u : 0u;
-                s_rmask[me * kRaw + c_stage] = (uint16_t)mask;
-                if (!which && (e0 == -1 || e1 == -1)) q8_flag(a, NOVA_ERR_BAD_TABLE);
-            }
-            const uint32_t dst = base + kOffRaw + c_stage * (2 * kSlab) + (uint32_t)(which * kSlab + w * 2048);
+            const int key = c_key + c_i * 2 * kKeys;
+            const uint32_t st = (uint32_t)(issued & (kRaw - 1)), dst = raw0 + st * 4096u + (uint32_t)(lrow * 128);
+            int mine = 0;                                  // the entry behind key `lane`
 #pragma unroll
-            for (int hf = 0; hf < 2; ++hf) {               // eight rows each: one page of 8, or half of the 16 slots
-                const int e = p8 && hf ? e1 : e0, s0 = p8 ? 0 : slot + 8 * hf;
-                if (e < 0) continue;
-                const unsigned char* src = pool_u + (uint64_t)(uint32_t)e * page_bytes + (uint32_t)s0 * row_bytes;
-                cp_async16(dst + (uint32_t)((8 * hf + lrow) * 128 + ((lch ^ lrow) << 4)), src);
-                cp_async16(dst + (uint32_t)((8 * hf + lrow + 4) * 128 + ((lch ^ (lrow + 4)) << 4)), src + 4 * row_bytes);
-                if ((lane >> 1) == hf)                      // scales: four keys a lane
-                    cp_async16(base + kOffSc + c_stage * 512u + (uint32_t)(which * 256 + w * 64 + 16 * lane), scale_u + (uint64_t)(uint32_t)e * page_scales + s0);
+            for (int g8 = 0; g8 < 4; ++g8) {               // eight rows each: one page of 8, or half of 16 slots
+                int e = __shfl_sync(0xffffffffu, b0, (2 * c_i + (g8 >> 1)) & 31);
+                if (p8) {
+                    const int f = __shfl_sync(0xffffffffu, b1, (2 * c_i + (g8 >> 1)) & 31);
+                    if (g8 & 1) e = f;
+                }
+                if (lrow == g8) mine = e;
+                if (e >= 0) {
+                    const int s0 = (key + 8 * g8) & slot_mask;
+                    const unsigned char* src = pool_u + (uint64_t)(uint32_t)e * page_bytes + (uint32_t)s0 * row_bytes;
+                    cp_async16(dst + (uint32_t)(g8 * 1024 + ((lch ^ lrow) << 4)), src);
+                    cp_async16(dst + (uint32_t)(g8 * 1024 + 512 + ((lch ^ (lrow + 4)) << 4)), src + 4 * row_bytes);
+                    if ((lane >> 1) == g8) cp_async16(rsc0 + st * 128u + (uint32_t)(16 * lane), scale_u + (uint64_t)(uint32_t)e * page_scales + s0);      // four keys a lane
+                }
+            }
+            const uint32_t mask = __ballot_sync(0xffffffffu, mine >= 0 && key + lane < u.keys_end);
+            const bool bad = __any_sync(0xffffffffu, mine == -1);
+            if (lane == 0) {
+                s_rmask[me * kRaw + st] = mask;
+                if (bad && !which) q8_flag(a, NOVA_ERR_BAD_TABLE);
             }
             ++c_i;
             ++issued;
-            if (++c_stage == kRaw) c_stage = 0;
         };
         // ---- what is converted now.  Eight lanes share two rows that differ in bits 0 and 2: four 16-byte pieces of each, apart both
         // where they are read (piece c of row r sits at c ^ (r & 7)) and where they are written (pieces 2c and 2c + 1, likewise).
         const int r8 = (lane >> 3) ^ (5 * (lane >> 2 & 1)), c4 = lane & 3;
-        const uint32_t bar_full = which ? bar_vfull : bar_kfull, bar_free = which ? bar_vfree : bar_kfree;
-        const uint32_t dst0 = base + (which ? kOffV : kOffK) + (uint32_t)(16 * w + r8) * 128u, src0 = base + kOffRaw + (uint32_t)(which * kSlab) + (uint32_t)(16 * w + r8) * 128u;
-        const uint32_t sc0 = base + kOffSc + (uint32_t)(which * 256 + (16 * w + r8) * 4);
+        const uint32_t bar_full = (which ? bar_vfull : bar_kfull) + 8u * (uint32_t)par, bar_free = (which ? bar_vfree : bar_kfree) + 8u * (uint32_t)par;
+        const uint32_t dst0 = base + (which ? kOffV : kOffK) + (uint32_t)par * (2 * kSlab) + (uint32_t)(32 * hw + r8) * 128u;
         const float div = which ? 1.f : 1.f / kKDiv;
         for (int k = 0; k < kRaw; ++k) {
             issue_next();
             asm volatile("cp.async.commit_group;" ::: "memory");
         }
-        uint32_t stage = 0;
 #pragma unroll 1
-        for (int t = 0; t < issued; ++t) {
+        for (int j = 0; j < issued; ++j) {                          // tile 2 j + par of the CTA's line
             asm volatile("cp.async.wait_group %0;" ::"n"(kRaw - 1) : "memory");      // (a group per tile, empty ones at the end)
             __syncwarp();
-            const bool ok = t < 2 || t5_wait(bar_free + 8u * (uint32_t)(t & 1), (uint32_t)(t / 2 - 1) & 1u, &s_abort);
-            if (!__all_sync(0xffffffffu, ok)) { failed = true; break; }
-            const uint32_t mask = s_rmask[me * kRaw + stage];
-            if (!which && lane == 0) s_mask[4 * (t & (kMasks - 1)) + w] = (uint16_t)mask;
-            const uint32_t src = src0 + stage * (2 * kSlab), dst = dst0 + (uint32_t)(t & 1) * (2 * kSlab);
-            uint4 code[4];                                          // rows r8 and r8 + 8, dims of slab 0 and 1
-            float f[2];
+            if (j > 0 && !__all_sync(0xffffffffu, t5_wait(bar_free, (uint32_t)(j - 1) & 1u, &s_abort))) { failed = true; break; }
+            const uint32_t st = (uint32_t)(j & (kRaw - 1)), mask = s_rmask[me * kRaw + st];
+            if (!which && lane == 0) s_mask[2 * ((2 * j + par) & (kMasks - 1)) + hw] = mask;
+            const uint32_t src = raw0 + st * 4096u + (uint32_t)r8 * 128u;
+            // two rows (r8 and r8 + 8) at a time
 #pragma unroll
-            for (int e = 0; e < 4; ++e) code[e] = lds128(src + (uint32_t)(e >> 1) * 1024u + (((uint32_t)(4 * (e & 1) + c4) ^ (uint32_t)r8) << 4));
+            for (int q = 0; q < 2; ++q) {
+                uint4 code[4];                                      // dims of slab 0 and 1 of each
+                float f[2];
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                f[e] = lds_f1(sc0 + stage * 512u + (uint32_t)e * 32u);
-                if (!(mask >> (8 * e + r8) & 1u)) {                   // what does not exist may hold anything: zeros instead
-                    code[2 * e] = code[2 * e + 1] = make_uint4(0u, 0u, 0u, 0u);
-                    f[e] = 0.f;
-                }
-            }
+                for (int e = 0; e < 4; ++e) code[e] = lds128(src + (uint32_t)(q * 2048 + (e >> 1) * 1024) + (((uint32_t)(4 * (e & 1) + c4) ^ (uint32_t)r8) << 4));
 #pragma unroll
-            for (int e2 = 0; e2 < 2; ++e2) {
-                const float fs = fminf(f[e2] * div, 65504.f / q8_qmax<kFmt>());
-                const __half hi1 = __float2half_rn(fs);
-                const __half2 hi2 = __half2half2(hi1), lo2 = __half2half2(__float2half_rn(fs - __half2float(hi1)));
-#pragma unroll
-                for (int e = 2 * e2; e < 2 * e2 + 2; ++e) {
-                    uint32_t h[8];
-                    q8_to_h2<kFmt>(code[e].x, h[0], h[1]);
-                    q8_to_h2<kFmt>(code[e].y, h[2], h[3]);
-                    q8_to_h2<kFmt>(code[e].z, h[4], h[5]);
-                    q8_to_h2<kFmt>(code[e].w, h[6], h[7]);
-#pragma unroll
-                    for (int b = 0; b < 8; ++b) {
-                        const __half2 x = *reinterpret_cast<const __half2*>(&h[b]);
-                        const __half2 y = __hfma2(x, hi2, __hmul2(x, lo2));
-                        h[b] = *reinterpret_cast<const uint32_t*>(&y);
+                for (int e = 0; e < 2; ++e) {
+                    f[e] = lds_f1(rsc0 + st * 128u + (uint32_t)((16 * q + 8 * e + r8) * 4));
+                    if (!(mask >> (16 * q + 8 * e + r8) & 1u)) {      // what does not exist may hold anything: zeros instead
+                        code[2 * e] = code[2 * e + 1] = make_uint4(0u, 0u, 0u, 0u);
+                        f[e] = 0.f;
                     }
-                    const uint32_t de = dst + (uint32_t)(e2 * 1024 + (e & 1) * kSlab);
-                    asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(de + (((uint32_t)(2 * c4) ^ (uint32_t)r8) << 4)), "r"(h[0]), "r"(h[1]), "r"(h[2]), "r"(h[3]) : "memory");
-                    asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(de + (((uint32_t)(2 * c4 + 1) ^ (uint32_t)r8) << 4)), "r"(h[4]), "r"(h[5]), "r"(h[6]), "r"(h[7]) : "memory");
+                }
+#pragma unroll
+                for (int e2 = 0; e2 < 2; ++e2) {
+                    const float fs = fminf(f[e2] * div, 65504.f / q8_qmax<kFmt>());
+                    const __half hi1 = __float2half_rn(fs);
+                    const __half2 hi2 = __half2half2(hi1), lo2 = __half2half2(__float2half_rn(fs - __half2float(hi1)));
+#pragma unroll
+                    for (int e = 2 * e2; e < 2 * e2 + 2; ++e) {
+                        uint32_t h[8];
+                        q8_to_h2<kFmt>(code[e].x, h[0], h[1]);
+                        q8_to_h2<kFmt>(code[e].y, h[2], h[3]);
+                        q8_to_h2<kFmt>(code[e].z, h[4], h[5]);
+                        q8_to_h2<kFmt>(code[e].w, h[6], h[7]);
+#pragma unroll
+                        for (int b = 0; b < 8; ++b) {
+                            const __half2 x = *reinterpret_cast<const __half2*>(&h[b]);
+                            const __half2 y = __hfma2(x, hi2, __hmul2(x, lo2));
+                            h[b] = *reinterpret_cast<const uint32_t*>(&y);
+                        }
+                        const uint32_t de = dst0 + (uint32_t)(q * 2048 + e2 * 1024 + (e & 1) * kSlab);
+                        asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(de + (((uint32_t)(2 * c4) ^ (uint32_t)r8) << 4)), "r"(h[0]), "r"(h[1]), "r"(h[2]), "r"(h[3]) : "memory");
+                        asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(de + (((uint32_t)(2 * c4 + 1) ^ (uint32_t)r8) << 4)), "r"(h[4]), "r"(h[5]), "r"(h[6]), "r"(h[7]) : "memory");
+                    }
                 }
             }
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
-            if (lane == 0) mbar_arrive(bar_full + 8u * (uint32_t)(t & 1));
+            if (lane == 0) mbar_arrive(bar_full);
             issue_next();                                           // into the stage that has just been read
             asm volatile("cp.async.commit_group;" ::: "memory");
-            if (++stage == kRaw) stage = 0;
         }
         asm volatile("cp.async.wait_all;" ::: "memory");           // (nothing may land after the CTA is gone)
     }
@@ -768,7 +799,9 @@ __global__ void __launch_bounds__(128) q8_chunk_merge_kernel(Q8Launch a, ChunkSh
     build_plan(a, sh, plan, false);       // (positions and row starts: written before the attention kernel, which waited)
     const long long total = plan.line[a.n_sessions];
     const int n_ctas = plan_ctas(total, grid_split), c1 = (int)blockIdx.x + 1;
-    auto begin = [&](int c) -> long long { return (long long)c * total / n_ctas; };
+    Shares shares = {};
+    if (n_ctas > 0) shares = plan_shares(total, n_ctas);
+    auto begin = [&](int c) -> long long { return cta_begin(shares, c); };
     Unit u = {};
     int tile, count, c_end = 0;
     bool todo = c1 < n_ctas;
