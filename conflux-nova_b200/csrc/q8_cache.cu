@@ -5,7 +5,6 @@
 // 448 (e4m3).  The three fp32 operations are rounded once each, so the codes are the same wherever the formula is followed.
 // Reading: value = code * scale.
 #include <cstring>
-#include <type_traits>
 
 #include "q8_common.cuh"
 
@@ -13,214 +12,224 @@ namespace novab {
 namespace {
 
 // A CTA takes kJobs consecutive (token, row) jobs - a token's rows are its K heads, its V heads and, where q is rotated in place
-// too, its query heads - a warp eight of them, 16 lanes a row, 8 values a lane.  What the rows hold is asked for before it is
-// known where they go (session, position, page: a chain of dependent loads, one thread per token), so that one wait covers
-// both.  Bound by HBM: 2 * 128 * (io bytes) read and 2 * 132 written per token and kv head.
+// too, its query heads - a warp eight of them, eight lanes a row: lane c the values 8c .. 8c + 7 and 64 + 8c .. 64 + 8c + 7, so that
+// both kinds of rotary pairs sit in one lane.  What the rows hold is asked for before it is known where they go (session,
+// position, page: a chain of dependent loads, one thread per token), so that one wait covers both.
+// HBM should bound it (2 * 128 * (io bytes) read and 2 * 132 written per token and kv head); with 16 lanes a row, addresses in 64
+// bits and two divisions in every lane the instructions did (1300 per warp: 253 MB in 141 us).
 constexpr int kJobs = 64;
 struct Place {
-    int64_t page;      // page of the pools (layer included), or -1
-    int64_t pos;       // position, or -1: nobody's row
-    int slot;
+    int64_t row;       // code row of kv head 0 in the pools, or -1: nowhere
+    int64_t scale;     // scale of kv head 0
+    int pos;           // position, or -1: nobody's row
 };
 
-__device__ __forceinline__ void q8_places(const Q8Launch& a, Place* places, int64_t job0, int units) {
+constexpr int kStarts = 256;       // row starts kept in shared memory (more sessions: searched where they are)
+struct PlaceSmem {
+    Place places[kJobs];
+    int starts[kStarts];
+};
+
+// The chain row starts -> (session) position and slice -> page is three round trips to memory.
+__device__ __forceinline__ void q8_places(const Q8Launch& a, PlaceSmem& sm, int64_t job0, int units) {
     const int tok0 = (int)(job0 / units);
     const int64_t last = (job0 + kJobs - 1) / units;
     const int tok1 = last < a.n_tokens - 1 ? (int)last : a.n_tokens - 1;
+    const bool staged = a.tok_start && a.n_sessions <= kStarts;
+    if (staged) {
+        for (int i = (int)threadIdx.x; i < a.n_sessions; i += (int)blockDim.x) sm.starts[i] = __ldg(a.tok_start + i);
+        __syncthreads();
+    }
     for (int i = (int)threadIdx.x; i <= tok1 - tok0; i += (int)blockDim.x) {
         Place p;
-        p.page = p.pos = -1;
-        p.slot = 0;
-        int t;
-        const int s = q8_session_of(a, tok0 + i, t);
+        p.row = p.scale = -1;
+        p.pos = -1;
+        int t, s;
+        if (staged) {
+            int lo = 0, up = a.n_sessions;
+            while (up - lo > 1) {
+                const int mid = (lo + up) >> 1;
+                if (sm.starts[mid] <= tok0 + i) lo = mid; else up = mid;
+            }
+            int first, count;
+            q8_rows(a, lo, first, count);
+            t = tok0 + i - first;
+            s = t >= 0 && t < count ? lo : -1;
+        } else {
+            s = q8_session_of(a, tok0 + i, t);
+        }
         if (s >= 0) {
             const int64_t pos = (int64_t)__ldg(a.n_past + s) + t;
-            if (pos < 0) {
+            const int32_t* const table = q8_table(a, s);
+            if (pos < 0 || pos > 0x7fffffff) {
                 q8_flag(a, NOVA_ERR_INVALID);
             } else {
-                p.pos = pos;
+                p.pos = (int)pos;
                 const int64_t lb = pos >> a.kv_shift;
-                const int phys = lb < a.table_stride ? __ldg(q8_table(a, s) + lb) : -1;
-                if (phys >= 0 && phys < a.nb) p.page = (int64_t)a.layer * a.nb + phys;
-                else q8_flag(a, NOVA_ERR_BAD_TABLE);
-                p.slot = (int)(pos & ((1 << a.kv_shift) - 1));
+                const int phys = lb < a.table_stride ? __ldg(table + lb) : -1;
+                if (phys >= 0 && phys < a.nb) {
+                    const int64_t page = (int64_t)a.layer * a.nb + phys;
+                    const int slot = (int)(pos & ((1 << a.kv_shift) - 1));
+                    p.row = ((page << a.kv_shift) + slot) * a.n_kv_heads;
+                    p.scale = ((page * a.n_kv_heads) << a.kv_shift) + slot;
+                } else {
+                    q8_flag(a, NOVA_ERR_BAD_TABLE);
+                }
             }
         }
-        places[i] = p;
+        sm.places[i] = p;
     }
     __syncthreads();
 }
 
-template <typename T>
-__device__ __forceinline__ void load8(const void* base, int64_t elem, float (&x)[8]) {
-    const T* p = static_cast<const T*>(base) + elem;
-    if constexpr (sizeof(T) == 2) {
-        const uint4 u = __ldg(reinterpret_cast<const uint4*>(p));
-        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            if constexpr (std::is_same<T, __half>::value) {
-                const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[e]));
-                x[2 * e] = f.x;
-                x[2 * e + 1] = f.y;
-            } else {
-                x[2 * e] = __uint_as_float(w[e] << 16);
-                x[2 * e + 1] = __uint_as_float(w[e] & 0xffff0000u);
-            }
-        }
-    } else {
-        const float4 u = *reinterpret_cast<const float4*>(p), v = *reinterpret_cast<const float4*>(p + 4);
-        x[0] = u.x; x[1] = u.y; x[2] = u.z; x[3] = u.w;
-        x[4] = v.x; x[5] = v.y; x[6] = v.z; x[7] = v.w;
-    }
-}
-
-// Rotates a row of which this lane (of 16) holds the values 8 l .. 8 l + 7.  All lanes of the warp.
-__device__ __forceinline__ void rotate8(float (&x)[8], int64_t pos, int l, const Q8Launch& a) {
-    if (a.neox) {               // pairs (d, d + 64): the partner sits 8 lanes away
-        const int64_t i = pos * 64 + 8 * (l & 7);
-        float c[8], n[8];
-        load8<float>(a.rope_cs, i, c);
-        load8<float>(a.rope_sn, i, n);
+// Rotates a row of which this lane holds x0 (8c ..) and x1 (64 + 8c ..).
+__device__ __forceinline__ void rotate16(float (&x0)[8], float (&x1)[8], int pos, int c, const Q8Launch& a) {
+    const int64_t i = (int64_t)pos * 64 + (a.neox ? 8 : 4) * c;
+    const int second = a.neox ? 4 : 32;           // neox: the pairs (d, d + 64); else neighbours, in both halves of the dims
+    const float4 c0 = __ldg(reinterpret_cast<const float4*>(a.rope_cs + i)), c1 = __ldg(reinterpret_cast<const float4*>(a.rope_cs + i + second));
+    const float4 s0 = __ldg(reinterpret_cast<const float4*>(a.rope_sn + i)), s1 = __ldg(reinterpret_cast<const float4*>(a.rope_sn + i + second));
+    const float cc[8] = {c0.x, c0.y, c0.z, c0.w, c1.x, c1.y, c1.z, c1.w}, ss[8] = {s0.x, s0.y, s0.z, s0.w, s1.x, s1.y, s1.z, s1.w};
+    if (a.neox) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-            const float y = __shfl_xor_sync(0xffffffffu, x[e], 8);
-            x[e] = l < 8 ? __fmaf_rn(x[e], c[e], -__fmul_rn(y, n[e])) : __fmaf_rn(y, n[e], __fmul_rn(x[e], c[e]));
+            const float y0 = x0[e], y1 = x1[e];
+            x0[e] = __fmaf_rn(y0, cc[e], -__fmul_rn(y1, ss[e]));
+            x1[e] = __fmaf_rn(y0, ss[e], __fmul_rn(y1, cc[e]));
         }
     } else {
-        const float4 c = *reinterpret_cast<const float4*>(a.rope_cs + pos * 64 + 4 * l), n = *reinterpret_cast<const float4*>(a.rope_sn + pos * 64 + 4 * l);
-        const float cc[4] = {c.x, c.y, c.z, c.w}, nn[4] = {n.x, n.y, n.z, n.w};
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const float x0 = x[2 * e], x1 = x[2 * e + 1];
-            x[2 * e] = __fmaf_rn(x0, cc[e], -__fmul_rn(x1, nn[e]));
-            x[2 * e + 1] = __fmaf_rn(x0, nn[e], __fmul_rn(x1, cc[e]));
+        for (int e = 0; e < 8; ++e) {
+            float* const y = e < 4 ? x0 : x1;
+            const float y0 = y[2 * (e & 3)], y1 = y[2 * (e & 3) + 1];
+            y[2 * (e & 3)] = __fmaf_rn(y0, cc[e], -__fmul_rn(y1, ss[e]));
+            y[2 * (e & 3) + 1] = __fmaf_rn(y0, ss[e], __fmul_rn(y1, cc[e]));
         }
     }
 }
 
 template <int kFmt, typename T>
-__global__ void __launch_bounds__(256) q8_append_kernel(Q8Launch a) {
-    __shared__ Place places[kJobs];
-    const int lane = (int)threadIdx.x & 31, warp = (int)threadIdx.x >> 5, l = lane & 15;
+__global__ void __launch_bounds__(256, 4) q8_append_kernel(Q8Launch a) {
+    __shared__ PlaceSmem sm;
+    const int lane = (int)threadIdx.x & 31, warp = (int)threadIdx.x >> 5, c = lane & 7;
     const int NKV = a.n_kv_heads, units = 2 * NKV + (a.q_rot ? a.n_heads : 0);
-    const int64_t job0 = (int64_t)blockIdx.x * kJobs, jobs = (int64_t)a.n_tokens * units;
+    const int64_t job0 = (int64_t)blockIdx.x * kJobs;
     const int tok0 = (int)(job0 / units);
     pdl_wait();
-    float x[4][8];
-    int tok[4], unit[4];
+    pdl_launch_dependents();        // (a kernel that starts early reads nothing of the caller's that this one has not waited for)
+    float x0[2][8], x1[2][8];
+    int tok[2], unit[2];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int64_t job = job0 + 8 * warp + 2 * i + (lane >> 4);
-        tok[i] = job < jobs ? (int)(job / units) : -1;
-        unit[i] = job < jobs ? (int)(job - (int64_t)tok[i] * units) : 0;
+    for (int i = 0; i < 2; ++i) {
+        const unsigned j = (unsigned)(job0 - (int64_t)tok0 * units) + (unsigned)(8 * warp + 4 * i + (lane >> 3)), dt = j / (unsigned)units;
+        tok[i] = tok0 + (int)dt < a.n_tokens ? tok0 + (int)dt : -1;
+        unit[i] = (int)(j - dt * (unsigned)units);
         if (tok[i] >= 0) {
             const bool is_v = unit[i] >= NKV;
-            if (unit[i] < 2 * NKV) load8<T>(is_v ? a.v : a.k, tok[i] * (is_v ? a.v_stride : a.k_stride) + (int64_t)(is_v ? unit[i] - NKV : unit[i]) * kHeadDim + 8 * l, x[i]);
-            else load8<float>(a.q_rot, ((int64_t)tok[i] * a.n_heads + unit[i] - 2 * NKV) * kHeadDim + 8 * l, x[i]);
+            if (unit[i] < 2 * NKV) {
+                const int64_t at = tok[i] * (is_v ? a.v_stride : a.k_stride) + (is_v ? unit[i] - NKV : unit[i]) * kHeadDim + 8 * c;
+                load8<T>(is_v ? a.v : a.k, at, x0[i]);
+                load8<T>(is_v ? a.v : a.k, at + 64, x1[i]);
+            } else {
+                const int64_t at = ((int64_t)tok[i] * a.n_heads + unit[i] - 2 * NKV) * kHeadDim + 8 * c;
+                load8<float>(a.q_rot, at, x0[i]);
+                load8<float>(a.q_rot, at + 64, x1[i]);
+            }
         } else {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) x[i][e] = 0.f;
+            for (int e = 0; e < 8; ++e) x0[i][e] = x1[i][e] = 0.f;
         }
     }
-    q8_places(a, places, job0, units);
+    q8_places(a, sm, job0, units);
+    float amax[2];
+    Place p[2];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const Place p = tok[i] >= 0 ? places[tok[i] - tok0] : Place{-1, -1, 0};
+    for (int i = 0; i < 2; ++i) {
+        if (tok[i] >= 0) p[i] = sm.places[tok[i] - tok0];
+        else p[i].row = p[i].pos = -1;
         const bool is_q = unit[i] >= 2 * NKV, is_v = !is_q && unit[i] >= NKV;
-        bool real = p.pos >= 0;
-        if (a.rope_cs) {
-            if (real && !is_v && p.pos >= a.rope_rows) {
-                real = false;
-                if (l == 0) q8_flag(a, NOVA_ERR_INVALID);
-            }
-            const bool turn = real && !is_v;
-            if (__any_sync(0xffffffffu, turn)) {
-                float y[8];
-#pragma unroll
-                for (int e = 0; e < 8; ++e) y[e] = x[i][e];
-                rotate8(y, turn ? p.pos : 0, l, a);
-#pragma unroll
-                for (int e = 0; e < 8; ++e)
-                    if (turn) x[i][e] = y[e];
-            }
-            float* const back = !turn ? nullptr : is_q ? a.q_rot + ((int64_t)tok[i] * a.n_heads + unit[i] - 2 * NKV) * kHeadDim
-                                        : a.k_rot ? a.k_rot + ((int64_t)tok[i] * NKV + unit[i]) * kHeadDim : nullptr;
-            if (back) {
-                *reinterpret_cast<float4*>(back + 8 * l) = make_float4(x[i][0], x[i][1], x[i][2], x[i][3]);
-                *reinterpret_cast<float4*>(back + 8 * l + 4) = make_float4(x[i][4], x[i][5], x[i][6], x[i][7]);
+        if (a.rope_cs && p[i].pos >= 0 && !is_v) {
+            if (p[i].pos >= a.rope_rows) {
+                p[i].row = -1;
+                if (c == 0) q8_flag(a, NOVA_ERR_INVALID);
+            } else {
+                rotate16(x0[i], x1[i], p[i].pos, c, a);
+                float* const back = is_q ? a.q_rot + ((int64_t)tok[i] * a.n_heads + unit[i] - 2 * NKV) * kHeadDim
+                                         : a.k_rot ? a.k_rot + ((int64_t)tok[i] * NKV + unit[i]) * kHeadDim : nullptr;
+                if (back) {
+                    *reinterpret_cast<float4*>(back + 8 * c) = make_float4(x0[i][0], x0[i][1], x0[i][2], x0[i][3]);
+                    *reinterpret_cast<float4*>(back + 8 * c + 4) = make_float4(x0[i][4], x0[i][5], x0[i][6], x0[i][7]);
+                    *reinterpret_cast<float4*>(back + 64 + 8 * c) = make_float4(x1[i][0], x1[i][1], x1[i][2], x1[i][3]);
+                    *reinterpret_cast<float4*>(back + 64 + 8 * c + 4) = make_float4(x1[i][4], x1[i][5], x1[i][6], x1[i][7]);
+                }
             }
         }
-        float amax = 0.f;
+        if (is_q) p[i].row = -1;
+        float m = 0.f;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) amax = fmaxf(amax, fabsf(x[i][e]));
+        for (int e = 0; e < 8; ++e) m = fmaxf(m, fmaxf(fabsf(x0[i][e]), fabsf(x1[i][e])));
 #pragma unroll
-        for (int o = 8; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-        if (is_q || !real || p.page < 0) continue;
-        amax = fmaxf(amax, kQ8MinAmax);
-        const float inv = __fdiv_rn(q8_qmax<kFmt>(), amax);
-        float y[8];
+        for (int o = 4; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+        amax[i] = fmaxf(m, kQ8MinAmax);
+    }
+    // the divisions of the warp's eight rows in one go: lane c of a row takes amax[c & 1]
+    const float am = c & 1 ? amax[1] : amax[0];
+    const float inv_c = __fdiv_rn(q8_qmax<kFmt>(), am), scale_c = __fdiv_rn(am, q8_qmax<kFmt>());
 #pragma unroll
-        for (int e = 0; e < 8; ++e) y[e] = __fmul_rn(x[i][e], inv);
-        const uint2 code = make_uint2(q8_encode4<kFmt>(make_float4(y[0], y[1], y[2], y[3])), q8_encode4<kFmt>(make_float4(y[4], y[5], y[6], y[7])));
+    for (int i = 0; i < 2; ++i) {
+        const float inv = __shfl_sync(0xffffffffu, inv_c, (lane & 24) + i);
+        if (p[i].row < 0) continue;
+        const bool is_v = unit[i] >= NKV;
         const int h = is_v ? unit[i] - NKV : unit[i];
-        unsigned char* const pool = static_cast<unsigned char*>(is_v ? a.pool_v : a.pool_k);
-        *reinterpret_cast<uint2*>(pool + (((p.page << a.kv_shift) + p.slot) * NKV + h) * kHeadDim + 8 * l) = code;
-        if (l == 0) (is_v ? a.scale_v : a.scale_k)[((p.page * NKV + h) << a.kv_shift) + p.slot] = __fdiv_rn(amax, q8_qmax<kFmt>());
+        float y0[8], y1[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            y0[e] = __fmul_rn(x0[i][e], inv);
+            y1[e] = __fmul_rn(x1[i][e], inv);
+        }
+        unsigned char* const dst = static_cast<unsigned char*>(is_v ? a.pool_v : a.pool_k) + (p[i].row + h) * kHeadDim + 8 * c;
+        *reinterpret_cast<uint2*>(dst) = make_uint2(q8_encode4<kFmt>(make_float4(y0[0], y0[1], y0[2], y0[3])), q8_encode4<kFmt>(make_float4(y0[4], y0[5], y0[6], y0[7])));
+        *reinterpret_cast<uint2*>(dst + 64) = make_uint2(q8_encode4<kFmt>(make_float4(y1[0], y1[1], y1[2], y1[3])), q8_encode4<kFmt>(make_float4(y1[4], y1[5], y1[6], y1[7])));
+        if (c == i) (is_v ? a.scale_v : a.scale_k)[p[i].scale + ((int64_t)h << a.kv_shift)] = scale_c;
     }
 }
 
-template <int kFmt>
+// Eight lanes a row: lane c the values 16 c .. 16 c + 15, a 16-byte load each.
+template <int kFmt, typename T>
 __global__ void __launch_bounds__(256) q8_read_kernel(Q8Launch a) {
-    __shared__ Place places[kJobs];
-    const int lane = (int)threadIdx.x & 31, warp = (int)threadIdx.x >> 5, l = lane & 15;
+    __shared__ PlaceSmem sm;
+    const int lane = (int)threadIdx.x & 31, warp = (int)threadIdx.x >> 5, c = lane & 7;
     const int NKV = a.n_kv_heads, units = 2 * NKV;
-    const int64_t job0 = (int64_t)blockIdx.x * kJobs, jobs = (int64_t)a.n_tokens * units;
+    const int64_t job0 = (int64_t)blockIdx.x * kJobs;
     const int tok0 = (int)(job0 / units);
     pdl_wait();
-    q8_places(a, places, job0, units);
-    uint2 code[4];
-    float scale[4];
-    int64_t dst[4];
+    q8_places(a, sm, job0, units);
+    uint4 code[2];
+    float scale[2];
+    T* dst[2];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int64_t job = job0 + 8 * warp + 2 * i + (lane >> 4);
-        dst[i] = -1;
-        if (job >= jobs) continue;
-        const int tok = (int)(job / units), unit = (int)(job - (int64_t)tok * units);
-        const Place p = places[tok - tok0];
-        if (p.page < 0) continue;
+    for (int i = 0; i < 2; ++i) {
+        const unsigned j = (unsigned)(job0 - (int64_t)tok0 * units) + (unsigned)(8 * warp + 4 * i + (lane >> 3)), dt = j / (unsigned)units;
+        const int tok = tok0 + (int)dt, unit = (int)(j - dt * (unsigned)units);
+        dst[i] = nullptr;
+        if (tok >= a.n_tokens) continue;
+        const Place p = sm.places[tok - tok0];
+        if (p.row < 0) continue;
         const bool is_v = unit >= NKV;
         const int h = is_v ? unit - NKV : unit;
-        const unsigned char* const pool = static_cast<const unsigned char*>(is_v ? a.pool_v : a.pool_k);
-        code[i] = __ldg(reinterpret_cast<const uint2*>(pool + (((p.page << a.kv_shift) + p.slot) * NKV + h) * kHeadDim + 8 * l));
-        scale[i] = __ldg((is_v ? a.scale_v : a.scale_k) + ((p.page * NKV + h) << a.kv_shift) + p.slot);
-        dst[i] = ((int64_t)tok * NKV + h) * kHeadDim + 8 * l;
-        if (is_v) dst[i] |= (int64_t)1 << 62;
+        code[i] = __ldg(reinterpret_cast<const uint4*>(static_cast<const unsigned char*>(is_v ? a.pool_v : a.pool_k) + (p.row + h) * kHeadDim + 16 * c));
+        scale[i] = __ldg((is_v ? a.scale_v : a.scale_k) + p.scale + ((int64_t)h << a.kv_shift));
+        dst[i] = static_cast<T*>(is_v ? a.v_out : a.k_out) + ((int64_t)tok * NKV + h) * kHeadDim + 16 * c;
     }
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        if (dst[i] < 0) continue;
-        void* const out = dst[i] >> 62 ? a.v_out : a.k_out;
-        const int64_t at = dst[i] & (((int64_t)1 << 62) - 1);
-        const float4 x = q8_decode4<kFmt>(code[i].x), y = q8_decode4<kFmt>(code[i].y);
+    for (int i = 0; i < 2; ++i) {
+        if (!dst[i]) continue;
+        const uint32_t w[4] = {code[i].x, code[i].y, code[i].z, code[i].w};
         const float f = scale[i];
-        const float v[8] = {x.x * f, x.y * f, x.z * f, x.w * f, y.x * f, y.y * f, y.z * f, y.w * f};
-        if (a.io == NOVA_IO_F32) {
-            *reinterpret_cast<float4*>(static_cast<float*>(out) + at) = make_float4(v[0], v[1], v[2], v[3]);
-            *reinterpret_cast<float4*>(static_cast<float*>(out) + at + 4) = make_float4(v[4], v[5], v[6], v[7]);
-        } else {
-            uint32_t w[4];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                if (a.io == NOVA_IO_F16) {
-                    w[e] = pack_h2(v[2 * e], v[2 * e + 1]);
-                } else {
-                    const __nv_bfloat162 b = __floats2bfloat162_rn(v[2 * e], v[2 * e + 1]);
-                    w[e] = *reinterpret_cast<const uint32_t*>(&b);
-                }
-            }
-            *reinterpret_cast<uint4*>(static_cast<unsigned char*>(out) + 2 * at) = make_uint4(w[0], w[1], w[2], w[3]);
+        for (int e = 0; e < 4; e += 2) {
+            const float4 x = q8_decode4<kFmt>(w[e]), y = q8_decode4<kFmt>(w[e + 1]);
+            const float v[8] = {x.x * f, x.y * f, x.z * f, x.w * f, y.x * f, y.y * f, y.z * f, y.w * f};
+            store8(dst[i] + 4 * e, v);
         }
     }
 }
@@ -273,6 +282,13 @@ static cudaError_t append_as(const Q8Launch& a, unsigned blocks, cudaStream_t s)
     return launch_kernel_pdl(q8_append_kernel<kFmt, __nv_bfloat16>, dim3(blocks), dim3(256), 0, s, true, a);
 }
 
+template <int kFmt>
+static cudaError_t read_as(const Q8Launch& a, unsigned blocks, cudaStream_t s) {
+    if (a.io == NOVA_IO_F32) return launch_kernel_pdl(q8_read_kernel<kFmt, float>, dim3(blocks), dim3(256), 0, s, true, a);
+    if (a.io == NOVA_IO_F16) return launch_kernel_pdl(q8_read_kernel<kFmt, __half>, dim3(blocks), dim3(256), 0, s, true, a);
+    return launch_kernel_pdl(q8_read_kernel<kFmt, __nv_bfloat16>, dim3(blocks), dim3(256), 0, s, true, a);
+}
+
 int launch_q8_append(const Q8Launch& a, cudaStream_t s) {
     if (a.n_tokens <= 0 || a.n_sessions <= 0) return NOVA_OK;
     const int64_t blocks = ((int64_t)a.n_tokens * (2 * a.n_kv_heads + (a.q_rot ? a.n_heads : 0)) + kJobs - 1) / kJobs;
@@ -290,8 +306,7 @@ int launch_q8_read(const Q8Launch& a, cudaStream_t s) {
     if (a.n_tokens <= 0 || a.n_sessions <= 0) return NOVA_OK;
     const int64_t blocks = ((int64_t)a.n_tokens * 2 * a.n_kv_heads + kJobs - 1) / kJobs;
     if (blocks > 0x7fffffffLL) return NOVA_ERR_TOO_LARGE;
-    const cudaError_t e = a.fmt == NOVA_KV_I8 ? launch_kernel_pdl(q8_read_kernel<NOVA_KV_I8>, dim3((unsigned)blocks), dim3(256), 0, s, true, a)
-                                              : launch_kernel_pdl(q8_read_kernel<NOVA_KV_E4M3>, dim3((unsigned)blocks), dim3(256), 0, s, true, a);
+    const cudaError_t e = a.fmt == NOVA_KV_I8 ? read_as<NOVA_KV_I8>(a, (unsigned)blocks, s) : read_as<NOVA_KV_E4M3>(a, (unsigned)blocks, s);
     if (e != cudaSuccess) {
         set_cuda_error(e, "8-bit read launch");
         return NOVA_ERR_CUDA;

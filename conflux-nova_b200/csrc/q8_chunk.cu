@@ -51,6 +51,9 @@ static_assert(kSmem <= 232448, "shared memory of one CTA");
 constexpr int kTmemCols = 512;                        // S of half h, buffer b: columns 128 h + 64 b (P over its first 32); O: 256 + 128 h
 constexpr uint32_t kColO = 256;
 constexpr float kKDiv = 16.f;                         // K goes in divided by this: magnitudes up to 2^20
+// As kQ8Step and kQ8Top (single tokens), but the reference moves less often, which costs more here (O rescaled in tensor
+// memory): weights are 2^7 .. 2^15 at the largest, with fp16's 11 bits down to 2^-21 of the reference.
+constexpr float kStep = 8.f, kTop = 7.f;
 constexpr int kSetup = 2;                             // what starting a unit costs, in tiles
 constexpr int kMinTiles = 4;                          // a CTA gets at least that many
 constexpr uint32_t kIdescS = (1u << 4) | ((uint32_t)(kKeys >> 3) << 17) | ((uint32_t)(kHalfRows >> 4) << 24);
@@ -215,7 +218,7 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16
 template <int kRegs> __device__ __forceinline__ void regs_up() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegs)); }
 template <int kRegs> __device__ __forceinline__ void regs_down() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegs)); }
 
-template <int kFmt>
+template <int kFmt, typename T>
 __global__ void __launch_bounds__(kThreads, 1)
 q8_chunk_kernel(Q8Launch a, ChunkShape sh) {
     // No static shared memory: the dynamic region then starts at the front of the CTA's window, which is 1024-byte aligned as the
@@ -258,15 +261,17 @@ q8_chunk_kernel(Q8Launch a, ChunkShape sh) {
         s_abort = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    // Nothing of the caller's is read before the kernels before this one are done; the merge kernel, which reads positions and
-    // row starts before its own wait, is let go only then.
-    pdl_wait();
+    // Nothing of the caller's is read before the kernels before this one are done, nor is the merge kernel let go, which reads
+    // positions and row starts before its own wait.  Behind the append kernel only the cache itself is waited for (by the
+    // converters): that kernel lets this one start once everything before it is done, and writes nothing else.
+    if (!a.append) pdl_wait();
     pdl_launch_dependents();
     build_plan(a, sh, plan, blockIdx.x == 0);
     const long long total = plan.line[a.n_sessions];
     const int n_ctas = plan_ctas(total, (int)gridDim.x);
     if ((int)blockIdx.x >= n_ctas || (base & 1023u) != 0) {            // uniform over the CTA; nothing has been allocated yet
         if ((base & 1023u) != 0 && threadIdx.x == 0) q8_flag(a, NOVA_ERR_UNSUPPORTED);
+        pdl_wait();                   // (a grid must not be done before the one that it follows)
         return;
     }
     const Shares shares = plan_shares(total, n_ctas);
@@ -329,19 +334,13 @@ q8_chunk_kernel(Q8Launch a, ChunkShape sh) {
                 for (int e8 = 0; e8 < 8; ++e8) {
                     const int r = 32 * (warp & 3) + 4 * e8 + (lane >> 3), rt = (row0 + r) / G, rg = row0 + r - rt * G;
                     const int rpos = u.past + u.t0 + rt;
-                    float x[16];
+                    float x0[8], x1[8];
 #pragma unroll
-                    for (int e = 0; e < 16; ++e) x[e] = 0.f;
+                    for (int e = 0; e < 8; ++e) x0[e] = x1[e] = 0.f;
                     if (rt < u.t_cnt && !(a.rope_cs && rpos >= a.rope_rows)) {
                         const int64_t qe = (tok0 + rt) * a.q_stride + (int64_t)(u.kvh * G + rg) * kHeadDim + 8 * c;
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const float4 v = q8_load4(a.q, qe + (e >> 1) * 64 + 4 * (e & 1), a.io);
-                            x[4 * e] = v.x;
-                            x[4 * e + 1] = v.y;
-                            x[4 * e + 2] = v.z;
-                            x[4 * e + 3] = v.w;
-                        }
+                        load8<T>(a.q, qe, x0);
+                        load8<T>(a.q, qe + 64, x1);
                         if (a.rope_cs) {
                             const float* cr = a.rope_cs + (int64_t)rpos * 64 + (a.neox ? 8 : 4) * c;
                             const float* sr = a.rope_sn + (int64_t)rpos * 64 + (a.neox ? 8 : 4) * c;
@@ -349,16 +348,20 @@ q8_chunk_kernel(Q8Launch a, ChunkShape sh) {
                             const float4 c0 = *reinterpret_cast<const float4*>(cr), c1 = *reinterpret_cast<const float4*>(cr + second);
                             const float4 s0 = *reinterpret_cast<const float4*>(sr), s1 = *reinterpret_cast<const float4*>(sr + second);
                             const float cc[8] = {c0.x, c0.y, c0.z, c0.w, c1.x, c1.y, c1.z, c1.w}, ss[8] = {s0.x, s0.y, s0.z, s0.w, s1.x, s1.y, s1.z, s1.w};
+                            if (a.neox) {
 #pragma unroll
-                            for (int e = 0; e < 8; ++e) {
-                                const float x0 = a.neox ? x[e] : x[2 * e], x1 = a.neox ? x[e + 8] : x[2 * e + 1];
-                                const float y0 = __fmaf_rn(x0, cc[e], -__fmul_rn(x1, ss[e])), y1 = __fmaf_rn(x0, ss[e], __fmul_rn(x1, cc[e]));
-                                if (a.neox) {
-                                    x[e] = y0;
-                                    x[e + 8] = y1;
-                                } else {
-                                    x[2 * e] = y0;
-                                    x[2 * e + 1] = y1;
+                                for (int e = 0; e < 8; ++e) {
+                                    const float y0 = x0[e], y1 = x1[e];
+                                    x0[e] = __fmaf_rn(y0, cc[e], -__fmul_rn(y1, ss[e]));
+                                    x1[e] = __fmaf_rn(y0, ss[e], __fmul_rn(y1, cc[e]));
+                                }
+                            } else {
+#pragma unroll
+                                for (int e = 0; e < 8; ++e) {
+                                    float* const y = e < 4 ? x0 : x1;
+                                    const float y0 = y[2 * (e & 3)], y1 = y[2 * (e & 3) + 1];
+                                    y[2 * (e & 3)] = __fmaf_rn(y0, cc[e], -__fmul_rn(y1, ss[e]));
+                                    y[2 * (e & 3) + 1] = __fmaf_rn(y0, ss[e], __fmul_rn(y1, cc[e]));
                                 }
                             }
                         }
@@ -366,7 +369,7 @@ q8_chunk_kernel(Q8Launch a, ChunkShape sh) {
 #pragma unroll
                     for (int hf = 0; hf < 2; ++hf) {
                         const uint32_t dst = base + (uint32_t)((2 * half + hf) * kQSlab + r * 128 + ((c ^ (r & 7)) << 4));
-                        const float* y = x + 8 * hf;
+                        const float* y = hf ? x1 : x0;
                         asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(dst), "r"(pack_h2(y[0] * kQ, y[1] * kQ)), "r"(pack_h2(y[2] * kQ, y[3] * kQ)),
                                      "r"(pack_h2(y[4] * kQ, y[5] * kQ)), "r"(pack_h2(y[6] * kQ, y[7] * kQ))
                                      : "memory");
@@ -424,11 +427,11 @@ q8_chunk_kernel(Q8Launch a, ChunkShape sh) {
                     mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
                 }
                 float scale = 1.f;
-                if (mx > m_ref + kQ8Step || (m_ref == -INFINITY && mx > -INFINITY)) {
+                if (mx > m_ref + kStep || (m_ref == -INFINITY && mx > -INFINITY)) {
                     scale = m_ref == -INFINITY ? 0.f : ex2(m_ref - mx);
                     m_ref = mx;
                 }
-                const float ms = m_ref == -INFINITY ? 0.f : kQ8Top - m_ref;         // nothing visible yet: keep exp arguments finite
+                const float ms = m_ref == -INFINITY ? 0.f : kTop - m_ref;         // nothing visible yet: keep exp arguments finite
                 const unsigned long long ms2 = pack_f2(ms, ms);
                 unsigned long long sum2[2] = {0ull, 0ull};
 #pragma unroll 1
@@ -539,7 +542,7 @@ q8_chunk_kernel(Q8Launch a, ChunkShape sh) {
                             v = make_float4(fmaf(__uint_as_float(y.x), w1, v.x), fmaf(__uint_as_float(y.y), w1, v.y), fmaf(__uint_as_float(y.z), w1, v.z),
                                             fmaf(__uint_as_float(y.w), w1, v.w));
                         }
-                        if (whole) q8_store4(a.out, oe + 32 * cc + c, a.io, v);
+                        if (whole) Q8Io<T>::store4(static_cast<T*>(a.out) + oe + 32 * cc + c, v);
                         else *reinterpret_cast<float4*>(slot + 4 * (size_t)sh.rows_cap + ((size_t)(8 * cc + (c >> 2)) * sh.rows_cap + row) * 4) = v;
                     }
                 }
@@ -647,7 +650,7 @@ q8_chunk_kernel(Q8Launch a, ChunkShape sh) {
         const unsigned char* pool_u = nullptr;             // rows of the part's kv head, this lane's row and piece
         const float* scale_u = nullptr;
         const uint32_t row_bytes = (uint32_t)a.n_kv_heads * kHeadDim, page_bytes = row_bytes << a.kv_shift, page_scales = (uint32_t)a.n_kv_heads << a.kv_shift;
-        bool more = true;
+        bool more = true, waited = !a.append;
         int c_i = 0, c_key = 0, c_own = 0, b0 = 0, b1 = 0, n0 = 0, n1 = 0, issued = 0;      // c_i, c_own: own tiles of the part, done and in all
         // block-table entry of the page that holds a key; -1: a bad one, -2: there is no such key
         auto entry = [&](int key) -> int {
@@ -688,6 +691,10 @@ q8_chunk_kernel(Q8Launch a, ChunkShape sh) {
                 b0 = n0;
                 b1 = n1;
                 fetch(c_i + 16);
+            }
+            if (!waited) {
+                pdl_wait();                                // the append before us has written the new rows
+                waited = true;
             }
             const int key = c_key + c_i * 2 * kKeys;
             const uint32_t st = (uint32_t)(issued & (kRaw - 1)), dst = raw0 + st * 4096u + (uint32_t)(lrow * 128);
@@ -790,8 +797,9 @@ q8_chunk_kernel(Q8Launch a, ChunkShape sh) {
 }
 
 // Merge of the units that several CTAs worked on: the unit that the place where CTA blockIdx.x + 1 begins falls into, unless an
-// earlier such place falls into it too.  blockIdx.y takes a share of the (32-row, 4-dim) pieces; thread = row.
-__global__ void __launch_bounds__(128) q8_chunk_merge_kernel(Q8Launch a, ChunkShape sh, int grid_split) {
+// earlier such place falls into it too.  blockIdx.y takes a share of the (32-row, 4-dim) pieces; thread = row.  A CTA is small enough
+// (two warps of 64 registers, 10 KiB) to wait beside an attention CTA, its plan and its unit already worked out.
+__global__ void __launch_bounds__(64, 16) q8_chunk_merge_kernel(Q8Launch a, ChunkShape sh, int grid_split) {
     __shared__ ChunkPlan plan;
     const int lane = (int)threadIdx.x & 31, warp = (int)threadIdx.x >> 5;
     const int G = a.n_heads / a.n_kv_heads;
@@ -819,7 +827,7 @@ __global__ void __launch_bounds__(128) q8_chunk_merge_kernel(Q8Launch a, ChunkSh
     if (!todo) return;
     const size_t slot_floats = (size_t)sh.rows_cap * kSlotW;
     const int rows = u.t_cnt * G, blocks = (rows + 31) / 32;
-    for (int piece = (int)blockIdx.y * 4 + warp; piece < blocks * 32; piece += (int)gridDim.y * 4) {
+    for (int piece = (int)blockIdx.y * 2 + warp; piece < blocks * 32; piece += (int)gridDim.y * 2) {
         const int row = (piece >> 5) * 32 + lane, d4 = piece & 31;
         if (row >= rows) continue;
         float M = -INFINITY, L = 0.f;
@@ -872,6 +880,7 @@ int launch_q8_chunk(const Q8Launch& a, cudaStream_t s) {
         b.n_past = a.n_past + s0;
         if (a.slice_ids) b.slice_ids = a.slice_ids + s0;
         else b.tables = a.tables + (int64_t)s0 * a.table_stride;
+        if (s0 > 0) b.append = 0;          // (its rows are written: this launch comes after another attention, which waited for them)
         if (a.tok_start) {
             b.tok_start = a.tok_start + s0;
         } else {
@@ -879,12 +888,13 @@ int launch_q8_chunk(const Q8Launch& a, cudaStream_t s) {
             b.q = static_cast<const unsigned char*>(a.q) + rows * a.q_stride * (int64_t)io_bytes;
             b.out = static_cast<unsigned char*>(a.out) + rows * a.out_stride * (int64_t)io_bytes;
         }
-        auto* kernel = a.fmt == NOVA_KV_I8 ? q8_chunk_kernel<NOVA_KV_I8> : q8_chunk_kernel<NOVA_KV_E4M3>;
+        auto* kernel = a.fmt == NOVA_KV_I8 ? (a.io == NOVA_IO_F32 ? q8_chunk_kernel<NOVA_KV_I8, float> : a.io == NOVA_IO_F16 ? q8_chunk_kernel<NOVA_KV_I8, __half> : q8_chunk_kernel<NOVA_KV_I8, __nv_bfloat16>)
+                                           : (a.io == NOVA_IO_F32 ? q8_chunk_kernel<NOVA_KV_E4M3, float> : a.io == NOVA_IO_F16 ? q8_chunk_kernel<NOVA_KV_E4M3, __half> : q8_chunk_kernel<NOVA_KV_E4M3, __nv_bfloat16>);
         NOVA_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem));
         cudaError_t e = launch_kernel_pdl(kernel, dim3((unsigned)ctas), dim3(kThreads), (size_t)kSmem, s, true, b, sh);
         if (e == cudaSuccess) {
             count_launch();
-            e = launch_kernel_pdl(q8_chunk_merge_kernel, dim3((unsigned)ctas - 1, 4u), dim3(128), 0, s, true, b, sh, ctas);
+            e = launch_kernel_pdl(q8_chunk_merge_kernel, dim3((unsigned)ctas - 1, 8u), dim3(64), 0, s, true, b, sh, ctas);
         }
         if (e != cudaSuccess) {
             set_cuda_error(e, "8-bit chunk attention launch");

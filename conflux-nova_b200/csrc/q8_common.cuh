@@ -7,6 +7,7 @@
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_fp8.h>
+#include <type_traits>
 
 #include "mma_common.cuh"
 
@@ -134,6 +135,48 @@ __device__ __forceinline__ void q8_store4(void* base, int64_t elem, int io, floa
     if (io == NOVA_IO_F32) Q8Io<float>::store4(static_cast<float*>(base) + elem, v);
     else if (io == NOVA_IO_F16) Q8Io<__half>::store4(static_cast<__half*>(base) + elem, v);
     else Q8Io<__nv_bfloat16>::store4(static_cast<__nv_bfloat16*>(base) + elem, v);
+}
+
+// Eight consecutive values (16 or 32 bytes).
+template <typename T>
+__device__ __forceinline__ void load8(const void* base, int64_t elem, float (&x)[8]) {
+    const T* p = static_cast<const T*>(base) + elem;
+    if constexpr (sizeof(T) == 2) {
+        const uint4 u = __ldg(reinterpret_cast<const uint4*>(p));
+        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            if constexpr (std::is_same<T, __half>::value) {
+                const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[e]));
+                x[2 * e] = f.x;
+                x[2 * e + 1] = f.y;
+            } else {
+                x[2 * e] = __uint_as_float(w[e] << 16);
+                x[2 * e + 1] = __uint_as_float(w[e] & 0xffff0000u);
+            }
+        }
+    } else {
+        const float4 u = *reinterpret_cast<const float4*>(p), v = *reinterpret_cast<const float4*>(p + 4);
+        x[0] = u.x; x[1] = u.y; x[2] = u.z; x[3] = u.w;
+        x[4] = v.x; x[5] = v.y; x[6] = v.z; x[7] = v.w;
+    }
+}
+
+__device__ __forceinline__ void store8(float* p, const float (&v)[8]) {
+    *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
+    *reinterpret_cast<float4*>(p + 4) = make_float4(v[4], v[5], v[6], v[7]);
+}
+__device__ __forceinline__ void store8(__half* p, const float (&v)[8]) {
+    *reinterpret_cast<uint4*>(p) = make_uint4(pack_h2(v[0], v[1]), pack_h2(v[2], v[3]), pack_h2(v[4], v[5]), pack_h2(v[6], v[7]));
+}
+__device__ __forceinline__ void store8(__nv_bfloat16* p, const float (&v)[8]) {
+    uint32_t w[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        const __nv_bfloat162 b = __floats2bfloat162_rn(v[2 * e], v[2 * e + 1]);
+        w[e] = *reinterpret_cast<const uint32_t*>(&b);
+    }
+    *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
 }
 
 // ---- codes: four of them in a word

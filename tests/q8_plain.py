@@ -209,7 +209,7 @@ def attention_bound(case, o, a, spread, floor, exact_q):
     truncated to 24 bits), the exponential's argument by 2^-23 of a magnitude below 2 spread.  Weights go to fp16 (2^-11; hi + lo: 2^-21),
     in chunks V too (2^-11 for its scale, 2^-11 for the product; below fp16's normal range 2^-25),
     their sums are rounded once per 16 keys (2^-23 each).  A weight below fp16's normal range is off by 2^-25 whatever it is, and
-    the largest weight of a row (p times v's scale) goes in as 2^11 or more: floor 2^-36 in all.  Last the rounding of the output
+    the largest weight of a row (p times v's scale) goes in as 2^11 or more, in chunks 2^7: floor 2^-36, 2^-32 in all.  Last the rounding of the output
     itself, half a step."""
     keys = max([p + n for p, n in zip(case.past, case.new)] + [1])
     chunk = max(case.new) > 1 or case.H // case.N > 8
@@ -220,4 +220,4 @@ def attention_bound(case, o, a, spread, floor, exact_q):
     rel = 2 * (e * (1 + e) + p_err) + (keys / 16 + 64) * 2.0 ** -23
     half = {"f32": 2.0 ** -24, "f16": 2.0 ** -11, "bf16": 2.0 ** -8}[case.io]
     tiny = {"f32": 1e-37, "f16": 2.0 ** -25, "bf16": 1e-37}[case.io]
-    return a * rel[..., None] + floor * 2.0 ** -36 + o.abs() * half + tiny + (2.0 ** -25 if chunk else 0.0)
+    return a * rel[..., None] + floor * 2.0 ** (-32 if chunk else -36) + o.abs() * half + tiny + (2.0 ** -25 if chunk else 0.0)
