@@ -141,6 +141,13 @@ class Ctx:
         return [float(x) for x in t.cpu().numpy()]
 
 
+KV_NAMES = {"f16": "fp16", "f32": "fp32", "i8": "int8", "e4m3": "e4m3"}
+
+
+def kv_type(nv, name):
+    return {"f16": nv.KV_F16, "f32": nv.KV_F32, "i8": nv.KV_I8, "e4m3": nv.KV_E4M3}[name]
+
+
 def configure_batch(nv, batch, args, prefix=False):
     """Kernel choice and launch options of a batch as the flags ask for them."""
     kernel = args.kernel
@@ -157,7 +164,7 @@ def configure_batch(nv, batch, args, prefix=False):
         batch.set_split_ctas(args.split_ctas)
     if kernel == 1 and args.prefill_kernel >= 0:
         nv.lib.nova_batch_set_prefill_kernel(batch.h, args.prefill_kernel)       # refused for page sizes it does not take
-    cascade = bool(kernel == 1 and prefix and not args.no_cascade)
+    cascade = bool(kernel == 1 and prefix and not args.no_cascade and args.kv in ("f16", "f32"))
     if cascade:
         batch.set_cascade(1)          # shared prefix pages attended once for all sessions (per-layer launches)
     return dict(kernel=kernel, fused=fused, pdl=bool(fused and not args.no_pdl), cascade=cascade)
@@ -242,7 +249,7 @@ def run_ours(args):
     PF_REPS = 3
     total_steps = 7 * (W + K) + (W + KE) + 8 + (PF_REPS + 1) * 512
     work = wl.Workload(w["model"], lens, seed=seed, steps=total_steps, device=local_rank,
-                       shared_prefix=w.get("prefix", 0), kv_dtype=nv.KV_F32 if args.kv == "f32" else nv.KV_F16,
+                       shared_prefix=w.get("prefix", 0), kv_dtype=kv_type(nv, args.kv),
                        kv_block=args.page_tokens)
     eng, batch = work.eng, work.batch
     opt = configure_batch(nv, batch, args, prefix=bool(w.get("prefix", 0)))
@@ -365,7 +372,7 @@ def run_ours(args):
             "higher_is_better": True, "scaling": w["scaling"], "vs_baseline": None,
             "dtype": args.kv, "data": "synthetic",
             "config": {"workload": f"{args.workload}: {w['text']}", "sessions_per_gpu": S,
-                       "context_tokens": lens, "layers": L, "kv_dtype": "fp16" if args.kv == "f16" else "fp32", "page_tokens": args.page_tokens,
+                       "context_tokens": lens, "layers": L, "kv_dtype": KV_NAMES[args.kv], "page_tokens": args.page_tokens,
                        "launch": args.launch, "attention_kernel": "mma" if kernel == 1 else "simt", "fused_append": fused,
                        "pdl": opt["pdl"], "late_inputs": late_main,
                        "cascade_shared_pages": batch.shared_prefix_pages() if cascade else 0,
@@ -867,8 +874,8 @@ def main():
     ap.add_argument("--no-pdl", action="store_true", help="no programmatic dependent launch between layers")
     ap.add_argument("--late-inputs", action="store_true",
                     help="headline with q / new k / new v read only after the previous layer's kernels have finished")
-    ap.add_argument("--kv", default="f16", choices=["f16", "f32"],
-                    help="KV pool element type (f32 = the reference's own format)")
+    ap.add_argument("--kv", default="f16", choices=list(KV_NAMES),
+                    help="KV pool element type (f32 = the reference's own format; i8, e4m3: 8-bit codes with a scale per row)")
     ap.add_argument("--page-tokens", type=int, default=16, choices=[8, 16, 32, 64],
                     help="tokens per KV page (the reference's NOVA_KV_BLOCK; single-GPU workloads)")
     ap.add_argument("--prefill-kernel", type=int, default=-1,

@@ -105,7 +105,7 @@ SIGNATURES = {
     "nova_pool_get_free_list": (i32, [vp, c_i32p, i32]), "nova_pool_get_free_slices": (i32, [vp, c_i32p, i32]),
     "nova_pool_get_live_slices": (i32, [vp, c_i32p, i32]),
     "nova_engine_create": (i32, [C.POINTER(EngineDesc), C.POINTER(vp)]), "nova_engine_destroy": (None, [vp]),
-    "nova_engine_desc_get": (i32, [vp, C.POINTER(EngineDesc)]),
+    "nova_engine_desc_get": (i32, [vp, C.POINTER(EngineDesc)]), "nova_engine_q8_cache": (i32, [vp, i32, C.POINTER(Q8Cache)]),
     "nova_kv_k_base": (vp, [vp]), "nova_kv_v_base": (vp, [vp]), "nova_kv_table_slot": (vp, [vp, i32]),
     "nova_kv_nb": (i32, [vp]), "nova_kv_nblocks": (i32, [vp]), "nova_kv_width": (i32, [vp]),
     "nova_kv_page_bytes": (sz, [vp]), "nova_rope_cos": (vp, [vp]), "nova_rope_sin": (vp, [vp]),
@@ -420,7 +420,7 @@ class Engine:
         self.h = h
         check(lib.nova_engine_desc_get(self.h, C.byref(self.desc)))
         self.pool = PoolView(lib.nova_engine_pool(self.h))
-        self.kv_np = np.float16 if kv_dtype == KV_F16 else np.float32
+        self.kv_np = {KV_F16: np.float16, KV_I8: np.int8, KV_E4M3: np.uint8}.get(kv_dtype, np.float32)      # e4m3: the codes
 
     def close(self):
         if getattr(self, "h", None):
@@ -453,6 +453,12 @@ class Engine:
     def shape(self) -> KvShape:
         d = self.desc
         return KvShape(d.n_heads, d.n_kv_heads, d.head_dim, d.kv_block, d.kv_dtype, d.rope_neox)
+
+    def q8_cache(self, layer=0) -> Q8Cache:
+        """8-bit pools: the cache of one layer, for the q8_* calls (its tables: one per slice)."""
+        c = Q8Cache()
+        check(lib.nova_engine_q8_cache(self.h, layer, C.byref(c)), "nova_engine_q8_cache")
+        return c
 
     # sessions
     def session_create(self): return check(lib.nova_session_create(self.h), "nova_session_create")
@@ -489,6 +495,13 @@ class Engine:
         shp = (self.L, self.nb, self.desc.kv_block, self.NKV, self.HD)
         return (download_ptr(self.k_base, self.kv_np, n).reshape(shp),
                 download_ptr(self.v_base, self.kv_np, n).reshape(shp))
+
+    def read_scales(self):
+        """8-bit pools: the scales of K and V, [layers][nb][n_kv_heads][page tokens]."""
+        c = self.q8_cache()
+        shp = (self.L, self.nb, self.NKV, self.desc.kv_block)
+        n = int(np.prod(shp))
+        return download_ptr(c.scale_k, np.float32, n).reshape(shp), download_ptr(c.scale_v, np.float32, n).reshape(shp)
 
     def batch(self, sessions) -> "Batch":
         return Batch(self, sessions)

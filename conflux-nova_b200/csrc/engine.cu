@@ -15,6 +15,7 @@
 
 #include "common.cuh"
 #include "handles.hpp"
+#include "q8_common.cuh"
 
 using namespace novab;
 
@@ -32,6 +33,9 @@ struct nova_engine {
     nova_pool pool;
     void* pool_k = nullptr;
     void* pool_v = nullptr;
+    float* scale_k = nullptr;        // 8-bit pools: [L][NB][NKV][page tokens]
+    float* scale_v = nullptr;
+    size_t scale_bytes = 0;          // scales of one page of one layer of one pool (0: no 8-bit pools)
     int32_t* tables = nullptr;       // [n_slices][nblocks]
     float* cs = nullptr;
     float* sn = nullptr;
@@ -59,7 +63,7 @@ struct nova_batch {
     int32_t* d_n_past = nullptr;
     int32_t* h_n_past = nullptr;     // pinned staging
     float* part = nullptr;
-    int kernel = 0;                  // 0 SIMT, 1 tensor-core
+    int kernel = 0;                  // 0 SIMT, 1 tensor-core (the only one on 8-bit pools)
     int fused = 0;                   // 1: RoPE+append done inside the tensor-core attention launch
     int pdl = 0;                     // 1: layers after the first of a step launch as programmatic dependents; 2: the same, but
                                      // they read their q / new k / new v only once the launches before them have finished
@@ -88,12 +92,16 @@ struct nova_batch {
 
 namespace {
 
+bool is_q8(int kv_dtype) { return kv_dtype == NOVA_KV_I8 || kv_dtype == NOVA_KV_E4M3; }
+bool is_q8(const nova_engine* e) { return is_q8(e->d.kv_dtype); }
+
 int check_desc(const nova_engine_desc& d) {
     if (d.n_layers <= 0 || d.n_heads <= 0 || d.n_kv_heads <= 0 || d.n_slices <= 0 || d.ctx <= 0) return NOVA_ERR_INVALID;
     if (d.n_heads % d.n_kv_heads) return NOVA_ERR_INVALID;
     if (d.head_dim != kHeadDim || kv_shift_of_block(d.kv_block) < 0) return NOVA_ERR_UNSUPPORTED;
-    if (d.kv_dtype != NOVA_KV_F32 && d.kv_dtype != NOVA_KV_F16) return NOVA_ERR_UNSUPPORTED;
     const int g = d.n_heads / d.n_kv_heads;
+    if (is_q8(d.kv_dtype)) return g <= 128 ? NOVA_OK : NOVA_ERR_UNSUPPORTED;      // any number of kv heads
+    if (d.kv_dtype != NOVA_KV_F32 && d.kv_dtype != NOVA_KV_F16) return NOVA_ERR_UNSUPPORTED;
     if (!(g == 1 || g == 2 || (g >= 4 && g <= 8))) return NOVA_ERR_UNSUPPORTED;
     const int kvg = d.n_kv_heads < 4 ? d.n_kv_heads : 4;
     if (d.n_kv_heads % kvg) return NOVA_ERR_UNSUPPORTED;
@@ -139,6 +147,61 @@ int collect_cow(nova_engine* e, int slice, int64_t pos0, int n, std::vector<CowE
     return NOVA_OK;
 }
 
+// Copy-on-write copies of all pools (8-bit: the codes, whose launch also rewrites the table entries, then the scales).
+int copy_pages(nova_engine* e, std::vector<CowEvent>& ev, cudaStream_t s) {
+    int rc = launch_cow_copy(e->pool_k, e->pool_v, e->d.n_layers, e->nb, e->page_bytes, ev.data(), (int)ev.size(), s);
+    if (rc != NOVA_OK || !is_q8(e)) return rc;
+    for (CowEvent& c : ev) c.table_entry = nullptr;
+    return launch_cow_copy(e->scale_k, e->scale_v, e->d.n_layers, e->nb, e->scale_bytes, ev.data(), (int)ev.size(), s);
+}
+
+bool misaligned(const void* a, const void* b = nullptr, const void* c = nullptr) { return ((uintptr_t)a | (uintptr_t)b | (uintptr_t)c) & 15; }
+
+// The batch's launch on 8-bit pools: one layer, n_tok tokens per session.
+void fill_q8(const nova_batch* b, int layer, int n_tok, Q8Launch& a) {
+    const nova_engine* e = b->e;
+    std::memset(&a, 0, sizeof(a));
+    a.pool_k = e->pool_k; a.pool_v = e->pool_v; a.scale_k = e->scale_k; a.scale_v = e->scale_v;
+    a.tables = e->tables; a.table_stride = e->nblocks; a.slice_ids = b->d_slices; a.n_past = b->d_n_past;
+    a.status = e->status;
+    a.n_sessions = b->n; a.n_tokens = b->n * n_tok; a.max_tokens = a.uniform_tokens = n_tok;
+    a.q_stride = a.out_stride = (int64_t)e->d.n_heads * kHeadDim;
+    a.k_stride = a.v_stride = (int64_t)e->d.n_kv_heads * kHeadDim;
+    a.io = NOVA_IO_F32; a.fmt = e->d.kv_dtype; a.neox = e->d.rope_neox;
+    a.layer = layer; a.nb = e->nb; a.n_heads = e->d.n_heads; a.n_kv_heads = e->d.n_kv_heads; a.kv_shift = e->kv_shift;
+}
+void q8_rope(const nova_batch* b, Q8Launch& a) {
+    a.rope_cs = b->e->cs; a.rope_sn = b->e->sn; a.rope_rows = b->e->d.rope_positions;
+}
+// RopeKvOp: q (may be NULL) and k rotated in place, k / v written.
+int q8_append(const nova_batch* b, int layer, int n_tok, float* q, float* k, const float* v, cudaStream_t s) {
+    if (misaligned(q, k, v)) return NOVA_ERR_INVALID;
+    Q8Launch a;
+    fill_q8(b, layer, n_tok, a);
+    q8_rope(b, a);
+    a.k = k; a.v = v; a.q_rot = q; a.k_rot = k;
+    return launch_q8_append(a, s);
+}
+// AttnOp: q as it is (rotated).
+int q8_attn(const nova_batch* b, int layer, int n_tok, int window, const float* q, float* out, cudaStream_t s) {
+    if (misaligned(q, out)) return NOVA_ERR_INVALID;
+    Q8Launch a;
+    fill_q8(b, layer, n_tok, a);
+    a.q = q; a.out = out; a.window = window;
+    a.part = b->part;
+    return launch_q8_attn(a, s);
+}
+// Both in one: q read un-rotated, k rotated in place.
+int q8_append_attn(const nova_batch* b, int layer, const float* q, float* k, const float* v, float* out, cudaStream_t s) {
+    if (misaligned(q, k, v) || misaligned(out)) return NOVA_ERR_INVALID;
+    Q8Launch a;
+    fill_q8(b, layer, 1, a);
+    q8_rope(b, a);
+    a.q = q; a.k = k; a.v = v; a.k_rot = k; a.out = out;
+    a.append = 1;
+    a.part = b->part;
+    return launch_q8_attn(a, s);
+}
 void fill_attn(const nova_batch* b, AttnLaunch& a) {
     const nova_engine* e = b->e;
     std::memset(&a, 0, sizeof(a));
@@ -244,7 +307,7 @@ int run_attn(const nova_batch* b, const AttnLaunch& a, cudaStream_t s) {
     return launch_attn_combine(a, ctas, s);
 }
 
-bool use_fused(const nova_batch* b) { return b->fused && b->kernel == 1 && b->e->d.rope_neox; }
+bool use_fused(const nova_batch* b) { return b->fused && b->kernel == 1 && (b->e->d.rope_neox || is_q8(b->e)); }
 
 // CTAs of one tensor-core attention launch.  A launch of a programmatic chain (one layer per launch) that has
 // little to stream - fewer than 16 pages per CTA, so that a CTA's start-up outweighs its streaming - takes only
@@ -289,6 +352,14 @@ int run_attn_fused(const nova_batch* b, int layer0, int n_layers, const float* q
                    float* out, cudaStream_t s, bool pdl = false, float* out_part = nullptr, int64_t page_lo = 0,
                    int64_t page_hi = -1) {
     const nova_engine* e = b->e;
+    if (is_q8(e)) {
+        const size_t qs = (size_t)b->n * e->d.n_heads * kHeadDim, ks = (size_t)b->n * e->d.n_kv_heads * kHeadDim;
+        for (int l = 0; l < n_layers; ++l) {
+            const int rc = q8_append_attn(b, layer0 + l, q + l * qs, k + l * ks, v + l * ks, out + l * qs, s);
+            if (rc != NOVA_OK) return rc;
+        }
+        return NOVA_OK;
+    }
     AttnLaunch a;
     fill_attn(b, a);
     a.q = q; a.out = out;
@@ -331,6 +402,40 @@ void fill_append(const nova_batch* b, AppendLaunch& a) {
     a.kv_dtype = e->d.kv_dtype;
 }
 
+// RopeKvOp / AttnOp for layers [layer0, layer0 + n_layers), whatever the pools hold.
+int append_layers(const nova_batch* b, int layer0, int n_layers, float* q, float* k, const float* v, cudaStream_t s) {
+    const nova_engine* e = b->e;
+    if (is_q8(e)) {
+        const size_t qs = (size_t)b->n * e->d.n_heads * kHeadDim, ks = (size_t)b->n * e->d.n_kv_heads * kHeadDim;
+        for (int l = 0; l < n_layers; ++l) {
+            const int rc = q8_append(b, layer0 + l, 1, q ? q + l * qs : nullptr, k + l * ks, v + l * ks, s);
+            if (rc != NOVA_OK) return rc;
+        }
+        return NOVA_OK;
+    }
+    AppendLaunch a;
+    fill_append(b, a);
+    a.q = q; a.k = k; a.v = v;
+    a.layer0 = layer0; a.n_layers = n_layers;
+    return launch_rope_append(a, s);
+}
+int attn_layers(const nova_batch* b, int layer0, int n_layers, const float* q, float* out, cudaStream_t s) {
+    const nova_engine* e = b->e;
+    if (is_q8(e)) {
+        const size_t qs = (size_t)b->n * e->d.n_heads * kHeadDim;
+        for (int l = 0; l < n_layers; ++l) {
+            const int rc = q8_attn(b, layer0 + l, 1, 0, q + l * qs, out + l * qs, s);
+            if (rc != NOVA_OK) return rc;
+        }
+        return NOVA_OK;
+    }
+    AttnLaunch a;
+    fill_attn(b, a);
+    a.q = q; a.out = out;
+    a.layer0 = layer0; a.n_layers = n_layers;
+    return run_attn(b, a, s);
+}
+
 }  // namespace
 
 extern "C" {
@@ -354,8 +459,11 @@ int nova_engine_create(const nova_engine_desc* desc, nova_engine** out) {
     e->pool.p.init(d.n_slices, d.ctx);
     e->nblocks = e->pool.p.nblocks();
     e->nb = e->pool.p.nb_total();
-    e->elem_bytes = d.kv_dtype == NOVA_KV_F16 ? 2 : 4;
+    const bool q8 = is_q8(d.kv_dtype);
+    if (q8 && (int64_t)d.n_layers * e->nb * d.kv_block > 0x7fffffffLL) { delete e; return NOVA_ERR_TOO_LARGE; }      // slot rows are 32-bit
+    e->elem_bytes = q8 ? 1 : d.kv_dtype == NOVA_KV_F16 ? 2 : 4;
     e->page_bytes = (size_t)d.kv_block * d.n_kv_heads * d.head_dim * e->elem_bytes;
+    e->scale_bytes = q8 ? (size_t)d.kv_block * d.n_kv_heads * sizeof(float) : 0;
     e->kv_group = kv_group_of(d.n_kv_heads);
     e->kv_shift = kv_shift_of_block(d.kv_block);
     e->sess.resize((size_t)d.max_sessions);
@@ -365,6 +473,8 @@ int nova_engine_create(const nova_engine_desc* desc, nova_engine** out) {
     cudaError_t ce = cudaSuccess;
     if (ce == cudaSuccess) ce = cudaMalloc(&e->pool_k, pool_bytes);
     if (ce == cudaSuccess) ce = cudaMalloc(&e->pool_v, pool_bytes);
+    if (ce == cudaSuccess && q8) ce = cudaMalloc((void**)&e->scale_k, (size_t)d.n_layers * (size_t)e->nb * e->scale_bytes);
+    if (ce == cudaSuccess && q8) ce = cudaMalloc((void**)&e->scale_v, (size_t)d.n_layers * (size_t)e->nb * e->scale_bytes);
     if (ce == cudaSuccess) ce = cudaMalloc((void**)&e->tables, (size_t)d.n_slices * e->nblocks * sizeof(int32_t));
     if (ce == cudaSuccess) ce = cudaMalloc((void**)&e->cs, rope_bytes);
     if (ce == cudaSuccess) ce = cudaMalloc((void**)&e->sn, rope_bytes);
@@ -407,6 +517,8 @@ void nova_engine_destroy(nova_engine* e) {
         if (s.used && s.stream) cudaStreamDestroy(s.stream);
     cudaFree(e->pool_k);
     cudaFree(e->pool_v);
+    cudaFree(e->scale_k);
+    cudaFree(e->scale_v);
     cudaFree(e->tables);
     cudaFree(e->cs);
     cudaFree(e->sn);
@@ -430,6 +542,19 @@ int nova_kv_nb(const nova_engine* e) { return e ? e->nb : 0; }
 int nova_kv_nblocks(const nova_engine* e) { return e ? e->nblocks : 0; }
 int nova_kv_width(const nova_engine* e) { return e ? e->d.n_kv_heads * e->d.head_dim : 0; }
 size_t nova_kv_page_bytes(const nova_engine* e) { return e ? e->page_bytes : 0; }
+int nova_engine_q8_cache(const nova_engine* e, int layer, nova_q8_cache* out) {
+    if (!e || !out || layer < 0 || layer >= e->d.n_layers) return NOVA_ERR_INVALID;
+    if (!is_q8(e)) return NOVA_ERR_UNSUPPORTED;
+    std::memset(out, 0, sizeof(*out));
+    out->shape.n_heads = e->d.n_heads; out->shape.n_kv_heads = e->d.n_kv_heads; out->shape.head_dim = e->d.head_dim;
+    out->shape.kv_block = e->d.kv_block; out->shape.kv_dtype = e->d.kv_dtype; out->shape.rope_neox = e->d.rope_neox;
+    out->pool_k = e->pool_k; out->pool_v = e->pool_v; out->scale_k = e->scale_k; out->scale_v = e->scale_v;
+    out->layer = layer; out->nb = e->nb;
+    out->tables = e->tables; out->table_stride = e->nblocks;
+    out->rope_cs = e->cs; out->rope_sn = e->sn; out->rope_rows = e->d.rope_positions;
+    out->status = e->status;
+    return NOVA_OK;
+}
 const float* nova_rope_cos(const nova_engine* e) { return e ? e->cs : nullptr; }
 const float* nova_rope_sin(const nova_engine* e) { return e ? e->sn : nullptr; }
 nova_pool* nova_engine_pool(nova_engine* e) { return e ? &e->pool : nullptr; }
@@ -460,6 +585,9 @@ int nova_session_create(nova_engine* e) {
     int rc = upload_table(e, slice, st);
     if (rc == NOVA_OK && e->d.zero_pages)
         rc = launch_zero_pages(e->pool_k, e->pool_v, e->d.n_layers, e->nb, e->page_bytes,
+                               e->tables + (size_t)slice * e->nblocks, e->nblocks, st);
+    if (rc == NOVA_OK && e->d.zero_pages && is_q8(e))
+        rc = launch_zero_pages(e->scale_k, e->scale_v, e->d.n_layers, e->nb, e->scale_bytes,
                                e->tables + (size_t)slice * e->nblocks, e->nblocks, st);
     if (rc == NOVA_OK) {
         ce = cudaStreamSynchronize(st);
@@ -586,7 +714,7 @@ int nova_engine_telemetry(const nova_engine* e, nova_telemetry* out) {
     int live = 0;
     for (const SessionRec& s : e->sess) live += s.used ? 1 : 0;
     out->sessions_live = live;
-    const uint64_t per_page = (uint64_t)e->page_bytes * 2ull * (uint64_t)e->d.n_layers;
+    const uint64_t per_page = (uint64_t)(e->page_bytes + e->scale_bytes) * 2ull * (uint64_t)e->d.n_layers;
     out->kv_bytes_cap = per_page * (uint64_t)pp.nb_total();
     out->kv_bytes_used = per_page * (uint64_t)(pp.nb_total() - pp.free_pages());
     return NOVA_OK;
@@ -599,8 +727,7 @@ int nova_session_cow_on(nova_engine* e, int session, int64_t pos0, int n, nova_s
     const int rc = collect_cow(e, r->slice, pos0, n, ev);
     if (!ev.empty()) {
         NOVA_CUDA_TRY(cudaSetDevice(e->d.device));
-        const int lrc = launch_cow_copy(e->pool_k, e->pool_v, e->d.n_layers, e->nb, e->page_bytes, ev.data(),
-                                        (int)ev.size(), (cudaStream_t)stream);
+        const int lrc = copy_pages(e, ev, (cudaStream_t)stream);
         if (lrc != NOVA_OK) return lrc;
     }
     return rc != NOVA_OK ? rc : (int)ev.size();
@@ -714,7 +841,7 @@ int nova_launch_attn_decode_paged(const nova_kv_shape* sh, const float* q, const
                                   const int32_t* table, int layer, int nb, int n_keys, float* o, float* scratch,
                                   nova_stream_t s) {
     if (!sh || !q || !pool_k || !pool_v || !table || !o || !scratch || layer < 0 || nb <= 0) return NOVA_ERR_INVALID;
-    if (sh->head_dim != kHeadDim || kv_shift_of_block(sh->kv_block) < 0) return NOVA_ERR_UNSUPPORTED;
+    if (sh->head_dim != kHeadDim || kv_shift_of_block(sh->kv_block) < 0 || is_q8(sh->kv_dtype)) return NOVA_ERR_UNSUPPORTED;
     if (sh->n_kv_heads <= 0 || sh->n_heads % sh->n_kv_heads) return NOVA_ERR_INVALID;
     AttnLaunch a;
     std::memset(&a, 0, sizeof(a));
@@ -803,7 +930,7 @@ int nova_lse_merge_peers(const float* part, void* const* peer_base, int n_ranks,
 int nova_batch_create(nova_engine* e, const int32_t* sessions, int n, nova_batch** out) {
     if (!e || !sessions || n <= 0 || !out) return NOVA_ERR_INVALID;
     *out = nullptr;
-    if ((int64_t)n * (e->d.n_kv_heads / e->kv_group) > kMaxRowsSmem) return NOVA_ERR_TOO_LARGE;
+    if (!is_q8(e) && (int64_t)n * (e->d.n_kv_heads / e->kv_group) > kMaxRowsSmem) return NOVA_ERR_TOO_LARGE;
     nova_batch* b = new (std::nothrow) nova_batch();
     if (!b) return NOVA_ERR_INVALID;
     b->e = e;
@@ -825,7 +952,13 @@ int nova_batch_create(nova_engine* e, const int32_t* sessions, int n, nova_batch
     const int64_t rows = (int64_t)e->d.n_layers * n * (e->d.n_kv_heads / e->kv_group);
     const int heads_per_row = e->kv_group * (e->d.n_heads / e->d.n_kv_heads);
     const int64_t rows_alloc = rows > kMaxRowsSmem ? rows : kMaxRowsSmem;   // a prefill launch has up to kMaxRowsSmem rows
-    const size_t part_floats = (size_t)(rows_alloc + kMaxSplitCtas) * heads_per_row * kSlotW;
+    size_t part_floats = (size_t)(rows_alloc + kMaxSplitCtas) * heads_per_row * kSlotW;
+    if (is_q8(e)) {
+        // a decode step's partials, or those of any prefill (2 a CTA, 256 rows at most)
+        part_floats = std::max(q8_work_bytes(e->d.n_heads, e->d.n_kv_heads, n, n, 1), q8_chunk_work_bytes(e->d.n_heads, e->d.n_kv_heads, 8192)) /
+                      sizeof(float);
+        b->kernel = 1;
+    }
     cudaError_t ce = cudaSuccess;
     if (ce == cudaSuccess) ce = cudaMalloc((void**)&b->d_slices, (size_t)n * sizeof(int32_t));
     if (ce == cudaSuccess) ce = cudaMalloc((void**)&b->d_n_past, (size_t)n * sizeof(int32_t));
@@ -896,6 +1029,7 @@ int nova_batch_sync_positions(nova_batch* b, nova_stream_t s) {
 
 int nova_batch_set_kernel(nova_batch* b, int which) {
     if (!b || which < 0 || which > 1) return NOVA_ERR_INVALID;
+    if (is_q8(b->e)) return which == 1 ? NOVA_OK : NOVA_ERR_UNSUPPORTED;
     if (which == 1 && !b->e->tmaps_ok) return NOVA_ERR_UNSUPPORTED;      // (fp32 pools: 16-token pages only)
     b->kernel = which;
     if (which != 1) b->fused = 0;
@@ -914,7 +1048,7 @@ int nova_batch_set_timeline(nova_batch* b, void* dev_buf) {
 }
 int nova_batch_set_fused_append(nova_batch* b, int on) {
     if (!b) return NOVA_ERR_INVALID;
-    if (on && (b->kernel != 1 || !b->e->d.rope_neox)) return NOVA_ERR_UNSUPPORTED;
+    if (on && (b->kernel != 1 || (!b->e->d.rope_neox && !is_q8(b->e)))) return NOVA_ERR_UNSUPPORTED;
     b->fused = on ? 1 : 0;
     if (b->graph) { cudaGraphExecDestroy(b->graph); b->graph = nullptr; }
     return NOVA_OK;
@@ -927,6 +1061,7 @@ int nova_batch_set_row_setup_pages(nova_batch* b, int pages) {
 }
 int nova_batch_set_prefill_kernel(nova_batch* b, int which) {
     if (!b || which < 0 || which > 1) return NOVA_ERR_INVALID;
+    if (is_q8(b->e)) return which == 1 ? NOVA_OK : NOVA_ERR_UNSUPPORTED;
     if (which == 1 && (b->e->d.kv_dtype != NOVA_KV_F16 || !b->e->tmaps_ok || b->e->kv_shift < 4)) return NOVA_ERR_UNSUPPORTED;
     b->prefill_tc5 = which;
     return NOVA_OK;
@@ -982,7 +1117,7 @@ static int shared_prefix_pages(const nova_batch* b) {
 
 int nova_batch_set_cascade(nova_batch* b, int on) {
     if (!b) return NOVA_ERR_INVALID;
-    if (on && b->kernel != 1) return NOVA_ERR_UNSUPPORTED;
+    if (on && (b->kernel != 1 || is_q8(b->e))) return NOVA_ERR_UNSUPPORTED;
     nova_engine* e = b->e;
     if (on && !b->casc_parts) {
         NOVA_CUDA_TRY(cudaSetDevice(e->d.device));
@@ -1017,8 +1152,7 @@ int nova_batch_cow(nova_batch* b, nova_stream_t s) {
         b->casc_pages = pages;
     }
     if (!ev.empty()) {
-        const int lrc = launch_cow_copy(e->pool_k, e->pool_v, e->d.n_layers, e->nb, e->page_bytes, ev.data(),
-                                        (int)ev.size(), (cudaStream_t)s);
+        const int lrc = copy_pages(e, ev, (cudaStream_t)s);
         if (lrc != NOVA_OK) return lrc;
     }
     return rc != NOVA_OK ? rc : (int)ev.size();
@@ -1026,30 +1160,18 @@ int nova_batch_cow(nova_batch* b, nova_stream_t s) {
 
 int nova_batch_append(nova_batch* b, int layer, float* q, float* k, const float* v, nova_stream_t s) {
     if (!b || !q || !k || !v || layer < 0 || layer >= b->e->d.n_layers) return NOVA_ERR_INVALID;
-    AppendLaunch a;
-    fill_append(b, a);
-    a.q = q; a.k = k; a.v = v;
-    a.layer0 = layer; a.n_layers = 1;
-    return launch_rope_append(a, (cudaStream_t)s);
+    return append_layers(b, layer, 1, q, k, v, (cudaStream_t)s);
 }
 
 int nova_batch_append_layers(nova_batch* b, int layer0, int n_layers, float* q, float* k, const float* v,
                              nova_stream_t s) {
     if (!b || !k || !v || layer0 < 0 || n_layers < 1 || layer0 + n_layers > b->e->d.n_layers) return NOVA_ERR_INVALID;
-    AppendLaunch a;
-    fill_append(b, a);
-    a.q = q; a.k = k; a.v = v;
-    a.layer0 = layer0; a.n_layers = n_layers;
-    return launch_rope_append(a, (cudaStream_t)s);
+    return append_layers(b, layer0, n_layers, q, k, v, (cudaStream_t)s);
 }
 
 int nova_batch_attn(nova_batch* b, int layer, const float* q, float* out, nova_stream_t s) {
     if (!b || !q || !out || layer < 0 || layer >= b->e->d.n_layers) return NOVA_ERR_INVALID;
-    AttnLaunch a;
-    fill_attn(b, a);
-    a.q = q; a.out = out;
-    a.layer0 = layer; a.n_layers = 1;
-    return run_attn(b, a, (cudaStream_t)s);
+    return attn_layers(b, layer, 1, q, out, (cudaStream_t)s);
 }
 
 int nova_batch_advance_by(nova_batch* b, int n_tokens, nova_stream_t s) {
@@ -1088,11 +1210,15 @@ int nova_batch_prefill(nova_batch* b, int layer, int n_tokens, float* q, float* 
             rc = collect_cow(e, b->slices[(size_t)i], st->n_past, n_tokens, ev);
         }
         if (!ev.empty()) {
-            const int lrc = launch_cow_copy(e->pool_k, e->pool_v, e->d.n_layers, e->nb, e->page_bytes, ev.data(),
-                                            (int)ev.size(), (cudaStream_t)s);
+            const int lrc = copy_pages(e, ev, (cudaStream_t)s);
             if (lrc != NOVA_OK) return lrc;
         }
         if (rc != NOVA_OK) return rc;
+    }
+    if (is_q8(e)) {
+        int rc = q8_append(b, layer, n_tokens, q, k, v, (cudaStream_t)s);
+        if (rc == NOVA_OK) rc = q8_attn(b, layer, n_tokens, b->window, q, out, (cudaStream_t)s);
+        return rc;
     }
     AppendLaunch ap;
     fill_append(b, ap);
@@ -1113,17 +1239,9 @@ int nova_batch_prefill(nova_batch* b, int layer, int n_tokens, float* q, float* 
 int nova_batch_step_all_layers(nova_batch* b, float* q, float* k, const float* v, float* out, nova_stream_t s) {
     if (!b || !q || !k || !v || !out) return NOVA_ERR_INVALID;
     if (use_fused(b)) return run_attn_fused(b, 0, b->e->d.n_layers, q, k, v, out, (cudaStream_t)s);
-    AppendLaunch ap;
-    fill_append(b, ap);
-    ap.q = q; ap.k = k; ap.v = v;
-    ap.layer0 = 0; ap.n_layers = b->e->d.n_layers;
-    int rc = launch_rope_append(ap, (cudaStream_t)s);
+    const int rc = append_layers(b, 0, b->e->d.n_layers, q, k, v, (cudaStream_t)s);
     if (rc != NOVA_OK) return rc;
-    AttnLaunch at;
-    fill_attn(b, at);
-    at.q = q; at.out = out;
-    at.layer0 = 0; at.n_layers = b->e->d.n_layers;
-    return run_attn(b, at, (cudaStream_t)s);
+    return attn_layers(b, 0, b->e->d.n_layers, q, out, (cudaStream_t)s);
 }
 
 static int ensure_staging(nova_batch* b);
@@ -1337,18 +1455,10 @@ int nova_batch_run_steps(nova_batch* b, int n_steps, float* q, float* k, const f
                 if (attn_ms) NOVA_CUDA_TRY(cudaEventRecord(b->ev[ev_used++], st));
                 rc = run_attn_fused(b, 0, e->d.n_layers, qi, ki, vi, oi, st);
             } else {
-                AppendLaunch ap;
-                fill_append(b, ap);
-                ap.q = qi; ap.k = ki; ap.v = vi;
-                ap.layer0 = 0; ap.n_layers = e->d.n_layers;
-                rc = launch_rope_append(ap, st);
+                rc = append_layers(b, 0, e->d.n_layers, qi, ki, vi, st);
                 if (rc != NOVA_OK) return rc;
                 if (attn_ms) NOVA_CUDA_TRY(cudaEventRecord(b->ev[ev_used++], st));
-                AttnLaunch at;
-                fill_attn(b, at);
-                at.q = qi; at.out = oi;
-                at.layer0 = 0; at.n_layers = e->d.n_layers;
-                rc = run_attn(b, at, st);
+                rc = attn_layers(b, 0, e->d.n_layers, qi, oi, st);
             }
             if (rc != NOVA_OK) return rc;
             if (attn_ms) NOVA_CUDA_TRY(cudaEventRecord(b->ev[ev_used++], st));
@@ -1402,6 +1512,7 @@ int nova_batch_attn_partial_layers(nova_batch* b, int layer0, int n_layers, cons
     if (!b || !q || !part || layer0 < 0 || n_layers < 1 || layer0 + n_layers > b->e->d.n_layers || page0 < 0 ||
         page1 < page0)
         return NOVA_ERR_INVALID;
+    if (is_q8(b->e)) return NOVA_ERR_UNSUPPORTED;
     AttnLaunch a;
     fill_attn(b, a);
     a.q = q;
@@ -1424,6 +1535,7 @@ int nova_batch_step_partial_peers(nova_batch* b, float* q, float* k, const float
         my_rank >= n_ranks || n_slots < 2 || epoch0 < 1 || page0 < 0 || page1 < page0 || timeout_ms < 1)
         return NOVA_ERR_INVALID;
     nova_engine* e = b->e;
+    if (is_q8(e)) return NOVA_ERR_UNSUPPORTED;
     const int L = e->d.n_layers;
     const int rows = b->n * e->d.n_heads;
     if (epoch0 + L > 0x7fffffffLL) return NOVA_ERR_INVALID;

@@ -655,7 +655,6 @@ __global__ void __launch_bounds__(128) q8_decode_merge_kernel(Q8Launch a, int kv
 }
 
 int dec_group(int n_kv_heads) { return n_kv_heads % 4 == 0 ? 4 : (n_kv_heads % 2 == 0 ? 2 : 1); }
-bool is_decode(int n_heads, int n_kv_heads, int max_tokens) { return max_tokens <= 1 && n_heads / n_kv_heads <= 8; }
 
 template <int KVG, int kFmt, bool kLo>
 int launch_decode_as(const Q8Launch& a, const CUtensorMap& tmk, const CUtensorMap& tmv, int ctas, cudaStream_t s) {
@@ -677,17 +676,18 @@ int launch_decode(const Q8Launch& a, const CUtensorMap& tmk, const CUtensorMap& 
 
 }  // namespace
 
+bool q8_is_decode(int n_heads, int n_kv_heads, int max_tokens) { return max_tokens <= 1 && n_heads / n_kv_heads <= 8; }
+
 size_t q8_work_bytes(int n_heads, int n_kv_heads, int n_sessions, int, int max_tokens) {
-    if (!is_decode(n_heads, n_kv_heads, max_tokens)) return q8_chunk_work_bytes(n_heads, n_kv_heads, max_tokens);
+    if (!q8_is_decode(n_heads, n_kv_heads, max_tokens)) return q8_chunk_work_bytes(n_heads, n_kv_heads, max_tokens);
     const int kvg = dec_group(n_kv_heads), groups = n_kv_heads / kvg;
     const int64_t rows = (int64_t)n_sessions * groups;
-    return (size_t)((rows < kMaxRowsSmem ? rows : kMaxRowsSmem) + kMaxSms) * (size_t)(kvg * (n_heads / n_kv_heads)) * kSlotW * sizeof(float);
+    return (size_t)((rows < kMaxRowsSmem ? rows : kMaxRowsSmem) + kQ8MaxCtas) * (size_t)(kvg * (n_heads / n_kv_heads)) * kSlotW * sizeof(float);
 }
 
-int launch_q8_attn(const Q8Launch& a_in, size_t, cudaStream_t s) {
-    Q8Launch a = a_in;
+int launch_q8_attn(const Q8Launch& a, cudaStream_t s) {
     if (a.n_tokens <= 0 || a.n_sessions <= 0) return NOVA_OK;
-    if (is_decode(a.n_heads, a.n_kv_heads, a.max_tokens)) {
+    if (q8_is_decode(a.n_heads, a.n_kv_heads, a.max_tokens)) {
         const int kvg = dec_group(a.n_kv_heads), groups = a.n_kv_heads / kvg;
         if (groups > kMaxRowsSmem) return NOVA_ERR_TOO_LARGE;
         alignas(64) CUtensorMap tmk, tmv;
@@ -697,7 +697,7 @@ int launch_q8_attn(const Q8Launch& a_in, size_t, cudaStream_t s) {
         if (rc == NOVA_OK) rc = attn_make_tmap(&tmv, a.pool_v, slot_rows, a.n_kv_heads, kvg, box, 1);
         if (rc != NOVA_OK) return rc;
         int ctas = sm_count();
-        if (ctas > kMaxSms) ctas = kMaxSms;
+        if (ctas > kQ8MaxCtas) ctas = kQ8MaxCtas;
         const int most = kMaxRowsSmem / groups;                    // sessions of one launch (the row table's size)
         const int all = a.n_sessions;
         const size_t io_bytes = a.io == NOVA_IO_F32 ? 4 : 2;

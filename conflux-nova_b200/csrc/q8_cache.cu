@@ -363,7 +363,7 @@ static int q8_attn(const nova_q8_cache* c, const nova_q8_rows* r, const void* q,
         a.k = k; a.v = v;
         a.append = 1;
     }
-    return launch_q8_attn(a, work_bytes, (cudaStream_t)s);
+    return launch_q8_attn(a, (cudaStream_t)s);
 }
 
 int nova_launch_q8_attn(const nova_q8_cache* c, const nova_q8_rows* r, const void* q, void* out, int window, void* work, size_t work_bytes,

@@ -866,13 +866,13 @@ ChunkShape chunk_shape(int n_heads, int n_kv_heads, int max_tokens) {
 }  // namespace
 
 size_t q8_chunk_work_bytes(int n_heads, int n_kv_heads, int max_tokens) {
-    return (size_t)2 * kMaxSms * chunk_shape(n_heads, n_kv_heads, max_tokens).rows_cap * kSlotW * sizeof(float);
+    return (size_t)2 * kQ8MaxCtas * chunk_shape(n_heads, n_kv_heads, max_tokens).rows_cap * kSlotW * sizeof(float);
 }
 
 int launch_q8_chunk(const Q8Launch& a, cudaStream_t s) {
     const ChunkShape sh = chunk_shape(a.n_heads, a.n_kv_heads, a.max_tokens);
     int ctas = sm_count();
-    if (ctas > kMaxSms) ctas = kMaxSms;
+    if (ctas > kQ8MaxCtas) ctas = kQ8MaxCtas;
     const size_t io_bytes = a.io == NOVA_IO_F32 ? 4 : 2;
     for (int s0 = 0; s0 < a.n_sessions; s0 += kMaxSessions) {           // (the plan's size)
         Q8Launch b = a;

@@ -24,6 +24,8 @@ constexpr float kQ8MinScale = 8.4703294725430034e-22f;     // 2^-70
 // keeps fp16's 11 bits down to 2^-25 of the reference (below: steps of 2^-35 of it).
 constexpr float kQ8Step = 4.f, kQ8Top = 11.f;
 
+constexpr int kQ8MaxCtas = 160;      // CTAs of an attention launch, one per SM (sizes the workspaces)
+
 struct Q8Launch {
     void* pool_k;
     void* pool_v;
@@ -305,7 +307,8 @@ __device__ __forceinline__ uint32_t movmatrix(uint32_t x) {
 // q8_cache.cu, q8_attn.cu (single tokens), q8_chunk.cu (everything else)
 int launch_q8_append(const Q8Launch& a, cudaStream_t s);
 int launch_q8_read(const Q8Launch& a, cudaStream_t s);
-int launch_q8_attn(const Q8Launch& a, size_t work_bytes, cudaStream_t s);
+int launch_q8_attn(const Q8Launch& a, cudaStream_t s);
+bool q8_is_decode(int n_heads, int n_kv_heads, int max_tokens);      // single tokens, at most 8 query heads per kv head: q8_attn.cu's kernel
 int launch_q8_chunk(const Q8Launch& a, cudaStream_t s);
 size_t q8_chunk_work_bytes(int n_heads, int n_kv_heads, int max_tokens);
 size_t q8_work_bytes(int n_heads, int n_kv_heads, int n_sessions, int n_tokens, int max_tokens);

@@ -11,7 +11,7 @@ import ctypes as C
 
 import numpy as np
 
-from . import (KV_F16, DevBuf, Engine, KvShape, check, lib, synth_key)
+from . import (IO_F32, KV_E4M3, KV_F16, KV_F32, KV_I8, DevBuf, Engine, KvShape, Q8Rows, check, lib, q8_append, synth_key)
 
 # (layers, q heads, kv heads); head_dim 128, page 16 tokens, RoPE theta 1e6 (NeoX pairs)
 SHAPES = {"qwen25_1p5b": (28, 12, 2), "qwen25_7b": (28, 28, 4), "qwen25_14b": (48, 40, 8)}
@@ -97,7 +97,7 @@ class Workload:
         ks = session if key_session is None else key_session
         row = e.NKV * e.HD
         sh = e.shape()
-        kbuf, vbuf = DevBuf(min(n, chunk) * row * 4), DevBuf(min(n, chunk) * row * 4)
+        kbuf, vbuf, pos = DevBuf(min(n, chunk) * row * 4), DevBuf(min(n, chunk) * row * 4), DevBuf(4)
         table = lib.nova_kv_table_slot(e.h, e.session_slice(session))
         cs, sn = lib.nova_rope_cos(e.h), lib.nova_rope_sin(e.h)
         for layer in range(e.L):
@@ -106,12 +106,20 @@ class Workload:
                 m = min(chunk, pos0 + n - p)
                 check(lib.nova_synth_normal(kbuf.ptr, m * row, kk, p * row, None))
                 check(lib.nova_synth_normal(vbuf.ptr, m * row, kv, p * row, None))
-                check(lib.nova_launch_rope_append_paged(C.byref(sh), e.k_base, e.v_base, table, layer, e.nb, m, p,
-                                                        None, kbuf.ptr, vbuf.ptr, cs, sn, None), "context fill")
+                if sh.kv_dtype in (KV_I8, KV_E4M3):
+                    cache = e.q8_cache(layer)
+                    cache.tables = table
+                    pos.upload(np.array([p], np.int32))
+                    q8_append(cache, Q8Rows(1, m, m, IO_F32, pos.ptr), kbuf.ptr, vbuf.ptr)
+                    check(lib.dev_sync())
+                else:
+                    check(lib.nova_launch_rope_append_paged(C.byref(sh), e.k_base, e.v_base, table, layer, e.nb, m, p,
+                                                            None, kbuf.ptr, vbuf.ptr, cs, sn, None), "context fill")
         check(lib.dev_sync())
         e.set_n_past(session, max(e.n_past(session), pos0 + n))
         kbuf.free()
         vbuf.free()
+        pos.free()
 
     # -- per-step inputs ------------------------------------------------------------------
     def step_input_sizes(self):
@@ -150,23 +158,26 @@ class Workload:
         check(lib.dev_sync())
         return dq, dk, dv
 
+    def row_bytes(self) -> int:
+        """Bytes of one cached row (one token of one kv head in one pool): its elements and, on 8-bit pools, its scale."""
+        e = self.eng
+        return {KV_F32: 4 * e.HD, KV_F16: 2 * e.HD}.get(e.desc.kv_dtype, e.HD + 4)
+
     def kv_bytes_per_step(self, n_past=None) -> int:
         """Algorithmic KV bytes of one decode step: every cached key's K and V row read once per
         kv head in every layer (the reference profiler's definition, code/graph/dense.h:88), plus
         the appended rows."""
         e = self.eng
-        es = 2 if e.desc.kv_dtype == KV_F16 else 4
         n_past = [e.n_past(s) for s in self.sessions] if n_past is None else n_past
         keys = sum(n + 1 for n in n_past)
-        per_tok = 2 * e.NKV * e.HD * es * e.L
+        per_tok = 2 * e.NKV * self.row_bytes() * e.L
         return keys * per_tok + len(self.sessions) * per_tok
 
     def unique_kv_bytes_per_step(self, n_past=None) -> int:
         """The same with shared-prefix pages counted once (the least HBM traffic a step can have)."""
         e = self.eng
-        es = 2 if e.desc.kv_dtype == KV_F16 else 4
         n_past = [e.n_past(s) for s in self.sessions] if n_past is None else n_past
-        per_tok = 2 * e.NKV * e.HD * es * e.L
+        per_tok = 2 * e.NKV * self.row_bytes() * e.L
         if not self.shared_prefix:
             return self.kv_bytes_per_step(n_past)
         full_pages = (self.shared_prefix // self.kv_block) * self.kv_block      # the tail page is private after its COW

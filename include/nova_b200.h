@@ -177,7 +177,7 @@ typedef struct {
     int32_t n_kv_heads;     /* Model::NKV (NH % NKV == 0)                         */
     int32_t head_dim;       /* Model::HD; 128 only                                */
     int32_t kv_block;       /* kKvBlock = NOVA_KV_BLOCK (code/graph/kv_pool_cfg.h:12-26): 8, 16, 32 or 64 */
-    int32_t kv_dtype;       /* NOVA_KV_F32 | NOVA_KV_F16                          */
+    int32_t kv_dtype;       /* NOVA_KV_F32 | NOVA_KV_F16 | NOVA_KV_I8 | NOVA_KV_E4M3 */
     int32_t rope_theta;     /* Model::theta (1000000 / 500000 / 10000)            */
     int32_t rope_neox;      /* 1 = pairs (i, i+HD/2) (Qwen2), 0 = (2i, 2i+1)      */
     int32_t n_slices;       /* KvPool::init(n_slices, ctx): slices == max sessions */
@@ -200,7 +200,7 @@ int32_t*    nova_kv_table_slot(const nova_engine* e, int slice);
 int         nova_kv_nb(const nova_engine* e);
 int         nova_kv_nblocks(const nova_engine* e);
 int         nova_kv_width(const nova_engine* e);
-size_t      nova_kv_page_bytes(const nova_engine* e);     /* one page of one layer of one pool */
+size_t      nova_kv_page_bytes(const nova_engine* e);     /* one page of one layer of one pool (8-bit pools: its codes) */
 const float* nova_rope_cos(const nova_engine* e);
 const float* nova_rope_sin(const nova_engine* e);
 nova_pool*  nova_engine_pool(nova_engine* e);             /* the engine's KvPool (kv_pool(), kv_pool.h:199) */
@@ -359,9 +359,10 @@ int nova_launch_q8_append(const nova_q8_cache* c, const nova_q8_rows* r, const v
 int nova_launch_q8_read(const nova_q8_cache* c, const nova_q8_rows* r, void* k_out, void* v_out, nova_stream_t s);
 /* Attention of the rows of q ([n_tokens][n_heads][128]) over the cached keys: the query at position p sees the keys [0, p], or
  * (p - window, p] where window > 0.  The keys of the new rows must be in the cache; a query that sees none gets zeros.
- * Codes are exact; q (rotated) and the softmax weights are rounded to fp16 on their way into the tensor cores, or, for fp32
- * activations of one row per session and at most 8 query heads per kv head, taken as two fp16 parts (2^-21); sums and the
- * softmax are fp32.  q and out must not overlap.  work: nova_q8_workspace_bytes() bytes, no state in it
+ * q (rotated) and the softmax weights are rounded to fp16 on their way into the tensor cores; sums and the softmax are fp32.
+ * One row per session and at most 8 query heads per kv head: the codes go in exactly and the scales are applied in fp32; with
+ * fp32 activations q and the weights are taken as two fp16 parts each (2^-21).  Anything else: keys and values go in as fp16 values,
+ * code * scale rounded once (|k| saturates at 2^20, |v| at 65504).  q and out must not overlap.  work: nova_q8_workspace_bytes() bytes, no state in it
  * between calls; calls that may overlap on the GPU need a workspace each. */
 size_t nova_q8_workspace_bytes(const nova_kv_shape* sh, const nova_q8_rows* r);
 int nova_launch_q8_attn(const nova_q8_cache* c, const nova_q8_rows* r, const void* q, void* out, int window, void* work,
@@ -370,10 +371,20 @@ int nova_launch_q8_attn(const nova_q8_cache* c, const nova_q8_rows* r, const voi
 int nova_launch_q8_append_attn(const nova_q8_cache* c, const nova_q8_rows* r, const void* q, const void* k, const void* v, void* out,
                                int window, void* work, size_t work_bytes, nova_stream_t s);
 
+/* The cache of one layer of an engine whose pools are 8-bit (nova_engine_desc.kv_dtype NOVA_KV_I8 | NOVA_KV_E4M3) as these calls take
+ * it: its codes, scales, all its block tables (one per slice: give the sessions' slices as slice_ids), rotary tables and status
+ * word.  NOVA_ERR_UNSUPPORTED for other pools. */
+int nova_engine_q8_cache(const nova_engine* e, int layer, nova_q8_cache* out);
+
 /* ------------------------------------------- batched decode over sessions */
 /* Engine::decode_batch's hot-path calls (model.cpp:281-289) for any number of
  * sessions in one launch per op.  A batch owns device copies of the sessions'
- * slice ids and write positions, and the scratch of the split-K attention. */
+ * slice ids and write positions, and the scratch of the split-K attention.
+ * On 8-bit pools the calls below run the kernels of the section above on fp32 activations, one launch per layer: append, attention,
+ * both at once, prefill (sliding windows too), whole steps, graphs, copy-on-write and shared prefixes work as on other pools.
+ * nova_batch_get_kernel is 1 from the start and 0 is refused; the cascade and partial attention (page ranges, peers) are
+ * refused with NOVA_ERR_UNSUPPORTED; fused append works with either rotary pairing; the tuning knobs (pdl, row_setup_pages,
+ * split_ctas, prefill kernel 1) are taken and change nothing.  Buffers have to be 16-byte aligned (NOVA_ERR_INVALID). */
 typedef struct nova_batch nova_batch;
 int  nova_batch_create(nova_engine* e, const int32_t* sessions, int n, nova_batch** out);
 void nova_batch_destroy(nova_batch* b);
