@@ -5,7 +5,7 @@
 // scales), against 4 * 128 * G flops.
 //
 //   * One persistent CTA per SM; the 16-key tiles of all (session, kv group) rows form one line that is dealt out evenly
-//     (attn_plan.cuh); rows that several CTAs worked on are merged by the kernel behind it.
+//     (DecLine); rows that several CTAs worked on are merged by the kernel behind it.
 //   * Four producer warps.  Two bring in the codes of K and V with TMA: boxes [128 B][16 slots][kv group], 128-byte swizzle (a row
 //     of codes is one swizzle line).  Two load the scales, four keys of a head per lane, and leave what the consumers need
 //     of them in shared memory.
@@ -22,13 +22,13 @@
 //     activations: q (rotated) and p rounded to fp16.
 //   * The scale of K multiplies the finished score.  The scale of V goes into the exponent: w_j = 2^(x_j + log2 sv_j - ref), so
 //     the weights that multiply the codes stay inside fp16's range whatever the scales are; the softmax sum adds w_j / sv_j.
-#include "attn_plan.cuh"
 #include "q8_common.cuh"
 
 namespace novab {
 namespace {
 
 constexpr int kSetupTiles = 2;       // work-split weight of starting a row inside a CTA, in tiles
+constexpr int kDecRows = 512;        // (session, kv group) rows of a launch
 constexpr int kMinTiles = 4;         // a CTA gets at least that many tiles (fewer partial rows to merge for short contexts)
 
 template <int KVG>
@@ -39,7 +39,7 @@ struct DecCfg {
     static constexpr int kHalf = KVG * 2048;                // K (or V) codes of a tile
     static constexpr int kTile = 2 * kHalf;
     static constexpr int kScales = KVG * 192;               // K scales | logarithms of V's | reciprocals of V's
-    static constexpr int kMergeFloats = KVG * (kSub - 1) * 36 * 32;
+    static constexpr int kMergeFloats = KVG * kSub * 36 * 32;
     static constexpr int kRawSteps = 8;                     // rings of raw scales (K, V), steps of 512 bytes
     static constexpr int kSmem = kStages * (kTile + kScales) + 2 * kRawSteps * 512 + kMergeFloats * 4 + 1024;
     static constexpr int kThreads = 32 * (kCons + 4);
@@ -47,67 +47,104 @@ struct DecCfg {
     static_assert(kStages % kSub == 0, "stages and consumer warps");
 };
 
-// Keys, first tile and tile count of every (session, group) row; a row without a new token has no tiles.
+// The line of work: per (session, group) row kSetupTiles and its tiles (a row without a new token: nothing), in 32 bits, cut off
+// where it would pass them.
 struct DecPlan {
-    int prefix[kMaxRowsSmem + 1];
-    int keys[kMaxRowsSmem];
-    int row[kMaxRowsSmem];
-    int slice[kMaxRowsSmem];
+    int prefix[kDecRows + 1];
+    int keys[kDecRows];
+    int row[kDecRows];
+    int slice[kDecRows];
 };
 
 __device__ __forceinline__ int dec_first_tile(const Q8Launch& a, int keys) { return a.window > 0 && keys > a.window ? (keys - a.window) >> 4 : 0; }
 
 __device__ inline void dec_build_plan(const Q8Launch& a, DecPlan& p, int n_groups, bool flag) {
+    for (int s = (int)threadIdx.x; s < a.n_sessions; s += (int)blockDim.x) {      // (all loads at once: one trip to memory)
+        int first, count;
+        q8_rows(a, s, first, count);
+        const int pos = __ldg(a.n_past + s), slice = a.slice_ids ? __ldg(a.slice_ids + s) : s;
+        int keys = 0;
+        if (count > 0) {
+            if (pos < 0 || pos == 0x7fffffff || (a.rope_cs && pos >= a.rope_rows)) {
+                if (flag) q8_flag(a, NOVA_ERR_INVALID);
+            } else {
+                keys = pos + 1;
+            }
+        }
+        p.keys[s] = keys;
+        p.row[s] = first;
+        p.slice[s] = slice;
+    }
+    __syncthreads();
     if (threadIdx.x < 32) {
         const int lane = (int)threadIdx.x, rows = a.n_sessions * n_groups;
-        int carry = 0;
+        uint32_t carry = 0;
         if (lane == 0) p.prefix[0] = 0;
         for (int base = 0; base < rows; base += 32) {
-            const int r = base + lane;
-            int v = 0;
-            if (r < rows) {
-                const int s = r / n_groups;
-                int first, count;
-                q8_rows(a, s, first, count);
-                const int pos = __ldg(a.n_past + s);
-                int keys = 0;
-                if (count > 0) {
-                    if (pos < 0 || pos == 0x7fffffff || (a.rope_cs && pos >= a.rope_rows)) {
-                        if (flag) q8_flag(a, NOVA_ERR_INVALID);
-                    } else {
-                        keys = pos + 1;
-                    }
-                }
-                if (r - s * n_groups == 0) {
-                    p.keys[s] = keys;
-                    p.row[s] = first;
-                    p.slice[s] = a.slice_ids ? __ldg(a.slice_ids + s) : s;
-                }
-                v = keys > 0 ? ((keys + 15) >> 4) - dec_first_tile(a, keys) + kSetupTiles : 0;
-            }
+            const int r = base + lane, keys = r < rows ? p.keys[r / n_groups] : 0;
+            uint32_t v = keys > 0 ? (uint32_t)(((keys + 15) >> 4) - dec_first_tile(a, keys) + kSetupTiles) : 0u;
+            v = min(v, 0x7ffffffu);                            // (the sum of 32 stays inside 32 bits)
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
-                const int t = __shfl_up_sync(0xffffffffu, v, o);
+                const uint32_t t = __shfl_up_sync(0xffffffffu, v, o);
                 if (lane >= o) v += t;
             }
-            if (r < rows) p.prefix[r + 1] = carry + v;
-            carry += __shfl_sync(0xffffffffu, v, 31);
+            const uint32_t sum = min(carry + min(v, 0x7fffffffu), 0x7fffffffu);
+            if (r < rows) p.prefix[r + 1] = (int)sum;
+            carry = __shfl_sync(0xffffffffu, sum, 31);
         }
+        if (flag && lane == 0 && carry == 0x7fffffffu) q8_flag(a, NOVA_ERR_INVALID);
     }
     __syncthreads();
 }
 
-__device__ __forceinline__ PlanView dec_view(const Q8Launch& a, const DecPlan& p, int n_groups, int grid) {
-    PlanView pv;
-    pv.prefix = p.prefix;
-    pv.rows_per_layer = a.n_sessions * n_groups;
-    pv.n_groups = n_groups;
-    pv.pages_per_layer = p.prefix[pv.rows_per_layer];
-    pv.pages_total = pv.pages_per_layer;
-    const int64_t most = (pv.pages_total + kMinTiles - 1) / kMinTiles;
-    pv.n_ctas = most < grid ? (int)most : grid;
-    plan_finish(pv);
-    return pv;
+// The line dealt out evenly: the first `extra` CTAs get per + 1 entries, the others per.
+struct DecLine {
+    int rows, n_groups, total, n_ctas, per, extra;
+    __device__ __forceinline__ int begin(int c) const { return c * per + min(c, extra); }
+    __device__ __forceinline__ int owner(int t) const {
+        const int wide = extra * (per + 1);
+        return t < wide ? t / (per + 1) : extra + (t - wide) / per;
+    }
+};
+__device__ __forceinline__ DecLine dec_line(const Q8Launch& a, const DecPlan& p, int n_groups, int grid) {
+    DecLine ln;
+    ln.rows = a.n_sessions * n_groups;
+    ln.n_groups = n_groups;
+    ln.total = p.prefix[ln.rows];
+    const int most = ln.total / kMinTiles + (ln.total % kMinTiles != 0);
+    ln.n_ctas = most < grid ? most : grid;
+    ln.per = ln.total > 0 ? ln.total / ln.n_ctas : 0;
+    ln.extra = ln.total - ln.per * ln.n_ctas;
+    return ln;
+}
+
+// What a CTA does of one row: from entry pos of the line to the row's end or hi.  By whole warps.
+struct DecSegment {
+    int row, session, group;
+    int first, count;      // tiles, counted from the row's first
+    int span;              // entries of the line
+    bool whole;            // no other CTA works on the row
+};
+__device__ __forceinline__ DecSegment dec_segment(const DecPlan& p, const DecLine& ln, int pos, int lo, int hi) {
+    const int lane = (int)threadIdx.x & 31, stride = (ln.rows + 31) >> 5;
+    // the last row that begins at pos or before (rows without work begin where the next one does)
+    int at = lane * stride;
+    int row = (__popc(__ballot_sync(0xffffffffu, at < ln.rows && p.prefix[at] <= pos)) - 1) * stride;
+    if (stride > 1) {
+        at = row + lane;
+        row += __popc(__ballot_sync(0xffffffffu, lane < stride && at < ln.rows && p.prefix[at] <= pos)) - 1;
+    }
+    DecSegment sg;
+    const int begin = p.prefix[row], row_end = p.prefix[row + 1], end = row_end < hi ? row_end : hi;
+    sg.row = row;
+    sg.session = row / ln.n_groups;
+    sg.group = row - sg.session * ln.n_groups;
+    sg.span = end - pos;
+    sg.first = max(pos - begin - kSetupTiles, 0);
+    sg.count = max(end - begin - kSetupTiles, 0) - sg.first;
+    sg.whole = begin >= lo && row_end <= hi;
+    return sg;
 }
 
 // kLo: q and p in two fp16 parts (fp32 activations)
@@ -151,9 +188,9 @@ q8_decode_kernel(Q8Launch a, const __grid_constant__ CUtensorMap tmk, const __gr
     pdl_wait();
     pdl_launch_dependents();
     dec_build_plan(a, s_plan, n_groups, blockIdx.x == 0);
-    const PlanView pv = dec_view(a, s_plan, n_groups, (int)gridDim.x);
-    if (pv.pages_total == 0 || (int)blockIdx.x >= pv.n_ctas) return;
-    const int64_t lo = plan_cta_begin(pv, (int)blockIdx.x), hi = plan_cta_begin(pv, (int)blockIdx.x + 1);
+    const DecLine ln = dec_line(a, s_plan, n_groups, (int)gridDim.x);
+    if ((int)blockIdx.x >= ln.n_ctas) return;
+    const int lo = ln.begin((int)blockIdx.x), hi = ln.begin((int)blockIdx.x + 1);
 
     // ------------------------------------------------------------------------------------------------ producers
     // Each of the four goes through ALL tiles in order: a stage's fill waits for the release of the fill before, which the same
@@ -185,28 +222,28 @@ q8_decode_kernel(Q8Launch a, const __grid_constant__ CUtensorMap tmk, const __gr
         const CUtensorMap* const tm = is_v ? &tmv : &tmk;
         const int row0 = (a.layer * a.nb) << a.kv_shift;
         uint32_t it0 = 0;                                                   // tiles before this segment
-        for (int64_t pos = lo; pos < hi;) {
-            const Segment sg = plan_segment(pv, pos, hi, kSetupTiles);
+        for (int pos = lo; pos < hi;) {
+            const DecSegment sg = dec_segment(s_plan, ln, pos, lo, hi);
             pos += sg.span;
             const int keys = s_plan.keys[sg.session];
-            const int t0 = dec_first_tile(a, keys) + sg.page_first, low = a.window > 0 && keys > a.window ? keys - a.window : 0;
+            const int t0 = dec_first_tile(a, keys) + sg.first, low = a.window > 0 && keys > a.window ? keys - a.window : 0;
             const int32_t* table = a.tables + (int64_t)s_plan.slice[sg.session] * a.table_stride;
             int n0, n1, c0 = 0, c1 = 0;
-            fetch(table, keys, t0 + lane, lane < sg.page_count, n0, n1);
+            fetch(table, keys, t0 + lane, lane < sg.count, n0, n1);
             uint32_t stage = (it0 + (uint32_t)lane) % kStages, round = (it0 + (uint32_t)lane) / kStages;
 #pragma unroll 1
-            for (int b = 0; b < sg.page_count; b += Cfg::kBatch) {
+            for (int b = 0; b < sg.count; b += Cfg::kBatch) {
                 if ((b & 31) == 0) {                                        // 32 entries at a time, the next 32 on their way
                     c0 = n0;
                     c1 = n1;
                     const int nx = b + 32 + lane;
-                    fetch(table, keys, t0 + nx, nx < sg.page_count, n0, n1);
+                    fetch(table, keys, t0 + nx, nx < sg.count, n0, n1);
                 }
                 const int i = b + lane, t = t0 + i;
                 const int e0 = __shfl_sync(0xffffffffu, c0, i & 31);
                 int e1 = -2;
                 if (p8) e1 = __shfl_sync(0xffffffffu, c1, i & 31);
-                const bool mine = lane < Cfg::kBatch && i < sg.page_count;
+                const bool mine = lane < Cfg::kBatch && i < sg.count;
                 const bool free = !mine || round == 0 || mbar_wait(smem_u32(&s_empty[stage]), (round - 1) & 1, &s_abort);
                 if (!__all_sync(0xffffffffu, free)) {
                     if (lane == 0) q8_flag(a, NOVA_ERR_TIMEOUT);
@@ -237,7 +274,7 @@ q8_decode_kernel(Q8Launch a, const __grid_constant__ CUtensorMap tmk, const __gr
                     ++round;
                 }
             }
-            it0 += (uint32_t)sg.page_count;
+            it0 += (uint32_t)sg.count;
         }
         return;
     }
@@ -253,15 +290,15 @@ q8_decode_kernel(Q8Launch a, const __grid_constant__ CUtensorMap tmk, const __gr
         const uint32_t dst0 = scale0 + (uint32_t)((is_v ? KVG * 64 : 0) + h * 64 + quad * 16);
         const int slot_mask = p8 ? 0 : (1 << a.kv_shift) - 1, slot_add = p8 ? 4 * (quad & 1) : 4 * quad;
         uint32_t it0 = 0;
-        for (int64_t pos = lo; pos < hi;) {
-            const Segment sg = plan_segment(pv, pos, hi, kSetupTiles);
+        for (int pos = lo; pos < hi;) {
+            const DecSegment sg = dec_segment(s_plan, ln, pos, lo, hi);
             pos += sg.span;
-            const int keys = s_plan.keys[sg.session], t0 = dec_first_tile(a, keys) + sg.page_first;
+            const int keys = s_plan.keys[sg.session], t0 = dec_first_tile(a, keys) + sg.first;
             const int32_t* table = a.tables + (int64_t)s_plan.slice[sg.session] * a.table_stride;
             const float* const mine0 = (is_v ? a.scale_v : a.scale_k) + ((((int64_t)a.layer * a.nb) * a.n_kv_heads + sg.group * KVG + h) << a.kv_shift);
-            const int steps = (sg.page_count + kPer - 1) / kPer;
+            const int steps = (sg.count + kPer - 1) / kPer;
             int n0, n1, c0 = 0, c1 = 0;
-            fetch(table, keys, t0 + lane, lane < sg.page_count, n0, n1);
+            fetch(table, keys, t0 + lane, lane < sg.count, n0, n1);
             uint32_t stage = (it0 + (uint32_t)sub_tile) % kStages, round = (it0 + (uint32_t)sub_tile) / kStages;
             int i = sub_tile - kDepth * kPer;                               // the tile that this step converts
 #pragma unroll 1
@@ -272,7 +309,7 @@ q8_decode_kernel(Q8Launch a, const __grid_constant__ CUtensorMap tmk, const __gr
                         c0 = n0;
                         c1 = n1;
                         const int nx = f + 32 + lane;
-                        fetch(table, keys, t0 + nx, nx < sg.page_count, n0, n1);
+                        fetch(table, keys, t0 + nx, nx < sg.count, n0, n1);
                     }
                     int e = __shfl_sync(0xffffffffu, c0, (f + sub_tile) & 31);       // (below 0 behind the segment's last tile too)
                     if (p8) {
@@ -287,7 +324,7 @@ q8_decode_kernel(Q8Launch a, const __grid_constant__ CUtensorMap tmk, const __gr
                 asm volatile("cp.async.commit_group;" ::: "memory");
                 if (step < kDepth) continue;
                 asm volatile("cp.async.wait_group %0;" ::"n"(kDepth) : "memory");
-                const bool mine = i < sg.page_count;                        // a lane converts what it has brought itself
+                const bool mine = i < sg.count;                        // a lane converts what it has brought itself
                 const uint4 u = lds128(raw0 + (uint32_t)((step - kDepth) & (Cfg::kRawSteps - 1)) * 512u);
                 const float4 v = make_float4(__uint_as_float(u.x), __uint_as_float(u.y), __uint_as_float(u.z), __uint_as_float(u.w));
                 const bool free = !mine || round == 0 || mbar_wait(smem_u32(&s_empty[stage]), (round - 1) & 1, &s_abort);
@@ -313,7 +350,7 @@ q8_decode_kernel(Q8Launch a, const __grid_constant__ CUtensorMap tmk, const __gr
                     ++round;
                 }
             }
-            it0 += (uint32_t)sg.page_count;
+            it0 += (uint32_t)sg.count;
         }
         asm volatile("cp.async.wait_all;" ::: "memory");
         return;
@@ -325,11 +362,11 @@ q8_decode_kernel(Q8Launch a, const __grid_constant__ CUtensorMap tmk, const __gr
     uint32_t it = 0;                                  // tiles of the segments before
     int stage = sub;                                  // of this warp's next tile, and the parity of its fill
     uint32_t parity = 0;
-    for (int64_t pos = lo; pos < hi;) {
-        const Segment sg = plan_segment(pv, pos, hi, kSetupTiles);
+    for (int pos = lo; pos < hi;) {
+        const DecSegment sg = dec_segment(s_plan, ln, pos, lo, hi);
         pos += sg.span;
         const int s = sg.session, kvh = sg.group * KVG + w;
-        const int keys = s_plan.keys[s], row = s_plan.row[s], t0 = dec_first_tile(a, keys) + sg.page_first;
+        const int keys = s_plan.keys[s], row = s_plan.row[s], t0 = dec_first_tile(a, keys) + sg.first;
         const int head = kvh * G + (g < G ? g : 0);
 
         // q fragments of head g: this lane's dims are 32 t .. 32 t + 31, four per contraction step
@@ -337,27 +374,25 @@ q8_decode_kernel(Q8Launch a, const __grid_constant__ CUtensorMap tmk, const __gr
         float off0 = 0.f, off1 = 0.f;             // what the accumulators of heads 2 t and 2 t + 1 start at
         {
             float qsum = 0.f;
-            const int64_t qe = (int64_t)row * a.q_stride + (int64_t)head * kHeadDim;
+            const int64_t qe = (int64_t)row * a.q_stride + (int64_t)head * kHeadDim + 32 * t;
+            // all loads before their first use: they are one trip to memory
+            constexpr int kRaw = kLo ? 8 : 4;
+            uint4 raw[kRaw];
+            const uint4* const qp = reinterpret_cast<const uint4*>(static_cast<const unsigned char*>(a.q) + qe * (kLo ? 4 : 2));
 #pragma unroll
-            for (int ks = 0; ks < 8; ++ks) {
-                float4 x = q8_load4(a.q, qe + 32 * t + 4 * ks, a.io);
-                if (a.rope_cs) {
-                    const int64_t cpos = (int64_t)(keys - 1) * 64;
-                    if (a.neox) {
-                        const float4 y = q8_load4(a.q, qe + ((32 * t) ^ 64) + 4 * ks, a.io);
-                        const float4 c = *reinterpret_cast<const float4*>(a.rope_cs + cpos + ((32 * t) & 63) + 4 * ks);
-                        const float4 n = *reinterpret_cast<const float4*>(a.rope_sn + cpos + ((32 * t) & 63) + 4 * ks);
-                        if (t < 2) x = make_float4(__fmaf_rn(x.x, c.x, -__fmul_rn(y.x, n.x)), __fmaf_rn(x.y, c.y, -__fmul_rn(y.y, n.y)),
-                                                   __fmaf_rn(x.z, c.z, -__fmul_rn(y.z, n.z)), __fmaf_rn(x.w, c.w, -__fmul_rn(y.w, n.w)));
-                        else x = make_float4(__fmaf_rn(y.x, n.x, __fmul_rn(x.x, c.x)), __fmaf_rn(y.y, n.y, __fmul_rn(x.y, c.y)),
-                                             __fmaf_rn(y.z, n.z, __fmul_rn(x.z, c.z)), __fmaf_rn(y.w, n.w, __fmul_rn(x.w, c.w)));
-                    } else {
-                        const float2 c = *reinterpret_cast<const float2*>(a.rope_cs + cpos + 16 * t + 2 * ks);
-                        const float2 n = *reinterpret_cast<const float2*>(a.rope_sn + cpos + 16 * t + 2 * ks);
-                        x = make_float4(__fmaf_rn(x.x, c.x, -__fmul_rn(x.y, n.x)), __fmaf_rn(x.x, n.x, __fmul_rn(x.y, c.x)),
-                                        __fmaf_rn(x.z, c.y, -__fmul_rn(x.w, n.y)), __fmaf_rn(x.z, n.y, __fmul_rn(x.w, c.y)));
-                    }
+            for (int e = 0; e < kRaw; ++e) raw[e] = __ldg(qp + e);
+            const bool bf = a.io == NOVA_IO_BF16;
+            auto load = [&](int ks) {
+                if constexpr (kLo) {
+                    return make_float4(__uint_as_float(raw[ks].x), __uint_as_float(raw[ks].y), __uint_as_float(raw[ks].z), __uint_as_float(raw[ks].w));
+                } else {
+                    const uint32_t u0 = ks & 1 ? raw[ks >> 1].z : raw[ks >> 1].x, u1 = ks & 1 ? raw[ks >> 1].w : raw[ks >> 1].y;
+                    const float2 h0 = __half22float2(*reinterpret_cast<const __half2*>(&u0)), h1 = __half22float2(*reinterpret_cast<const __half2*>(&u1));
+                    return bf ? make_float4(__uint_as_float(u0 << 16), __uint_as_float(u0 & 0xffff0000u), __uint_as_float(u1 << 16), __uint_as_float(u1 & 0xffff0000u))
+                              : make_float4(h0.x, h0.y, h1.x, h1.y);
                 }
+            };
+            auto put = [&](int ks, float4 x) {
                 const float f[4] = {x.x * 0.125f, x.y * 0.125f, x.z * 0.125f, x.w * 0.125f};
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
@@ -367,6 +402,47 @@ q8_decode_kernel(Q8Launch a, const __grid_constant__ CUtensorMap tmk, const __gr
                     qsum += kLo ? f[2 * e] + f[2 * e + 1] : b.x + b.y;
                     if constexpr (kLo) ql[ks][e] = g < G ? pack_h2(f[2 * e] - b.x, f[2 * e + 1] - b.y) : 0u;
                 }
+            };
+            const int64_t cpos = (int64_t)(keys - 1) * 64;
+            if (a.rope_cs && a.neox) {
+                const float4* const cp = reinterpret_cast<const float4*>(a.rope_cs + cpos + ((32 * t) & 63));
+                const float4* const np = reinterpret_cast<const float4*>(a.rope_sn + cpos + ((32 * t) & 63));
+#pragma unroll
+                for (int k0 = 0; k0 < 8; k0 += 4) {
+                    float4 c[4], n[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        c[e] = __ldg(cp + k0 + e);
+                        n[e] = __ldg(np + k0 + e);
+                    }
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const float4 x = load(k0 + e);              // the other half of the pair: dims 32 (t ^ 2) ..
+                        const float4 y = make_float4(__shfl_xor_sync(0xffffffffu, x.x, 2), __shfl_xor_sync(0xffffffffu, x.y, 2),
+                                                     __shfl_xor_sync(0xffffffffu, x.z, 2), __shfl_xor_sync(0xffffffffu, x.w, 2));
+                        const float4 lo4 = make_float4(__fmaf_rn(x.x, c[e].x, -__fmul_rn(y.x, n[e].x)), __fmaf_rn(x.y, c[e].y, -__fmul_rn(y.y, n[e].y)),
+                                                       __fmaf_rn(x.z, c[e].z, -__fmul_rn(y.z, n[e].z)), __fmaf_rn(x.w, c[e].w, -__fmul_rn(y.w, n[e].w)));
+                        const float4 hi4 = make_float4(__fmaf_rn(y.x, n[e].x, __fmul_rn(x.x, c[e].x)), __fmaf_rn(y.y, n[e].y, __fmul_rn(x.y, c[e].y)),
+                                                       __fmaf_rn(y.z, n[e].z, __fmul_rn(x.z, c[e].z)), __fmaf_rn(y.w, n[e].w, __fmul_rn(x.w, c[e].w)));
+                        put(k0 + e, t < 2 ? lo4 : hi4);
+                    }
+                }
+            } else if (a.rope_cs) {
+                float2 c[8], n[8];
+#pragma unroll
+                for (int ks = 0; ks < 8; ++ks) {
+                    c[ks] = __ldg(reinterpret_cast<const float2*>(a.rope_cs + cpos + 16 * t) + ks);
+                    n[ks] = __ldg(reinterpret_cast<const float2*>(a.rope_sn + cpos + 16 * t) + ks);
+                }
+#pragma unroll
+                for (int ks = 0; ks < 8; ++ks) {
+                    const float4 x = load(ks);
+                    put(ks, make_float4(__fmaf_rn(x.x, c[ks].x, -__fmul_rn(x.y, n[ks].x)), __fmaf_rn(x.x, n[ks].x, __fmul_rn(x.y, c[ks].x)),
+                                        __fmaf_rn(x.z, c[ks].y, -__fmul_rn(x.w, n[ks].y)), __fmaf_rn(x.z, n[ks].y, __fmul_rn(x.w, c[ks].y))));
+                }
+            } else {
+#pragma unroll
+                for (int ks = 0; ks < 8; ++ks) put(ks, load(ks));
             }
             if constexpr (kFmt == NOVA_KV_I8) {
                 qsum += __shfl_xor_sync(0xffffffffu, qsum, 1);
@@ -382,7 +458,7 @@ q8_decode_kernel(Q8Launch a, const __grid_constant__ CUtensorMap tmk, const __gr
 #pragma unroll
         for (int j = 0; j < 8; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
 
-        const uint32_t it_end = it + (uint32_t)sg.page_count;
+        const uint32_t it_end = it + (uint32_t)sg.count;
         for (uint32_t i = it + (((uint32_t)sub + kSub - it % kSub) % kSub); i < it_end; i += kSub) {
             if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(&s_full[stage]), parity, &s_abort))) {
                 if (lane == 0) q8_flag(a, NOVA_ERR_TIMEOUT);      // the result is void; the warp still meets its siblings below
@@ -535,123 +611,158 @@ q8_decode_kernel(Q8Launch a, const __grid_constant__ CUtensorMap tmk, const __gr
             l0 += __shfl_xor_sync(0xffffffffu, l0, sh);
             l1 += __shfl_xor_sync(0xffffffffu, l1, sh);
         }
-        if constexpr (kSub > 1) {
-            float* mine = merge + (size_t)(w * (kSub - 1)) * 36 * 32 + lane;
-            if (sub > 0) {
-                float* p = mine + (size_t)(sub - 1) * 36 * 32;
+        // every warp leaves its 32 sums a lane; each then adds up and writes some of them: piece un is four dims of a lane's head
+        // 2 t + (un & 1), o[j][e] and o[j][2 + e] being the dims 16 g + 2 j and 16 g + 2 j + 1
+        float* const all = merge + (size_t)w * kSub * 36 * 32 + lane;
+        {
+            float* p = all + (size_t)sub * 36 * 32;
 #pragma unroll
-                for (int j = 0; j < 32; ++j) p[32 * j] = o[j >> 2][j & 3];
-                p[32 * 32] = ref0;
-                p[33 * 32] = ref1;
-                p[34 * 32] = l0;
-                p[35 * 32] = l1;
-            }
-            asm volatile("bar.sync %0, %1;" ::"r"(1 + w), "r"(32 * kSub) : "memory");
-            if (sub == 0) {
+            for (int j = 0; j < 32; ++j) p[32 * j] = o[j >> 2][j & 3];
+            p[32 * 32] = ref0;
+            p[33 * 32] = ref1;
+            p[34 * 32] = l0;
+            p[35 * 32] = l1;
+        }
+        asm volatile("bar.sync %0, %1;" ::"r"(1 + w), "r"(32 * kSub) : "memory");
 #pragma unroll 1
-                for (int u = 0; u < kSub - 1; ++u) {
-                    const float* p = mine + (size_t)u * 36 * 32;
-                    const float u0 = p[32 * 32], u1 = p[33 * 32];
-                    const float n0 = fmaxf(ref0, u0), n1 = fmaxf(ref1, u1);
-                    const float a0 = ref0 == -INFINITY ? 0.f : ex2(ref0 - n0), b0 = u0 == -INFINITY ? 0.f : ex2(u0 - n0);
-                    const float a1 = ref1 == -INFINITY ? 0.f : ex2(ref1 - n1), b1 = u1 == -INFINITY ? 0.f : ex2(u1 - n1);
-                    l0 = l0 * a0 + p[34 * 32] * b0;
-                    l1 = l1 * a1 + p[35 * 32] * b1;
+        for (int un = sub; un < 8; un += kSub) {
+            const int e = un & 1, j = un & 6, hd = 2 * t + e;
+            float M = -INFINITY, L = 0.f;
+            float wt[kSub];
 #pragma unroll
-                    for (int j = 0; j < 32; ++j) o[j >> 2][j & 3] = o[j >> 2][j & 3] * (j & 1 ? a1 : a0) + p[32 * j] * (j & 1 ? b1 : b0);
-                    ref0 = n0;
-                    ref1 = n1;
-                }
+            for (int u = 0; u < kSub; ++u) {
+                wt[u] = all[(size_t)u * 36 * 32 + 32 * (32 + e)];
+                M = fmaxf(M, wt[u]);
             }
-            asm volatile("bar.sync %0, %1;" ::"r"(1 + w), "r"(32 * kSub) : "memory");
-            if (sub > 0) continue;
-        }
+            float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {                       // heads 2 t + e: o[j][e], o[j][2 + e] are the dims 16 g + 2 j, 16 g + 2 j + 1
-            const int hd = 2 * t + e;
+            for (int u = 0; u < kSub; ++u) {
+                const float* p = all + (size_t)u * 36 * 32;
+                const float l = p[32 * (34 + e)], c = l != 0.f ? ex2(wt[u] - M) : 0.f;      // (a NaN stays one)
+                L = fmaf(l, c, L);
+                y = make_float4(fmaf(p[32 * (4 * j + e)], c, y.x), fmaf(p[32 * (4 * j + 2 + e)], c, y.y), fmaf(p[32 * (4 * j + 4 + e)], c, y.z),
+                                fmaf(p[32 * (4 * j + 6 + e)], c, y.w));
+            }
             if (hd >= G) continue;
-            const float l = e ? l1 : l0;
-            if (sg.c_last == sg.c_first) {
-                const float inv = l > 0.f ? 1.f / l : 0.f;
-                const int64_t oe = (int64_t)row * a.out_stride + (int64_t)(kvh * G + hd) * kHeadDim + 16 * g;
-#pragma unroll
-                for (int j = 0; j < 8; j += 2)
-                    q8_store4(a.out, oe + 2 * j, a.io, make_float4(o[j][e] * inv, o[j][2 + e] * inv, o[j + 1][e] * inv, o[j + 1][2 + e] * inv));
+            if (sg.whole) {
+                const float inv = L > 0.f ? 1.f / L : 0.f;
+                q8_store4(a.out, (int64_t)row * a.out_stride + (int64_t)(kvh * G + hd) * kHeadDim + 16 * g + 2 * j, a.io,
+                          make_float4(y.x * inv, y.y * inv, y.z * inv, y.w * inv));
             } else {
-                float* p = a.part + ((size_t)((int64_t)blockIdx.x + sg.row_id) * heads_per_row + (size_t)(w * G + hd)) * kSlotW;
-                if (g == 0) *reinterpret_cast<float2*>(p) = make_float2(e ? ref1 : ref0, l);
-#pragma unroll
-                for (int j = 0; j < 8; j += 2)
-                    *reinterpret_cast<float4*>(p + 4 + 16 * g + 2 * j) = make_float4(o[j][e], o[j][2 + e], o[j + 1][e], o[j + 1][2 + e]);
+                float* p = a.part + ((size_t)((int)blockIdx.x + sg.row) * heads_per_row + (size_t)(w * G + hd)) * kSlotW;
+                if (g == 0 && j == 0) *reinterpret_cast<float2*>(p) = make_float2(M, L);
+                *reinterpret_cast<float4*>(p + 4 + 16 * g + 2 * j) = y;
             }
         }
+        asm volatile("bar.sync %0, %1;" ::"r"(1 + w), "r"(32 * kSub) : "memory");
     }
 }
 
-// Merge of the rows that several CTAs worked on.  One CTA of four warps per (row, head); the warps take the contributors in
-// turn, four at a time, a lane four dims; the warps' sums meet in shared memory, always in the same order.
-__global__ void __launch_bounds__(128) q8_decode_merge_kernel(Q8Launch a, int kvg, int grid_split) {
+// Merge of the rows that several CTAs worked on: W warps per (row, head).  The first finds every contributor's weight; the
+// contributors are dealt to the warps, eight at a time, a lane four dims; the warps' sums are added in order.
+template <int W>
+__global__ void __launch_bounds__(W == 16 ? 512 : 128) q8_decode_merge_kernel(Q8Launch a, int kvg, int grid_split) {
+    constexpr int kWarps = W == 16 ? 16 : 4, kUnits = kWarps / W;
     __shared__ DecPlan s_plan;
-    __shared__ float s_ml[8];
-    __shared__ float4 s_acc[128];
-    const int lane = (int)threadIdx.x & 31, warp = (int)threadIdx.x >> 5;
+    __shared__ float s_w[kUnits][kQ8MaxCtas];
+    __shared__ float s_inv[kUnits];
+    __shared__ float4 s_acc[W == 1 ? 1 : kWarps * 32];
+    const int lane = (int)threadIdx.x & 31, warp = (int)threadIdx.x >> 5, mine = warp / W, part = warp % W;
     const int G = a.n_heads / a.n_kv_heads, n_groups = a.n_kv_heads / kvg, heads_per_row = kvg * G;
     pdl_launch_dependents();
     dec_build_plan(a, s_plan, n_groups, false);           // (positions and row starts: written before the split, which waited)
-    const PlanView pv = dec_view(a, s_plan, n_groups, grid_split);
-    const int units = pv.pages_total > 0 ? pv.rows_per_layer * heads_per_row : 0;
+    const DecLine ln = dec_line(a, s_plan, n_groups, grid_split);
+    const int units = ln.total > 0 ? ln.rows * heads_per_row : 0;
+    auto sync = [] {
+        if constexpr (W == 1) __syncwarp();
+        else __syncthreads();
+    };
+    // contributors of a unit: CTAs c0 .. c0 + n - 1 (n == 1: written by the split kernel)
+    int r = 0, hr = 0, c0 = 0, n = 1;
+    auto find = [&](int u) {
+        n = 1;
+        if (u >= units) return;
+        r = u / heads_per_row;
+        hr = u - r * heads_per_row;
+        if (s_plan.prefix[r + 1] == s_plan.prefix[r]) return;
+        c0 = ln.owner(s_plan.prefix[r]);
+        n = ln.owner(s_plan.prefix[r + 1] - 1) - c0 + 1;
+    };
+    int u = (int)blockIdx.x * kUnits + mine;
+    find(u);
     pdl_wait();
-    for (int u = (int)blockIdx.x; u < units; u += (int)gridDim.x) {
-        const int r = u / heads_per_row, hr = u - r * heads_per_row;
-        if (s_plan.prefix[r + 1] == s_plan.prefix[r]) continue;
-        const int c0 = plan_owner(pv, s_plan.prefix[r]), n = plan_owner(pv, s_plan.prefix[r + 1] - 1) - c0 + 1;
-        if (n == 1) continue;                              // written by the split kernel
+    for (; u < units; u += (int)gridDim.x * kUnits, find(u)) {
+        if (n == 1) continue;
         const size_t step = (size_t)heads_per_row * kSlotW;
         const float* base = a.part + ((size_t)(c0 + r) * heads_per_row + hr) * kSlotW;
-        float M = -INFINITY, L = 0.f;
-        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-        for (int i = 4 * warp; i < n; i += 16) {
-            float2 ml[4];
-            float4 x[4];
+        constexpr int kBatch = 8;
+        float4 x[kBatch];
+        auto bring = [&](int i0) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const float* p = base + (size_t)(i + e < n ? i + e : i) * step;
-                ml[e] = __ldcg(reinterpret_cast<const float2*>(p));
-                x[e] = __ldcg(reinterpret_cast<const float4*>(p + 4 + 4 * lane));
+            for (int e = 0; e < kBatch; ++e)
+                if (i0 + e * W < n) x[e] = __ldcg(reinterpret_cast<const float4*>(base + (size_t)(i0 + e * W) * step + 4 + 4 * lane));
+        };
+        bring(part);
+        if (part == 0) {
+            float2 ml[kQ8MaxCtas / 32];
+            float M = -INFINITY, L = 0.f;
+#pragma unroll
+            for (int e = 0; e < kQ8MaxCtas / 32; ++e) {
+                ml[e] = make_float2(-INFINITY, 0.f);
+                if (32 * e + lane < n) ml[e] = __ldcg(reinterpret_cast<const float2*>(base + (size_t)(32 * e + lane) * step));
             }
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                if (i + e >= n || !(ml[e].y > 0.f)) continue;
-                const float mn = fmaxf(M, ml[e].x), cm = M == -INFINITY ? 0.f : ex2(M - mn), cx = ex2(ml[e].x - mn);
-                M = mn;
-                L = L * cm + ml[e].y * cx;
-                acc = make_float4(acc.x * cm + x[e].x * cx, acc.y * cm + x[e].y * cx, acc.z * cm + x[e].z * cx, acc.w * cm + x[e].w * cx);
+            for (int e = 0; e < kQ8MaxCtas / 32; ++e)
+                if (ml[e].y != 0.f) M = fmaxf(M, ml[e].x);
+#pragma unroll
+            for (int o = 16; o; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+#pragma unroll
+            for (int e = 0; e < kQ8MaxCtas / 32; ++e) {
+                const float c = ml[e].y != 0.f ? ex2(ml[e].x - M) : 0.f;
+                L += ml[e].y * c;
+                if (32 * e + lane < n) s_w[mine][32 * e + lane] = c;
+            }
+#pragma unroll
+            for (int o = 16; o; o >>= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
+            if (lane == 0) s_inv[mine] = L > 0.f ? 1.f / L : 0.f;
+        }
+        sync();
+        float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int i0 = part; i0 < n; i0 += kBatch * W) {
+            if (i0 != part) bring(i0);
+#pragma unroll
+            for (int e = 0; e < kBatch; ++e) {
+                if (i0 + e * W >= n) break;
+                const float c = s_w[mine][i0 + e * W];
+                y = make_float4(fmaf(x[e].x, c, y.x), fmaf(x[e].y, c, y.y), fmaf(x[e].z, c, y.z), fmaf(x[e].w, c, y.w));
             }
         }
-        if (lane == 0) {
-            s_ml[2 * warp] = M;
-            s_ml[2 * warp + 1] = L;
-        }
-        s_acc[threadIdx.x] = acc;
-        __syncthreads();
-        if (warp == 0) {
-            float Mx = -INFINITY, Lx = 0.f;
-            float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
-            for (int v = 0; v < 4; ++v) Mx = fmaxf(Mx, s_ml[2 * v]);
-            for (int v = 0; v < 4; ++v) {
-                if (s_ml[2 * v] == -INFINITY) continue;
-                const float cw = ex2(s_ml[2 * v] - Mx);
-                const float4 z = s_acc[32 * v + lane];
-                Lx += s_ml[2 * v + 1] * cw;
-                y = make_float4(y.x + z.x * cw, y.y + z.y * cw, y.z + z.z * cw, y.w + z.w * cw);
+        if constexpr (W > 1) {
+            s_acc[threadIdx.x] = y;
+            sync();
+            if (part == 0) {
+#pragma unroll
+                for (int v = 1; v < (n < W ? n : W); ++v) {
+                    const float4 z = s_acc[32 * v + lane];
+                    y = make_float4(y.x + z.x, y.y + z.y, y.z + z.z, y.w + z.w);
+                }
             }
-            const float inv = Lx > 0.f ? 1.f / Lx : 0.f;
+        }
+        if (part == 0) {
+            const float inv = s_inv[mine];
             const int s = r / n_groups, head = (r - s * n_groups) * heads_per_row + hr;
             q8_store4(a.out, (int64_t)s_plan.row[s] * a.out_stride + (int64_t)head * kHeadDim + 4 * lane, a.io,
                       make_float4(y.x * inv, y.y * inv, y.z * inv, y.w * inv));
         }
-        __syncthreads();
+        sync();
     }
+}
+
+template <int W>
+cudaError_t merge_as(const Q8Launch& a, int kvg, int ctas, cudaStream_t s) {
+    constexpr int kUnits = W == 1 ? 4 : 1;
+    const int64_t units = ((int64_t)a.n_sessions * a.n_heads + kUnits - 1) / kUnits, cap = 4 * sm_count();
+    return launch_kernel_pdl(q8_decode_merge_kernel<W>, dim3((unsigned)(units < cap ? units : cap)), dim3(W == 16 ? 512 : 128), 0, s, true, a, kvg, ctas);
 }
 
 int dec_group(int n_kv_heads) { return n_kv_heads % 4 == 0 ? 4 : (n_kv_heads % 2 == 0 ? 2 : 1); }
@@ -682,14 +793,14 @@ size_t q8_work_bytes(int n_heads, int n_kv_heads, int n_sessions, int, int max_t
     if (!q8_is_decode(n_heads, n_kv_heads, max_tokens)) return q8_chunk_work_bytes(n_heads, n_kv_heads, max_tokens);
     const int kvg = dec_group(n_kv_heads), groups = n_kv_heads / kvg;
     const int64_t rows = (int64_t)n_sessions * groups;
-    return (size_t)((rows < kMaxRowsSmem ? rows : kMaxRowsSmem) + kQ8MaxCtas) * (size_t)(kvg * (n_heads / n_kv_heads)) * kSlotW * sizeof(float);
+    return (size_t)((rows < kDecRows ? rows : kDecRows) + kQ8MaxCtas) * (size_t)(kvg * (n_heads / n_kv_heads)) * kSlotW * sizeof(float);
 }
 
 int launch_q8_attn(const Q8Launch& a, cudaStream_t s) {
     if (a.n_tokens <= 0 || a.n_sessions <= 0) return NOVA_OK;
     if (q8_is_decode(a.n_heads, a.n_kv_heads, a.max_tokens)) {
         const int kvg = dec_group(a.n_kv_heads), groups = a.n_kv_heads / kvg;
-        if (groups > kMaxRowsSmem) return NOVA_ERR_TOO_LARGE;
+        if (groups > kDecRows) return NOVA_ERR_TOO_LARGE;
         alignas(64) CUtensorMap tmk, tmv;
         const int64_t slot_rows = ((int64_t)(a.layer + 1) * a.nb) << a.kv_shift;
         const int box = a.kv_shift == 3 ? 8 : 16;
@@ -698,7 +809,7 @@ int launch_q8_attn(const Q8Launch& a, cudaStream_t s) {
         if (rc != NOVA_OK) return rc;
         int ctas = sm_count();
         if (ctas > kQ8MaxCtas) ctas = kQ8MaxCtas;
-        const int most = kMaxRowsSmem / groups;                    // sessions of one launch (the row table's size)
+        const int most = kDecRows / groups;                    // sessions of one launch (the row table's size)
         const int all = a.n_sessions;
         const size_t io_bytes = a.io == NOVA_IO_F32 ? 4 : 2;
         auto ahead = [&](const void* p, int64_t elems) -> const void* { return p ? static_cast<const unsigned char*>(p) + elems * (int64_t)io_bytes : nullptr; };
@@ -728,9 +839,8 @@ int launch_q8_attn(const Q8Launch& a, cudaStream_t s) {
                 else rc = launch_decode<1, NOVA_KV_E4M3>(b, tmk, tmv, ctas, s);
             }
             if (rc != NOVA_OK) return rc;
-            const int units = b.n_sessions * a.n_heads;
-            const int cap = 4 * sm_count();
-            const cudaError_t e = launch_kernel_pdl(q8_decode_merge_kernel, dim3((unsigned)(units < cap ? units : cap)), dim3(128), 0, s, true, b, kvg, ctas);
+            const int per_row = ctas / (b.n_sessions * groups);           // contributors of a row
+            const cudaError_t e = per_row > 16 ? merge_as<16>(b, kvg, ctas, s) : per_row > 4 ? merge_as<4>(b, kvg, ctas, s) : merge_as<1>(b, kvg, ctas, s);
             if (e != cudaSuccess) {
                 set_cuda_error(e, "8-bit decode merge launch");
                 return NOVA_ERR_CUDA;
