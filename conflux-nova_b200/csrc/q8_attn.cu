@@ -27,7 +27,7 @@
 namespace novab {
 namespace {
 
-constexpr int kSetupTiles = 2;       // work-split weight of starting a row inside a CTA, in tiles
+constexpr int kSetupTiles = 8;       // work-split weight of starting a row inside a CTA, in tiles
 constexpr int kDecRows = 512;        // (session, kv group) rows of a launch
 constexpr int kMinTiles = 4;         // a CTA gets at least that many tiles (fewer partial rows to merge for short contexts)
 
@@ -58,6 +58,8 @@ struct DecPlan {
 
 __device__ __forceinline__ int dec_first_tile(const Q8Launch& a, int keys) { return a.window > 0 && keys > a.window ? (keys - a.window) >> 4 : 0; }
 
+__device__ __forceinline__ int dec_setup(int row) { return row > 0 ? kSetupTiles : 0; }
+
 __device__ inline void dec_build_plan(const Q8Launch& a, DecPlan& p, int n_groups, bool flag) {
     for (int s = (int)threadIdx.x; s < a.n_sessions; s += (int)blockDim.x) {      // (all loads at once: one trip to memory)
         int first, count;
@@ -82,7 +84,7 @@ __device__ inline void dec_build_plan(const Q8Launch& a, DecPlan& p, int n_group
         if (lane == 0) p.prefix[0] = 0;
         for (int base = 0; base < rows; base += 32) {
             const int r = base + lane, keys = r < rows ? p.keys[r / n_groups] : 0;
-            uint32_t v = keys > 0 ? (uint32_t)(((keys + 15) >> 4) - dec_first_tile(a, keys) + kSetupTiles) : 0u;
+            uint32_t v = keys > 0 ? (uint32_t)(((keys + 15) >> 4) - dec_first_tile(a, keys) + dec_setup(r)) : 0u;
             v = min(v, 0x7ffffffu);                            // (the sum of 32 stays inside 32 bits)
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
@@ -141,8 +143,8 @@ __device__ __forceinline__ DecSegment dec_segment(const DecPlan& p, const DecLin
     sg.session = row / ln.n_groups;
     sg.group = row - sg.session * ln.n_groups;
     sg.span = end - pos;
-    sg.first = max(pos - begin - kSetupTiles, 0);
-    sg.count = max(end - begin - kSetupTiles, 0) - sg.first;
+    sg.first = max(pos - begin - dec_setup(row), 0);
+    sg.count = max(end - begin - dec_setup(row), 0) - sg.first;
     sg.whole = begin >= lo && row_end <= hi;
     return sg;
 }
@@ -367,90 +369,88 @@ q8_decode_kernel(Q8Launch a, const __grid_constant__ CUtensorMap tmk, const __gr
         pos += sg.span;
         const int s = sg.session, kvh = sg.group * KVG + w;
         const int keys = s_plan.keys[s], row = s_plan.row[s], t0 = dec_first_tile(a, keys) + sg.first;
-        const int head = kvh * G + (g < G ? g : 0);
 
-        // q fragments of head g: this lane's dims are 32 t .. 32 t + 31, four per contraction step
+        // q of the kv head's query heads: its warps rotate, scale and round them together, 8 dims a thread, and leave them in shared
+        // memory (each warp for itself took 2 us instead of 1: all of them would do the same work); then a lane takes head g's
+        // dims 32 t .. 32 t + 31, four per contraction step.  Row of a head: its 16-byte chunk 4 t + k at place 4 k + t, xor 4 in
+        // odd rows, so that the fragments' loads meet no bank twice.
         uint32_t qh[8][2], ql[kLo ? 8 : 1][2];
         float off0 = 0.f, off1 = 0.f;             // what the accumulators of heads 2 t and 2 t + 1 start at
         {
-            float qsum = 0.f;
-            const int64_t qe = (int64_t)row * a.q_stride + (int64_t)head * kHeadDim + 32 * t;
-            // all loads before their first use: they are one trip to memory
-            constexpr int kRaw = kLo ? 8 : 4;
-            uint4 raw[kRaw];
-            const uint4* const qp = reinterpret_cast<const uint4*>(static_cast<const unsigned char*>(a.q) + qe * (kLo ? 4 : 2));
-#pragma unroll
-            for (int e = 0; e < kRaw; ++e) raw[e] = __ldg(qp + e);
-            const bool bf = a.io == NOVA_IO_BF16;
-            auto load = [&](int ks) {
-                if constexpr (kLo) {
-                    return make_float4(__uint_as_float(raw[ks].x), __uint_as_float(raw[ks].y), __uint_as_float(raw[ks].z), __uint_as_float(raw[ks].w));
-                } else {
-                    const uint32_t u0 = ks & 1 ? raw[ks >> 1].z : raw[ks >> 1].x, u1 = ks & 1 ? raw[ks >> 1].w : raw[ks >> 1].y;
-                    const float2 h0 = __half22float2(*reinterpret_cast<const __half2*>(&u0)), h1 = __half22float2(*reinterpret_cast<const __half2*>(&u1));
-                    return bf ? make_float4(__uint_as_float(u0 << 16), __uint_as_float(u0 & 0xffff0000u), __uint_as_float(u1 << 16), __uint_as_float(u1 & 0xffff0000u))
-                              : make_float4(h0.x, h0.y, h1.x, h1.y);
+            const uint32_t stash = smem_u32(merge) + (uint32_t)w * kSub * 36u * 128u;       // [8][256] fp16, its second part, [8] sums
+#pragma unroll 1
+            for (int un = 32 * sub + lane; un < 16 * G + (16 * G & 16); un += 32 * kSub) {  // (whole warps)
+                const int hd = un >> 4, i = un & 15;
+                const bool real = hd < G;
+                const int d0 = a.neox || !a.rope_cs ? 4 * i : 8 * i, d1 = a.neox || !a.rope_cs ? 64 + 4 * i : 8 * i + 4;
+                float4 x0 = make_float4(0.f, 0.f, 0.f, 0.f), x1 = x0, c = x0, n = x0;
+                if (real) {
+                    const int64_t qe = (int64_t)row * a.q_stride + (int64_t)(kvh * G + hd) * kHeadDim;
+                    if (a.rope_cs) {
+                        c = __ldg(reinterpret_cast<const float4*>(a.rope_cs + (int64_t)(keys - 1) * 64) + i);
+                        n = __ldg(reinterpret_cast<const float4*>(a.rope_sn + (int64_t)(keys - 1) * 64) + i);
+                    }
+                    if constexpr (kLo) {
+                        x0 = __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(a.q) + qe + d0));
+                        x1 = __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(a.q) + qe + d1));
+                    } else {
+                        x0 = q8_load4(a.q, qe + d0, a.io);
+                        x1 = q8_load4(a.q, qe + d1, a.io);
+                    }
                 }
-            };
-            auto put = [&](int ks, float4 x) {
-                const float f[4] = {x.x * 0.125f, x.y * 0.125f, x.z * 0.125f, x.w * 0.125f};
+                if (a.rope_cs) {
+                    float4 u, v;
+                    if (a.neox) {
+                        u = make_float4(__fmaf_rn(x0.x, c.x, -__fmul_rn(x1.x, n.x)), __fmaf_rn(x0.y, c.y, -__fmul_rn(x1.y, n.y)),
+                                        __fmaf_rn(x0.z, c.z, -__fmul_rn(x1.z, n.z)), __fmaf_rn(x0.w, c.w, -__fmul_rn(x1.w, n.w)));
+                        v = make_float4(__fmaf_rn(x0.x, n.x, __fmul_rn(x1.x, c.x)), __fmaf_rn(x0.y, n.y, __fmul_rn(x1.y, c.y)),
+                                        __fmaf_rn(x0.z, n.z, __fmul_rn(x1.z, c.z)), __fmaf_rn(x0.w, n.w, __fmul_rn(x1.w, c.w)));
+                    } else {
+                        u = make_float4(__fmaf_rn(x0.x, c.x, -__fmul_rn(x0.y, n.x)), __fmaf_rn(x0.x, n.x, __fmul_rn(x0.y, c.x)),
+                                        __fmaf_rn(x0.z, c.y, -__fmul_rn(x0.w, n.y)), __fmaf_rn(x0.z, n.y, __fmul_rn(x0.w, c.y)));
+                        v = make_float4(__fmaf_rn(x1.x, c.z, -__fmul_rn(x1.y, n.z)), __fmaf_rn(x1.x, n.z, __fmul_rn(x1.y, c.z)),
+                                        __fmaf_rn(x1.z, c.w, -__fmul_rn(x1.w, n.w)), __fmaf_rn(x1.z, n.w, __fmul_rn(x1.w, c.w)));
+                    }
+                    x0 = u;
+                    x1 = v;
+                }
+                float sum = 0.f;
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
-                    const __half2 h = __floats2half2_rn(f[2 * e], f[2 * e + 1]);
-                    const float2 b = __half22float2(h);
-                    qh[ks][e] = g < G ? *reinterpret_cast<const uint32_t*>(&h) : 0u;
-                    qsum += kLo ? f[2 * e] + f[2 * e + 1] : b.x + b.y;
-                    if constexpr (kLo) ql[ks][e] = g < G ? pack_h2(f[2 * e] - b.x, f[2 * e + 1] - b.y) : 0u;
-                }
-            };
-            const int64_t cpos = (int64_t)(keys - 1) * 64;
-            if (a.rope_cs && a.neox) {
-                const float4* const cp = reinterpret_cast<const float4*>(a.rope_cs + cpos + ((32 * t) & 63));
-                const float4* const np = reinterpret_cast<const float4*>(a.rope_sn + cpos + ((32 * t) & 63));
-#pragma unroll
-                for (int k0 = 0; k0 < 8; k0 += 4) {
-                    float4 c[4], n[4];
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        c[e] = __ldg(cp + k0 + e);
-                        n[e] = __ldg(np + k0 + e);
-                    }
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const float4 x = load(k0 + e);              // the other half of the pair: dims 32 (t ^ 2) ..
-                        const float4 y = make_float4(__shfl_xor_sync(0xffffffffu, x.x, 2), __shfl_xor_sync(0xffffffffu, x.y, 2),
-                                                     __shfl_xor_sync(0xffffffffu, x.z, 2), __shfl_xor_sync(0xffffffffu, x.w, 2));
-                        const float4 lo4 = make_float4(__fmaf_rn(x.x, c[e].x, -__fmul_rn(y.x, n[e].x)), __fmaf_rn(x.y, c[e].y, -__fmul_rn(y.y, n[e].y)),
-                                                       __fmaf_rn(x.z, c[e].z, -__fmul_rn(y.z, n[e].z)), __fmaf_rn(x.w, c[e].w, -__fmul_rn(y.w, n[e].w)));
-                        const float4 hi4 = make_float4(__fmaf_rn(y.x, n[e].x, __fmul_rn(x.x, c[e].x)), __fmaf_rn(y.y, n[e].y, __fmul_rn(x.y, c[e].y)),
-                                                       __fmaf_rn(y.z, n[e].z, __fmul_rn(x.z, c[e].z)), __fmaf_rn(y.w, n[e].w, __fmul_rn(x.w, c[e].w)));
-                        put(k0 + e, t < 2 ? lo4 : hi4);
+                    const float4 x = e ? x1 : x0;
+                    const float f[4] = {x.x * 0.125f, x.y * 0.125f, x.z * 0.125f, x.w * 0.125f};
+                    const __half2 h0 = __floats2half2_rn(f[0], f[1]), h1 = __floats2half2_rn(f[2], f[3]);
+                    const float2 b0 = __half22float2(h0), b1 = __half22float2(h1);
+                    const int d = e ? d1 : d0, chunk = d >> 3;
+                    const uint32_t dst = stash + (uint32_t)hd * 256u + (uint32_t)(((4 * (chunk & 3) + (chunk >> 2)) ^ (4 * (hd & 1))) * 16 + (d & 4) * 2);
+                    sum += kLo ? (f[0] + f[1]) + (f[2] + f[3]) : (b0.x + b0.y) + (b1.x + b1.y);
+                    if (real) {
+                        sts64(dst, *reinterpret_cast<const uint32_t*>(&h0), *reinterpret_cast<const uint32_t*>(&h1));
+                        if constexpr (kLo) sts64(dst + 2048u, pack_h2(f[0] - b0.x, f[1] - b0.y), pack_h2(f[2] - b1.x, f[3] - b1.y));
                     }
                 }
-            } else if (a.rope_cs) {
-                float2 c[8], n[8];
+                if constexpr (kFmt == NOVA_KV_I8) {
 #pragma unroll
-                for (int ks = 0; ks < 8; ++ks) {
-                    c[ks] = __ldg(reinterpret_cast<const float2*>(a.rope_cs + cpos + 16 * t) + ks);
-                    n[ks] = __ldg(reinterpret_cast<const float2*>(a.rope_sn + cpos + 16 * t) + ks);
+                    for (int o = 8; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+                    if (real && i == 0) sts_f1(stash + 4096u + (uint32_t)hd * 4u, sum);
                 }
+            }
+            asm volatile("bar.sync %0, %1;" ::"r"(1 + w), "r"(32 * kSub) : "memory");
 #pragma unroll
-                for (int ks = 0; ks < 8; ++ks) {
-                    const float4 x = load(ks);
-                    put(ks, make_float4(__fmaf_rn(x.x, c[ks].x, -__fmul_rn(x.y, n[ks].x)), __fmaf_rn(x.x, n[ks].x, __fmul_rn(x.y, c[ks].x)),
-                                        __fmaf_rn(x.z, c[ks].y, -__fmul_rn(x.w, n[ks].y)), __fmaf_rn(x.z, n[ks].y, __fmul_rn(x.w, c[ks].y))));
+            for (int k = 0; k < 4; ++k) {
+                const uint32_t src = stash + (uint32_t)g * 256u + (uint32_t)(((4 * k + t) ^ (4 * (g & 1))) * 16);
+                const uint4 h = g < G ? lds128(src) : make_uint4(0u, 0u, 0u, 0u);
+                qh[2 * k][0] = h.x, qh[2 * k][1] = h.y, qh[2 * k + 1][0] = h.z, qh[2 * k + 1][1] = h.w;
+                if constexpr (kLo) {
+                    const uint4 l = g < G ? lds128(src + 2048u) : make_uint4(0u, 0u, 0u, 0u);
+                    ql[2 * k][0] = l.x, ql[2 * k][1] = l.y, ql[2 * k + 1][0] = l.z, ql[2 * k + 1][1] = l.w;
                 }
-            } else {
-#pragma unroll
-                for (int ks = 0; ks < 8; ++ks) put(ks, load(ks));
             }
-            if constexpr (kFmt == NOVA_KV_I8) {
-                qsum += __shfl_xor_sync(0xffffffffu, qsum, 1);
-                qsum += __shfl_xor_sync(0xffffffffu, qsum, 2);
-                if (g >= G) qsum = 0.f;
-                off0 = -7.62939453125e-06f * __shfl_sync(0xffffffffu, qsum, 8 * t);             // 128 * 2^-24
-                off1 = -7.62939453125e-06f * __shfl_sync(0xffffffffu, qsum, 8 * t + 4);
+            if constexpr (kFmt == NOVA_KV_I8) {                                                     // 128 * 2^-24
+                if (2 * t < G) off0 = -7.62939453125e-06f * lds_f1(stash + 4096u + 8u * t);
+                if (2 * t + 1 < G) off1 = -7.62939453125e-06f * lds_f1(stash + 4096u + 8u * t + 4u);
             }
+            asm volatile("bar.sync %0, %1;" ::"r"(1 + w), "r"(32 * kSub) : "memory");               // (the merge uses the same place)
         }
         // heads 2 t and 2 t + 1: reference maximum (log2 units), this lane's share of the sum, dims 16 g .. 16 g + 15
         float ref0 = -INFINITY, ref1 = -INFINITY, l0 = 0.f, l1 = 0.f;
@@ -624,7 +624,7 @@ q8_decode_kernel(Q8Launch a, const __grid_constant__ CUtensorMap tmk, const __gr
             p[35 * 32] = l1;
         }
         asm volatile("bar.sync %0, %1;" ::"r"(1 + w), "r"(32 * kSub) : "memory");
-#pragma unroll 1
+#pragma unroll 1                                              // (unrolled, it waits longer for its instructions than it saves)
         for (int un = sub; un < 8; un += kSub) {
             const int e = un & 1, j = un & 6, hd = 2 * t + e;
             float M = -INFINITY, L = 0.f;
@@ -695,7 +695,7 @@ __global__ void __launch_bounds__(W == 16 ? 512 : 128) q8_decode_merge_kernel(Q8
         if (n == 1) continue;
         const size_t step = (size_t)heads_per_row * kSlotW;
         const float* base = a.part + ((size_t)(c0 + r) * heads_per_row + hr) * kSlotW;
-        constexpr int kBatch = 8;
+        constexpr int kBatch = W == 16 ? kQ8MaxCtas / W : 8;
         float4 x[kBatch];
         auto bring = [&](int i0) {
 #pragma unroll
