@@ -55,6 +55,7 @@ constexpr float kKDiv = 16.f;                         // K goes in divided by th
 // memory): weights are 2^7 .. 2^15 at the largest, with fp16's 11 bits down to 2^-21 of the reference.
 constexpr float kStep = 8.f, kTop = 7.f;
 constexpr int kSetup = 2;                             // what starting a unit costs, in tiles
+constexpr int kFewTiles = 4;                          // token tiles that a thread counts for itself
 constexpr int kMinTiles = 4;                          // a CTA gets at least that many
 constexpr uint32_t kIdescS = (1u << 4) | ((uint32_t)(kKeys >> 3) << 17) | ((uint32_t)(kHalfRows >> 4) << 24);
 constexpr uint32_t kIdescPV = (1u << 4) | (1u << 16) | ((uint32_t)(kHeadDim >> 3) << 17) | ((uint32_t)(kHalfRows >> 4) << 24);
@@ -78,6 +79,7 @@ __device__ __forceinline__ int unit_tiles(const Q8Launch& a, int tq, int past, i
 
 // All threads of the CTA; ends with __syncthreads().
 __device__ inline void build_plan(const Q8Launch& a, const ChunkShape& sh, ChunkPlan& p, bool flag) {
+    bool many = false;
     for (int s = (int)threadIdx.x; s < a.n_sessions; s += (int)blockDim.x) {
         int first, count;
         q8_rows(a, s, first, count);
@@ -87,13 +89,27 @@ __device__ inline void build_plan(const Q8Launch& a, const ChunkShape& sh, Chunk
             count = 0;
         }
         long long len = 0;
-        for (int qt = 0; qt * sh.tq < count; ++qt) len += unit_tiles(a, sh.tq, past, count, qt) + kSetup;
+        if (count <= kFewTiles * sh.tq)
+            for (int qt = 0; qt * sh.tq < count; ++qt) len += unit_tiles(a, sh.tq, past, count, qt) + kSetup;
+        else
+            many = true;                                  // (a thread for itself needs 40 cycles a token tile)
         p.line[s + 1] = len * a.n_kv_heads;
         p.first[s] = first;
         p.count[s] = count;
         p.past[s] = past;
     }
-    __syncthreads();
+    if (__syncthreads_or(many)) {
+        for (int s = (int)threadIdx.x >> 5; s < a.n_sessions; s += (int)blockDim.x >> 5) {
+            const int count = p.count[s], past = p.past[s];
+            if (count <= kFewTiles * sh.tq) continue;
+            long long len = 0;
+            for (int qt = (int)threadIdx.x & 31; qt * sh.tq < count; qt += 32) len += unit_tiles(a, sh.tq, past, count, qt) + kSetup;
+#pragma unroll
+            for (int o = 16; o; o >>= 1) len += __shfl_xor_sync(0xffffffffu, len, o);
+            if ((threadIdx.x & 31) == 0) p.line[s + 1] = len * a.n_kv_heads;
+        }
+        __syncthreads();
+    }
     if (threadIdx.x < 32) {
         const int lane = (int)threadIdx.x;
         long long carry = 0;
@@ -209,6 +225,12 @@ __device__ __forceinline__ unsigned long long add_f2(unsigned long long x, unsig
     asm("add.rn.f32x2 %0, %1, %2;" : "=l"(v) : "l"(x), "l"(y));
     return v;
 }
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+                 : "r"(taddr)
+                 : "memory");
+}
 __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
     asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr), "r"(r[0]), "r"(r[1]),
                  "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]),
@@ -245,19 +267,19 @@ q8_chunk_kernel(Q8Launch a, ChunkShape sh) {
             mbar_init(bar_kfree + 8u * i, sh.dual ? 1 : 2);
             mbar_init(bar_vfull + 8u * i, kConv / 4);
             mbar_init(bar_vfree + 8u * i, sh.dual ? 1 : 2);
-            mbar_init(bar_qready + 8u * i, kHalfRows);
+            mbar_init(bar_qready + 8u * i, 4);
         }
         for (int i = 0; i < 4; ++i) {
             mbar_init(bar_sready + 8u * i, 1);
-            mbar_init(bar_pready + 8u * i, kHalfRows);
+            mbar_init(bar_pready + 8u * i, 4);
             mbar_init(bar_pvdone + 8u * i, 1);
         }
         for (int i = 0; i < kParts; ++i) {
             mbar_init(bar_partfull + 8u * i, 1);
             mbar_init(bar_partfree + 8u * i, 18);      // every warp but the one that walks and the one that idles
         }
-        mbar_init(bar_xfull, kHalfRows);
-        mbar_init(bar_xfree, kHalfRows);
+        mbar_init(bar_xfull, 4);
+        mbar_init(bar_xfree, 4);
         s_abort = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -309,13 +331,18 @@ q8_chunk_kernel(Q8Launch a, ChunkShape sh) {
 
     if (warp < 8) {
         // ---------------------------------------------------------------------------------------- softmax: thread = one row
-        regs_up<120>();
+        regs_up<136>();
         const int half = warp >> 2, hrow = (int)threadIdx.x & (kHalfRows - 1);
         const uint32_t t_lane = tmem + ((uint32_t)(32 * (warp & 3)) << 16);
         const uint32_t col_s = 128u * (uint32_t)half, col_o = kColO + 128u * (uint32_t)half;
         const uint32_t my_sready = bar_sready + 16u * (uint32_t)half, my_pready = bar_pready + 16u * (uint32_t)half, my_pvdone = bar_pvdone + 16u * (uint32_t)half;
         const int row0 = sh.dual ? 0 : half * kHalfRows, row = row0 + hrow, tk = row / G, g = row - tk * G;
+        const uint32_t per_g = (65536u + (uint32_t)G - 1u) / (uint32_t)G;       // rows / G by this: exact below 256 rows, G at most 128
         uint32_t xround = 0;
+        auto arrive_warp = [&](uint32_t b) {                   // what all lanes have done so far
+            __syncwarp();
+            if (lane == 0) mbar_arrive(b);
+        };
         while (!failed && next_part()) {
             const int tiles = u.tiles;
             // this half's tiles of the unit: every tile, or those whose place on the CTA's line is even (odd)
@@ -328,55 +355,85 @@ q8_chunk_kernel(Q8Launch a, ChunkShape sh) {
             {
                 // ---- q: rotated, scaled, fp16, K-major 128-byte swizzle; eight lanes a row, dims 8c .. and 64 + 8c .. each.  The scores
                 // of the unit before are all computed (this thread has waited for the last of them), so the operand can be overwritten.
+                // The loads of kRows rows go out together (one after the other they took 9 us a unit).
                 constexpr float kQ = kAttnScale * kLog2e * kKDiv;
-                const int c = lane & 7;
-#pragma unroll 4
-                for (int e8 = 0; e8 < 8; ++e8) {
-                    const int r = 32 * (warp & 3) + 4 * e8 + (lane >> 3), rt = (row0 + r) / G, rg = row0 + r - rt * G;
-                    const int rpos = u.past + u.t0 + rt;
-                    float x0[8], x1[8];
+                constexpr int kRows = 2, kVec = sizeof(T) / 2;
+                const int c = lane & 7, second = a.neox ? 4 : 32;          // neox: the pairs (d, d + 64); else neighbours, in both halves of the dims
+#pragma unroll 1
+                for (int e8 = 0; e8 < 8; e8 += kRows) {
+                    const int r0 = 32 * (warp & 3) + 4 * e8 + (lane >> 3);
+                    if (__all_sync(0xffffffffu, (row0 + r0 - (lane >> 3)) >= u.t_cnt * G)) {      // none of these rows exists
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) x0[e] = x1[e] = 0.f;
-                    if (rt < u.t_cnt && !(a.rope_cs && rpos >= a.rope_rows)) {
-                        const int64_t qe = (tok0 + rt) * a.q_stride + (int64_t)(u.kvh * G + rg) * kHeadDim + 8 * c;
-                        load8<T>(a.q, qe, x0);
-                        load8<T>(a.q, qe + 64, x1);
-                        if (a.rope_cs) {
-                            const float* cr = a.rope_cs + (int64_t)rpos * 64 + (a.neox ? 8 : 4) * c;
-                            const float* sr = a.rope_sn + (int64_t)rpos * 64 + (a.neox ? 8 : 4) * c;
-                            const int second = a.neox ? 4 : 32;        // neox: the pairs (d, d + 64); else neighbours, in both halves of the dims
-                            const float4 c0 = *reinterpret_cast<const float4*>(cr), c1 = *reinterpret_cast<const float4*>(cr + second);
-                            const float4 s0 = *reinterpret_cast<const float4*>(sr), s1 = *reinterpret_cast<const float4*>(sr + second);
-                            const float cc[8] = {c0.x, c0.y, c0.z, c0.w, c1.x, c1.y, c1.z, c1.w}, ss[8] = {s0.x, s0.y, s0.z, s0.w, s1.x, s1.y, s1.z, s1.w};
-                            if (a.neox) {
+                        for (int e = 0; e < kRows; ++e)
 #pragma unroll
-                                for (int e = 0; e < 8; ++e) {
-                                    const float y0 = x0[e], y1 = x1[e];
-                                    x0[e] = __fmaf_rn(y0, cc[e], -__fmul_rn(y1, ss[e]));
-                                    x1[e] = __fmaf_rn(y0, ss[e], __fmul_rn(y1, cc[e]));
-                                }
-                            } else {
+                            for (int hf = 0; hf < 2; ++hf)
+                                sts128(base + (uint32_t)((2 * half + hf) * kQSlab + (r0 + 4 * e) * 128 + ((c ^ ((r0 + 4 * e) & 7)) << 4)), make_float4(0.f, 0.f, 0.f, 0.f));
+                        continue;
+                    }
+                    uint4 raw[kRows][2 * kVec];
+                    float4 rc[kRows][2], rs[kRows][2];
 #pragma unroll
-                                for (int e = 0; e < 8; ++e) {
-                                    float* const y = e < 4 ? x0 : x1;
-                                    const float y0 = y[2 * (e & 3)], y1 = y[2 * (e & 3) + 1];
-                                    y[2 * (e & 3)] = __fmaf_rn(y0, cc[e], -__fmul_rn(y1, ss[e]));
-                                    y[2 * (e & 3) + 1] = __fmaf_rn(y0, ss[e], __fmul_rn(y1, cc[e]));
-                                }
+                    for (int e = 0; e < kRows; ++e) {
+                        const int rr = row0 + r0 + 4 * e, rt = (int)((uint32_t)rr * per_g >> 16), rg = rr - rt * G, rpos = u.past + u.t0 + rt;
+#pragma unroll
+                        for (int v = 0; v < 2 * kVec; ++v) raw[e][v] = make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll
+                        for (int v = 0; v < 2; ++v) rc[e][v] = rs[e][v] = make_float4(0.f, 0.f, 0.f, 0.f);
+                        if (rt < u.t_cnt && !(a.rope_cs && rpos >= a.rope_rows)) {
+                            const uint4* const src = reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + (tok0 + rt) * a.q_stride + (int64_t)(u.kvh * G + rg) * kHeadDim + 8 * c);
+#pragma unroll
+                            for (int v = 0; v < kVec; ++v) {
+                                raw[e][v] = __ldg(src + v);
+                                raw[e][kVec + v] = __ldg(src + 8 * kVec + v);
+                            }
+                            if (a.rope_cs) {
+                                const float* cr = a.rope_cs + (int64_t)rpos * 64 + (a.neox ? 8 : 4) * c;
+                                const float* sr = a.rope_sn + (int64_t)rpos * 64 + (a.neox ? 8 : 4) * c;
+                                rc[e][0] = __ldg(reinterpret_cast<const float4*>(cr));
+                                rc[e][1] = __ldg(reinterpret_cast<const float4*>(cr + second));
+                                rs[e][0] = __ldg(reinterpret_cast<const float4*>(sr));
+                                rs[e][1] = __ldg(reinterpret_cast<const float4*>(sr + second));
                             }
                         }
                     }
 #pragma unroll
-                    for (int hf = 0; hf < 2; ++hf) {
-                        const uint32_t dst = base + (uint32_t)((2 * half + hf) * kQSlab + r * 128 + ((c ^ (r & 7)) << 4));
-                        const float* y = hf ? x1 : x0;
-                        asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(dst), "r"(pack_h2(y[0] * kQ, y[1] * kQ)), "r"(pack_h2(y[2] * kQ, y[3] * kQ)),
-                                     "r"(pack_h2(y[4] * kQ, y[5] * kQ)), "r"(pack_h2(y[6] * kQ, y[7] * kQ))
-                                     : "memory");
+                    for (int e = 0; e < kRows; ++e) {
+                        const int r = r0 + 4 * e;
+                        float x0[8], x1[8];
+                        q8_unpack8<T>(&raw[e][0], x0);
+                        q8_unpack8<T>(&raw[e][kVec], x1);
+                        if (a.rope_cs) {
+                            const float cc[8] = {rc[e][0].x, rc[e][0].y, rc[e][0].z, rc[e][0].w, rc[e][1].x, rc[e][1].y, rc[e][1].z, rc[e][1].w};
+                            const float ss[8] = {rs[e][0].x, rs[e][0].y, rs[e][0].z, rs[e][0].w, rs[e][1].x, rs[e][1].y, rs[e][1].z, rs[e][1].w};
+                            if (a.neox) {
+#pragma unroll
+                                for (int d = 0; d < 8; ++d) {
+                                    const float y0 = x0[d], y1 = x1[d];
+                                    x0[d] = __fmaf_rn(y0, cc[d], -__fmul_rn(y1, ss[d]));
+                                    x1[d] = __fmaf_rn(y0, ss[d], __fmul_rn(y1, cc[d]));
+                                }
+                            } else {
+#pragma unroll
+                                for (int d = 0; d < 8; ++d) {
+                                    float* y = d < 4 ? x0 : x1;
+                                    const float y0 = y[2 * (d & 3)], y1 = y[2 * (d & 3) + 1];
+                                    y[2 * (d & 3)] = __fmaf_rn(y0, cc[d], -__fmul_rn(y1, ss[d]));
+                                    y[2 * (d & 3) + 1] = __fmaf_rn(y0, ss[d], __fmul_rn(y1, cc[d]));
+                                }
+                            }
+                        }
+#pragma unroll
+                        for (int hf = 0; hf < 2; ++hf) {
+                            const uint32_t dst = base + (uint32_t)((2 * half + hf) * kQSlab + r * 128 + ((c ^ (r & 7)) << 4));
+                            const float* y = hf ? x1 : x0;
+                            asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(dst), "r"(pack_h2(y[0] * kQ, y[1] * kQ)), "r"(pack_h2(y[2] * kQ, y[3] * kQ)),
+                                         "r"(pack_h2(y[4] * kQ, y[5] * kQ)), "r"(pack_h2(y[6] * kQ, y[7] * kQ))
+                                         : "memory");
+                        }
                     }
                 }
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                mbar_arrive(bar_qready + 8u * (uint32_t)half);
+                arrive_warp(bar_qready + 8u * (uint32_t)half);
             }
             const int row_pos = u.past + u.t0 + tk;
             const bool in_tile = tk < u.t_cnt, beyond = in_tile && a.rope_cs && row_pos >= a.rope_rows;
@@ -386,6 +443,8 @@ q8_chunk_kernel(Q8Launch a, ChunkShape sh) {
             const int row_lim = row_ok ? row_pos : 0x7fffffff;
             const int row_lo = row_ok && a.window > 0 ? row_pos - a.window + 1 : 0;
             const bool idle = __all_sync(0xffffffffu, !row_ok);
+            // keys that all of the warp's rows see: [see_lo, see_hi]
+            const int see_hi = __reduce_min_sync(0xffffffffu, row_lim), see_lo = __reduce_max_sync(0xffffffffu, row_lo);
             float m_ref = -INFINITY, l = 0.f;
             int m = sh.dual ? (n + mine0) >> 1 : n;            // tiles of this half so far: which score buffer, which parity
 #pragma unroll 1
@@ -393,39 +452,34 @@ q8_chunk_kernel(Q8Launch a, ChunkShape sh) {
                 const int t = n + i;
                 if (!__all_sync(0xffffffffu, t5_wait(my_sready + 8u * (uint32_t)(m & 1), (uint32_t)(m >> 1) & 1u, &s_abort))) { failed = true; break; }
                 if (idle) {                                     // what P and O hold in these rows is nobody's
-                    mbar_arrive(my_pready + 8u * (uint32_t)(m & 1));
+                    arrive_warp(my_pready + 8u * (uint32_t)(m & 1));
                     continue;
                 }
                 tc_fence_after();
                 const uint32_t s_col = t_lane + col_s + 64u * (uint32_t)(m & 1);
                 const int key0 = (u.first16 << 4) + (u.tile0 + i) * kKeys;
-                const int hi_k = row_lim - key0, lo_k = row_lo - key0;       // first and last visible column
+                // All 64 scores in registers at once (read twice, 32 columns at a time, they took 12 % longer).
+                uint32_t sv[2][32];
+                tmem_ld32(s_col, sv[0]);
+                tmem_ld32(s_col + 32u, sv[1]);
                 const unsigned long long there = *reinterpret_cast<const unsigned long long*>(s_mask + 2 * (t & (kMasks - 1)));    // (a page missing, or the last key passed)
-                const bool all_seen = __all_sync(0xffffffffu, hi_k >= kKeys - 1 && lo_k <= 0) && there == ~0ull;
-                // Two passes over the scores, 32 columns at a time, both read from tensor memory: half the code and half the registers
-                // of one pass over 64 (with that, instruction fetches were the largest stall: sixteen warps run five loops here).
-                float mx = -INFINITY;
-#pragma unroll 1
-                for (int hf = 0; hf < 2; ++hf) {
-                    uint32_t sv[32];
-                    tmem_ld32(s_col + 32u * (uint32_t)hf, sv);
-                    tmem_wait_ld();
-                    if (!all_seen) {
-                        const int hk = hi_k - 32 * hf, lk = lo_k - 32 * hf;
-                        uint32_t vis = (uint32_t)(there >> (32 * hf));
-                        if (hk < 31) vis &= hk < 0 ? 0u : (2u << hk) - 1u;
-                        if (lk > 0) vis &= lk > 31 ? 0u : ~((1u << lk) - 1u);
+                tmem_wait_ld();
+                if (key0 + kKeys - 1 > see_hi || key0 < see_lo || there != ~0ull) {
+                    const int hi_k = row_lim - key0, lo_k = row_lo - key0;       // first and last visible column
+                    unsigned long long vis = there;
+                    if (hi_k < 63) vis &= hi_k < 0 ? 0ull : (2ull << hi_k) - 1ull;
+                    if (lo_k > 0) vis &= lo_k > 63 ? 0ull : ~((1ull << lo_k) - 1ull);
+                    const uint32_t v0 = (uint32_t)vis, v1 = (uint32_t)(vis >> 32);
 #pragma unroll
-                        for (int c = 0; c < 32; ++c)
-                            if (!(vis >> c & 1u)) sv[c] = 0xff800000u;          // -inf
-                        tmem_st32(s_col + 32u * (uint32_t)hf, sv);
-                        tmem_wait_st();
+                    for (int c = 0; c < 32; ++c) {                             // -inf
+                        if (!(v0 >> c & 1u)) sv[0][c] = 0xff800000u;
+                        if (!(v1 >> c & 1u)) sv[1][c] = 0xff800000u;
                     }
-                    float m4[4] = {mx, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-                    for (int c = 0; c < 32; ++c) m4[c & 3] = fmaxf(m4[c & 3], __uint_as_float(sv[c]));
-                    mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
                 }
+                float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                for (int c = 0; c < 64; c += 2) m4[(c >> 1) & 3] = fmaxf(m4[(c >> 1) & 3], fmaxf(__uint_as_float(sv[c >> 5][c & 31]), __uint_as_float(sv[c >> 5][(c & 31) + 1])));
+                const float mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
                 float scale = 1.f;
                 if (mx > m_ref + kStep || (m_ref == -INFINITY && mx > -INFINITY)) {
                     scale = m_ref == -INFINITY ? 0.f : ex2(m_ref - mx);
@@ -434,15 +488,13 @@ q8_chunk_kernel(Q8Launch a, ChunkShape sh) {
                 const float ms = m_ref == -INFINITY ? 0.f : kTop - m_ref;         // nothing visible yet: keep exp arguments finite
                 const unsigned long long ms2 = pack_f2(ms, ms);
                 unsigned long long sum2[2] = {0ull, 0ull};
-#pragma unroll 1
+#pragma unroll
                 for (int hf = 0; hf < 2; ++hf) {
-                    uint32_t sv[32], pk[16];
-                    tmem_ld32(s_col + 32u * (uint32_t)hf, sv);
-                    tmem_wait_ld();
+                    uint32_t pk[16];
 #pragma unroll
                     for (int c = 0; c < 32; c += 2) {
                         float y0, y1;
-                        unpack_f2(add_f2(pack_f2(__uint_as_float(sv[c]), __uint_as_float(sv[c + 1])), ms2), y0, y1);
+                        unpack_f2(add_f2(pack_f2(__uint_as_float(sv[hf][c]), __uint_as_float(sv[hf][c + 1])), ms2), y0, y1);
                         y0 = ex2(y0);
                         y1 = ex2(y1);
                         sum2[(c >> 1) & 1] = add_f2(pack_f2(y0, y1), sum2[(c >> 1) & 1]);
@@ -470,7 +522,7 @@ q8_chunk_kernel(Q8Launch a, ChunkShape sh) {
                 }
                 tmem_wait_st();
                 tc_fence_before();
-                mbar_arrive(my_pready + 8u * (uint32_t)(m & 1));
+                arrive_warp(my_pready + 8u * (uint32_t)(m & 1));
             }
             n += tiles;
             if (failed) break;
@@ -478,23 +530,24 @@ q8_chunk_kernel(Q8Launch a, ChunkShape sh) {
             if (!__all_sync(0xffffffffu, t5_wait(my_pvdone + 8u * (uint32_t)((m - 1) & 1), (uint32_t)((m - 1) >> 1) & 1u, &s_abort))) { failed = true; break; }
             tc_fence_after();
             const bool whole = u.whole, fold = sh.dual && tiles > 1;
+            const int xrows = sh.rows_cap <= 64 ? 64 : kHalfRows, xparts = sh.rows_cap <= 64 ? 1 : 2;       // rounds of handing over: all dims of 64 rows fit, or 64 of 128
             const uint32_t xbase = base + 2u * kQSlab, xml = base + kOffX;      // (the second half's q is no longer needed)
             if (fold && half == 1) {
                 // both halves have a share of the rows: the second hands its own over, 64 dims at a time
                 sts_f1(xml + 8u * (uint32_t)hrow, m_ref);
                 sts_f1(xml + 8u * (uint32_t)hrow + 4u, l);
-                for (int part = 0; part < 2 && !failed; ++part) {
+                for (int part = 0; part < xparts && !failed; ++part) {
 #pragma unroll 1
-                    for (int cc = 0; cc < 2 && !idle; ++cc) {
+                    for (int cc = 0; cc < 4 / xparts && !idle; ++cc) {
                         uint32_t ov[32];
                         tmem_ld32(t_lane + col_o + 64u * (uint32_t)part + 32u * (uint32_t)cc, ov);
                         tmem_wait_ld();
 #pragma unroll
                         for (int c = 0; c < 32; c += 4)
-                            sts128(xbase + (uint32_t)((8 * cc + (c >> 2)) * kHalfRows + hrow) * 16u,
+                            sts128(xbase + (uint32_t)((8 * cc + (c >> 2)) * xrows + hrow) * 16u,
                                    make_float4(__uint_as_float(ov[c]), __uint_as_float(ov[c + 1]), __uint_as_float(ov[c + 2]), __uint_as_float(ov[c + 3])));
                     }
-                    mbar_arrive(bar_xfull);
+                    arrive_warp(bar_xfull);
                     if (!__all_sync(0xffffffffu, t5_wait(bar_xfree, xround & 1u, &s_abort))) failed = true;
                     ++xround;
                 }
@@ -507,7 +560,7 @@ q8_chunk_kernel(Q8Launch a, ChunkShape sh) {
             float w0 = 1.f, w1 = 0.f;                 // what this half's and the other half's accumulators are multiplied by
 #pragma unroll 1
             for (int cc = 0; cc < 4; ++cc) {
-                if (fold && (cc & 1) == 0) {
+                if (fold && (cc & (4 / xparts - 1)) == 0) {
                     if (!__all_sync(0xffffffffu, t5_wait(bar_xfull, xround & 1u, &s_abort))) { failed = true; break; }
                     ++xround;
                 }
@@ -535,23 +588,35 @@ q8_chunk_kernel(Q8Launch a, ChunkShape sh) {
                 }
                 if (row_ok) {
 #pragma unroll
-                    for (int c = 0; c < 32; c += 4) {
-                        float4 v = make_float4(__uint_as_float(ov[c]) * w0, __uint_as_float(ov[c + 1]) * w0, __uint_as_float(ov[c + 2]) * w0, __uint_as_float(ov[c + 3]) * w0);
+                    for (int c = 0; c < 32; c += 8) {
+                        float v[8];
+#pragma unroll
+                        for (int d = 0; d < 8; ++d) v[d] = __uint_as_float(ov[c + d]) * w0;
                         if (fold) {
-                            const uint4 y = lds128(xbase + (uint32_t)((8 * (cc & 1) + (c >> 2)) * kHalfRows + hrow) * 16u);
-                            v = make_float4(fmaf(__uint_as_float(y.x), w1, v.x), fmaf(__uint_as_float(y.y), w1, v.y), fmaf(__uint_as_float(y.z), w1, v.z),
-                                            fmaf(__uint_as_float(y.w), w1, v.w));
+#pragma unroll
+                            for (int d = 0; d < 8; d += 4) {
+                                const uint4 y = lds128(xbase + (uint32_t)((8 * (cc & (4 / xparts - 1)) + ((c + d) >> 2)) * xrows + hrow) * 16u);
+                                v[d] = fmaf(__uint_as_float(y.x), w1, v[d]);
+                                v[d + 1] = fmaf(__uint_as_float(y.y), w1, v[d + 1]);
+                                v[d + 2] = fmaf(__uint_as_float(y.z), w1, v[d + 2]);
+                                v[d + 3] = fmaf(__uint_as_float(y.w), w1, v[d + 3]);
+                            }
                         }
-                        if (whole) Q8Io<T>::store4(static_cast<T*>(a.out) + oe + 32 * cc + c, v);
-                        else *reinterpret_cast<float4*>(slot + 4 * (size_t)sh.rows_cap + ((size_t)(8 * cc + (c >> 2)) * sh.rows_cap + row) * 4) = v;
+                        if (whole) {
+                            store8(static_cast<T*>(a.out) + oe + 32 * cc + c, v);
+                        } else {
+#pragma unroll
+                            for (int d = 0; d < 8; d += 4)
+                                *reinterpret_cast<float4*>(slot + 4 * (size_t)sh.rows_cap + ((size_t)(8 * cc + ((c + d) >> 2)) * sh.rows_cap + row) * 4) = make_float4(v[d], v[d + 1], v[d + 2], v[d + 3]);
+                        }
                     }
                 }
-                if (fold && (cc & 1) == 1) mbar_arrive(bar_xfree);
+                if (fold && (cc & (4 / xparts - 1)) == 4 / xparts - 1) arrive_warp(bar_xfree);
             }
             tc_fence_before();
         }
     } else if (warp < 12) {
-        regs_down<64>();
+        regs_down<48>();
         if (warp < 10) {
             // ------------------------------------------------------------------------------------ MMA issue: one warp per half
             const int h = warp - 8;
@@ -637,7 +702,7 @@ q8_chunk_kernel(Q8Launch a, ChunkShape sh) {
         // kRaw tiles ahead, with 16-byte asynchronous copies into a ring of its own, which needs no barrier.  (As TMA boxes the rows of one
         // head are 2 KiB a copy, too little: one warp issuing all of a tile's copies took 1900 cycles a tile, eight warps with a box
         // and a run of scales each 900.  16 keys of every tile a warp: 1500 cycles a tile, most of it latency.)
-        regs_down<88>();
+        regs_down<80>();
         const int me = warp - 12, which = me >> 2, par = me >> 1 & 1, hw = me & 1;
         const bool p8 = a.kv_shift == 3;
         const unsigned char* const pool = static_cast<const unsigned char*>(which ? a.pool_v : a.pool_k);

@@ -139,13 +139,11 @@ __device__ __forceinline__ void q8_store4(void* base, int64_t elem, int io, floa
     else Q8Io<__nv_bfloat16>::store4(static_cast<__nv_bfloat16*>(base) + elem, v);
 }
 
-// Eight consecutive values (16 or 32 bytes).
+// Eight consecutive values (16 or 32 bytes), as loaded.
 template <typename T>
-__device__ __forceinline__ void load8(const void* base, int64_t elem, float (&x)[8]) {
-    const T* p = static_cast<const T*>(base) + elem;
+__device__ __forceinline__ void q8_unpack8(const uint4* u, float (&x)[8]) {
+    const uint32_t w[4] = {u[0].x, u[0].y, u[0].z, u[0].w};
     if constexpr (sizeof(T) == 2) {
-        const uint4 u = __ldg(reinterpret_cast<const uint4*>(p));
-        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             if constexpr (std::is_same<T, __half>::value) {
@@ -158,10 +156,21 @@ __device__ __forceinline__ void load8(const void* base, int64_t elem, float (&x)
             }
         }
     } else {
-        const float4 u = *reinterpret_cast<const float4*>(p), v = *reinterpret_cast<const float4*>(p + 4);
-        x[0] = u.x; x[1] = u.y; x[2] = u.z; x[3] = u.w;
-        x[4] = v.x; x[5] = v.y; x[6] = v.z; x[7] = v.w;
+        const uint32_t v[4] = {u[1].x, u[1].y, u[1].z, u[1].w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            x[e] = __uint_as_float(w[e]);
+            x[4 + e] = __uint_as_float(v[e]);
+        }
     }
+}
+template <typename T>
+__device__ __forceinline__ void load8(const void* base, int64_t elem, float (&x)[8]) {
+    const uint4* const p = reinterpret_cast<const uint4*>(static_cast<const T*>(base) + elem);
+    uint4 u[sizeof(T) / 2];
+#pragma unroll
+    for (int e = 0; e < (int)sizeof(T) / 2; ++e) u[e] = sizeof(T) == 2 ? __ldg(p + e) : p[e];
+    q8_unpack8<T>(u, x);
 }
 
 __device__ __forceinline__ void store8(float* p, const float (&v)[8]) {
