@@ -25,7 +25,7 @@
 namespace novab {
 namespace {
 
-constexpr int kThreads = 640;
+constexpr int kThreads = 640, kMergeThreads = 128;
 constexpr int kConv = 8;                              // converting warps
 constexpr int kKeys = 64;                             // keys of a tile
 constexpr int kHalfRows = 128;                        // rows of a half = M of the MMAs
@@ -862,9 +862,9 @@ q8_chunk_kernel(Q8Launch a, ChunkShape sh) {
 }
 
 // Merge of the units that several CTAs worked on: the unit that the place where CTA blockIdx.x + 1 begins falls into, unless an
-// earlier such place falls into it too.  blockIdx.y takes a share of the (32-row, 4-dim) pieces; thread = row.  A CTA is small enough
-// (two warps of 64 registers, 10 KiB) to wait beside an attention CTA, its plan and its unit already worked out.
-__global__ void __launch_bounds__(64, 16) q8_chunk_merge_kernel(Q8Launch a, ChunkShape sh, int grid_split) {
+// earlier such place falls into it too.  blockIdx.y takes a share of the (32-row, 16-dim) pieces; thread = row, and what four
+// contributors have for it is on its way at a time (one after the other the loads took 42 us for 8 x (301-512) tokens).
+__global__ void __launch_bounds__(kMergeThreads, 4) q8_chunk_merge_kernel(Q8Launch a, ChunkShape sh, int grid_split) {
     __shared__ ChunkPlan plan;
     const int lane = (int)threadIdx.x & 31, warp = (int)threadIdx.x >> 5;
     const int G = a.n_heads / a.n_kv_heads;
@@ -891,29 +891,53 @@ __global__ void __launch_bounds__(64, 16) q8_chunk_merge_kernel(Q8Launch a, Chun
     pdl_wait();                            // by every CTA: this grid must not be done before the one that it follows
     if (!todo) return;
     const size_t slot_floats = (size_t)sh.rows_cap * kSlotW;
-    const int rows = u.t_cnt * G, blocks = (rows + 31) / 32;
-    for (int piece = (int)blockIdx.y * 2 + warp; piece < blocks * 32; piece += (int)gridDim.y * 2) {
-        const int row = (piece >> 5) * 32 + lane, d4 = piece & 31;
-        if (row >= rows) continue;
-        float M = -INFINITY, L = 0.f;
-        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-        for (int c = c1 - 1; c < c_end; ++c) {
-            unit_part(u, begin(c), begin(c + 1), tile, count);
-            if (count == 0) continue;
-            const float* slot = a.part + (size_t)(2 * c + (u.begin > begin(c) ? 1 : 0)) * slot_floats;
-            const float2 ml = __ldcg(reinterpret_cast<const float2*>(slot + 2 * row));
-            const float4 x = __ldcg(reinterpret_cast<const float4*>(slot + 4 * (size_t)sh.rows_cap + ((size_t)d4 * sh.rows_cap + row) * 4));
-            if (!(ml.y > 0.f)) continue;
-            const float mn = fmaxf(M, ml.x), cm = M == -INFINITY ? 0.f : ex2(M - mn), cx = ex2(ml.x - mn);
-            M = mn;
-            L = L * cm + ml.y * cx;
-            acc = make_float4(acc.x * cm + x.x * cx, acc.y * cm + x.y * cx, acc.z * cm + x.z * cx, acc.w * cm + x.w * cx);
-        }
+    const int rows = u.t_cnt * G, pieces = (rows + 31) / 32 * 8;
+    for (int piece = (int)blockIdx.y * (kMergeThreads / 32) + warp; piece < pieces; piece += (int)gridDim.y * (kMergeThreads / 32)) {
+        const int row = (piece >> 3) * 32 + lane, d4 = (piece & 7) * 4;
         const int tk = row / G, g = row - tk * G;
-        if (a.rope_cs && u.past + u.t0 + tk >= a.rope_rows) continue;
+        if (row >= rows || (a.rope_cs && u.past + u.t0 + tk >= a.rope_rows)) continue;
+        float M = -INFINITY, L = 0.f;
+        float4 acc[4];
+#pragma unroll
+        for (int d = 0; d < 4; ++d) acc[d] = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int c = c1 - 1; c < c_end; c += 4) {
+            float2 ml[4];
+            float4 x[4][4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                ml[e] = make_float2(-INFINITY, 0.f);
+                count = 0;
+                if (c + e < c_end) unit_part(u, begin(c + e), begin(c + e + 1), tile, count);
+                if (count > 0) {
+                    const float* slot = a.part + (size_t)(2 * (c + e) + (u.begin > begin(c + e) ? 1 : 0)) * slot_floats;
+                    ml[e] = __ldcg(reinterpret_cast<const float2*>(slot + 2 * row));
+#pragma unroll
+                    for (int d = 0; d < 4; ++d) x[e][d] = __ldcg(reinterpret_cast<const float4*>(slot + 4 * (size_t)sh.rows_cap + ((size_t)(d4 + d) * sh.rows_cap + row) * 4));
+                }
+            }
+            float mn = M;
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (ml[e].y != 0.f) mn = fmaxf(mn, ml[e].x);
+            const float cm = M == -INFINITY ? 0.f : ex2(M - mn);
+            M = mn;
+            L *= cm;
+#pragma unroll
+            for (int d = 0; d < 4; ++d) acc[d] = make_float4(acc[d].x * cm, acc[d].y * cm, acc[d].z * cm, acc[d].w * cm);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                if (ml[e].y == 0.f) continue;                 // nothing of the row's; a NaN stays one
+                const float cx = ex2(ml[e].x - mn);
+                L = fmaf(ml[e].y, cx, L);
+#pragma unroll
+                for (int d = 0; d < 4; ++d)
+                    acc[d] = make_float4(fmaf(x[e][d].x, cx, acc[d].x), fmaf(x[e][d].y, cx, acc[d].y), fmaf(x[e][d].z, cx, acc[d].z), fmaf(x[e][d].w, cx, acc[d].w));
+            }
+        }
         const float inv = L > 0.f ? 1.f / L : 0.f;
-        q8_store4(a.out, ((int64_t)plan.first[u.s] + u.t0 + tk) * a.out_stride + (int64_t)(u.kvh * G + g) * kHeadDim + 4 * d4, a.io,
-                  make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv));
+        const int64_t oe = ((int64_t)plan.first[u.s] + u.t0 + tk) * a.out_stride + (int64_t)(u.kvh * G + g) * kHeadDim + 4 * d4;
+#pragma unroll
+        for (int d = 0; d < 4; ++d) q8_store4(a.out, oe + 4 * d, a.io, make_float4(acc[d].x * inv, acc[d].y * inv, acc[d].z * inv, acc[d].w * inv));
     }
 }
 
@@ -959,7 +983,7 @@ int launch_q8_chunk(const Q8Launch& a, cudaStream_t s) {
         cudaError_t e = launch_kernel_pdl(kernel, dim3((unsigned)ctas), dim3(kThreads), (size_t)kSmem, s, true, b, sh);
         if (e == cudaSuccess) {
             count_launch();
-            e = launch_kernel_pdl(q8_chunk_merge_kernel, dim3((unsigned)ctas - 1, 8u), dim3(64), 0, s, true, b, sh, ctas);
+            e = launch_kernel_pdl(q8_chunk_merge_kernel, dim3((unsigned)ctas - 1, 8u), dim3(kMergeThreads), 0, s, true, b, sh, ctas);
         }
         if (e != cudaSuccess) {
             set_cuda_error(e, "8-bit chunk attention launch");
