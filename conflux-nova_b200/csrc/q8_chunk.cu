@@ -206,12 +206,24 @@ struct __align__(16) Part {
 };
 constexpr int kParts = 4;
 static_assert(sizeof(Part) == 48 && kOffBar - kOffParts == kParts * (int)sizeof(Part), "ring of parts");
-// The part [lo, hi) of the line that a CTA takes of a unit, as tiles of the unit.
-__device__ __forceinline__ void unit_part(const Unit& u, long long lo, long long hi, int& tile, int& count) {
-    const long long b = (lo > u.begin ? lo : u.begin) - u.begin - kSetup, e = (hi < u.end ? hi : u.end) - u.begin - kSetup;
+// The part [lo, hi) of the line that a CTA takes of the unit [begin, end), as tiles of the unit.
+__device__ __forceinline__ void unit_part(long long begin, long long end, long long lo, long long hi, int& tile, int& count) {
+    const long long b = (lo > begin ? lo : begin) - begin - kSetup, e = (hi < end ? hi : end) - begin - kSetup;
     tile = (int)(b > 0 ? b : 0);
     count = (int)(e > 0 ? e : 0) - tile;
     if (count < 0) count = 0;
+}
+
+// What the merge kernel needs of the unit that a CTA begins inside of; behind the partial slots.
+struct __align__(16) Seam {
+    long long begin, end;            // the unit on the line
+    long long each, more;            // Shares
+    int todo, c0, c_end;             // whether there is something to merge here; contributors c0 .. c_end - 1
+    int token, t_cnt, pos, kvh, pad; // first row of q / out, rows, position of the first, kv head
+};
+static_assert(sizeof(Seam) == 64, "records of the seams");
+__device__ __forceinline__ Seam* seams(const Q8Launch& a, const ChunkShape& sh) {
+    return reinterpret_cast<Seam*>(a.part + (size_t)2 * kQ8MaxCtas * sh.rows_cap * kSlotW);
 }
 
 __device__ __forceinline__ unsigned long long pack_f2(float x, float y) {
@@ -294,6 +306,7 @@ q8_chunk_kernel(Q8Launch a, ChunkShape sh) {
     if ((int)blockIdx.x >= n_ctas || (base & 1023u) != 0) {            // uniform over the CTA; nothing has been allocated yet
         if ((base & 1023u) != 0 && threadIdx.x == 0) q8_flag(a, NOVA_ERR_UNSUPPORTED);
         pdl_wait();                   // (a grid must not be done before the one that it follows)
+        if (threadIdx.x == 0) seams(a, sh)[blockIdx.x].todo = 0;
         return;
     }
     const Shares shares = plan_shares(total, n_ctas);
@@ -678,7 +691,7 @@ q8_chunk_kernel(Q8Launch a, ChunkShape sh) {
                 q.tiles = 0;
                 while (pos < hi && q.tiles == 0) {
                     const Unit v = find_unit(a, sh, plan, pos);
-                    unit_part(v, lo, hi, q.tile0, q.tiles);
+                    unit_part(v.begin, v.end, lo, hi, q.tile0, q.tiles);
                     pos = v.end;
                     q.s = v.s; q.kvh = v.kvh; q.t0 = v.t0; q.t_cnt = v.t_cnt; q.past = v.past; q.first16 = v.first16; q.keys_end = v.keys_end;
                     q.whole = q.tiles == v.tiles;
@@ -694,6 +707,22 @@ q8_chunk_kernel(Q8Launch a, ChunkShape sh) {
                 ++k;
                 if (q.tiles == 0) break;
             }
+            // the unit that this CTA begins inside of is merged by its first such CTA, unless all its tiles went to one
+            const Unit v = find_unit(a, sh, plan, lo);
+            const int c1 = (int)blockIdx.x;
+            Seam z = {};
+            if (lo != v.begin && c1 > 0 && cta_begin(shares, c1 - 1) <= v.begin) {
+                int c_end = c1, tile, some = 0;
+                for (int c = c1 - 1, count; c < n_ctas && cta_begin(shares, c) < v.end; ++c) {
+                    unit_part(v.begin, v.end, cta_begin(shares, c), cta_begin(shares, c + 1), tile, count);
+                    some += count > 0;
+                    c_end = c + 1;
+                }
+                z.begin = v.begin; z.end = v.end; z.each = shares.each; z.more = shares.more;
+                z.todo = some > 1; z.c0 = c1 - 1; z.c_end = c_end;
+                z.token = plan.first[v.s] + v.t0; z.t_cnt = v.t_cnt; z.pos = v.past + v.t0; z.kvh = v.kvh;
+            }
+            if (lane == 0) seams(a, sh)[c1] = z;
         }
     } else {
         // ---------------------------------------------------------------------------------------- codes -> fp16 operands
@@ -861,55 +890,44 @@ q8_chunk_kernel(Q8Launch a, ChunkShape sh) {
     if (warp == 0) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"((uint32_t)kTmemCols) : "memory");
 }
 
-// Merge of the units that several CTAs worked on: the unit that the place where CTA blockIdx.x + 1 begins falls into, unless an
-// earlier such place falls into it too.  blockIdx.y takes a share of the (32-row, 16-dim) pieces; thread = row, and what four
-// contributors have for it is on its way at a time (one after the other the loads took 42 us for 8 x (301-512) tokens).
-__global__ void __launch_bounds__(kMergeThreads, 4) q8_chunk_merge_kernel(Q8Launch a, ChunkShape sh, int grid_split) {
-    __shared__ ChunkPlan plan;
+// Merge of the units that several CTAs worked on, by the record of CTA blockIdx.x + 1.  blockIdx.y takes a share of the (32-row,
+// 16-dim) pieces; thread = row, and what four contributors have for it is on its way at a time (with the loads one after the other, and
+// the plan worked out again here, the merge took 42 us for 8 x (301-512) tokens).
+__global__ void __launch_bounds__(kMergeThreads, 4) q8_chunk_merge_kernel(Q8Launch a, ChunkShape sh) {
     const int lane = (int)threadIdx.x & 31, warp = (int)threadIdx.x >> 5;
     const int G = a.n_heads / a.n_kv_heads;
     pdl_launch_dependents();
-    build_plan(a, sh, plan, false);       // (positions and row starts: written before the attention kernel, which waited)
-    const long long total = plan.line[a.n_sessions];
-    const int n_ctas = plan_ctas(total, grid_split), c1 = (int)blockIdx.x + 1;
-    Shares shares = {};
-    if (n_ctas > 0) shares = plan_shares(total, n_ctas);
-    auto begin = [&](int c) -> long long { return cta_begin(shares, c); };
-    Unit u = {};
-    int tile, count, c_end = 0;
-    bool todo = c1 < n_ctas;
-    if (todo) {
-        u = find_unit(a, sh, plan, begin(c1));
-        todo = begin(c1) != u.begin && begin(c1 - 1) <= u.begin;        // a seam of this unit, and its first
-        for (c_end = c1; c_end < n_ctas && begin(c_end) < u.end; ++c_end) {}      // contributors c1 - 1 .. c_end - 1
-        // (one of two contributors may have got nothing but the set-up weight)
-        unit_part(u, begin(c1 - 1), begin(c1), tile, count);
-        if (count == u.tiles) todo = false;
-        unit_part(u, begin(c1), begin(c1 + 1), tile, count);
-        if (c_end == c1 + 1 && count == u.tiles) todo = false;
-    }
     pdl_wait();                            // by every CTA: this grid must not be done before the one that it follows
-    if (!todo) return;
+    const int4* const rec = reinterpret_cast<const int4*>(seams(a, sh) + blockIdx.x + 1);
+    int4 w[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) w[e] = __ldcg(rec + e);
+    const Seam z = *reinterpret_cast<const Seam*>(w);
+    if (!z.todo) return;
+    Shares shares;
+    shares.each = z.each;
+    shares.more = z.more;
+    auto begin = [&](int c) -> long long { return cta_begin(shares, c); };
     const size_t slot_floats = (size_t)sh.rows_cap * kSlotW;
-    const int rows = u.t_cnt * G, pieces = (rows + 31) / 32 * 8;
+    const int rows = z.t_cnt * G, pieces = (rows + 31) / 32 * 8;
     for (int piece = (int)blockIdx.y * (kMergeThreads / 32) + warp; piece < pieces; piece += (int)gridDim.y * (kMergeThreads / 32)) {
         const int row = (piece >> 3) * 32 + lane, d4 = (piece & 7) * 4;
         const int tk = row / G, g = row - tk * G;
-        if (row >= rows || (a.rope_cs && u.past + u.t0 + tk >= a.rope_rows)) continue;
+        if (row >= rows || (a.rope_cs && z.pos + tk >= a.rope_rows)) continue;
         float M = -INFINITY, L = 0.f;
         float4 acc[4];
 #pragma unroll
         for (int d = 0; d < 4; ++d) acc[d] = make_float4(0.f, 0.f, 0.f, 0.f);
-        for (int c = c1 - 1; c < c_end; c += 4) {
+        for (int c = z.c0; c < z.c_end; c += 4) {
             float2 ml[4];
             float4 x[4][4];
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 ml[e] = make_float2(-INFINITY, 0.f);
-                count = 0;
-                if (c + e < c_end) unit_part(u, begin(c + e), begin(c + e + 1), tile, count);
+                int tile, count = 0;
+                if (c + e < z.c_end) unit_part(z.begin, z.end, begin(c + e), begin(c + e + 1), tile, count);
                 if (count > 0) {
-                    const float* slot = a.part + (size_t)(2 * (c + e) + (u.begin > begin(c + e) ? 1 : 0)) * slot_floats;
+                    const float* slot = a.part + (size_t)(2 * (c + e) + (z.begin > begin(c + e) ? 1 : 0)) * slot_floats;
                     ml[e] = __ldcg(reinterpret_cast<const float2*>(slot + 2 * row));
 #pragma unroll
                     for (int d = 0; d < 4; ++d) x[e][d] = __ldcg(reinterpret_cast<const float4*>(slot + 4 * (size_t)sh.rows_cap + ((size_t)(d4 + d) * sh.rows_cap + row) * 4));
@@ -935,7 +953,7 @@ __global__ void __launch_bounds__(kMergeThreads, 4) q8_chunk_merge_kernel(Q8Laun
             }
         }
         const float inv = L > 0.f ? 1.f / L : 0.f;
-        const int64_t oe = ((int64_t)plan.first[u.s] + u.t0 + tk) * a.out_stride + (int64_t)(u.kvh * G + g) * kHeadDim + 4 * d4;
+        const int64_t oe = ((int64_t)z.token + tk) * a.out_stride + (int64_t)(z.kvh * G + g) * kHeadDim + 4 * d4;
 #pragma unroll
         for (int d = 0; d < 4; ++d) q8_store4(a.out, oe + 4 * d, a.io, make_float4(acc[d].x * inv, acc[d].y * inv, acc[d].z * inv, acc[d].w * inv));
     }
@@ -955,7 +973,7 @@ ChunkShape chunk_shape(int n_heads, int n_kv_heads, int max_tokens) {
 }  // namespace
 
 size_t q8_chunk_work_bytes(int n_heads, int n_kv_heads, int max_tokens) {
-    return (size_t)2 * kQ8MaxCtas * chunk_shape(n_heads, n_kv_heads, max_tokens).rows_cap * kSlotW * sizeof(float);
+    return (size_t)2 * kQ8MaxCtas * chunk_shape(n_heads, n_kv_heads, max_tokens).rows_cap * kSlotW * sizeof(float) + kQ8MaxCtas * sizeof(Seam);
 }
 
 int launch_q8_chunk(const Q8Launch& a, cudaStream_t s) {
@@ -983,7 +1001,7 @@ int launch_q8_chunk(const Q8Launch& a, cudaStream_t s) {
         cudaError_t e = launch_kernel_pdl(kernel, dim3((unsigned)ctas), dim3(kThreads), (size_t)kSmem, s, true, b, sh);
         if (e == cudaSuccess) {
             count_launch();
-            e = launch_kernel_pdl(q8_chunk_merge_kernel, dim3((unsigned)ctas - 1, 8u), dim3(kMergeThreads), 0, s, true, b, sh, ctas);
+            if (ctas > 1) e = launch_kernel_pdl(q8_chunk_merge_kernel, dim3((unsigned)ctas - 1, (unsigned)(sh.rows_cap / 16)), dim3(kMergeThreads), 0, s, true, b, sh);
         }
         if (e != cudaSuccess) {
             set_cuda_error(e, "8-bit chunk attention launch");
