@@ -368,50 +368,63 @@ q8_chunk_kernel(Q8Launch a, ChunkShape sh) {
             {
                 // ---- q: rotated, scaled, fp16, K-major 128-byte swizzle; eight lanes a row, dims 8c .. and 64 + 8c .. each.  The scores
                 // of the unit before are all computed (this thread has waited for the last of them), so the operand can be overwritten.
-                // The loads of kRows rows go out together (one after the other they took 9 us a unit).
+                // A warp takes four rows of every sixteen, two such groups at a time; the next two groups' q is on its way meanwhile (one
+                // row after the other took 9 us a unit).
                 constexpr float kQ = kAttnScale * kLog2e * kKDiv;
-                constexpr int kRows = 2, kVec = sizeof(T) / 2;
+                constexpr int kRows = sizeof(T) == 4 ? 1 : 2, kVec = sizeof(T) / 2;
                 const int c = lane & 7, second = a.neox ? 4 : 32;          // neox: the pairs (d, d + 64); else neighbours, in both halves of the dims
+                const int rfirst = 4 * (warp & 3) + (lane >> 3), n_rows = u.t_cnt * G - row0;
+                uint4 next[kRows][2 * kVec];
+                auto bring = [&](int e8) {
+#pragma unroll
+                    for (int e = 0; e < kRows; ++e) {
+                        const int rr = row0 + rfirst + 16 * (e8 + e), rt = (int)((uint32_t)rr * per_g >> 16), rg = rr - rt * G, rpos = u.past + u.t0 + rt;
+#pragma unroll
+                        for (int v = 0; v < 2 * kVec; ++v) next[e][v] = make_uint4(0u, 0u, 0u, 0u);
+                        if (e8 < 8 && rt < u.t_cnt && !(a.rope_cs && rpos >= a.rope_rows)) {
+                            const uint4* const src = reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + (tok0 + rt) * a.q_stride + (int64_t)(u.kvh * G + rg) * kHeadDim + 8 * c);
+#pragma unroll
+                            for (int v = 0; v < kVec; ++v) {
+                                next[e][v] = __ldg(src + v);
+                                next[e][kVec + v] = __ldg(src + 8 * kVec + v);
+                            }
+                        }
+                    }
+                };
+                bring(0);
 #pragma unroll 1
                 for (int e8 = 0; e8 < 8; e8 += kRows) {
-                    const int r0 = 32 * (warp & 3) + 4 * e8 + (lane >> 3);
-                    if (__all_sync(0xffffffffu, (row0 + r0 - (lane >> 3)) >= u.t_cnt * G)) {      // none of these rows exists
+                    const int r0 = rfirst + 16 * e8;
+                    if (16 * e8 >= n_rows) {                               // none of these rows exists
 #pragma unroll
                         for (int e = 0; e < kRows; ++e)
 #pragma unroll
                             for (int hf = 0; hf < 2; ++hf)
-                                sts128(base + (uint32_t)((2 * half + hf) * kQSlab + (r0 + 4 * e) * 128 + ((c ^ ((r0 + 4 * e) & 7)) << 4)), make_float4(0.f, 0.f, 0.f, 0.f));
+                                sts128(base + (uint32_t)((2 * half + hf) * kQSlab + (r0 + 16 * e) * 128 + ((c ^ ((r0 + 16 * e) & 7)) << 4)), make_float4(0.f, 0.f, 0.f, 0.f));
                         continue;
                     }
                     uint4 raw[kRows][2 * kVec];
                     float4 rc[kRows][2], rs[kRows][2];
 #pragma unroll
                     for (int e = 0; e < kRows; ++e) {
-                        const int rr = row0 + r0 + 4 * e, rt = (int)((uint32_t)rr * per_g >> 16), rg = rr - rt * G, rpos = u.past + u.t0 + rt;
 #pragma unroll
-                        for (int v = 0; v < 2 * kVec; ++v) raw[e][v] = make_uint4(0u, 0u, 0u, 0u);
+                        for (int v = 0; v < 2 * kVec; ++v) raw[e][v] = next[e][v];
 #pragma unroll
                         for (int v = 0; v < 2; ++v) rc[e][v] = rs[e][v] = make_float4(0.f, 0.f, 0.f, 0.f);
-                        if (rt < u.t_cnt && !(a.rope_cs && rpos >= a.rope_rows)) {
-                            const uint4* const src = reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + (tok0 + rt) * a.q_stride + (int64_t)(u.kvh * G + rg) * kHeadDim + 8 * c);
-#pragma unroll
-                            for (int v = 0; v < kVec; ++v) {
-                                raw[e][v] = __ldg(src + v);
-                                raw[e][kVec + v] = __ldg(src + 8 * kVec + v);
-                            }
-                            if (a.rope_cs) {
-                                const float* cr = a.rope_cs + (int64_t)rpos * 64 + (a.neox ? 8 : 4) * c;
-                                const float* sr = a.rope_sn + (int64_t)rpos * 64 + (a.neox ? 8 : 4) * c;
-                                rc[e][0] = __ldg(reinterpret_cast<const float4*>(cr));
-                                rc[e][1] = __ldg(reinterpret_cast<const float4*>(cr + second));
-                                rs[e][0] = __ldg(reinterpret_cast<const float4*>(sr));
-                                rs[e][1] = __ldg(reinterpret_cast<const float4*>(sr + second));
-                            }
+                        const int rt = (int)((uint32_t)(row0 + r0 + 16 * e) * per_g >> 16), rpos = u.past + u.t0 + rt;
+                        if (rt < u.t_cnt && a.rope_cs && rpos < a.rope_rows) {
+                            const float* cr = a.rope_cs + (int64_t)rpos * 64 + (a.neox ? 8 : 4) * c;
+                            const float* sr = a.rope_sn + (int64_t)rpos * 64 + (a.neox ? 8 : 4) * c;
+                            rc[e][0] = __ldg(reinterpret_cast<const float4*>(cr));
+                            rc[e][1] = __ldg(reinterpret_cast<const float4*>(cr + second));
+                            rs[e][0] = __ldg(reinterpret_cast<const float4*>(sr));
+                            rs[e][1] = __ldg(reinterpret_cast<const float4*>(sr + second));
                         }
                     }
+                    bring(e8 + kRows);
 #pragma unroll
                     for (int e = 0; e < kRows; ++e) {
-                        const int r = r0 + 4 * e;
+                        const int r = r0 + 16 * e;
                         float x0[8], x1[8];
                         q8_unpack8<T>(&raw[e][0], x0);
                         q8_unpack8<T>(&raw[e][kVec], x1);
