@@ -167,7 +167,8 @@ void fill_q8(const nova_batch* b, int layer, int n_tok, Q8Launch& a) {
     a.n_sessions = b->n; a.n_tokens = b->n * n_tok; a.max_tokens = a.uniform_tokens = n_tok;
     a.q_stride = a.out_stride = (int64_t)e->d.n_heads * kHeadDim;
     a.k_stride = a.v_stride = (int64_t)e->d.n_kv_heads * kHeadDim;
-    a.io = NOVA_IO_F32; a.fmt = e->d.kv_dtype; a.neox = e->d.rope_neox;
+    a.io = NOVA_IO_F32; a.one_part = 1;      // (q and the weights rounded to fp16 once, as on fp16 pools)
+    a.fmt = e->d.kv_dtype; a.neox = e->d.rope_neox;
     a.layer = layer; a.nb = e->nb; a.n_heads = e->d.n_heads; a.n_kv_heads = e->d.n_kv_heads; a.kv_shift = e->kv_shift;
 }
 void q8_rope(const nova_batch* b, Q8Launch& a) {

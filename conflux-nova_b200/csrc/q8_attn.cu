@@ -149,7 +149,7 @@ __device__ __forceinline__ DecSegment dec_segment(const DecPlan& p, const DecLin
     return sg;
 }
 
-// kLo: q and p in two fp16 parts (fp32 activations)
+// kLo: q and p in two fp16 parts (fp32 activations, unless one_part)
 template <int KVG, int kFmt, bool kLo>
 __global__ void __launch_bounds__(DecCfg<KVG>::kThreads, 1)
 q8_decode_kernel(Q8Launch a, const __grid_constant__ CUtensorMap tmk, const __grid_constant__ CUtensorMap tmv) {
@@ -770,7 +770,7 @@ int dec_group(int n_kv_heads) { return n_kv_heads % 4 == 0 ? 4 : (n_kv_heads % 2
 template <int KVG, int kFmt, bool kLo>
 int launch_decode_as(const Q8Launch& a, const CUtensorMap& tmk, const CUtensorMap& tmv, int ctas, cudaStream_t s) {
     using Cfg = DecCfg<KVG>;
-    NOVA_CUDA_TRY((cudaFuncSetAttribute(q8_decode_kernel<KVG, kFmt, kLo>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::kSmem)));
+    NOVA_CUDA_TRY((q8_allow_smem<q8_decode_kernel<KVG, kFmt, kLo>>(Cfg::kSmem)));
     const cudaError_t e = launch_kernel_pdl(q8_decode_kernel<KVG, kFmt, kLo>, dim3((unsigned)ctas), dim3(Cfg::kThreads), (size_t)Cfg::kSmem, s, true, a, tmk, tmv);
     if (e != cudaSuccess) {
         set_cuda_error(e, "8-bit decode attention launch");
@@ -782,7 +782,7 @@ int launch_decode_as(const Q8Launch& a, const CUtensorMap& tmk, const CUtensorMa
 
 template <int KVG, int kFmt>
 int launch_decode(const Q8Launch& a, const CUtensorMap& tmk, const CUtensorMap& tmv, int ctas, cudaStream_t s) {
-    return a.io == NOVA_IO_F32 ? launch_decode_as<KVG, kFmt, true>(a, tmk, tmv, ctas, s) : launch_decode_as<KVG, kFmt, false>(a, tmk, tmv, ctas, s);
+    return a.io == NOVA_IO_F32 && !a.one_part ? launch_decode_as<KVG, kFmt, true>(a, tmk, tmv, ctas, s) : launch_decode_as<KVG, kFmt, false>(a, tmk, tmv, ctas, s);
 }
 
 }  // namespace

@@ -18,7 +18,6 @@
 //     A lane's rows are chosen so that neither the reads (rows r and r ^ 5 side by side) nor the writes meet in a bank.
 //   * q (rotated) and P are rounded to fp16; everything else is fp32.
 //   * Every wait is bounded; tensor memory is released on every path.
-#include "attn_plan.cuh"
 #include "q8_common.cuh"
 #include "tc5_common.cuh"
 
@@ -972,6 +971,17 @@ __global__ void __launch_bounds__(kMergeThreads, 4) q8_chunk_merge_kernel(Q8Laun
     }
 }
 
+template <int kFmt, typename T>
+cudaError_t launch_chunk_as(const Q8Launch& a, const ChunkShape& sh, int ctas, cudaStream_t s) {
+    const cudaError_t e = q8_allow_smem<q8_chunk_kernel<kFmt, T>>(kSmem);
+    return e != cudaSuccess ? e : launch_kernel_pdl(q8_chunk_kernel<kFmt, T>, dim3((unsigned)ctas), dim3(kThreads), (size_t)kSmem, s, true, a, sh);
+}
+template <int kFmt>
+cudaError_t launch_chunk(const Q8Launch& a, const ChunkShape& sh, int ctas, cudaStream_t s) {
+    return a.io == NOVA_IO_F32 ? launch_chunk_as<kFmt, float>(a, sh, ctas, s)
+         : a.io == NOVA_IO_F16 ? launch_chunk_as<kFmt, __half>(a, sh, ctas, s) : launch_chunk_as<kFmt, __nv_bfloat16>(a, sh, ctas, s);
+}
+
 ChunkShape chunk_shape(int n_heads, int n_kv_heads, int max_tokens) {
     ChunkShape sh;
     const int G = n_heads / n_kv_heads;
@@ -1008,10 +1018,7 @@ int launch_q8_chunk(const Q8Launch& a, cudaStream_t s) {
             b.q = static_cast<const unsigned char*>(a.q) + rows * a.q_stride * (int64_t)io_bytes;
             b.out = static_cast<unsigned char*>(a.out) + rows * a.out_stride * (int64_t)io_bytes;
         }
-        auto* kernel = a.fmt == NOVA_KV_I8 ? (a.io == NOVA_IO_F32 ? q8_chunk_kernel<NOVA_KV_I8, float> : a.io == NOVA_IO_F16 ? q8_chunk_kernel<NOVA_KV_I8, __half> : q8_chunk_kernel<NOVA_KV_I8, __nv_bfloat16>)
-                                           : (a.io == NOVA_IO_F32 ? q8_chunk_kernel<NOVA_KV_E4M3, float> : a.io == NOVA_IO_F16 ? q8_chunk_kernel<NOVA_KV_E4M3, __half> : q8_chunk_kernel<NOVA_KV_E4M3, __nv_bfloat16>);
-        NOVA_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem));
-        cudaError_t e = launch_kernel_pdl(kernel, dim3((unsigned)ctas), dim3(kThreads), (size_t)kSmem, s, true, b, sh);
+        cudaError_t e = a.fmt == NOVA_KV_I8 ? launch_chunk<NOVA_KV_I8>(b, sh, ctas, s) : launch_chunk<NOVA_KV_E4M3>(b, sh, ctas, s);
         if (e == cudaSuccess) {
             count_launch();
             if (ctas > 1) e = launch_kernel_pdl(q8_chunk_merge_kernel, dim3((unsigned)ctas - 1, (unsigned)(sh.rows_cap / 16)), dim3(kMergeThreads), 0, s, true, b, sh);

@@ -5,6 +5,7 @@
 // scale per (token, kv head) [layer][NB][NKV][page tokens], kv head major within a page so that the scales of one
 // head's tile of keys are one contiguous piece.
 #pragma once
+#include <atomic>
 #include <cuda_bf16.h>
 #include <cuda_fp8.h>
 #include <type_traits>
@@ -51,6 +52,7 @@ struct Q8Launch {
     int32_t* status;
     float* part;                  // workspace of the attention
     int32_t n_sessions, n_tokens, max_tokens, uniform_tokens;
+    int32_t one_part;             // single tokens, fp32 activations: q and the weights as one fp16 value instead of two parts
     int32_t io, fmt, neox;
     int32_t layer, nb, n_heads, n_kv_heads, kv_shift;
     int32_t window;
@@ -164,15 +166,6 @@ __device__ __forceinline__ void q8_unpack8(const uint4* u, float (&x)[8]) {
         }
     }
 }
-template <typename T>
-__device__ __forceinline__ void load8(const void* base, int64_t elem, float (&x)[8]) {
-    const uint4* const p = reinterpret_cast<const uint4*>(static_cast<const T*>(base) + elem);
-    uint4 u[sizeof(T) / 2];
-#pragma unroll
-    for (int e = 0; e < (int)sizeof(T) / 2; ++e) u[e] = sizeof(T) == 2 ? __ldg(p + e) : p[e];
-    q8_unpack8<T>(u, x);
-}
-
 __device__ __forceinline__ void store8(float* p, const float (&v)[8]) {
     *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
     *reinterpret_cast<float4*>(p + 4) = make_float4(v[4], v[5], v[6], v[7]);
@@ -302,9 +295,6 @@ __device__ __forceinline__ void sts128(uint32_t addr, float4 v) {
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
-__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
-    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
-}
 // Transpose of an 8 x 8 matrix of 16-bit values over the warp (lane 4 r + c holds row r, columns 2c and 2c + 1).
 __device__ __forceinline__ uint32_t movmatrix(uint32_t x) {
     uint32_t y;
@@ -313,6 +303,20 @@ __device__ __forceinline__ uint32_t movmatrix(uint32_t x) {
 }
 
 #endif  // __CUDACC__
+
+// Lets a kernel have `bytes` of dynamic shared memory on the current device; asked of the driver once per kernel and device.
+template <auto kKernel>
+inline cudaError_t q8_allow_smem(int bytes) {
+    static std::atomic<uint64_t> done{0};
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    const uint64_t bit = dev < 64 ? 1ull << dev : 0ull;
+    if (bit & done.load(std::memory_order_relaxed)) return cudaSuccess;
+    e = cudaFuncSetAttribute(kKernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_relaxed);
+    return e;
+}
 
 // q8_cache.cu, q8_attn.cu (single tokens), q8_chunk.cu (everything else)
 int launch_q8_append(const Q8Launch& a, cudaStream_t s);

@@ -380,7 +380,8 @@ int nova_engine_q8_cache(const nova_engine* e, int layer, nova_q8_cache* out);
 /* Engine::decode_batch's hot-path calls (model.cpp:281-289) for any number of
  * sessions in one launch per op.  A batch owns device copies of the sessions'
  * slice ids and write positions, and the scratch of the split-K attention.
- * On 8-bit pools the calls below run the kernels of the section above on fp32 activations, one launch per layer: append, attention,
+ * On 8-bit pools the calls below run the kernels of the section above on fp32 activations (q and the softmax weights rounded to
+ * fp16 once, as on fp16 pools), one launch per layer: append, attention,
  * both at once, prefill (sliding windows too), whole steps, graphs, copy-on-write and shared prefixes work as on other pools.
  * nova_batch_get_kernel is 1 from the start and 0 is refused; the cascade and partial attention (page ranges, peers) are
  * refused with NOVA_ERR_UNSUPPORTED; fused append works with either rotary pairing; the tuning knobs (pdl, row_setup_pages,

@@ -61,7 +61,7 @@ class Run:
             c.window = window
             o, a, spread, floor = c.attend()
             got = torch.from_numpy(out[c.layer]).double()
-            bound = attention_bound(c, o, a, spread, floor, n == 1 and self.H // self.N <= 8)
+            bound = attention_bound(c, o, a, spread, floor, False)         # q and the weights are rounded to fp16, by the header's word
             assert bool(torch.isfinite(got).all()) and bool(((got - o).abs() <= bound).all()), float(((got - o).abs() / bound).max())
 
     def prefill(self, b, n, check=True, window=0):
