@@ -306,6 +306,17 @@ class PoolView:
 
 # ------------------------------------------------------------------------------ 8-bit paged cache
 # The operators of nova_launch_q8_*: cache and rows are Q8Cache / Q8Rows, everything else device addresses and a stream handle.
+def q8_values(codes: np.ndarray, kv_dtype) -> np.ndarray:
+    """The numbers that 8-bit codes stand for (fp32, without the scales): int8 as they are, e4m3 from their bits."""
+    if kv_dtype == KV_I8:
+        return codes.view(np.int8).astype(np.float32)
+    c = np.arange(256)
+    e, m = c >> 3 & 15, c & 7
+    v = np.where(e == 0, m * 2.0 ** -9, (8 + m) * 2.0 ** (e - 10.0))
+    v[(e == 15) & (m == 7)] = np.nan
+    return np.where(c >> 7, -v, v).astype(np.float32)[codes.view(np.uint8)]
+
+
 def q8_append(cache: Q8Cache, rows: Q8Rows, k, v, stream=None):
     return check(lib.nova_launch_q8_append(cache, rows, k, v, stream), "q8_append")
 

@@ -9,7 +9,7 @@
 //     of all units form one line that is dealt out evenly over one CTA per SM, so neither short sessions, nor long ones, nor
 //     the causal triangle leave SMs idle.  Units that several CTAs worked on are merged by the kernel behind it.
 //   * Twenty warps: 8 softmax (thread = row), 2 issuing MMAs (one per half), 8 converting, each of which brings in its own keys'
-//     codes and scales.  The pipe runs on from one unit to the next.
+//     codes and scales, one that walks the line (and one idle).  The pipe runs on from one unit to the next.
 //   * The tensor cores want fp16 operands, so a tile's codes become fp16 VALUES in shared memory, code times scale, in the
 //     128-byte-swizzle layout that is the K-major form for S = Q.K^T and the MN-major form for O += P.V.  A scale (K's over 16;
 //     q is multiplied by 16 / sqrt(128) log2 e) goes in as two fp16 parts and the product is rounded once (2^-11).
@@ -17,6 +17,11 @@
 //     from shared memory, which took 1500 cycles of a 64-key tile.  So |K| saturates at 2^20 and |V| at 65504 here.
 //     A lane's rows are chosen so that neither the reads (rows r and r ^ 5 side by side) nor the writes meet in a bank.
 //   * q (rotated) and P are rounded to fp16; everything else is fp32.
+//   * Measured (graph replay, append included): 2048 tokens over 16384, 28 / 4 heads: 860 us = 850 TFLOP/s; 8 x (301-512) tokens over
+//     2k-8k: 340 us = 750 TFLOP/s; 16 x (0-8) tokens over 2k-8k: 51 us = 1.5 TB/s; a window of 512: 52 us.  A 64-key tile of 256 rows
+//     takes 2350 cycles.  The tensor cores are busy for 1020 of them, the special-function units for 1024; what sets the pace is
+//     the softmax warps' own chain of some 300 dependent instructions per tile (two warps per scheduler; without the exponentials
+//     it would still be 2200).  A unit costs 5 us of q and 4 us of outputs beside its tiles.
 //   * Every wait is bounded; tensor memory is released on every path.
 #include "q8_common.cuh"
 #include "tc5_common.cuh"
@@ -53,7 +58,7 @@ constexpr float kKDiv = 16.f;                         // K goes in divided by th
 // As kQ8Step and kQ8Top (single tokens), but the reference moves less often, which costs more here (O rescaled in tensor
 // memory): weights are 2^7 .. 2^15 at the largest, with fp16's 11 bits down to 2^-21 of the reference.
 constexpr float kStep = 8.f, kTop = 7.f;
-constexpr int kSetup = 2;                             // what starting a unit costs, in tiles
+constexpr int kSetup = 8;                             // what a unit costs beside its tiles, in tiles (8 x (301-512) tokens: 2 362 us, 5 349, 8 340, 12 342)
 constexpr int kFewTiles = 4;                          // token tiles that a thread counts for itself
 constexpr int kMinTiles = 4;                          // a CTA gets at least that many
 constexpr uint32_t kIdescS = (1u << 4) | ((uint32_t)(kKeys >> 3) << 17) | ((uint32_t)(kHalfRows >> 4) << 24);
@@ -878,7 +883,9 @@ q8_chunk_kernel(Q8Launch a, ChunkShape sh) {
 #pragma unroll
                         for (int b = 0; b < 8; ++b) {
                             const __half2 x = *reinterpret_cast<const __half2*>(&h[b]);
-                            const __half2 y = __hfma2(x, hi2, __hmul2(x, lo2));
+                            __half2 y = __hfma2(x, hi2, __hmul2(x, lo2));
+                            // V's NaN codes become the largest number: a query that does not see the key multiplies it by zero
+                            if (kFmt == NOVA_KV_E4M3 && which) y = __hmin2(y, __half2half2(__ushort_as_half(0x7bff)));
                             h[b] = *reinterpret_cast<const uint32_t*>(&y);
                         }
                         const uint32_t de = dst0 + (uint32_t)(q * 2048 + e2 * 1024 + (e & 1) * kSlab);

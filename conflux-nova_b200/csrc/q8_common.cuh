@@ -52,7 +52,7 @@ struct Q8Launch {
     int32_t* status;
     float* part;                  // workspace of the attention
     int32_t n_sessions, n_tokens, max_tokens, uniform_tokens;
-    int32_t one_part;             // single tokens, fp32 activations: q and the weights as one fp16 value instead of two parts
+    int32_t one_part;             // single tokens, fp32 or fp16 activations: q and the weights as one fp16 value instead of two parts
     int32_t io, fmt, neox;
     int32_t layer, nb, n_heads, n_kv_heads, kv_shift;
     int32_t window;

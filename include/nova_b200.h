@@ -317,7 +317,8 @@ int nova_launch_attn_decode_paged_static(const nova_kv_shape* sh, const float* q
  *   scales scale_k / scale_v [layers][nb][n_kv_heads][kv_block] fp32
  * A row (one token of one kv head) is written as  amax = max(max|x|, 2^-60),  scale = amax / Q,  code = rn(x * (Q / amax)),
  * Q = 127 or 448, in fp32 with one rounding per operation (ties to even).  A NaN becomes code 0 (int8) or NaN (e4m3); a row
- * with an infinity gets an infinite scale and reads back as NaN.
+ * with an infinity gets an infinite scale and reads back as NaN; of queries that see such keys or values, or NaN ones, nothing is
+ * promised (others are not touched by them).
  * The block tables are those of the rest of this header: `tables` is an array of tables of table_stride entries, session s
  * uses table slice_ids[s] (slice_ids NULL: table s).  An entry outside [0, nb) is never followed: its keys are skipped, its
  * rows are neither written nor read back, and *status (device, may be NULL) becomes NOVA_ERR_BAD_TABLE.
@@ -361,8 +362,8 @@ int nova_launch_q8_read(const nova_q8_cache* c, const nova_q8_rows* r, void* k_o
  * (p - window, p] where window > 0.  The keys of the new rows must be in the cache; a query that sees none gets zeros.
  * q (rotated) and the softmax weights are rounded to fp16 on their way into the tensor cores; sums and the softmax are fp32.
  * One row per session and at most 8 query heads per kv head: the codes go in exactly and the scales are applied in fp32; with
- * fp32 activations q and the weights are taken as two fp16 parts each (2^-21).  Anything else: keys and values go in as fp16 values,
- * code * scale rounded once (|k| saturates at 2^20, |v| at 65504).  q and out must not overlap.  work: nova_q8_workspace_bytes() bytes, no state in it
+ * fp32 or fp16 activations q and the weights are taken as two fp16 parts each (2^-21).  Anything else: keys and values go in as fp16
+ * values, code * scale rounded once (|k| saturates at 2^20, |v| at 65504).  q and out must not overlap.  work: nova_q8_workspace_bytes() bytes, no state in it
  * between calls; calls that may overlap on the GPU need a workspace each. */
 size_t nova_q8_workspace_bytes(const nova_kv_shape* sh, const nova_q8_rows* r);
 int nova_launch_q8_attn(const nova_q8_cache* c, const nova_q8_rows* r, const void* q, void* out, int window, void* work,

@@ -6,7 +6,7 @@ import math
 import pytest
 import torch
 
-from q8_plain import HD, IO, Cache, attention_bound, call
+from q8_plain import HD, IO, Cache, attention_bound, call, quantise, rotate
 
 pytestmark = pytest.mark.gpu
 
@@ -40,7 +40,7 @@ def check_out(case, d):
     got = d["out"].cpu()
     assert bool((got[T:] == 7).all()), "rows behind the last session"
     o, a, spread, floor = case.attend()
-    exact_q = case.io == "f32" and max(case.new) == 1 and case.H // case.N <= 8        # fp16 hi + lo, by the header's word
+    exact_q = case.io != "bf16" and max(case.new) == 1 and case.H // case.N <= 8        # fp16 hi + lo, by the header's word
     bound = attention_bound(case, o, a, spread, floor, exact_q)
     off = (got[:T].double() - o).abs()
     assert bool(torch.isfinite(got[:T]).all()), "finite"
@@ -184,6 +184,53 @@ def test_chunk_long(nv):
     run_and_check(nv, Cache([1500, 40], [300, 700], 7, 1, 16, "i8", "bf16", layers=1, layer=0, poison=False))
     run_and_check(nv, Cache([6000, 2500, 900], [5, 1, 8], 14, 2, 32, "e4m3", "f16", layers=1, layer=0, poison=False))
     run_and_check(nv, Cache([300, 20], [12, 9], 8, 2, 16, "i8", "f16", scale_spread=3.0))
+
+
+@pytest.mark.parametrize("fmt", ["i8", "e4m3"])
+@pytest.mark.parametrize("past,new,heads,kv_heads", [(40, 12, 4, 2), (0, 90, 14, 2)])
+def test_what_a_later_token_holds_touches_no_earlier_one(nv, fmt, past, new, heads, kv_heads):
+    """NaN and infinities in the keys and values of a chunk's last tokens: the queries before them see nothing of it."""
+    case = Cache([past], [new], heads, kv_heads, 16, fmt, "bf16", layers=1, layer=0)
+    n = new - 4
+    first = Cache([past], [new], heads, kv_heads, 16, fmt, "bf16", layers=1, layer=0)
+    first.new, first.start = [n], [0, n]
+    first.q, first.k, first.v = case.q[:n].clone(), case.k[:n].clone(), case.v[:n].clone()
+    case.v[n, :, 3], case.k[n + 1, 0, 5], case.v[n + 2, -1, 70], case.k[n + 3] = math.nan, math.nan, math.inf, -math.inf
+    d = case.device(nv)
+    call(nv, d, "append_attn")
+    torch.cuda.synchronize()
+    first.append()
+    o, a, spread, floor = first.attend()
+    off = (d["out"][:n].cpu().double() - o).abs()
+    assert bool((off <= attention_bound(first, o, a, spread, floor, False)).all())
+
+
+def test_chunk_many_sessions(nv):
+    """More sessions than a launch's plan holds (512), and than the row starts kept by the writing kernel (256)."""
+    g = torch.Generator().manual_seed(9)
+    past = torch.randint(0, 70, (610,), generator=g).tolist()
+    new = torch.randint(0, 4, (610,), generator=g).tolist()
+    run_and_check(nv, Cache(past, new, 4, 2, 16, "e4m3", "bf16", layers=1, layer=0))
+    run_and_check(nv, Cache(past, [2] * 610, 4, 2, 8, "i8", "f32", layers=1, layer=0, uniform=True), extra_rows=0)
+
+
+@pytest.mark.parametrize("kv_heads,tokens,io", [(16, [7, 5000, 0, 6001], "bf16"), (5, [40000, 1, 9001], "f16"), (5, [45501], "f32")])
+def test_many_rows_are_written_in_several_turns(nv, kv_heads, tokens, io):
+    """So many rows that a CTA takes several turns of 64 (a token's rows begin anywhere in one)."""
+    case = Cache([0] * len(tokens), tokens, kv_heads, kv_heads, 16, "i8", io, layers=1, layer=0, seed=kv_heads)
+    d = case.device(nv)
+    call(nv, d, "append")
+    call(nv, d, "read")
+    torch.cuda.synchronize()
+    assert int(d["status"]) == 0
+    pos = case.positions()
+    rows = (rotate(case.k, pos, case.cs, case.sn, case.rope), case.v.float())
+    table = torch.cat([case.tables[int(case.slices[s])].long()[torch.arange(n) // 16] for s, n in enumerate(tokens)])
+    for i in (0, 1):
+        c, sc = quantise(rows[i], "i8")
+        codes, scales = d["codes"][i].cpu()[0, table, pos % 16], d["scales"][i].cpu()[0, table, :, pos % 16]
+        assert same_bits(codes, c.view(torch.uint8)) and same_bits(scales, sc)
+        assert same_bits(d["back"][i], (c.float() * sc[..., None]).to(IO[io]))
 
 
 def test_attention_of_written_keys(nv):

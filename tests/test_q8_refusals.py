@@ -36,6 +36,14 @@ def test_bad_descriptors(nv, where, field, value, code):
     assert L.nova_launch_q8_append_attn(cache, rows, p, p, p, p, 0, p, 1 << 40, None) == want
 
 
+def test_values_of_codes(nv):
+    import numpy as np
+    import torch
+    c = torch.arange(256, dtype=torch.int32).to(torch.uint8)
+    assert np.array_equal(nv.q8_values(c.numpy(), nv.KV_E4M3), c.view(torch.float8_e4m3fn).float().numpy(), equal_nan=True)
+    assert np.array_equal(nv.q8_values(c.numpy(), nv.KV_I8), c.view(torch.int8).float().numpy())
+
+
 def test_bad_pointers_and_sizes(nv):
     cache, rows, p, keep = parts(nv)
     L, bad = nv.lib, nv.ERR_INVALID
