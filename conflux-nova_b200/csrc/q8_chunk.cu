@@ -17,7 +17,7 @@
 //     from shared memory, which took 1500 cycles of a 64-key tile.  So |K| saturates at 2^20 and |V| at 65504 here.
 //     A lane's rows are chosen so that neither the reads (rows r and r ^ 5 side by side) nor the writes meet in a bank.
 //   * q (rotated) and P are rounded to fp16; everything else is fp32.
-//   * Measured (graph replay, append included): 2048 tokens over 16384, 28 / 4 heads: 860 us = 850 TFLOP/s; 8 x (301-512) tokens over
+//   * Measured (graph replay, append included): 2048 tokens over 16384, 40 / 8 heads: 860 us = 850 TFLOP/s; 8 x (301-512) tokens over
 //     2k-8k: 340 us = 750 TFLOP/s; 16 x (0-8) tokens over 2k-8k: 51 us = 1.5 TB/s; a window of 512: 52 us.  A 64-key tile of 256 rows
 //     takes 2350 cycles.  The tensor cores are busy for 1020 of them, the special-function units for 1024; what sets the pace is
 //     the softmax warps' own chain of some 300 dependent instructions per tile (two warps per scheduler; without the exponentials
@@ -804,7 +804,8 @@ q8_chunk_kernel(Q8Launch a, ChunkShape sh) {
                 fetch(c_i + 16);
             }
             if (!waited) {
-                pdl_wait();                                // the append before us has written the new rows
+                pdl_wait();                                // the append before us has written the new rows (older keys too: another
+                                                           // session of the call may have written them; not waiting gained nothing)
                 waited = true;
             }
             const int key = c_key + c_i * 2 * kKeys;
