@@ -368,7 +368,9 @@ int nova_launch_q8_read(const nova_q8_cache* c, const nova_q8_rows* r, void* k_o
 size_t nova_q8_workspace_bytes(const nova_kv_shape* sh, const nova_q8_rows* r);
 int nova_launch_q8_attn(const nova_q8_cache* c, const nova_q8_rows* r, const void* q, void* out, int window, void* work,
                         size_t work_bytes, nova_stream_t s);
-/* nova_launch_q8_append followed by nova_launch_q8_attn: one decode step, or one chunk of a prompt, of a layer. */
+/* nova_launch_q8_append followed by nova_launch_q8_attn: one decode step, or one chunk of a prompt, of a layer.  The sessions of a
+ * call may share pages of old keys, but none may see a row that another one writes in the same call (single tokens are written
+ * while others are read); two sets of rows of one sequence go in as one session, or as two calls. */
 int nova_launch_q8_append_attn(const nova_q8_cache* c, const nova_q8_rows* r, const void* q, const void* k, const void* v, void* out,
                                int window, void* work, size_t work_bytes, nova_stream_t s);
 
