@@ -184,15 +184,27 @@ __device__ __forceinline__ void store8(__nv_bfloat16* p, const float (&v)[8]) {
 }
 
 // ---- codes: four of them in a word
-template <int kFmt> __device__ __forceinline__ float4 q8_decode4(uint32_t w) {
+// Four codes of a word -> two pairs of fp16, exactly.
+template <int kFmt> __device__ __forceinline__ void q8_to_h2(uint32_t w, uint32_t& h0, uint32_t& h1) {
     if constexpr (kFmt == NOVA_KV_I8) {
-        return make_float4((float)(int8_t)(w & 0xff), (float)(int8_t)((w >> 8) & 0xff), (float)(int8_t)((w >> 16) & 0xff), (float)(int8_t)(w >> 24));
+        // 0x6400 | (code + 128) is the fp16 number 1024 + 128 + code
+        const uint32_t u = w ^ 0x80808080u;
+        const uint32_t a = __byte_perm(u, 0x64646464u, 0x4140), b = __byte_perm(u, 0x64646464u, 0x4342);
+        const __half2 k = __halves2half2(__ushort_as_half(0x6480), __ushort_as_half(0x6480));      // 1152
+        const __half2 x = __hsub2(*reinterpret_cast<const __half2*>(&a), k), y = __hsub2(*reinterpret_cast<const __half2*>(&b), k);
+        h0 = *reinterpret_cast<const uint32_t*>(&x);
+        h1 = *reinterpret_cast<const uint32_t*>(&y);
     } else {
-        uint32_t h0, h1;
         asm("{ .reg .b16 l, h; mov.b32 {l, h}, %2; cvt.rn.f16x2.e4m3x2 %0, l; cvt.rn.f16x2.e4m3x2 %1, h; }" : "=r"(h0), "=r"(h1) : "r"(w));
-        const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&h0)), b = __half22float2(*reinterpret_cast<const __half2*>(&h1));
-        return make_float4(a.x, a.y, b.x, b.y);
     }
+}
+
+// The same in fp32 (through fp16: a conversion of an integer takes the special-function units, a quarter of the rate).
+template <int kFmt> __device__ __forceinline__ float4 q8_decode4(uint32_t w) {
+    uint32_t h0, h1;
+    q8_to_h2<kFmt>(w, h0, h1);
+    const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&h0)), b = __half22float2(*reinterpret_cast<const __half2*>(&h1));
+    return make_float4(a.x, a.y, b.x, b.y);
 }
 // Round to nearest, ties to even, in both formats.  |x| <= Q but for the rounding of the product; a NaN becomes code 0
 // (int8) or NaN (e4m3).
@@ -251,22 +263,7 @@ __device__ __forceinline__ float rcp(float x) {
     return y;
 }
 
-// Four codes of a word -> two pairs of fp16, exactly.
-template <int kFmt> __device__ __forceinline__ void q8_to_h2(uint32_t w, uint32_t& h0, uint32_t& h1) {
-    if constexpr (kFmt == NOVA_KV_I8) {
-        // 0x6400 | (code + 128) is the fp16 number 1024 + 128 + code
-        const uint32_t u = w ^ 0x80808080u;
-        const uint32_t a = __byte_perm(u, 0x64646464u, 0x4140), b = __byte_perm(u, 0x64646464u, 0x4342);
-        const __half2 k = __halves2half2(__ushort_as_half(0x6480), __ushort_as_half(0x6480));      // 1152
-        const __half2 x = __hsub2(*reinterpret_cast<const __half2*>(&a), k), y = __hsub2(*reinterpret_cast<const __half2*>(&b), k);
-        h0 = *reinterpret_cast<const uint32_t*>(&x);
-        h1 = *reinterpret_cast<const uint32_t*>(&y);
-    } else {
-        asm("{ .reg .b16 l, h; mov.b32 {l, h}, %2; cvt.rn.f16x2.e4m3x2 %0, l; cvt.rn.f16x2.e4m3x2 %1, h; }" : "=r"(h0), "=r"(h1) : "r"(w));
-    }
-}
-
-// The same for K: int8 codes as (code + 128) 2^-24, an fp16 subnormal whose bits are the byte.
+// q8_to_h2 for K: int8 codes as (code + 128) 2^-24, an fp16 subnormal whose bits are the byte.
 template <int kFmt> __device__ __forceinline__ void q8_k_to_h2(uint32_t w, uint32_t& h0, uint32_t& h1) {
     if constexpr (kFmt == NOVA_KV_I8) {
         const uint32_t u = w ^ 0x80808080u;
