@@ -30,6 +30,10 @@ namespace novab {
 namespace {
 
 constexpr int kThreads = 640, kMergeThreads = 128;
+// Registers a thread: at launch, and of the softmax, issuing and converting warps (120 / 64 / 88: 918 us for 2048 tokens over 16384,
+// 128 / 64 / 80: 880, 136 / 48 / 80: 873, 144 / 48 / 72: the same).
+constexpr int kRegsLaunch = 96, kRegsSoft = 136, kRegsIssue = 48, kRegsConv = 80;
+static_assert(256 * kRegsSoft + 128 * kRegsIssue + 256 * kRegsConv <= kThreads * kRegsLaunch, "registers of the roles");
 constexpr int kConv = 8;                              // converting warps
 constexpr int kKeys = 64;                             // keys of a tile
 constexpr int kHalfRows = 128;                        // rows of a half = M of the MMAs
@@ -348,7 +352,7 @@ q8_chunk_kernel(Q8Launch a, ChunkShape sh) {
 
     if (warp < 8) {
         // ---------------------------------------------------------------------------------------- softmax: thread = one row
-        regs_up<136>();
+        regs_up<kRegsSoft>();
         const int half = warp >> 2, hrow = (int)threadIdx.x & (kHalfRows - 1);
         const uint32_t t_lane = tmem + ((uint32_t)(32 * (warp & 3)) << 16);
         const uint32_t col_s = 128u * (uint32_t)half, col_o = kColO + 128u * (uint32_t)half;
@@ -646,7 +650,7 @@ q8_chunk_kernel(Q8Launch a, ChunkShape sh) {
             tc_fence_before();
         }
     } else if (warp < 12) {
-        regs_down<48>();
+        regs_down<kRegsIssue>();
         if (warp < 10) {
             // ------------------------------------------------------------------------------------ MMA issue: one warp per half
             const int h = warp - 8;
@@ -748,7 +752,7 @@ q8_chunk_kernel(Q8Launch a, ChunkShape sh) {
         // kRaw tiles ahead, with 16-byte asynchronous copies into a ring of its own, which needs no barrier.  (As TMA boxes the rows of one
         // head are 2 KiB a copy, too little: one warp issuing all of a tile's copies took 1900 cycles a tile, eight warps with a box
         // and a run of scales each 900.  16 keys of every tile a warp: 1500 cycles a tile, most of it latency.)
-        regs_down<80>();
+        regs_down<kRegsConv>();
         const int me = warp - 12, which = me >> 2, par = me >> 1 & 1, hw = me & 1;
         const bool p8 = a.kv_shift == 3;
         const unsigned char* const pool = static_cast<const unsigned char*>(which ? a.pool_v : a.pool_k);
@@ -981,7 +985,7 @@ __global__ void __launch_bounds__(kMergeThreads, 4) q8_chunk_merge_kernel(Q8Laun
 
 template <int kFmt, typename T>
 cudaError_t launch_chunk_as(const Q8Launch& a, const ChunkShape& sh, int ctas, cudaStream_t s) {
-    const cudaError_t e = q8_allow_smem<q8_chunk_kernel<kFmt, T>>(kSmem);
+    const cudaError_t e = q8_allow_smem<q8_chunk_kernel<kFmt, T>>(kSmem, kRegsLaunch);
     return e != cudaSuccess ? e : launch_kernel_pdl(q8_chunk_kernel<kFmt, T>, dim3((unsigned)ctas), dim3(kThreads), (size_t)kSmem, s, true, a, sh);
 }
 template <int kFmt>

@@ -301,15 +301,22 @@ __device__ __forceinline__ uint32_t movmatrix(uint32_t x) {
 
 #endif  // __CUDACC__
 
-// Lets a kernel have `bytes` of dynamic shared memory on the current device; asked of the driver once per kernel and device.
+// Lets a kernel have `bytes` of dynamic shared memory on the current device, and sees that it is launched with the `regs` registers a
+// thread that its roles share out (with fewer they would wait for good); asked of the driver once per kernel and device.
 template <auto kKernel>
-inline cudaError_t q8_allow_smem(int bytes) {
+inline cudaError_t q8_allow_smem(int bytes, int regs = 0) {
     static std::atomic<uint64_t> done{0};
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return e;
     const uint64_t bit = dev < 64 ? 1ull << dev : 0ull;
     if (bit & done.load(std::memory_order_relaxed)) return cudaSuccess;
+    if (regs > 0) {
+        cudaFuncAttributes at;
+        e = cudaFuncGetAttributes(&at, kKernel);
+        if (e != cudaSuccess) return e;
+        if (at.numRegs < regs) return cudaErrorInvalidConfiguration;
+    }
     e = cudaFuncSetAttribute(kKernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
     if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_relaxed);
     return e;
