@@ -11,10 +11,10 @@
 //   * Twenty warps: 8 softmax (thread = row), 2 issuing MMAs (one per half), 8 converting, each of which brings in its own keys'
 //     codes and scales, one that walks the line (and one idle).  The pipe runs on from one unit to the next.
 //   * The tensor cores want fp16 operands, so a tile's codes become fp16 VALUES in shared memory, code times scale, in the
-//     128-byte-swizzle layout that is the K-major form for S = Q.K^T and the MN-major form for O += P.V.  A scale (K's over 16;
-//     q is multiplied by 16 / sqrt(128) log2 e) goes in as two fp16 parts and the product is rounded once (2^-11).
+//     128-byte-swizzle layout that is the K-major form for S = Q.K^T and the MN-major form for O += P.V.  A scale (K's over 2;
+//     q is multiplied by 2 / sqrt(128) log2 e) goes in as two fp16 parts and the product is rounded once (2^-11).
 //     With exact codes as operands and the scales in the softmax instead, every thread had to read three floats per key
-//     from shared memory, which took 1500 cycles of a 64-key tile.  So |K| saturates at 2^20 and |V| at 65504 here.
+//     from shared memory, which took 1500 cycles of a 64-key tile.  So |K| saturates at 2^17 and |V| at 65504 here.
 //     A lane's rows are chosen so that neither the reads (rows r and r ^ 5 side by side) nor the writes meet in a bank.
 //   * q (rotated) and P are rounded to fp16; everything else is fp32.
 //   * Measured (graph replay, append included): 2048 tokens over 16384, 40 / 8 heads: 860 us = 850 TFLOP/s; 8 x (301-512) tokens over
@@ -58,7 +58,8 @@ constexpr int kSmem = kOffBar + 768;
 static_assert(kSmem <= 232448, "shared memory of one CTA");
 constexpr int kTmemCols = 512;                        // S of half h, buffer b: columns 128 h + 64 b (P over its first 32); O: 256 + 128 h
 constexpr uint32_t kColO = 256;
-constexpr float kKDiv = 16.f;                         // K goes in divided by this: magnitudes up to 2^20
+constexpr float kKDiv = 2.f;                          // K goes in divided by this: magnitudes up to 2^17 (rotated fp16 keys fit), and q, multiplied
+                                                      // by 0.255, the same
 // As kQ8Step and kQ8Top (single tokens), but the reference moves less often, which costs more here (O rescaled in tensor
 // memory): weights are 2^7 .. 2^15 at the largest, with fp16's 11 bits down to 2^-21 of the reference.
 constexpr float kStep = 8.f, kTop = 7.f;
