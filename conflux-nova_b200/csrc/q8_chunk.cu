@@ -12,7 +12,8 @@
 //     codes and scales, one that walks the line (and one idle).  The pipe runs on from one unit to the next.
 //   * The tensor cores want fp16 operands, so a tile's codes become fp16 VALUES in shared memory, code times scale, in the
 //     128-byte-swizzle layout that is the K-major form for S = Q.K^T and the MN-major form for O += P.V.  A scale (K's over 2;
-//     q is multiplied by 2 / sqrt(128) log2 e) goes in as two fp16 parts and the product is rounded once (2^-11).
+//     q is multiplied by 2 / sqrt(128) log2 e) goes in as two fp16 parts, 64 or 256 times as large and the codes as much
+//     smaller, and the product is rounded once: 2^-11; where fp16 has no more bits to give (its grid ends at 2^-24) 2^-23, of K 2^-22.
 //     With exact codes as operands and the scales in the softmax instead, every thread had to read three floats per key
 //     from shared memory, which took 1500 cycles of a 64-key tile.  So |K| saturates at 2^17 and |V| at 65504 here.
 //     A lane's rows are chosen so that neither the reads (rows r and r ^ 5 side by side) nor the writes meet in a bank.
@@ -846,7 +847,7 @@ q8_chunk_kernel(Q8Launch a, ChunkShape sh) {
         const int r8 = (lane >> 3) ^ (5 * (lane >> 2 & 1)), c4 = lane & 3;
         const uint32_t bar_full = (which ? bar_vfull : bar_kfull) + 8u * (uint32_t)par, bar_free = (which ? bar_vfree : bar_kfree) + 8u * (uint32_t)par;
         const uint32_t dst0 = base + (which ? kOffV : kOffK) + (uint32_t)par * (2 * kSlab) + (uint32_t)(32 * hw + r8) * 128u;
-        const float div = which ? 1.f : 1.f / kKDiv;
+        const float mul = kQ8CodeDiv<kFmt> * (which ? 1.f : 1.f / kKDiv);
         for (int k = 0; k < kRaw; ++k) {
             issue_next();
             asm volatile("cp.async.commit_group;" ::: "memory");
@@ -876,16 +877,16 @@ q8_chunk_kernel(Q8Launch a, ChunkShape sh) {
                 }
 #pragma unroll
                 for (int e2 = 0; e2 < 2; ++e2) {
-                    const float fs = fminf(f[e2] * div, 65504.f / q8_qmax<kFmt>());
+                    const float fs = fminf(f[e2] * mul, 65504.f * kQ8CodeDiv<kFmt> / q8_qmax<kFmt>());
                     const __half hi1 = __float2half_rn(fs);
                     const __half2 hi2 = __half2half2(hi1), lo2 = __half2half2(__float2half_rn(fs - __half2float(hi1)));
 #pragma unroll
                     for (int e = 2 * e2; e < 2 * e2 + 2; ++e) {
                         uint32_t h[8];
-                        q8_to_h2<kFmt>(code[e].x, h[0], h[1]);
-                        q8_to_h2<kFmt>(code[e].y, h[2], h[3]);
-                        q8_to_h2<kFmt>(code[e].z, h[4], h[5]);
-                        q8_to_h2<kFmt>(code[e].w, h[6], h[7]);
+                        q8_to_small_h2<kFmt>(code[e].x, h[0], h[1]);
+                        q8_to_small_h2<kFmt>(code[e].y, h[2], h[3]);
+                        q8_to_small_h2<kFmt>(code[e].z, h[4], h[5]);
+                        q8_to_small_h2<kFmt>(code[e].w, h[6], h[7]);
 #pragma unroll
                         for (int b = 0; b < 8; ++b) {
                             const __half2 x = *reinterpret_cast<const __half2*>(&h[b]);
