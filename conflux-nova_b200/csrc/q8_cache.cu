@@ -180,18 +180,16 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 ? 2 : 3) q8_append_kernel(
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
             const bool is_q = unit[i] >= 2 * NKV, is_v = !is_q && unit[i] >= NKV;
-            if (a.rope_cs && p[i].pos >= 0 && !is_v) {
-                if (p[i].pos >= a.rope_rows) {
-                    p[i].row = -1;
-                    if (c == 0) q8_flag(a, NOVA_ERR_INVALID);
-                } else {
-                    rotate16(x0[i], x1[i], p[i].pos, c, a);
-                    float* const back = is_q ? a.q_rot + ((int64_t)tok[i] * a.n_heads + unit[i] - 2 * NKV) * kHeadDim
-                                             : a.k_rot ? a.k_rot + ((int64_t)tok[i] * NKV + unit[i]) * kHeadDim : nullptr;
-                    if (back) {
-                        store8(back + 8 * c, x0[i]);
-                        store8(back + 64 + 8 * c, x1[i]);
-                    }
+            if (a.rope_cs && p[i].pos >= a.rope_rows) {              // (V's row too: the token is not written)
+                p[i].row = -1;
+                if (c == 0) q8_flag(a, NOVA_ERR_INVALID);
+            } else if (a.rope_cs && p[i].pos >= 0 && !is_v) {
+                rotate16(x0[i], x1[i], p[i].pos, c, a);
+                float* const back = is_q ? a.q_rot + ((int64_t)tok[i] * a.n_heads + unit[i] - 2 * NKV) * kHeadDim
+                                         : a.k_rot ? a.k_rot + ((int64_t)tok[i] * NKV + unit[i]) * kHeadDim : nullptr;
+                if (back) {
+                    store8(back + 8 * c, x0[i]);
+                    store8(back + 64 + 8 * c, x1[i]);
                 }
             }
             if (is_q) p[i].row = -1;

@@ -1,0 +1,49 @@
+"""The 8-bit cache operators at the limits of what they are given: positions behind the rotary tables or the block tables, row starts that
+are no row starts, pages that nobody needs any more.  What is skipped is left as it was, what is not is right."""
+import pytest
+import torch
+
+from q8_plain import Cache, attention_bound, call
+
+pytestmark = pytest.mark.gpu
+
+
+def bits(x):
+    return x.cpu().contiguous().view(torch.uint8)
+
+
+def check_rows(case, got, done):
+    """The rows of `done` against the plain form, all others as they were (7)."""
+    o, a, spread, floor = case.attend()
+    exact_q = case.io != "bf16" and max(case.new) == 1 and case.H // case.N <= 8
+    off, bound = (got.double() - o).abs(), attention_bound(case, o, a, spread, floor, exact_q)
+    assert bool((off <= bound)[done].all())
+    assert bool((got[~done] == 7).all()), "rows that are skipped"
+
+
+@pytest.mark.parametrize("fmt,io", [("i8", "f32"), ("e4m3", "bf16")])
+@pytest.mark.parametrize("past,new,heads,kv_heads,page,limit", [
+    ([40, 60], [1, 1], 4, 2, 16, 50), ([40, 60, 3], [1, 1, 1], 32, 2, 8, 41), ([40, 0, 5], [30, 100, 3], 4, 2, 16, 60),
+    ([64, 70], [2, 90], 14, 2, 64, 64), ([3000, 10, 3019], [40, 5, 2], 7, 1, 16, 3020)])
+def test_positions_behind_the_rotary_tables_are_skipped(nv, past, new, heads, kv_heads, page, limit, fmt, io):
+    """Neither keys nor values are written there, no output either; the rows before them and the other sessions are not touched by it."""
+    for what in ("append_attn", "append"):
+        case = Cache(past, new, heads, kv_heads, page, fmt, io, layers=1, layer=0, poison=False)
+        d = case.device(nv)
+        d["cache"].rope_rows = limit
+        before = [x.clone() for x in case.codes + case.scales]
+        case.append()
+        for x, old in zip(case.codes + case.scales, before):
+            for s, (p, n) in enumerate(zip(past, new)):
+                for t in range(n):
+                    if p + t >= limit:
+                        ph, slot = case.place(s, p + t)
+                        where = (0, ph, slot) if x.dtype == torch.uint8 else (0, ph, slice(None), slot)
+                        x[where] = old[where]
+        call(nv, d, what)
+        torch.cuda.synchronize()
+        assert int(d["status"]) == nv.ERR_INVALID
+        for x, y in zip(d["codes"] + d["scales"], case.codes + case.scales):
+            assert bool((bits(x) == bits(y)).all())
+        if what == "append_attn":
+            check_rows(case, d["out"].cpu(), case.positions() < limit)
