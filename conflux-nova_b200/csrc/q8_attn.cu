@@ -63,6 +63,12 @@ struct DecPlan {
 
 __device__ __forceinline__ int dec_first_tile(const Q8Launch& a, int keys) { return a.window > 0 && keys > a.window ? (keys - a.window) >> 4 : 0; }
 
+// Tiles of a row: keys behind the block table are not looked for, but there is always one tile.
+__device__ __forceinline__ int dec_tiles(const Q8Launch& a, int keys) {
+    const int end = keys < a.keys_cap ? keys : a.keys_cap;
+    return max(((end + 15) >> 4) - dec_first_tile(a, keys), 1);
+}
+
 __device__ __forceinline__ int dec_setup(int row) { return row > 0 ? kSetupTiles : 0; }
 
 __device__ inline void dec_build_plan(const Q8Launch& a, DecPlan& p, int n_groups, bool flag) {
@@ -72,10 +78,11 @@ __device__ inline void dec_build_plan(const Q8Launch& a, DecPlan& p, int n_group
         const int pos = __ldg(a.n_past + s), slice = a.slice_ids ? __ldg(a.slice_ids + s) : s;
         int keys = 0;
         if (count > 0) {
-            if (pos < 0 || pos == 0x7fffffff || (a.rope_cs && pos >= a.rope_rows)) {
+            if (pos < 0 || pos >= kQ8MaxPos || (a.rope_cs && pos >= a.rope_rows)) {
                 if (flag) q8_flag(a, NOVA_ERR_INVALID);
             } else {
                 keys = pos + 1;
+                if (flag && keys > a.keys_cap) q8_flag(a, NOVA_ERR_BAD_TABLE);
             }
         }
         p.keys[s] = keys;
@@ -89,7 +96,7 @@ __device__ inline void dec_build_plan(const Q8Launch& a, DecPlan& p, int n_group
         if (lane == 0) p.prefix[0] = 0;
         for (int base = 0; base < rows; base += 32) {
             const int r = base + lane, keys = r < rows ? p.keys[r / n_groups] : 0;
-            uint32_t v = keys > 0 ? (uint32_t)(((keys + 15) >> 4) - dec_first_tile(a, keys) + dec_setup(r)) : 0u;
+            uint32_t v = keys > 0 ? (uint32_t)(dec_tiles(a, keys) + dec_setup(r)) : 0u;
             v = min(v, 0x7ffffffu);                            // (the sum of 32 stays inside 32 bits)
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
@@ -796,8 +803,10 @@ size_t q8_work_bytes(int n_heads, int n_kv_heads, int n_sessions, int, int max_t
     return (size_t)((rows < kDecRows ? rows : kDecRows) + kQ8MaxCtas) * (size_t)(kvg * (n_heads / n_kv_heads)) * kSlotW * sizeof(float);
 }
 
-int launch_q8_attn(const Q8Launch& a, cudaStream_t s) {
-    if (a.n_tokens <= 0 || a.n_sessions <= 0) return NOVA_OK;
+int launch_q8_attn(const Q8Launch& call, cudaStream_t s) {
+    if (call.n_tokens <= 0 || call.n_sessions <= 0) return NOVA_OK;
+    Q8Launch a = call;
+    a.keys_cap = (int)(a.table_stride > (kQ8MaxPos >> a.kv_shift) ? kQ8MaxPos : a.table_stride << a.kv_shift);
     if (q8_is_decode(a.n_heads, a.n_kv_heads, a.max_tokens)) {
         const int kvg = dec_group(a.n_kv_heads), groups = a.n_kv_heads / kvg;
         if (groups > kDecRows) return NOVA_ERR_TOO_LARGE;

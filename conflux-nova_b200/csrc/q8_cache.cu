@@ -63,7 +63,7 @@ __device__ __forceinline__ void q8_places(const Q8Launch& a, PlaceSmem& sm, int6
         if (s >= 0) {
             const int64_t pos = (int64_t)__ldg(a.n_past + s) + t;
             const int32_t* const table = q8_table(a, s);
-            if (pos < 0 || pos > 0x7fffffff) {
+            if (pos < 0 || pos >= kQ8MaxPos) {
                 q8_flag(a, NOVA_ERR_INVALID);
             } else {
                 p.pos = (int)pos;

@@ -84,7 +84,8 @@ __device__ __forceinline__ int unit_first16(const Q8Launch& a, int past, int t0)
 }
 __device__ __forceinline__ int unit_tiles(const Q8Launch& a, int tq, int past, int count, int qt) {
     const int t1 = (qt + 1) * tq < count ? (qt + 1) * tq : count;
-    return (((past + t1 + 15) >> 4) - unit_first16(a, past, qt * tq) + 3) >> 2;
+    const int end = past + t1 < a.keys_cap ? past + t1 : a.keys_cap;          // (keys behind the block table are not looked for)
+    return max((((end + 15) >> 4) - unit_first16(a, past, qt * tq) + 3) >> 2, 1);
 }
 
 // All threads of the CTA; ends with __syncthreads().
@@ -94,10 +95,11 @@ __device__ inline void build_plan(const Q8Launch& a, const ChunkShape& sh, Chunk
         int first, count;
         q8_rows(a, s, first, count);
         const int past = __ldg(a.n_past + s);
-        if (count > 0 && (past < 0 || past > 0x7ff00000 - count)) {
+        if (count > 0 && (past < 0 || past > kQ8MaxPos - count)) {
             if (flag) q8_flag(a, NOVA_ERR_INVALID);
             count = 0;
         }
+        if (flag && count > 0 && past + count > a.keys_cap) q8_flag(a, NOVA_ERR_BAD_TABLE);
         long long len = 0;
         if (count <= kFewTiles * sh.tq)
             for (int qt = 0; qt * sh.tq < count; ++qt) len += unit_tiles(a, sh.tq, past, count, qt) + kSetup;

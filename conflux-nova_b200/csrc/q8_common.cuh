@@ -25,6 +25,7 @@ constexpr float kQ8MinScale = 8.4703294725430034e-22f;     // 2^-70
 // keeps fp16's 11 bits down to 2^-25 of the reference (below: steps of 2^-35 of it).
 constexpr float kQ8Step = 4.f, kQ8Top = 11.f;
 
+constexpr int kQ8MaxPos = 0x7ff00000;      // the largest position: what is added to one stays inside 32 bits
 constexpr int kQ8MaxCtas = 160;      // CTAs of an attention launch, one per SM (sizes the workspaces)
 
 struct Q8Launch {
@@ -56,6 +57,7 @@ struct Q8Launch {
     int32_t io, fmt, neox;
     int32_t layer, nb, n_heads, n_kv_heads, kv_shift;
     int32_t window;
+    int32_t keys_cap;             // attention: keys that a block table has entries for (none behind them is looked for)
     int32_t append;               // attention: write the (single) new token of every session on the way
 };
 

@@ -323,7 +323,8 @@ int nova_launch_attn_decode_paged_static(const nova_kv_shape* sh, const float* q
  * uses table slice_ids[s] (slice_ids NULL: table s).  An entry outside [0, nb) is never followed: its keys are skipped, its
  * rows are neither written nor read back, and *status (device, may be NULL) becomes NOVA_ERR_BAD_TABLE.
  * rope_cs / rope_sn [rope_rows][64] (both NULL: no rotation): k is rotated at its position before it is quantised, q when it
- * is read; neither buffer is changed.  A position beyond the tables is skipped and flagged (NOVA_ERR_INVALID).
+ * is read; neither buffer is changed.  A position beyond the tables is skipped and flagged (NOVA_ERR_INVALID), as is one below 0 or from
+ * 2^31 - 2^20 on; one that the block table has no entry for counts as an entry outside [0, nb).
  * All pointers 16-byte aligned (tables, positions and status: 4).  All calls act on the calling thread's current device,
  * are asynchronous, keep nothing from one call to the next, allocate nothing, and may be captured into a graph. */
 typedef struct {

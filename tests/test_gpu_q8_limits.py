@@ -47,3 +47,47 @@ def test_positions_behind_the_rotary_tables_are_skipped(nv, past, new, heads, kv
             assert bool((bits(x) == bits(y)).all())
         if what == "append_attn":
             check_rows(case, d["out"].cpu(), case.positions() < limit)
+
+
+@pytest.mark.parametrize("page", [8, 16, 64])
+@pytest.mark.parametrize("window", [0, 50])
+@pytest.mark.parametrize("far", [200, 2 ** 31 - 17, 2 ** 31 - 9, 0x7ff00000 - 70, 0x7ff00000 - 3, 0x7ff00000, 2 ** 31 - 1, -1, -2 ** 31])
+def test_positions_behind_the_block_table(nv, far, window, page):
+    """A query whose position has no table entry sees the keys that have one (none: zeros), its own is not written, the status says so; a
+    position that is none, or within 2^20 of 2^31, is skipped.  Nothing is walked that is not there: the call takes no longer."""
+    for new in ([1, 1, 1], [1, 5, 3]):
+        case = Cache([64, 30, 64], new, 6, 2, page, "i8", "bf16", rope="none", layers=1, layer=0, poison=False, seed=page)
+        width = 128 // page
+        case.tables = case.tables[:, :width].contiguous() if case.tables.shape[1] >= width else torch.nn.functional.pad(
+            case.tables, (0, width - case.tables.shape[1]), value=-1)
+        d = case.device(nv)
+        d["past"][0] = far
+        before = [x.clone() for x in case.codes + case.scales]
+        case.append()
+        ph, slot = case.place(0, 64)
+        for x, old in zip(case.codes + case.scales, before):
+            where = (0, ph, slot) if x.dtype == torch.uint8 else (0, ph, slice(None), slot)
+            x[where] = old[where]
+        call(nv, d, "append_attn", window)
+        torch.cuda.synchronize()
+        skipped = far < 0 or far >= 0x7ff00000
+        assert int(d["status"]) == (nv.ERR_INVALID if skipped else nv.ERR_BAD_TABLE)
+        for x, y in zip(d["codes"] + d["scales"], case.codes + case.scales):
+            assert bool((bits(x) == bits(y)).all())
+        got = d["out"].cpu()
+        if skipped:
+            assert bool((got[0] == 7).all())
+        elif window:
+            assert bool((got[0] == 0).all())
+        else:
+            k, v = (case.values(i, 0, 0, page * ((64 + page) // page))[0] for i in (0, 1))
+            for h in range(6):       # q, k, weights and v are rounded to fp16, the output to bf16 (attention_bound has the whole account)
+                q, kh, vh = case.q[0, h].double(), k[:, h // 3], v[:, h // 3]
+                w = torch.softmax((kh @ q) * 128 ** -0.5, -1)
+                e = float((kh.abs() @ q.abs()).max()) * 128 ** -0.5 * (2 * 2.0 ** -11 + 2.0 ** -18)
+                bound = (w @ vh.abs()) * (2 * (e * (1 + e) + 3 * 2.0 ** -11)) + (w @ vh).abs() * 2.0 ** -8
+                assert bool(((got[0, h].double() - w @ vh).abs() <= bound).all())
+        case.window = window
+        o, a, spread, floor = case.attend()
+        off, bound = (got.double() - o).abs(), attention_bound(case, o, a, spread, floor, False)
+        assert bool((off <= bound)[1:].all())
