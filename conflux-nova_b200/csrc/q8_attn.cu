@@ -61,7 +61,8 @@ struct DecPlan {
     int slice[kDecRows];
 };
 
-__device__ __forceinline__ int dec_first_tile(const Q8Launch& a, int keys) { return a.window > 0 && keys > a.window ? (keys - a.window) >> 4 : 0; }
+__device__ __forceinline__ int dec_low(const Q8Launch& a, int keys) { return a.window > 0 && keys > a.window ? keys - a.window : 0; }      // first key that is seen
+__device__ __forceinline__ int dec_first_tile(const Q8Launch& a, int keys) { return dec_low(a, keys) >> 4; }
 
 // Tiles of a row: keys behind the block table are not looked for, but there is always one tile.
 __device__ __forceinline__ int dec_tiles(const Q8Launch& a, int keys) {
@@ -210,10 +211,11 @@ q8_decode_kernel(Q8Launch a, const __grid_constant__ CUtensorMap tmk, const __gr
     // Each of the four goes through ALL tiles in order: a stage's fill waits for the release of the fill before, which the same
     // warp has taken part in, so a parity is never taken for the one two fills ago.
     const int tpp = a.kv_shift > 4 ? a.kv_shift - 4 : 0;               // log2(tiles per page)
-    // entries of the block table behind tile i of a segment (the second: 8-token pages); -1: a bad one, -2: nothing to bring
-    auto fetch = [&](const int32_t* table, int keys, int t, bool real, int& e0, int& e1) {
+    // entries of the block table behind tile i of a segment (the second: 8-token pages); -1: a bad one, -2: nothing to bring (no key of
+    // the page is there, or none is in the window: an 8-token page in front of one that is, whose entry may be gone)
+    auto fetch = [&](const int32_t* table, int keys, int low, int t, bool real, int& e0, int& e1) {
         auto entry = [&](int64_t page, int first_key) -> int {
-            if (first_key >= keys) return -2;
+            if (first_key >= keys || (p8 && first_key + 8 <= low)) return -2;
             if (page >= a.table_stride) return -1;
             const int e = __ldg(table + page);
             return e >= 0 && e < a.nb ? e : -1;
@@ -240,10 +242,10 @@ q8_decode_kernel(Q8Launch a, const __grid_constant__ CUtensorMap tmk, const __gr
             const DecSegment sg = dec_segment(s_plan, ln, pos, lo, hi);
             pos += sg.span;
             const int keys = s_plan.keys[sg.session];
-            const int t0 = dec_first_tile(a, keys) + sg.first, low = a.window > 0 && keys > a.window ? keys - a.window : 0;
+            const int t0 = dec_first_tile(a, keys) + sg.first, low = dec_low(a, keys);
             const int32_t* table = a.tables + (int64_t)s_plan.slice[sg.session] * a.table_stride;
             int n0, n1, c0 = 0, c1 = 0;
-            fetch(table, keys, t0 + lane, lane < sg.count, n0, n1);
+            fetch(table, keys, low, t0 + lane, lane < sg.count, n0, n1);
             uint32_t stage = (it0 + (uint32_t)lane) % kStages, round = (it0 + (uint32_t)lane) / kStages;
 #pragma unroll 1
             for (int b = 0; b < sg.count; b += Cfg::kBatch) {
@@ -251,7 +253,7 @@ q8_decode_kernel(Q8Launch a, const __grid_constant__ CUtensorMap tmk, const __gr
                     c0 = n0;
                     c1 = n1;
                     const int nx = b + 32 + lane;
-                    fetch(table, keys, t0 + nx, nx < sg.count, n0, n1);
+                    fetch(table, keys, low, t0 + nx, nx < sg.count, n0, n1);
                 }
                 const int i = b + lane, t = t0 + i;
                 const int e0 = __shfl_sync(0xffffffffu, c0, i & 31);
@@ -307,12 +309,12 @@ q8_decode_kernel(Q8Launch a, const __grid_constant__ CUtensorMap tmk, const __gr
         for (int pos = lo; pos < hi;) {
             const DecSegment sg = dec_segment(s_plan, ln, pos, lo, hi);
             pos += sg.span;
-            const int keys = s_plan.keys[sg.session], t0 = dec_first_tile(a, keys) + sg.first;
+            const int keys = s_plan.keys[sg.session], t0 = dec_first_tile(a, keys) + sg.first, low = dec_low(a, keys);
             const int32_t* table = a.tables + (int64_t)s_plan.slice[sg.session] * a.table_stride;
             const float* const mine0 = (is_v ? a.scale_v : a.scale_k) + ((((int64_t)a.layer * a.nb) * a.n_kv_heads + sg.group * KVG + h) << a.kv_shift);
             const int steps = (sg.count + kPer - 1) / kPer;
             int n0, n1, c0 = 0, c1 = 0;
-            fetch(table, keys, t0 + lane, lane < sg.count, n0, n1);
+            fetch(table, keys, low, t0 + lane, lane < sg.count, n0, n1);
             uint32_t stage = (it0 + (uint32_t)sub_tile) % kStages, round = (it0 + (uint32_t)sub_tile) / kStages;
             int i = sub_tile - kDepth * kPer;                               // the tile that this step converts
 #pragma unroll 1
@@ -323,7 +325,7 @@ q8_decode_kernel(Q8Launch a, const __grid_constant__ CUtensorMap tmk, const __gr
                         c0 = n0;
                         c1 = n1;
                         const int nx = f + 32 + lane;
-                        fetch(table, keys, t0 + nx, nx < sg.count, n0, n1);
+                        fetch(table, keys, low, t0 + nx, nx < sg.count, n0, n1);
                     }
                     int e = __shfl_sync(0xffffffffu, c0, (f + sub_tile) & 31);       // (below 0 behind the segment's last tile too)
                     if (p8) {

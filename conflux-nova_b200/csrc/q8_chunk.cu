@@ -771,9 +771,10 @@ q8_chunk_kernel(Q8Launch a, ChunkShape sh) {
         const uint32_t row_bytes = (uint32_t)a.n_kv_heads * kHeadDim, page_bytes = row_bytes << a.kv_shift, page_scales = (uint32_t)a.n_kv_heads << a.kv_shift;
         bool more = true, waited = !a.append;
         int c_i = 0, c_key = 0, c_own = 0, b0 = 0, b1 = 0, n0 = 0, n1 = 0, issued = 0;      // c_i, c_own: own tiles of the part, done and in all
-        // block-table entry of the page that holds a key; -1: a bad one, -2: there is no such key
+        // block-table entry of the page that holds a key; -1: a bad one, -2: there is no such key, or none of an 8-token page is in the
+        // window of any token (its entry may be gone)
         auto entry = [&](int key) -> int {
-            if (key >= u.keys_end) return -2;
+            if (key >= u.keys_end || (p8 && a.window > 0 && key + 8 <= u.past + u.t0 - a.window + 1)) return -2;
             const int64_t page = key >> a.kv_shift;
             if (page >= a.table_stride) return -1;
             const int e = __ldg(table + page);

@@ -360,7 +360,7 @@ int nova_launch_q8_append(const nova_q8_cache* c, const nova_q8_rows* r, const v
  * rounded once (keys come back as they are stored: rotated). */
 int nova_launch_q8_read(const nova_q8_cache* c, const nova_q8_rows* r, void* k_out, void* v_out, nova_stream_t s);
 /* Attention of the rows of q ([n_tokens][n_heads][128]) over the cached keys: the query at position p sees the keys [0, p], or
- * (p - window, p] where window > 0.  The keys of the new rows must be in the cache; a query that sees none gets zeros.
+ * (p - window, p] where window > 0 (pages of which no query sees a key need no table entry).  The keys of the new rows must be in the cache; a query that sees none gets zeros.
  * q (rotated) and the softmax weights are rounded to fp16 on their way into the tensor cores; sums and the softmax are fp32.
  * One row per session and at most 8 query heads per kv head: the codes go in exactly and the scales are applied in fp32; with
  * fp32 or fp16 activations q and the weights are taken as two fp16 parts each (2^-21).  Anything else: keys and values go in as fp16

@@ -91,3 +91,36 @@ def test_positions_behind_the_block_table(nv, far, window, page):
         o, a, spread, floor = case.attend()
         off, bound = (got.double() - o).abs(), attention_bound(case, o, a, spread, floor, False)
         assert bool((off <= bound)[1:].all())
+
+
+@pytest.mark.parametrize("fmt", ["i8", "e4m3"])
+@pytest.mark.parametrize("page", [8, 16, 32, 64])
+@pytest.mark.parametrize("window", [1, 7, 24, 100])
+def test_pages_behind_the_window_may_be_gone(nv, window, page, fmt):
+    """Pages of which no new token sees a key have no entry any more, and what lies in front of the window in the others is NaN: nothing is
+    flagged, and nothing of it shows."""
+    for past, new in (([200, 207, 31, 64, 111, 8], [1] * 6), ([200, 207, 31, 300, 111], [3, 40, 1, 9, 70])):
+        case = Cache(past, new, 4, 2, page, fmt, "bf16", window=window, seed=window)
+        gone = []
+        for s, p in enumerate(past):
+            first = max(0, p - window + 1)
+            for j in range(first):
+                ph, slot = case.place(s, j)
+                for x in case.codes:
+                    x[:, ph, slot] = 0x7f
+                for x in case.scales:
+                    x[:, ph, :, slot] = float("nan")
+            gone.append(first // page)
+        d = case.device(nv)
+        for s, n in enumerate(gone):
+            d["tables"][int(case.slices[s]), :n] = -1
+        case.append()
+        call(nv, d, "append_attn", window)
+        torch.cuda.synchronize()
+        assert int(d["status"]) == 0
+        for i in (0, 1):            # (the plain form multiplies what it does not see by zero)
+            x = case.codes[i], case.scales[i]
+            bad = x[1].isnan()
+            x[0][bad.permute(0, 1, 3, 2)] = 0
+            x[1][bad] = 1.0
+        check_rows(case, d["out"].cpu(), torch.ones(sum(new), dtype=torch.bool))
