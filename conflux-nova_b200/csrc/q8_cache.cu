@@ -285,7 +285,7 @@ __global__ void __launch_bounds__(256) q8_read_kernel(Q8Launch a, int iters) {
     }
 }
 
-bool misaligned(const void* p) { return ((uintptr_t)p & 15u) != 0; }
+bool misaligned(const void* p, unsigned to = 16) { return ((uintptr_t)p & (to - 1)) != 0; }
 
 // Descriptors -> launch description, with every check that the host can make.
 int q8_fill(const nova_q8_cache* c, const nova_q8_rows* r, Q8Launch& a) {
@@ -297,6 +297,7 @@ int q8_fill(const nova_q8_cache* c, const nova_q8_rows* r, Q8Launch& a) {
     if (sh.n_heads / sh.n_kv_heads > 128) return NOVA_ERR_UNSUPPORTED;
     if (c->layer < 0 || c->nb <= 0 || c->table_stride <= 0 || !c->pool_k || !c->pool_v || !c->scale_k || !c->scale_v || !c->tables) return NOVA_ERR_INVALID;
     if (misaligned(c->pool_k) || misaligned(c->pool_v) || misaligned(c->scale_k) || misaligned(c->scale_v)) return NOVA_ERR_INVALID;
+    if (misaligned(c->tables, 4) || misaligned(c->slice_ids, 4) || misaligned(c->status, 4) || misaligned(r->n_past, 4) || misaligned(r->tok_start, 4)) return NOVA_ERR_INVALID;
     if (!c->rope_cs != !c->rope_sn || (c->rope_cs && c->rope_rows <= 0) || misaligned(c->rope_cs) || misaligned(c->rope_sn)) return NOVA_ERR_INVALID;
     if (((int64_t)c->layer + 1) * c->nb * sh.kv_block > 0x7fffffffLL) return NOVA_ERR_TOO_LARGE;      // slot rows are 32-bit coordinates
     if (r->io_dtype != NOVA_IO_F32 && r->io_dtype != NOVA_IO_F16 && r->io_dtype != NOVA_IO_BF16) return NOVA_ERR_UNSUPPORTED;
