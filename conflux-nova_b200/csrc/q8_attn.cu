@@ -20,8 +20,11 @@
 //     contraction index may be permuted freely as long as q's fragments follow.  V needs pairs of keys side by side: bytes are
 //     interleaved with permutes, and the rows of product j are the dims 16 g + 2 j (+ 1).  P goes from the accumulator layout to
 //     the operand layout with movmatrix.
-//   * int8 K: the byte code + 128 is taken as an fp16 subnormal, (code + 128) 2^-24, which costs no arithmetic; the accumulators start
-//     at -128 2^-24 sum(q).  (Not for V: there the offset would be a sum of weights, hundreds of times the result.)
+//   * int8 K with q in one part: the byte code + 128 is taken as an fp16 subnormal, (code + 128) 2^-24, which costs no arithmetic; the
+//     accumulators start at -128 2^-24 sum(q).  What the offset's size takes from the accumulators' bits stays below what rounding q to
+//     fp16 does.  With q in two parts it would not (keys of small codes beside a large one, queries of one sign: 2^-15 of sum |q k|
+//     instead of 2^-21), so there the codes go in as they are, one subtraction a pair.  (Nor for V: there the offset would be a sum of
+//     weights, hundreds of times the result.)
 //   * fp32 and fp16 activations: q and p as fp16 hi + lo, two instructions each, so that outputs are as good as fp32 arithmetic gives
 //     them (rounded once, fp16 outputs would be 5e-4 off instead of 2e-4).  bf16 activations: q (rotated) and p rounded to fp16,
 //     which bf16's own 2^-9 hides.
@@ -182,8 +185,9 @@ q8_decode_kernel(Q8Launch a, const __grid_constant__ CUtensorMap tmk, const __gr
     const uint32_t tile0 = (smem_u32(smem_raw) + 1023u) & ~1023u;
     const uint32_t scale0 = tile0 + kStages * Cfg::kTile;
     float* const merge = reinterpret_cast<float*>(smem_raw + (scale0 - smem_u32(smem_raw)) + kStages * Cfg::kScales + 2 * Cfg::kRawSteps * 512);
-    // the operands are q / 8 (rotated fp16 values stay inside fp16) and codes, those of int8 K times 2^-24
-    constexpr float kToLog2 = kAttnScale * kLog2e * 8.f * (kFmt == NOVA_KV_I8 ? 16777216.f : 1.f);
+    // the operands are q / 8 (rotated fp16 values stay inside fp16) and codes, those of int8 K, with q in one part, plus 128 and times 2^-24
+    constexpr bool kOffset = kFmt == NOVA_KV_I8 && !kLo;
+    constexpr float kToLog2 = kAttnScale * kLog2e * 8.f * (kOffset ? 16777216.f : 1.f);
     // a page of 8 tokens is half a tile: two boxes of 8 slots, [half][kv head][8]; otherwise [kv head][16]
     const bool p8 = a.kv_shift == 3;
     const uint32_t head_step = p8 ? 1024u : 2048u, half_step = p8 ? KVG * 1024u : 1024u;
@@ -432,13 +436,13 @@ q8_decode_kernel(Q8Launch a, const __grid_constant__ CUtensorMap tmk, const __gr
                     const float2 b0 = __half22float2(h0), b1 = __half22float2(h1);
                     const int d = e ? d1 : d0, chunk = d >> 3;
                     const uint32_t dst = stash + (uint32_t)hd * 256u + (uint32_t)(((4 * (chunk & 3) + (chunk >> 2)) ^ (4 * (hd & 1))) * 16 + (d & 4) * 2);
-                    sum += kLo ? (f[0] + f[1]) + (f[2] + f[3]) : (b0.x + b0.y) + (b1.x + b1.y);
+                    sum += (b0.x + b0.y) + (b1.x + b1.y);
                     if (real) {
                         sts64(dst, *reinterpret_cast<const uint32_t*>(&h0), *reinterpret_cast<const uint32_t*>(&h1));
                         if constexpr (kLo) sts64(dst + 2048u, pack_h2(f[0] - b0.x, f[1] - b0.y), pack_h2(f[2] - b1.x, f[3] - b1.y));
                     }
                 }
-                if constexpr (kFmt == NOVA_KV_I8) {
+                if constexpr (kOffset) {
 #pragma unroll
                     for (int o = 8; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
                     if (real && i == 0) sts_f1(stash + 4096u + (uint32_t)hd * 4u, sum);
@@ -455,7 +459,7 @@ q8_decode_kernel(Q8Launch a, const __grid_constant__ CUtensorMap tmk, const __gr
                     ql[2 * k][0] = l.x, ql[2 * k][1] = l.y, ql[2 * k + 1][0] = l.z, ql[2 * k + 1][1] = l.w;
                 }
             }
-            if constexpr (kFmt == NOVA_KV_I8) {                                                     // 128 * 2^-24
+            if constexpr (kOffset) {                                                                // 128 * 2^-24
                 if (2 * t < G) off0 = -7.62939453125e-06f * lds_f1(stash + 4096u + 8u * t);
                 if (2 * t + 1 < G) off1 = -7.62939453125e-06f * lds_f1(stash + 4096u + 8u * t + 4u);
             }
@@ -529,8 +533,14 @@ q8_decode_kernel(Q8Launch a, const __grid_constant__ CUtensorMap tmk, const __gr
                     const uint4 wa = kw[ks >> 2][0], wb = kw[ks >> 2][1];
                     const int k4 = ks & 3;
                     uint32_t a0, a1, a2, a3;
-                    q8_k_to_h2<kFmt>(k4 == 0 ? wa.x : k4 == 1 ? wa.y : k4 == 2 ? wa.z : wa.w, a0, a2);
-                    q8_k_to_h2<kFmt>(k4 == 0 ? wb.x : k4 == 1 ? wb.y : k4 == 2 ? wb.z : wb.w, a1, a3);
+                    const uint32_t w0 = k4 == 0 ? wa.x : k4 == 1 ? wa.y : k4 == 2 ? wa.z : wa.w, w1 = k4 == 0 ? wb.x : k4 == 1 ? wb.y : k4 == 2 ? wb.z : wb.w;
+                    if constexpr (kOffset) {
+                        q8_k_to_h2(w0, a0, a2);
+                        q8_k_to_h2(w1, a1, a3);
+                    } else {
+                        q8_to_h2<kFmt>(w0, a0, a2);
+                        q8_to_h2<kFmt>(w1, a1, a3);
+                    }
                     mma_full(c, a0, a1, a2, a3, qh[ks][0], qh[ks][1]);
                     if constexpr (kLo) mma_full(c, a0, a1, a2, a3, ql[ks][0], ql[ks][1]);
                 }

@@ -288,15 +288,11 @@ __device__ __forceinline__ float rcp(float x) {
     return y;
 }
 
-// q8_to_h2 for K: int8 codes as (code + 128) 2^-24, an fp16 subnormal whose bits are the byte.
-template <int kFmt> __device__ __forceinline__ void q8_k_to_h2(uint32_t w, uint32_t& h0, uint32_t& h1) {
-    if constexpr (kFmt == NOVA_KV_I8) {
-        const uint32_t u = w ^ 0x80808080u;
-        h0 = __byte_perm(u, 0u, 0x4140);
-        h1 = __byte_perm(u, 0u, 0x4342);
-    } else {
-        q8_to_h2<kFmt>(w, h0, h1);
-    }
+// int8 codes as (code + 128) 2^-24, an fp16 subnormal whose bits are the byte.
+__device__ __forceinline__ void q8_k_to_h2(uint32_t w, uint32_t& h0, uint32_t& h1) {
+    const uint32_t u = w ^ 0x80808080u;
+    h0 = __byte_perm(u, 0u, 0x4140);
+    h1 = __byte_perm(u, 0u, 0x4342);
 }
 
 __device__ __forceinline__ uint4 lds128(uint32_t addr) {

@@ -2,7 +2,7 @@
 import pytest
 import torch
 
-from q8_plain import HD, IO, Cache, call
+from q8_plain import HD, IO, Cache, attention_bound, call
 
 pytestmark = pytest.mark.gpu
 HALF = {"f32": 2.0 ** -24, "f16": 2.0 ** -11, "bf16": 2.0 ** -8}        # half a step of the outputs' type, relative
@@ -132,3 +132,26 @@ def test_prefill_of_an_engine(nv, fmt, size):
         assert bool(((got[s] - want).abs() <= want.abs() * (2.0 ** -11 + VALUE + HALF["f32"]) + VALUE_LOW).all())
     b.close()
     eng.close()
+
+
+@pytest.mark.parametrize("fmt", ["i8", "e4m3"])
+@pytest.mark.parametrize("io", ["f32", "f16"])
+@pytest.mark.parametrize("mean", [0.0, 2.0, 6.0])
+def test_single_tokens_over_keys_with_one_large_number(nv, mean, io, fmt):
+    """Keys whose codes are small but for one (the scale is that one's), queries of mostly one sign: q is taken in two fp16 parts, so a score
+    is off by 2^-18 of sum |q k| at the most, whatever sum q is."""
+    past = [3, 7, 15, 2, 40, 5, 1, 6] * 4
+    case = Cache(past, [1] * len(past), 14, 2, 16, fmt, io, rope="none", seed=int(mean), poison=False, layers=1, layer=0)
+    g = torch.Generator().manual_seed(9)
+    case.q.copy_((torch.randn(case.q.shape, generator=g) * 0.5 + mean).to(IO[io]))
+    shape = case.codes[0].shape
+    small = torch.randint(-3, 4, shape, generator=g).float()
+    small[..., 77] = 127.0 if fmt == "i8" else 448.0
+    case.codes[0] = (small.to(torch.int8) if fmt == "i8" else small.to(torch.float8_e4m3fn)).view(torch.uint8)
+    case.scales[0].fill_(0.04)
+    case.k.copy_((torch.randint(-3, 4, case.k.shape, generator=g).float() * 0.04).to(IO[io]))
+    case.k[..., 77] = (127.0 if fmt == "i8" else 448.0) * 0.04
+    got = run(nv, case)
+    o, a, spread, floor = case.attend()
+    bound = attention_bound(case, o, a, spread, floor, True)
+    assert bool(((got - o).abs() <= bound).all()), f"{float(((got - o).abs() / bound).max()):.3g} of the bound"
