@@ -357,7 +357,8 @@ q8_decode_kernel(Q8Launch a, const __grid_constant__ CUtensorMap tmk, const __gr
                     if (!is_v) {
                         sts128(dst, make_float4(v.x * kToLog2, v.y * kToLog2, v.z * kToLog2, v.w * kToLog2));
                     } else {
-                        const float4 m = make_float4(fmaxf(v.x, kQ8MinScale), fmaxf(v.y, kQ8MinScale), fmaxf(v.z, kQ8MinScale), fmaxf(v.w, kQ8MinScale));
+                        auto at_least = [](float x) { return x < kQ8MinScale ? kQ8MinScale : x; };      // (a NaN stays one)
+                        const float4 m = make_float4(at_least(v.x), at_least(v.y), at_least(v.z), at_least(v.w));
                         sts128(dst, make_float4(lg2(m.x), lg2(m.y), lg2(m.z), lg2(m.w)));
                         sts128(dst + KVG * 64, make_float4(rcp(m.x), rcp(m.y), rcp(m.z), rcp(m.w)));
                     }

@@ -275,6 +275,7 @@ q8_chunk_kernel(Q8Launch a, ChunkShape sh) {
     volatile int& s_abort = *reinterpret_cast<volatile int*>(smem_raw + kOffBar + 516);
     uint32_t* const s_mask = reinterpret_cast<uint32_t*>(smem_raw + kOffBar + 520);       // [kMasks][2] which keys of a tile exist
     uint32_t* const s_rmask = reinterpret_cast<uint32_t*>(smem_raw + kOffBar + 584);      // [kConv][kRaw] the same of a converter's 32 keys
+    uint32_t* const s_show = reinterpret_cast<uint32_t*>(smem_raw + kOffBar + 648);       // ... whether what is no number among them shows
     const int lane = (int)threadIdx.x & 31;
     const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0);
     const int G = a.n_heads / a.n_kv_heads;
@@ -840,6 +841,7 @@ q8_chunk_kernel(Q8Launch a, ChunkShape sh) {
             const bool bad = __any_sync(0xffffffffu, mine == -1);
             if (lane == 0) {
                 s_rmask[me * kRaw + st] = mask;
+                s_show[me * kRaw + st] = !which || (key + 31 <= u.past + u.t0 && (a.window <= 0 || key >= u.keys_end - a.window));
                 if (bad && !which) q8_flag(a, NOVA_ERR_BAD_TABLE);
             }
             ++c_i;
@@ -862,6 +864,11 @@ q8_chunk_kernel(Q8Launch a, ChunkShape sh) {
             if (j > 0 && !__all_sync(0xffffffffu, t5_wait(bar_free, (uint32_t)(j - 1) & 1u, &s_abort))) { failed = true; break; }
             const uint32_t st = (uint32_t)(j & (kRaw - 1)), mask = s_rmask[me * kRaw + st];
             if (!which && lane == 0) s_mask[2 * ((2 * j + par) & (kMasks - 1)) + hw] = mask;
+            // What is no number stays none, so that it shows: the score of such a key is NaN for the queries that see it, and is taken out
+            // for the others.  But V of a key that a query does not see is multiplied by zero: unless all the unit's queries see all of
+            // these keys, it becomes the largest number.
+            const bool show = s_show[me * kRaw + st];
+            const __half2 most = __half2half2(__ushort_as_half(show ? 0x7fff : 0x7bff));            // (the minimum with NaN is the other)
             const uint32_t src = raw0 + st * 4096u + (uint32_t)r8 * 128u;
             // two rows (r8 and r8 + 8) at a time
 #pragma unroll
@@ -880,7 +887,8 @@ q8_chunk_kernel(Q8Launch a, ChunkShape sh) {
                 }
 #pragma unroll
                 for (int e2 = 0; e2 < 2; ++e2) {
-                    const float fs = fminf(f[e2] * mul, 65504.f * kQ8CodeDiv<kFmt> / q8_qmax<kFmt>());
+                    float fs = fminf(f[e2] * mul, 65504.f * kQ8CodeDiv<kFmt> / q8_qmax<kFmt>());
+                    if (show) fs = fmaf(f[e2], 0.f, fs);              // (NaN for a scale that is no number)
                     const __half hi1 = __float2half_rn(fs);
                     const __half2 hi2 = __half2half2(hi1), lo2 = __half2half2(__float2half_rn(fs - __half2float(hi1)));
 #pragma unroll
@@ -894,8 +902,7 @@ q8_chunk_kernel(Q8Launch a, ChunkShape sh) {
                         for (int b = 0; b < 8; ++b) {
                             const __half2 x = *reinterpret_cast<const __half2*>(&h[b]);
                             __half2 y = __hfma2(x, hi2, __hmul2(x, lo2));
-                            // V's NaN codes become the largest number: a query that does not see the key multiplies it by zero
-                            if (kFmt == NOVA_KV_E4M3 && which) y = __hmin2(y, __half2half2(__ushort_as_half(0x7bff)));
+                            if (kFmt == NOVA_KV_E4M3 && which) y = __hmin2(y, most);
                             h[b] = *reinterpret_cast<const uint32_t*>(&y);
                         }
                         const uint32_t de = dst0 + (uint32_t)(q * 2048 + e2 * 1024 + (e & 1) * kSlab);

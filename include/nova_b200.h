@@ -317,8 +317,8 @@ int nova_launch_attn_decode_paged_static(const nova_kv_shape* sh, const float* q
  *   scales scale_k / scale_v [layers][nb][n_kv_heads][kv_block] fp32
  * A row (one token of one kv head) is written as  amax = max(max|x|, 2^-60),  scale = amax / Q,  code = rn(x * (Q / amax)),
  * Q = 127 or 448, in fp32 with one rounding per operation (ties to even).  A NaN becomes code 0 (int8) or NaN (e4m3); a row
- * with an infinity gets an infinite scale and reads back as NaN; of queries that see such keys or values, or NaN ones, nothing is
- * promised (others are not touched by them).
+ * with an infinity gets an infinite scale and reads back as NaN.  Queries that see such keys or values, or NaN ones, get NaN, but in a
+ * chunk a value within 32 keys of where some of its tokens see it and others do not may give them any number; others are not touched.
  * The block tables are those of the rest of this header: `tables` is an array of tables of table_stride entries, session s
  * uses table slice_ids[s] (slice_ids NULL: table s).  An entry outside [0, nb) is never followed: its keys are skipped, its
  * rows are neither written nor read back, and *status (device, may be NULL) becomes NOVA_ERR_BAD_TABLE.

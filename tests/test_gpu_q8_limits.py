@@ -124,3 +124,39 @@ def test_pages_behind_the_window_may_be_gone(nv, window, page, fmt):
             x[0][bad.permute(0, 1, 3, 2)] = 0
             x[1][bad] = 1.0
         check_rows(case, d["out"].cpu(), torch.ones(sum(new), dtype=torch.bool))
+
+
+@pytest.mark.parametrize("fmt", ["i8", "e4m3"])
+@pytest.mark.parametrize("what", ["k inf", "v inf", "k nan", "v nan"])
+@pytest.mark.parametrize("window", [0, 200, 40])
+def test_cached_rows_that_are_no_numbers_show(nv, fmt, what, window):
+    """A cached row with an infinite scale, or with a NaN (e4m3 codes; int8 has none: its scale is NaN here), that all tokens of a chunk see,
+    or none (window 40): the outputs of those that see it are no numbers, in the head that has it; all others are right.  Single tokens the
+    same."""
+    for past, new in (([200, 70, 30], [40, 130, 5]), ([200, 70, 30], [1, 1, 1])):
+        case = Cache(past, new, 4, 2, 16, fmt, "bf16", rope="none", window=window, layers=1, layer=0, poison=False)
+        i, bad = "kv".index(what[0]), ((0, 150, 1), (1, 0, 0))             # (session, key, kv head)
+        d = case.device(nv)
+        for s, j, h in bad:
+            ph, slot = case.place(s, j)
+            if what.endswith("inf"):
+                d["scales"][i][0, ph, h, slot] = float("inf")
+                d["codes"][i][0, ph, slot, h] = 0
+            elif fmt == "e4m3":
+                d["codes"][i][0, ph, slot, h, 5] = 0x7f
+            else:
+                d["scales"][i][0, ph, h, slot] = float("nan")
+        case.append()
+        call(nv, d, "append_attn", window)
+        torch.cuda.synchronize()
+        assert int(d["status"]) == 0
+        hit = torch.zeros(sum(new), 4, dtype=torch.bool)
+        pos, session = case.positions(), torch.repeat_interleave(torch.arange(3), torch.tensor(new))
+        for s, j, h in bad:
+            hit[:, 2 * h:2 * h + 2] |= ((session == s) & ((pos - window < j) if window else True))[:, None]
+        got = d["out"].cpu()
+        o, a, spread, floor = case.attend()
+        off = (got.double() - o).abs()
+        assert bool((off <= attention_bound(case, o, a, spread, floor, False))[~hit].all())
+        dim = slice(5, 6) if what == "v nan" and fmt == "e4m3" else slice(None)
+        assert bool((~got[hit][:, dim].isfinite()).all())
