@@ -165,6 +165,14 @@ __device__ __forceinline__ DecSegment dec_segment(const DecPlan& p, const DecLin
     return sg;
 }
 
+// A CTA that has given up on a wait stays for a millisecond more: copies that it has on their way land in microseconds, and none may when
+// its shared memory is another's.
+__device__ __forceinline__ void dec_settle(const volatile int* aborted) {
+    if (!*aborted) return;
+    const unsigned long long t0 = now_ns();
+    for (int i = 0; i < 100000 && now_ns() - t0 < 1000000ull; ++i) __nanosleep(1000);
+}
+
 // kLo: q and p in two fp16 parts (fp32 and fp16 activations, unless one_part)
 template <int KVG, int kFmt, bool kLo>
 __global__ void __launch_bounds__(DecCfg<KVG>::kThreads, 1)
@@ -267,6 +275,7 @@ q8_decode_kernel(Q8Launch a, const __grid_constant__ CUtensorMap tmk, const __gr
                 const bool free = !mine || round == 0 || mbar_wait(smem_u32(&s_empty[stage]), (round - 1) & 1, &s_abort);
                 if (!__all_sync(0xffffffffu, free)) {
                     if (lane == 0) q8_flag(a, NOVA_ERR_TIMEOUT);
+                    dec_settle(&s_abort);
                     return;
                 }
                 if (mine) {
@@ -676,6 +685,7 @@ q8_decode_kernel(Q8Launch a, const __grid_constant__ CUtensorMap tmk, const __gr
         }
         asm volatile("bar.sync %0, %1;" ::"r"(1 + w), "r"(32 * kSub) : "memory");
     }
+    dec_settle(&s_abort);
 }
 
 // Merge of the rows that several CTAs worked on: W warps per (row, head).  The first finds every contributor's weight; the

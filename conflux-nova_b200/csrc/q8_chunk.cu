@@ -283,7 +283,7 @@ q8_chunk_kernel(Q8Launch a, ChunkShape sh) {
     const uint32_t bar = base + kOffBar;
     const uint32_t bar_partfull = bar, bar_partfree = bar + 32, bar_kfull = bar + 320, bar_kfree = bar + 336, bar_vfull = bar + 352, bar_vfree = bar + 368,
                    bar_sready = bar + 384 /* [half][buffer] */, bar_pready = bar + 416, bar_pvdone = bar + 448, bar_qready = bar + 480 /* [half] */,
-                   bar_xfull = bar + 496, bar_xfree = bar + 504;
+                   bar_xfull = bar + 496, bar_xfree = bar + 504, bar_drain = bar + 712 /* [half] */;
     // Every waiter waits for a phase whose successor on the same barrier needs that waiter's own next action (or one that follows it),
     // so a parity is never taken for a later one.
     if (threadIdx.x == 0) {
@@ -293,6 +293,7 @@ q8_chunk_kernel(Q8Launch a, ChunkShape sh) {
             mbar_init(bar_vfull + 8u * i, kConv / 4);
             mbar_init(bar_vfree + 8u * i, sh.dual ? 1 : 2);
             mbar_init(bar_qready + 8u * i, 4);
+            mbar_init(bar_drain + 8u * i, 1);
         }
         for (int i = 0; i < 4; ++i) {
             mbar_init(bar_sready + 8u * i, 1);
@@ -709,6 +710,13 @@ q8_chunk_kernel(Q8Launch a, ChunkShape sh) {
                 }
                 n += tiles;
             }
+            if (failed) {
+                // products that are under way finish before the tensor memory is given back (a bounded wait of its own)
+                if (elect_one()) umma_commit(bar_drain + 8u * (uint32_t)h);
+                __syncwarp();
+                for (int i = 0; i < 1 << 16 && !mbar_try(bar_drain + 8u * (uint32_t)h, 0u); ++i) {}
+                __syncwarp();
+            }
         } else if (warp == 10) {
             // ------------------------------------------------------------------------------------ the walk along the line
             int k = 0;
@@ -917,7 +925,8 @@ q8_chunk_kernel(Q8Launch a, ChunkShape sh) {
             issue_next();                                           // into the stage that has just been read
             asm volatile("cp.async.commit_group;" ::: "memory");
         }
-        asm volatile("cp.async.wait_all;" ::: "memory");           // (nothing may land after the CTA is gone)
+        asm volatile("cp.async.wait_all;" ::: "memory");           // nothing may land after the CTA is gone: no copy, and no arrival of the
+        if (!failed && issued > 0) t5_wait(bar_free, (uint32_t)(issued - 1) & 1u, &s_abort);      // products of the last tiles either
     }
     if (failed && lane == 0) q8_flag(a, NOVA_ERR_TIMEOUT);
     // ---- release the tensor memory (every path of every thread ends here)
