@@ -3,7 +3,7 @@ are no row starts, pages that nobody needs any more.  What is skipped is left as
 import pytest
 import torch
 
-from q8_plain import Cache, attention_bound, call
+from q8_plain import IO, Cache, attention_bound, call, quantise, rotate
 
 pytestmark = pytest.mark.gpu
 
@@ -160,3 +160,72 @@ def test_cached_rows_that_are_no_numbers_show(nv, fmt, what, window):
         assert bool((off <= attention_bound(case, o, a, spread, floor, False))[~hit].all())
         dim = slice(5, 6) if what == "v nan" and fmt == "e4m3" else slice(None)
         assert bool((~got[hit][:, dim].isfinite()).all())
+
+
+STARTS = [([1, 1, 1], [0, -50, 10 ** 9, 10 ** 9]), ([1, 1, 1], [7, 3, 2, 1]), ([1, 1, 1], [-3, -2, -1, 0]), ([1, 1, 1], [0, 1, 1, 10 ** 9]),
+          ([4, 5, 6], [0, -50, 10 ** 9, 10 ** 9]), ([4, 5, 6], [7, 3, 2, 1]), ([4, 5, 6], [-2 ** 31, 4, 9, 2 ** 31 - 1]), ([4, 5, 6], [15, 15, 15, 15]),
+          ([4, 5, 6], [20, 30, 40, 50]), ([4, 5, 6], [2, 3, 3, 8])]
+
+
+@pytest.mark.parametrize("fmt,io", [("i8", "bf16"), ("e4m3", "f32")])
+@pytest.mark.parametrize("new,starts", STARTS)
+def test_row_starts_that_are_none_touch_nothing_else(nv, new, starts, fmt, io):
+    """tok_start is device data.  Cut to [0, n_tokens], a session has the rows from its start to the next one's, at most max_tokens: those are
+    written, read back and attended, and everything else stays: spare rows, guard rows around all buffers, pages of sessions without rows."""
+    T, extra = sum(new), 2
+    case = Cache([20, 30, 40], new, 4, 2, 16, fmt, io, layers=1, layer=0, poison=False)
+    case.qkv = torch.cat((case.qkv, case.qkv[:extra]))
+    d = case.device(nv)
+    rows = []                                             # (row, session, token) that somebody has
+    cut = [min(max(x, 0), T) for x in starts]
+    for s in range(3):
+        rows += [(r, s, r - cut[s]) for r in range(cut[s], min(max(cut[s + 1], cut[s]), cut[s] + max(new)))]
+    d["rows"].n_tokens = T
+    d["start"].copy_(torch.tensor(starts, dtype=torch.int32))
+    fill = lambda n, *shape, t: torch.full((n + 8, *shape), 7, dtype=t, device="cuda")
+    out, back = fill(T, 4, 128, t=d["out"].dtype), [fill(T, 2, 128, t=d["out"].dtype) for _ in range(2)]
+    guard = []                                            # pools inside larger buffers
+    for name in ("codes", "scales"):
+        for i in (0, 1):
+            x = d[name][i].flatten()
+            big = torch.full((x.numel() + 512,), 7, dtype=x.dtype, device="cuda")
+            big[256:-256] = x
+            guard.append(big)
+            d[name][i] = big[256:-256].view(d[name][i].shape)
+    c = d["cache"]
+    c.pool_k, c.pool_v, c.scale_k, c.scale_v = (x.data_ptr() for x in d["codes"] + d["scales"])
+    ptr = lambda x: x[4:].data_ptr()
+    # the plain form: the same rows, session by session, token by token of the order they have
+    fresh = [quantise(x, fmt) for x in (rotate(case.qkv[[r for r, _, _ in rows], 4:6], torch.tensor([case.past[s] + t for _, s, t in rows], dtype=torch.long),
+                                               case.cs, case.sn, case.rope), case.qkv[[r for r, _, _ in rows], 6:].float())] if rows else []
+    for n, (r, s, t) in enumerate(rows):
+        ph, slot = case.place(s, case.past[s] + t)
+        for i in (0, 1):
+            case.codes[i][0, ph, slot] = fresh[i][0][n].view(torch.uint8)
+            case.scales[i][0, ph, :, slot] = fresh[i][1][n]
+    stream = torch.cuda.current_stream().cuda_stream
+    nv.q8_append_attn(c, d["rows"], d["q"].data_ptr(), d["k"].data_ptr(), d["v"].data_ptr(), ptr(out), 0, d["work"].data_ptr(), d["work"].numel(), stream)
+    nv.q8_read(c, d["rows"], ptr(back[0]), ptr(back[1]), stream)
+    torch.cuda.synchronize()
+    assert int(d["status"]) == 0
+    for big in guard:
+        assert bool((big[:256] == 7).all() and (big[-256:] == 7).all())
+    for x, y in zip(d["codes"] + d["scales"], case.codes + case.scales):
+        assert bool((bits(x) == bits(y)).all())
+    spare = torch.ones(T + 8, dtype=torch.bool)
+    spare[[4 + r for r, _, _ in rows]] = False
+    for x in [out] + back:
+        assert bool((x.cpu()[spare] == 7).all())
+    for s in range(3):
+        mine = [r for r, o, _ in rows if o == s]
+        if not mine:
+            continue
+        one = Cache([case.past[s]], [len(mine)], 4, 2, 16, fmt, io, layers=1, layer=0, poison=False)
+        one.codes, one.scales, one.tables, one.slices, one.cs, one.sn = case.codes, case.scales, case.tables, case.slices[s:s + 1], case.cs, case.sn
+        one.q = case.qkv[mine, :4]
+        o, a, spread, floor = one.attend()
+        off = (out.cpu()[[4 + r for r in mine]].double() - o).abs()
+        assert bool((off <= attention_bound(one, o, a, spread, floor, False)).all())
+        for i in (0, 1):
+            want = one.values(i, 0, one.past[0], one.past[0] + len(mine))[1].to(IO[io])
+            assert bool((bits(back[i][[4 + r for r in mine]]) == bits(want)).all())
