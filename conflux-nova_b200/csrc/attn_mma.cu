@@ -671,6 +671,23 @@ int launch_kvg(const AttnLaunch& a, int n_ctas, cudaStream_t s) {
 typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
                                   const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
                                   CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+typedef CUresult (*CtxGetCurrentFn)(CUcontext*);
+
+template <typename Fn>
+int driver_entry(const char* name, std::atomic<Fn>& known, Fn& out) {
+    out = known.load(std::memory_order_acquire);
+    if (out) return NOVA_OK;
+    cudaDriverEntryPointQueryResult q;
+    void* fn = nullptr;
+    const cudaError_t e = cudaGetDriverEntryPoint(name, &fn, cudaEnableDefault, &q);
+    if (e != cudaSuccess || q != cudaDriverEntryPointSuccess || !fn) {
+        set_cuda_error(e == cudaSuccess ? cudaErrorNotSupported : e, name);
+        return NOVA_ERR_CUDA;
+    }
+    out = (Fn)fn;
+    known.store(out, std::memory_order_release);
+    return NOVA_OK;
+}
 
 }  // namespace
 
@@ -681,16 +698,19 @@ size_t attn_tmap_bytes() { return sizeof(CUtensorMap); }
 // Tensor map over one pool (fp16; fp32 and 8-bit codes: the same with 4 or 1 bytes an element) [rows = L*NB*page tokens][NKV][128]: dim0 = 128 dims, dim1 = slot rows
 // (stride NKV*256 B), dim2 = kv head (stride 256 B); box = [64][box_rows = 16 or 8][kv_group], 128-byte swizzle.
 int attn_make_tmap(void* out_map, void* pool, int64_t slot_rows, int n_kv_heads, int kv_group, int box_rows, int elem_bytes) {
-    static EncodeTiledFn encode = nullptr;
-    if (!encode) {
-        cudaDriverEntryPointQueryResult q;
-        void* fn = nullptr;
-        const cudaError_t e = cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &q);
-        if (e != cudaSuccess || q != cudaDriverEntryPointSuccess || !fn) {
-            set_cuda_error(e == cudaSuccess ? cudaErrorNotSupported : e, "cuTensorMapEncodeTiled entry point");
-            return NOVA_ERR_CUDA;
-        }
-        encode = (EncodeTiledFn)fn;
+    static std::atomic<EncodeTiledFn> encode_known{nullptr};
+    static std::atomic<CtxGetCurrentFn> current_known{nullptr};
+    EncodeTiledFn encode;
+    CtxGetCurrentFn current;
+    int rc = driver_entry("cuTensorMapEncodeTiled", encode_known, encode);
+    if (rc == NOVA_OK) rc = driver_entry("cuCtxGetCurrent", current_known, current);
+    if (rc != NOVA_OK) return rc;
+    // The driver's call wants a current context, which a host thread that has not made a runtime call yet does not have.
+    CUcontext ctx = nullptr;
+    if (current(&ctx) != CUDA_SUCCESS || !ctx) {
+        int dev = 0;
+        NOVA_CUDA_TRY(cudaGetDevice(&dev));
+        NOVA_CUDA_TRY(cudaSetDevice(dev));
     }
     if (slot_rows <= 0 || slot_rows > 0x7fffffffLL) return NOVA_ERR_TOO_LARGE;
     if ((box_rows != 8 && box_rows != 16) || (elem_bytes != 1 && elem_bytes != 2 && elem_bytes != 4)) return NOVA_ERR_INVALID;
