@@ -229,3 +229,29 @@ def test_row_starts_that_are_none_touch_nothing_else(nv, new, starts, fmt, io):
         for i in (0, 1):
             want = one.values(i, 0, one.past[0], one.past[0] + len(mine))[1].to(IO[io])
             assert bool((bits(back[i][[4 + r for r in mine]]) == bits(want)).all())
+
+
+@pytest.mark.parametrize("new,io", [([1, 1, 1], "f16"), ([30, 0, 9], "bf16")])
+def test_pools_of_more_than_four_gigabytes(nv, new, io):
+    """The last layer of pools whose offsets pass 32 bits (5 GB of codes each): written, read back, attended."""
+    case = Cache([200, 5, 70], new, 16, 8, 16, "i8", io, layers=1, layer=0)
+    layer = 5 * 10 ** 9 // case.codes[0].numel()
+    d = case.device(nv)
+    big = [torch.empty((layer + 1) * x.numel(), dtype=x.dtype, device="cuda") for x in d["codes"] + d["scales"]]
+    for b, x in zip(big, d["codes"] + d["scales"]):
+        b[-x.numel():] = x.flatten()
+    c = d["cache"]
+    c.pool_k, c.pool_v, c.scale_k, c.scale_v = (b.data_ptr() for b in big)
+    c.layer = layer
+    case.append()
+    call(nv, d, "append_attn")
+    call(nv, d, "read")
+    torch.cuda.synchronize()
+    assert int(d["status"]) == 0
+    for b, x in zip(big, case.codes + case.scales):
+        assert bool((bits(b[-x.numel():]) == bits(x.flatten())).all())
+    check_rows(case, d["out"].cpu(), torch.ones(sum(new), dtype=torch.bool))
+    for got, want in zip(d["back"], case.read()):
+        assert bool((bits(got) == bits(want)).all())
+    del big
+    torch.cuda.empty_cache()
