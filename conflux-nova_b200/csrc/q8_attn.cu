@@ -4,9 +4,10 @@
 // This file: single new tokens (decode).  What bounds it is HBM: 264 bytes per key and kv head (two rows of codes, two
 // scales), against 4 * 128 * G flops.
 //
-// Measured (int8, bf16 activations, graph replay): 64 sessions x 8192 keys, 40 / 8 heads: 174 us = 6.4 TB/s, 97 % of a plain copy;
-// 1 x 131072: 35 us = 4.0 TB/s; 8 x (2048-8192), 28 / 4 heads: 20 us; 1 x 1024: 9 us, of which 1.2 are the plan, 0.4 the row,
-// 1.4 q, 0.5 the first tile, 0.8 the tiles, 0.9 the partials, 1.6 the gap to the merge, 1.6 the merge.
+// Measured (a graph replayed on one state): 64 sessions x 8192 keys, 40 / 8 heads, int8, bf16 activations: 174 us = 6.4 TB/s, 97 % of a
+// plain copy (200-213 us = 5.2-5.5 TB/s in calls on three such states in turn); 1 x 131072, int8, fp32: 35-37 us = 3.8 TB/s; 8 x
+// (2048-8192), 28 / 4 heads, e4m3, bf16: 20 us; 1 x 1024, int8, fp16: 9.3 us, of which 1.2 are the plan, 0.4 the row, 1.4 q, 0.5 the
+// first tile, 0.8 the tiles, 0.9 the partials, 1.6 the gap to the merge, 1.6 the merge.
 //
 //   * One persistent CTA per SM; the 16-key tiles of all (session, kv group) rows form one line that is dealt out evenly
 //     (DecLine); rows that several CTAs worked on are merged by the kernel behind it.

@@ -18,11 +18,12 @@
 //     from shared memory, which took 1500 cycles of a 64-key tile.  So |K| saturates at 2^17 and |V| at 65504 here.
 //     A lane's rows are chosen so that neither the reads (rows r and r ^ 5 side by side) nor the writes meet in a bank.
 //   * q (rotated) and P are rounded to fp16; everything else is fp32.
-//   * Measured (graph replay, append included): 2048 tokens over 16384, 40 / 8 heads: 860 us = 850 TFLOP/s; 8 x (301-512) tokens over
-//     2k-8k: 340 us = 750 TFLOP/s; 16 x (0-8) tokens over 2k-8k: 51 us = 1.5 TB/s; a window of 512: 52 us.  A 64-key tile of 256 rows
-//     takes 2350 cycles.  The tensor cores are busy for 1020 of them, the special-function units for 1024; what sets the pace is
+//   * Measured (graph replay, append included; in calls on several states in turn): 2048 tokens over 16384, 40 / 8 heads, int8: 900 us =
+//     810 TFLOP/s (917-936); 8 x (301-512) tokens over 2k-8k, e4m3: 355 us = 720 TFLOP/s (377); 16 x (0-8) tokens over 2k-8k, int8:
+//     52 us = 1.5 TB/s (55); a window of 512, e4m3: 52-55 us (54).  A 64-key tile of 256 rows
+//     takes some 2400 cycles.  The tensor cores are busy for 1020 of them, the special-function units for 1024; what sets the pace is
 //     the softmax warps' own chain of some 300 dependent instructions per tile (two warps per scheduler; without the exponentials
-//     it would still be 2200).  A unit costs 5 us of q and 4 us of outputs beside its tiles.
+//     it would still be 2200 or so).  A unit costs 5 us of q and 4 us of outputs beside its tiles.
 //   * Every wait is bounded; tensor memory is released on every path.
 #include "q8_common.cuh"
 #include "tc5_common.cuh"

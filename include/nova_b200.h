@@ -360,13 +360,16 @@ int nova_launch_q8_append(const nova_q8_cache* c, const nova_q8_rows* r, const v
  * rounded once (keys come back as they are stored: rotated). */
 int nova_launch_q8_read(const nova_q8_cache* c, const nova_q8_rows* r, void* k_out, void* v_out, nova_stream_t s);
 /* Attention of the rows of q ([n_tokens][n_heads][128]) over the cached keys: the query at position p sees the keys [0, p], or
- * (p - window, p] where window > 0 (pages of which no query sees a key need no table entry).  The keys of the new rows must be in the cache; a query that sees none gets zeros.
- * q (rotated) and the softmax weights are rounded to fp16 on their way into the tensor cores; sums and the softmax are fp32.
- * One row per session and at most 8 query heads per kv head: the codes go in exactly and the scales are applied in fp32; with
- * fp32 or fp16 activations q and the weights are taken as two fp16 parts each (2^-21).  Anything else: keys and values go in as fp16
- * values, code * scale rounded once (2^-11 of themselves), except that small ones are off by up to 2^-23 (v) or 2^-22 (k), as fp16's
- * grid ends at 2^-24; |k| saturates at 2^17, |v| at 65504.  |q|, rotated, may be up to 2^17.  q and out must not overlap.  work: nova_q8_workspace_bytes() bytes, no state in it
- * between calls; calls that may overlap on the GPU need a workspace each. */
+ * (p - window, p] where window > 0 (pages of which no query sees a key need no table entry).  The keys of the new rows must be
+ * in the cache; a query that sees none gets zeros.
+ * q (rotated, up to 2^17) and the softmax weights are rounded to fp16 on their way into the tensor cores; sums and the softmax are fp32.
+ *   One row per session and at most 8 query heads per kv head: the codes go in exactly and the scales are applied in fp32; with fp32
+ *     or fp16 activations q and the weights are taken as two fp16 parts each (2^-21).
+ *   Anything else: keys and values go in as fp16 values, code * scale rounded once (2^-11 of themselves), except that small ones are
+ *     off by up to 2^-23 (v) or 2^-22 (k), as fp16's grid ends at 2^-24; |k| saturates at 2^17, |v| at 65504; a key that weighs less
+ *     than 2^-32 of a query's heaviest may count as none.
+ * out overlaps none of q, k, v and the cache.  work: nova_q8_workspace_bytes() bytes, no state in it between calls; calls that may
+ * overlap on the GPU need a workspace each. */
 size_t nova_q8_workspace_bytes(const nova_kv_shape* sh, const nova_q8_rows* r);
 int nova_launch_q8_attn(const nova_q8_cache* c, const nova_q8_rows* r, const void* q, void* out, int window, void* work,
                         size_t work_bytes, nova_stream_t s);
